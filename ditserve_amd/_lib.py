@@ -75,6 +75,13 @@ SIGNATURES = {
     "ditk_check_cu_seqlens_pair": (c_int, [_P, c_int, _P, _P, c_int, _P, c_int, _P, _P]),
     "ditk_check_cu_seqlens": (c_int, [_P, c_int, c_int, _P, _P, _P]),
     "ditk_solver_step": (c_int, [_P, _P, _P, _P, _P, _P, _P, _P, _P, c_int64, _P, _P]),
+    "ditk_mx_quantize": (c_int, [_P, c_int64, _P, c_int64, _P, c_int64, c_int, c_int, c_int, _P]),
+    "ditk_mx_norm": (c_int, [_P, c_int64, _P, c_int64, _P, c_int64, _P, c_int64, _P, c_int64, c_int, c_int, _P, c_int,
+                             _P, _P, c_int64, _P, _P, c_float, c_int, _P]),
+    "ditk_mx_gemm": (c_int, [_P, c_int64, _P, c_int64, _P, c_int64, _P, c_int64, _P, _P, c_int64, _P, c_int64, c_int,
+                             c_int, c_int, c_int, c_int, _P, c_int64, _P, c_int64, _P, c_int, _P]),
+    "ditk_mx_matvec": (c_int, [_P, c_int64, _P, c_int64, _P, c_int64, _P, _P, c_int64, c_int, c_int, c_int, c_int, _P,
+                               c_int64, _P]),
     "ditk_flash_attn_varlen_noalloc": (c_int, [_P, c_int64, _P, c_int64, _P, c_int64, _P, c_int64, _P, c_int64,
                                                _P, _P, c_int, c_int, c_int, c_int, c_int, c_float, _P]),
 }

@@ -1,0 +1,356 @@
+"""Products of microscaled (MX) matrices: 8-bit activations and weights, 4-bit weights.
+
+An MX matrix holds for every 32 consecutive columns of a row one scale 2^e and the
+values over it in e4m3 ("fp8") or e2m1 ("fp4").  `norm` and `quantize` write them,
+`linear` multiplies two of them on the scaled MFMA (and can write the next one),
+`matvec` multiplies a few bf16 rows with a 4-bit weight:
+
+    w_up, w_down = mx.quantize(up_weight), mx.quantize(down_weight)   # once
+    y, h = mx.norm(x, residual, weight=w)                             # 8-bit rows, new residual
+    y = mx.linear(y, w_up, b_up, epilogue="gelu", out_fmt="fp8")
+    h = mx.linear(y, w_down, b_down, epilogue="res", residual=h)
+
+Checks, streams and errors are those of ditserve_amd.ops.  The reference has no
+counterpart: its products are in fp16 or bf16.
+"""
+import torch
+
+from . import _lib, ops
+from .ops import EPILOGUES, _check, _extent, _meet, _ptr, _rows, _vec
+
+FORMATS = {"fp8": 0, "fp4": 1}
+_BF16, _E4M3, _E8M0 = torch.bfloat16, torch.float8_e4m3fn, torch.float8_e8m0fnu
+_DATA_TYPE = {"fp8": _E4M3, "fp4": torch.uint8}
+
+
+def _data_bytes(cols, fmt):
+    """Bytes of a row's values with the padding to 128 columns."""
+    n = (cols + 127) // 128 * 128
+    return n // 2 if fmt == "fp4" else n
+
+
+def _scale_bytes(cols):
+    """Bytes of a row's scales with the padding to 16 blocks."""
+    return (cols + 511) // 512 * 16
+
+
+class MXTensor:
+    """An MX matrix of `cols` columns, a multiple of 32.
+
+    fmt     "fp8" or "fp4"
+    data    [rows, cols rounded up to 128] float8_e4m3fn, or half as many uint8 (the
+            even column in the low four bits); zeros behind `cols`
+    scales  [rows, cols / 32 rounded up to 16] float8_e8m0fnu; of each 16, the scale
+            of block 4 s + g stands at 4 g + s
+
+    Rows may be strided (multiples of 16 bytes)."""
+
+    __slots__ = ("fmt", "data", "scales", "cols")
+
+    def __init__(self, fmt, data, scales, cols):
+        if fmt not in FORMATS:
+            raise ValueError(f"an MX matrix is 'fp8' or 'fp4', got {fmt!r}")
+        _check(data, "data", _DATA_TYPE[fmt], 2)
+        _check(scales, "scales", _E8M0, 2)
+        cols = int(cols)
+        if cols <= 0 or cols % 32:
+            raise ValueError(f"an MX matrix has blocks of 32 columns, got {cols}")
+        if data.shape[1] != _data_bytes(cols, fmt) or scales.shape != (data.shape[0], _scale_bytes(cols)):
+            raise ValueError(f"{cols} {fmt} columns take data [rows, {_data_bytes(cols, fmt)}] and scales "
+                             f"[rows, {_scale_bytes(cols)}], got {tuple(data.shape)} and {tuple(scales.shape)}")
+        if data.device != scales.device:
+            raise ValueError(f"data is on {data.device}, scales on {scales.device}")
+        for t, name in ((data, "data"), (scales, "scales")):
+            st = t.stride()
+            if st[1] != 1 or st[0] % 16 or (t.shape[0] > 1 and st[0] < t.shape[1]) or t.data_ptr() % 16:
+                raise ValueError(f"{name} rows must have unit column stride and be 16-byte aligned, got strides {st}")
+        self.fmt, self.data, self.scales, self.cols = fmt, data, scales, cols
+
+    @classmethod
+    def empty(cls, rows, cols, device, fmt="fp8"):
+        """An uninitialised MX matrix (an output for quantize, norm or linear)."""
+        if fmt not in FORMATS or cols <= 0 or cols % 32:
+            raise ValueError(f"an MX matrix is 'fp8' or 'fp4' with blocks of 32 columns, got {fmt!r} and {cols}")
+        self = cls.__new__(cls)
+        self.fmt, self.cols = fmt, int(cols)
+        self.data = torch.empty((rows, _data_bytes(cols, fmt)), dtype=_DATA_TYPE[fmt], device=device)
+        self.scales = torch.empty((rows, _scale_bytes(cols)), dtype=_E8M0, device=device)
+        return self
+
+    @property
+    def rows(self):
+        return self.data.shape[0]
+
+    @property
+    def shape(self):
+        return (self.data.shape[0], self.cols)
+
+    @property
+    def device(self):
+        return self.data.device
+
+    def __getitem__(self, rows):
+        """A view of some rows (a slice with step 1)."""
+        if not isinstance(rows, slice) or rows.step not in (None, 1):
+            raise ValueError("an MX matrix is indexed by a slice of rows")
+        return MXTensor(self.fmt, self.data[rows], self.scales[rows], self.cols)
+
+    def record_stream(self, stream):
+        """Mark both tensors as in use by `stream` (for rows consumed on a side stream)."""
+        self.data.record_stream(stream)
+        self.scales.record_stream(stream)
+
+    def dequantize(self):
+        """The fp32 values [rows, cols], for inspection (plain torch operations)."""
+        rows, cols = self.shape
+        if self.fmt == "fp8":
+            v = self.data.float()
+        else:
+            table = torch.tensor([0, 0.5, 1, 1.5, 2, 3, 4, 6], device=self.device)
+            table = torch.cat([table, -table])
+            v = torch.stack([table[(self.data & 15).long()], table[(self.data >> 4).long()]], 2).reshape(rows, -1)
+        s = self.scales.float().reshape(rows, -1, 4, 4).transpose(2, 3).reshape(rows, -1)[:, :cols // 32]
+        return (v[:, :cols].reshape(rows, cols // 32, 32) * s.unsqueeze(2)).reshape(rows, cols)
+
+    def _args(self):
+        return _ptr(self.data), self.data.stride(0), _ptr(self.scales), self.scales.stride(0)
+
+
+def _call(device, name, *args):
+    """Launch on the current stream of `device`, which need not be the current device."""
+    if device.index == torch.cuda.current_device():
+        return _lib.call(name, *args, ops._stream())
+    with torch.cuda.device(device):
+        return _lib.call(name, *args, ops._stream())
+
+
+def _one_device(device, **tensors):
+    for name, t in tensors.items():
+        if t is not None and t.device != device:
+            raise ValueError(f"{name} is on {t.device}, the other operands on {device}")
+
+
+def _mx_check(m, name, fmt=None):
+    if not isinstance(m, MXTensor):
+        raise ValueError(f"{name} must be an MXTensor, got {type(m).__name__}")
+    if fmt is not None and m.fmt != fmt:
+        raise ValueError(f"{name} must be {fmt}, got {m.fmt}")
+
+
+def _mx_out(out, rows, cols, device, fmt):
+    if out is None:
+        return MXTensor.empty(rows, cols, device, fmt)
+    _mx_check(out, "out", fmt)
+    if out.shape != (rows, cols):
+        raise ValueError(f"out must be [{rows}, {cols}], got {out.shape}")
+    _one_device(device, out=out)
+    return out
+
+
+def _apart(fn, outs, operands, same=()):
+    """Refuse outputs that share memory with an operand or with each other.  same:
+    operands that an output may be as a whole (written where they are read)."""
+    spans = [(t, _extent(t)) for t in outs]
+    for i, (t, e) in enumerate(spans):
+        for u in (*operands, *same, *(o for o, _ in spans[i + 1:])):
+            if u is None or not _meet(e, _extent(u)):
+                continue
+            if any(u is s for s in same) and t.data_ptr() == u.data_ptr() and t.stride() == u.stride() \
+                    and t.dtype == u.dtype and t.shape == u.shape:
+                continue
+            raise ValueError(f"{fn}: an output overlaps an operand or another output")
+
+
+def quantize(x, fmt="fp8", out=None):
+    """The MX matrix of x [T, K] bf16 (a row view), K % 32 == 0.
+
+    Per block of 32 the scale is the smallest power of two (at least 2^-126) under
+    which no value passes 448 (fp8) or 6 (fp4); values are rounded to nearest even.
+    A block that holds an infinity or NaN becomes NaN (in fp4: by its scale)."""
+    if fmt not in FORMATS:
+        raise ValueError(f"fmt must be 'fp8' or 'fp4', got {fmt!r}")
+    _check(x, "x", _BF16, 2)
+    T, K = x.shape
+    ldx = _rows(x, "x")
+    if K == 0 or K % 32:
+        raise ValueError(f"x needs blocks of 32 columns, got {K}")
+    given = out
+    out = _mx_out(out, T, K, x.device, fmt)
+    if given is not None:
+        _apart("quantize", (out.data, out.scales), (x,))
+    _call(x.device, "ditk_mx_quantize", _ptr(x), ldx, *out._args(), T, K, FORMATS[fmt])
+    return out
+
+
+def norm(x, residual=None, shift=None, scale=None, segments=None, weight=None, bias=None, eps=1e-6, kind="rms",
+         out=None, residual_out=None):
+    """ops.adaln with the residual's addition before it and an fp8 MX output:
+    s = x + residual; MX(norm(s)[*w + b][*(1 + scale[seg]) + shift[seg]]).
+
+    x, residual [T, D] bf16 row views, D % 32 == 0, D <= 6144; the other arguments as
+    ops.adaln's, kind "rms" by default.  Returns the MX matrix, and with a residual
+    also s in bf16 (in residual_out if given, which may be x or residual itself);
+    the norm is that of the unrounded s."""
+    _check(x, "x", _BF16, 2)
+    T, D = x.shape
+    ldx = _rows(x, "x")
+    if D == 0 or D % 32:
+        raise ValueError(f"x needs blocks of 32 columns, got {D}")
+    if kind not in ("ln", "rms"):
+        raise ValueError(f"kind must be 'ln' or 'rms', got {kind!r}")
+    _one_device(x.device, residual=residual, shift=shift, scale=scale, weight=weight, bias=bias,
+                residual_out=residual_out, segments=None if segments is None else segments.dev)
+    h, ldr, ldh = None, 0, 0
+    if residual is not None:
+        _check(residual, "residual", _BF16, 2)
+        if residual.shape != (T, D):
+            raise ValueError(f"residual must be [{T}, {D}], got {tuple(residual.shape)}")
+        ldr = _rows(residual, "residual")
+        if residual_out is None:
+            h = torch.empty((T, D), dtype=_BF16, device=x.device)
+        else:
+            h = residual_out
+            _check(h, "residual_out", _BF16, 2)
+            if h.shape != (T, D):
+                raise ValueError(f"residual_out must be [{T}, {D}], got {tuple(h.shape)}")
+        ldh = _rows(h, "residual_out")
+    elif residual_out is not None:
+        raise ValueError("residual_out needs a residual")
+    mod_stride, cu, nseg = 0, None, 0
+    if (shift is None) != (scale is None):
+        raise ValueError("shift and scale go together")
+    if shift is not None:
+        _check(shift, "shift", torch.float32, 2)
+        _check(scale, "scale", torch.float32, 2)
+        if segments is None:
+            raise ValueError("modulation requires segments")
+        if shift.shape != (segments.nseg, D) or scale.shape != (segments.nseg, D):
+            raise ValueError(f"shift/scale must be [{segments.nseg}, {D}]")
+        if shift.stride(1) != 1 or scale.stride(1) != 1 or scale.stride(0) != shift.stride(0):
+            raise ValueError("shift/scale must share a row stride with unit column stride")
+        if segments.total != T:
+            raise ValueError(f"segments cover {segments.total} tokens, x has {T}")
+        mod_stride, cu, nseg = shift.stride(0), segments.dev, segments.nseg
+    for t, n in ((weight, "weight"), (bias, "bias")):
+        if t is not None:
+            _vec(t, n, D)
+    y = _mx_out(out, T, D, x.device, "fp8")
+    if out is not None or residual_out is not None:
+        outs = ([] if out is None else [y.data, y.scales]) + ([] if residual_out is None else [h])
+        _apart("norm", outs, (shift, scale, weight, bias), same=(x, residual))
+    _call(x.device, "ditk_mx_norm", _ptr(x), ldx, _ptr(residual), ldr, _ptr(h), ldh, *y._args(), T, D, _ptr(cu), nseg,
+          _ptr(shift), _ptr(scale), mod_stride, _ptr(weight), _ptr(bias), float(eps), 0 if kind == "ln" else 1)
+    return y if residual is None else (y, h)
+
+
+def _bf16_out(out, M, N, dtype, device):
+    if out is None:
+        return torch.empty((M, N), dtype=dtype, device=device)
+    _check(out, "out", dtype, 2)
+    ldc, unit = out.stride()
+    if out.shape != (M, N) or unit != 1 or ldc % 8 or out.data_ptr() % 16:
+        raise ValueError("out must be [M, N], unit column stride, leading dim % 8 == 0, 16-byte aligned")
+    return out
+
+
+def _residual(residual, M, N):
+    _check(residual, "residual", _BF16, 2)
+    ldr, unit = residual.stride()
+    if residual.shape != (M, N) or unit != 1 or ldr % 8 or residual.data_ptr() % 16:
+        raise ValueError("residual must be [M, N] row-major with 16-byte aligned rows")
+    return ldr
+
+
+def linear(x, w, b=None, epilogue="bias", residual=None, gate=None, segments=None, out=None, out_fmt=None):
+    """out = epilogue(x @ w.T + b) of fp8 MX matrices x [M, K], w [N, K] on the scaled MFMA.
+
+    b [N] fp32, N % 8 == 0.  Epilogues as ops.linear's: "bias", "gelu" (GELU-tanh),
+    "silu", "res" (residual + y), "gate_res" (residual + y * gate[seg]); all in fp32
+    with one rounding at the end.  Returns bf16 [M, N] (out may be the residual
+    itself), or with out_fmt="fp8" ("bias", "gelu" and "silu", N % 32 == 0) the MX
+    matrix of the result for the next product.  A row's result does not depend on
+    the other rows: packed and per-request products agree bitwise."""
+    _mx_check(x, "x", "fp8")
+    _mx_check(w, "w", "fp8")
+    (M, K), (N, Kw) = x.shape, w.shape
+    if Kw != K:
+        raise ValueError(f"weight is {w.shape}, input has K={K}")
+    if N == 0 or N % 8:
+        raise ValueError(f"linear needs N % 8 == 0 (got N={N})")
+    if epilogue not in EPILOGUES or epilogue == "f32":
+        raise ValueError(f"unknown epilogue {epilogue!r}")
+    if out_fmt not in (None, "fp8"):
+        raise ValueError(f"out_fmt must be None (bf16) or 'fp8', got {out_fmt!r}")
+    res = epilogue in ("res", "gate_res")
+    if out_fmt and res:
+        raise ValueError(f"epilogue {epilogue!r} writes bf16")
+    if out_fmt and N % 32:
+        raise ValueError(f"an MX output needs N % 32 == 0 (got N={N})")
+    if b is not None:
+        _vec(b, "bias", N)
+    _one_device(x.device, w=w, bias=b, residual=residual if res else None, gate=gate if res else None,
+                out=out, segments=None if segments is None else segments.dev)
+    ldr = _residual(residual, M, N) if res else 0
+    gate_stride, cu, nseg = 0, None, 0
+    if epilogue == "gate_res":
+        _check(gate, "gate", torch.float32, 2)
+        if segments is None or segments.total != M:
+            raise ValueError("gated epilogue needs segments covering M rows")
+        nseg, cu = segments.nseg, segments.dev
+        gate_stride, unit = gate.stride()
+        if gate.shape != (nseg, N) or unit != 1 or gate_stride % 4 or gate.data_ptr() % 16:
+            raise ValueError(f"gate must be [{nseg}, {N}] with unit column stride and 16-byte aligned rows")
+    given = out
+    if out_fmt:
+        out = _mx_out(out, M, N, x.device, "fp8")
+        c, outs = out._args(), (out.data, out.scales)
+    else:
+        out = _bf16_out(out, M, N, _BF16, x.device)
+        c, outs = (_ptr(out), out.stride(0), None, 0), (out,)
+    if given is not None:
+        _apart("linear", outs, (x.data, x.scales, w.data, w.scales, b, gate if res else None),
+               same=(residual,) if res else ())
+    _call(x.device, "ditk_mx_gemm", *x._args(), *w._args(), _ptr(b), *c, M, N, K, EPILOGUES[epilogue],
+          1 if out_fmt else 0, _ptr(residual) if res else None, ldr, _ptr(gate) if cu is not None else None,
+          gate_stride, _ptr(cu), nseg)
+    return out
+
+
+def matvec(x, w, b=None, epilogue="bias", residual=None, out=None):
+    """out = epilogue(x @ w.T + b) of a few bf16 rows and an fp4 MX weight w [N, K].
+
+    x [M, K] (a row view) or [K], b [N] fp32, N % 8 == 0.  Epilogues "bias", "gelu"
+    (GELU-tanh), "silu", "res" (residual + y), "f32" (fp32 output); in fp32 with one
+    rounding at the end.  Returns [M, N] (or [N]).  The weight is read once for every
+    64 rows: for many rows quantize them and use an fp8 weight and linear().  A row's
+    result does not depend on the other rows."""
+    _mx_check(w, "w", "fp4")
+    _check(x, "x", _BF16)
+    if x.dim() not in (1, 2):
+        raise ValueError(f"x must be [M, K] or [K], got shape {tuple(x.shape)}")
+    one = x.dim() == 1
+    if one:
+        x = x.unsqueeze(0)
+        residual = None if residual is None else residual.unsqueeze(0)
+        out = None if out is None else out.unsqueeze(0)
+    M, K = x.shape
+    N = w.rows
+    if w.cols != K:
+        raise ValueError(f"weight is {w.shape}, input has K={K}")
+    if N == 0 or N % 8:
+        raise ValueError(f"matvec needs N % 8 == 0 (got N={N})")
+    if epilogue not in EPILOGUES or epilogue == "gate_res":
+        raise ValueError(f"unknown epilogue {epilogue!r}")
+    ldx = _rows(x, "x")
+    if b is not None:
+        _vec(b, "bias", N)
+    res = epilogue == "res"
+    _one_device(x.device, w=w, bias=b, residual=residual if res else None, out=out)
+    ldr = _residual(residual, M, N) if res else 0
+    given = out
+    out = _bf16_out(out, M, N, torch.float32 if epilogue == "f32" else _BF16, x.device)
+    if given is not None:
+        _apart("matvec", (out,), (x, w.data, w.scales, b), same=(residual,) if res else ())
+    _call(x.device, "ditk_mx_matvec", _ptr(x), ldx, *w._args(), _ptr(b), _ptr(out), out.stride(0), M, N, K,
+          EPILOGUES[epilogue], _ptr(residual) if res else None, ldr)
+    return out[0] if one else out

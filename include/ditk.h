@@ -374,6 +374,67 @@ int ditk_flash_attn_varlen_noalloc(const void* q, int64_t ldq, const void* k, in
                                    const int32_t* cu_k, int nseg, int Tq, int Tk, int heads, int head_dim,
                                    float softmax_scale, ditk_stream_t stream);
 
+/*
+ * Microscaled (MX) matrices.  A block of 32 consecutive columns of a row has one
+ * scale 2^e, stored as the byte e + 127 (e8m0; 255 = NaN), and its values over
+ * that scale in e4m3 (fp8, one byte each) or e2m1 (fp4, two a byte, the even
+ * column in the low half).  A row of K columns holds K rounded up to a multiple
+ * of 128 (zeros behind K) and K / 32 rounded up to a multiple of 16 scale bytes
+ * (127 behind K / 32); within 16 blocks the scale of block 4 s + g is byte
+ * 4 g + s.  Row strides are in bytes, multiples of 16, and every pointer is
+ * 16-byte aligned.  Readers take any bytes (a scale byte 0, 2^-127, may count as
+ * zero) but rely on the zeros behind K.
+ * The reference has no counterpart: its products are in fp16 or bf16.
+ */
+#define DITK_MX_FP8 0
+#define DITK_MX_FP4 1
+
+/*
+ * data, scales = MX of x [T, K] bf16, K % 32 == 0: per block
+ * e = max(ceil(log2(amax / vmax)), -126), vmax 448 (fp8) or 6 (fp4), values
+ * rounded to nearest even.  A block with an infinity or NaN gets the scale NaN
+ * (and, in fp8, NaN values).
+ */
+int ditk_mx_quantize(const void* x, int64_t ldx, void* data, int64_t ldd, void* scales, int64_t lds, int T, int K,
+                     int fmt, ditk_stream_t stream);
+
+/*
+ * s = x (+ residual), h = s in bf16, and the fp8 MX matrix of
+ *   norm(s) [* weight + bias] [* (1 + scale[seg]) + shift[seg]]
+ * (norm_kind 0 = LayerNorm, 1 = RMSNorm, of the unrounded fp32 s; arguments as
+ * ditk_adaln's).  residual and h are both NULL or both given; h may be x or
+ * residual.  D % 32 == 0, D <= 6144.
+ */
+int ditk_mx_norm(const void* x, int64_t ldx, const void* residual, int64_t ldr, void* h, int64_t ldh, void* data,
+                 int64_t ldd, void* scales, int64_t lds, int T, int D, const int32_t* cu_seqlens, int nseg,
+                 const float* shift, const float* scale, int64_t mod_stride, const float* weight, const float* bias,
+                 float eps, int norm_kind, ditk_stream_t stream);
+
+/*
+ * C = epilogue(A W^T + bias) of fp8 MX matrices A [M, K] and W [N, K], K % 32 == 0,
+ * N % 8 == 0; fp32 accumulation, one rounding at the end.  epilogue 0 bias, 1
+ * GELU-tanh, 2 R + y * gate[seg], 3 R + y, 5 SiLU (as ditk_gemm's, which also
+ * rounds before the activation or residual).  out_kind 0: C bf16 [M, N], ldc in
+ * elements, ldc % 8 == 0, may be R itself.  out_kind 1 (epilogues 0, 1, 5; N % 32 ==
+ * 0): C, Cs the fp8 MX matrix of the result, padding included.  Every row is
+ * computed the same way whatever M is and wherever it sits.
+ */
+int ditk_mx_gemm(const void* A, int64_t lda, const void* As, int64_t ldas, const void* W, int64_t ldw, const void* Ws,
+                 int64_t ldws, const float* bias, void* C, int64_t ldc, void* Cs, int64_t ldcs, int M, int N, int K,
+                 int epilogue, int out_kind, const void* R, int64_t ldr, const float* gate, int64_t gate_stride,
+                 const int32_t* cu_seqlens, int nseg, ditk_stream_t stream);
+
+/*
+ * C = epilogue(x W^T + bias) of bf16 rows x [M, K] and an fp4 MX matrix W [N, K],
+ * K % 32 == 0, N % 8 == 0, for few rows: the weight is read once for every 64 rows.
+ * fp32 accumulation, one rounding at the end.  epilogue 0 bias, 1 GELU-tanh, 3 R + y,
+ * 4 fp32 output, 5 SiLU.  ldc, ldr in elements, multiples of 8; C may be R itself.
+ * Every row is computed the same way whatever M is.
+ */
+int ditk_mx_matvec(const void* x, int64_t ldx, const void* W, int64_t ldw, const void* Ws, int64_t ldws,
+                   const float* bias, void* C, int64_t ldc, int M, int N, int K, int epilogue, const void* R,
+                   int64_t ldr, ditk_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif
