@@ -16,9 +16,11 @@
 //
 // The k order is fixed and nothing is split along k, so an output element is the same
 // whatever M is, wherever its row sits and whichever tile computed it.
+#include <algorithm>
 #include <type_traits>
 
 #include "mx_common.h"
+#include "mx_l4_clobbers.h"
 
 namespace {
 
@@ -46,6 +48,7 @@ struct MxGemmArgs {
   const int32_t* cu;
   int nseg, M, N, K;
   int tiles_m, tiles_n, group_m;
+  bool stream;  // output stored past the caches
 };
 
 // 16 bytes per lane, global -> LDS; the wave's 64 lanes fill 1 KiB from slot0 on
@@ -59,87 +62,216 @@ __device__ __forceinline__ f32x4_t mfma_mx(i32x8_t w, i32x8_t x, f32x4_t c, uint
   return __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(w, x, c, 0, 0, S, (int)sw, S, (int)sx);
 }
 
-// The epilogue of a wave tile of FJ x 16 tokens and FI x 16 features: accumulators to
-// row-major order through LDS in fp32 (16 tokens at a time, in space of this wave's
-// own), so that the bias, the activation and the residual are added before the
-// one rounding, then 8 features of a token per lane.
-template <int EPI, int OUT, int FI, int FJ>
-__device__ __forceinline__ void mx_epilogue(const MxGemmArgs& p, const f32x4_t (&acc)[FI][FJ], f32x4_t* stage, int m0,
-                                            int n0, int lane) {
-  constexpr int WTN = FI * 16, CPR = WTN / 8, RPP = 64 / CPR, NPASS = 16 / RPP;
-  constexpr int ROW = WTN / 4 + 1;  // 16-byte units of a staged row, one spare: rows start 4 banks apart
-  static_assert(16 % RPP == 0, "whole passes");
-  const int ql = lane & 15, g = lane >> 4;
-  const int c8 = lane % CPR, t0 = lane / CPR;
-  const int n = n0 + c8 * 8;
-  const int nc = min(n, p.N - 8);
-  float bias[8];
+// Row and feature ranges of a workgroup tile.  A tile that would reach past M or N starts
+// earlier instead, so that the rows it loads are there; it stores rows from m0 and features
+// from n0 on, which no other tile has.
+struct MxTile {
+  int m0, n0;  // first row and feature of its own
+  int mb, nb;  // and of those it computes
+};
+
+// Exchanges halves between lanes l and l ^ 8 of each 16: of the first units of two 16-byte
+// registers, a (columns c ..) and b (columns c + 64 bytes ..) of 16 tokens by 4 lanes, to whole
+// 128-byte lines of 8 tokens by 8 lanes: `a` the tokens 0-7, `b` the tokens 8-15.
+__device__ __forceinline__ void to_lines(u32x4_t& a, u32x4_t& b, bool hi) {
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    const f32x4_t b4 = p.bias != nullptr ? *reinterpret_cast<const f32x4_t*>(p.bias + nc + 4 * h) : f32x4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int e = 0; e < 4; ++e) bias[4 * h + e] = b4[e];
+  for (int d = 0; d < 4; ++d) {
+    const uint32_t give = hi ? a[d] : b[d];
+    const uint32_t got = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)give, 0x128, 0xF, 0xF, true);  // row_ror:8
+    a[d] = hi ? got : a[d];
+    b[d] = hi ? b[d] : got;
   }
+}
+
+// The epilogue of a wave tile of FJ x 16 tokens and FI x 16 features, acc(i, j) its accumulators,
+// (m, n) its first row and feature; bias8 and gate8 give 8 features' bias and gate (gate8 where
+// the tile's rows are one segment).  A lane has features 4 g .. + 3 of a token per accumulator;
+// permlane16 swaps between the accumulators of features 32 f and 32 f + 16 leave it with 8
+// consecutive ones (32 f + 16 (g % 2) + 8 (g / 2) ..), a block of 32 among the four lanes of a
+// token.  Everything before the one rounding is in fp32, and nothing goes through LDS, where
+// the next tile's operands are arriving.  Stores are whole 128-byte lines: 65520 x 1536 x 1536
+// (201 MB out) 171 us with 64-byte segments, 159 with lines, 145 past the caches (stream).
+template <int EPI, int OUT, int FI, int FJ, class Acc, class Bias, class Gate>
+__device__ __forceinline__ void mx_epilogue(const MxGemmArgs& p, const Acc& acc, const Bias& bias8, const Gate& gate8,
+                                            bool one_seg, const MxTile& tile, int m, int n, int lane) {
+  static_assert(FI % 4 == 0, "lines of 64 features");
+  constexpr bool kRes = EPI == MXE_RES || EPI == MXE_GATE_RES;
+  constexpr int NF = FI / 2;
+  const int ql = lane & 15, g = lane >> 4;
+  const bool hi = lane & 8;
+  const int nl = n + (g & 1) * 16 + (g >> 1) * 8;
+  // Output and residual go through buffer descriptors at the wave's first row, and a row or column
+  // that is not the tile's has an offset past their range, where stores are dropped and loads
+  // give 0: no branches, behind which the compiler would wait for every store before it uses a load.
+  constexpr uint32_t kOut = 0x80000000u;
+  auto uniform = [](const void* q) {
+    const uint64_t x = (uint64_t)(uintptr_t)q;
+    const uint64_t lo = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)x);
+    const uint64_t hi32 = (uint32_t)__builtin_amdgcn_readfirstlane((int)(uint32_t)(x >> 32));
+    return reinterpret_cast<void*>((uintptr_t)(lo | hi32 << 32));
+  };
+  auto desc = [&](const void* base, int64_t row_bytes) {
+    return __builtin_amdgcn_make_buffer_rsrc(
+        uniform(reinterpret_cast<const char*>(base) + (base != nullptr ? m * row_bytes : 0)), 0, 0x7fffffff, 0x00020000);
+  };
+  const uint32_t ldc = (uint32_t)p.ldc * (OUT == MXO_FP8 ? 1 : 2), ldr = (uint32_t)p.ldr * 2, ldcs = (uint32_t)p.ldcs;
+  const __amdgpu_buffer_rsrc_t cdesc = desc(p.C, ldc), rdesc = desc(kRes ? p.R : nullptr, ldr),
+                               sdesc = desc(OUT == MXO_FP8 ? p.Cs : nullptr, ldcs);
+  const int t_lo = tile.m0 - m, t_hi = p.M - m;  // the tile's rows, from m
+  auto row_ok = [&](int t) { return t >= t_lo && t < t_hi; };
+  auto col_ok = [&](int col) { return col >= tile.n0 && col < p.N; };
+  auto store = [&](const u32x4_t& v, int t, int col, int esize) {
+    const uint32_t off = row_ok(t) && col_ok(col) ? (uint32_t)t * ldc + (uint32_t)(col * esize) : kOut;
+    if (p.stream) __builtin_amdgcn_raw_buffer_store_b128(v, cdesc, off, 0, 2);  // non-temporal
+    else __builtin_amdgcn_raw_buffer_store_b128(v, cdesc, off, 0, 0);
+  };
+  float bias[NF][8], gate[NF][8];
+#pragma unroll
+  for (int f = 0; f < NF; ++f) {
+    bias8(nl + f * 32, bias[f]);
+    if (EPI == MXE_GATE_RES && one_seg) gate8(nl + f * 32, gate[f]);
+  }
+  u32x4_t res[kRes ? FJ : 1][kRes ? NF : 1];  // all of them asked for at once: one latency for the tile
+  auto load_res = [&](int j) {
+    const int t = j * 16 + ql;
+#pragma unroll
+    for (int f = 0; f < NF; ++f)
+      res[j][f] = __builtin_amdgcn_raw_buffer_load_b128(
+          rdesc, row_ok(t) && col_ok(nl + f * 32) ? (uint32_t)t * ldr + (uint32_t)(nl + f * 32) * 2 : kOut, 0, 0);
+  };
+  if (kRes)
+#pragma unroll
+    for (int j = 0; j < FJ; ++j) load_res(j);
 #pragma unroll
   for (int j = 0; j < FJ; ++j) {
-    if (m0 + j * 16 >= p.M) break;  // the same for every lane
+    u32x4_t line[NF];
+    uint32_t q0[NF][2], scales = 0;
 #pragma unroll
-    for (int i = 0; i < FI; ++i) stage[ql * ROW + i * 4 + g] = acc[i][j];
-    __builtin_amdgcn_wave_barrier();
-#pragma unroll
-    for (int r = 0; r < NPASS; ++r) {
-      const int t = r * RPP + t0, m = m0 + j * 16 + t;
+    for (int f = 0; f < NF; ++f) {
+      const f32x4_t a = acc(2 * f, j), b = acc(2 * f + 1, j);
       float y[8];
 #pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const f32x4_t v = stage[t * ROW + c8 * 2 + h];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) y[4 * h + e] = v[e] + bias[4 * h + e];
+      for (int e = 0; e < 4; ++e) {
+        const auto s = __builtin_amdgcn_permlane16_swap(__float_as_uint(a[e]), __float_as_uint(b[e]), false, false);
+        y[e] = __uint_as_float(s[0]) + bias[f][e];
+        y[e + 4] = __uint_as_float(s[1]) + bias[f][e + 4];
       }
-      const bool on = m < p.M && n < p.N;
-      const int mc = min(m, p.M - 1);
       if (EPI == MXE_GELU) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) y[e] = gelu_tanh_f(y[e]);
       } else if (EPI == MXE_SILU) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) y[e] = silu_f(y[e]);
-      } else if (EPI == MXE_RES || EPI == MXE_GATE_RES) {
+      } else if (kRes) {
         float rv[8];
-        unpack8(*reinterpret_cast<const u32x4_t*>(p.R + (int64_t)mc * p.ldr + nc), rv);
+        unpack8(res[j][f], rv);
         if (EPI == MXE_GATE_RES) {
-          const float* gp = p.gate + (int64_t)find_segment(p.cu, p.nseg, mc) * p.gate_stride + nc;
-          const f32x4_t g0 = *reinterpret_cast<const f32x4_t*>(gp), g1 = *reinterpret_cast<const f32x4_t*>(gp + 4);
+          if (!one_seg) {
+            const int mc = min(m + j * 16 + ql, p.M - 1), nc = min(nl + f * 32, p.N - 8);
+            const float* gp = p.gate + (int64_t)find_segment(p.cu, p.nseg, mc) * p.gate_stride + nc;
+            const f32x4_t g0 = *reinterpret_cast<const f32x4_t*>(gp), g1 = *reinterpret_cast<const f32x4_t*>(gp + 4);
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            y[e] = fmaf(y[e], g0[e], rv[e]);
-            y[e + 4] = fmaf(y[e + 4], g1[e], rv[e + 4]);
+            for (int e = 0; e < 4; ++e) {
+              gate[f][e] = g0[e];
+              gate[f][e + 4] = g1[e];
+            }
           }
+#pragma unroll
+          for (int e = 0; e < 8; ++e) y[e] = fmaf(y[e], gate[f][e], rv[e]);
         } else {
 #pragma unroll
           for (int e = 0; e < 8; ++e) y[e] += rv[e];
         }
       }
       if (OUT == MXO_FP8) {
-        // N is whole blocks of 32 (checked on the host): a quad is on or off as one.
-        // What the tile holds behind N is padding.
-        uint32_t q[2];
-        uint32_t s = mx_quantise8<MX_FP8>(y, q);
-        if (n >= p.N) {
-          q[0] = q[1] = 0;
-          s = 127;
+        // N is whole blocks of 32 (checked on the host), tiles start at whole blocks
+        scales |= mx_quantise8<MX_FP8, true>(y, q0[f]) << (8 * (f & 3));
+        if (f & 1) {
+          // lanes g = 0, 1: 16 columns of block f - 1 each, g = 2, 3: of block f
+          const auto s0 = __builtin_amdgcn_permlane32_swap(q0[f - 1][0], q0[f][0], false, false);
+          const auto s1 = __builtin_amdgcn_permlane32_swap(q0[f - 1][1], q0[f][1], false, false);
+          line[f / 2] = u32x4_t{s0[0], s1[0], s0[1], s1[1]};
         }
-        if (m < p.M) {
-          if (n < (int)mx_cols(p.N))
-            *reinterpret_cast<u32x2_t*>(reinterpret_cast<uint8_t*>(p.C) + (int64_t)m * p.ldc + n) = u32x2_t{q[0], q[1]};
-          if ((c8 & 3) == 0 && n < (int)mx_scale_bytes(p.N) * 32)
-            p.Cs[(int64_t)m * p.ldcs + mx_scale_at(n >> 5)] = (uint8_t)s;
-        }
-      } else if (on) {
-        *reinterpret_cast<u32x4_t*>(reinterpret_cast<bf16_t*>(p.C) + (int64_t)m * p.ldc + n) = pack8(y);
+      } else {
+        line[f] = pack8(y);
       }
     }
-    __builtin_amdgcn_wave_barrier();
+    const int t = j * 16;
+    if (OUT == MXO_FP8) {
+      // 64 columns a register; lane g stores the scale of block g of each four
+      const int nb = n + (g >> 1) * 32 + (g & 1) * 16;
+      if (NF == 4) {
+        to_lines(line[0], line[1], hi);
+        store(line[0], t + (ql & 7), nb + (hi ? 64 : 0), 1);
+        store(line[1], t + 8 + (ql & 7), nb + (hi ? 64 : 0), 1);
+      } else {
+        store(line[0], t + ql, nb, 1);
+      }
+      const int col = n + g * 32;
+      __builtin_amdgcn_raw_buffer_store_b8(
+          (uint8_t)(scales >> (8 * g)), sdesc,
+          g < NF && row_ok(t + ql) && col_ok(col) ? (uint32_t)(t + ql) * ldcs + (uint32_t)mx_scale_at(col >> 5) : kOut, 0, 0);
+    } else {
+#pragma unroll
+      for (int f = 0; f < NF; f += 2) {
+        to_lines(line[f], line[f + 1], hi);
+        const int col = nl + f * 32 + (hi ? 32 : 0);
+        store(line[f], t + (ql & 7), col, 2);
+        store(line[f + 1], t + 8 + (ql & 7), col, 2);
+      }
+    }
+  }
+}
+
+// 8 consecutive floats, 16-byte aligned
+__device__ __forceinline__ void load8(const float* src, float (&out)[8]) {
+  const f32x4_t lo = *reinterpret_cast<const f32x4_t*>(src), hi = *reinterpret_cast<const f32x4_t*>(src + 4);
+#pragma unroll
+  for (int e = 0; e < 4; ++e) {
+    out[e] = lo[e];
+    out[e + 4] = hi[e];
+  }
+}
+__device__ __forceinline__ void zero8(float (&out)[8]) {
+#pragma unroll
+  for (int e = 0; e < 8; ++e) out[e] = 0.f;
+}
+
+// Whether the rows [m, m + rows) (the same for the wave) are one segment, and which: by scalar
+// loads, which do not wait for the vector loads and stores on their way.
+__device__ __forceinline__ bool one_segment(const MxGemmArgs& p, int m, int rows, int& seg) {
+  auto load = [&](int i) {
+    int v;
+    asm volatile("s_load_dword %0, %1, 0x0\n s_waitcnt lgkmcnt(0)"
+                 : "=s"(v)
+                 : "s"(p.cu + __builtin_amdgcn_readfirstlane(i))
+                 : "memory");
+    return v;
+  };
+  const int last = min(m + rows, p.M) - 1;
+  int lo = 0, hi = p.nseg - 1;
+  asm volatile("" : "+s"(hi));  // compared here, not kept as a mask across the k loop
+  m = min(m, p.M - 1);
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (load(mid) <= m) lo = mid;
+    else hi = mid - 1;
+  }
+  seg = lo;
+  asm volatile("" : "+s"(lo));
+  return lo + 1 >= p.nseg || load(lo + 1) > last;
+}
+
+// An MX output's padding behind N, by the whole launch: zeros up to a multiple of 128 columns,
+// scales 2^0 up to a multiple of 16.
+__device__ __forceinline__ void mx_out_padding(const MxGemmArgs& p) {
+  const int cols = ((int)mx_cols(p.N) - p.N) / 16, b0 = p.N / 32, sc = (int)mx_scale_bytes(p.N) - b0;
+  const int i = threadIdx.x & 31, per = blockDim.x / 32;  // 32 threads a row: at most 6 + 15 stores
+  if (cols + sc == 0) return;
+  for (int row = blockIdx.x * per + threadIdx.x / 32; row < p.M; row += gridDim.x * per) {
+    if (i < cols)
+      *reinterpret_cast<u32x4_t*>(reinterpret_cast<uint8_t*>(p.C) + (int64_t)row * p.ldc + p.N + i * 16) = u32x4_t{0, 0, 0, 0};
+    if (i >= 16 && i < 16 + sc) p.Cs[(int64_t)row * p.ldcs + mx_scale_at(b0 + i - 16)] = 127;
   }
 }
 
@@ -150,13 +282,11 @@ __global__ __launch_bounds__(WM * WN * 64, EU) void mx_gemm_kernel(MxGemmArgs p)
   constexpr int DA = GBM / 8 / GW, DW = GBN / 8 / GW;  // DMA instructions per wave and stage, 8 rows each
   constexpr int ROWS = GBM + GBN, SG = ROWS / 64;      // scale DMA instructions of a workgroup and four stages
   constexpr int STAGE = ROWS * 8;                      // 16-byte units of a stage
-  constexpr int EPI_UNITS = GW * 16 * (WTN / 4 + 1);
-  constexpr int UNITS = 2 * STAGE + 2 * ROWS;
   static_assert(DA >= 1 && DW >= 1 && DA * GW * 8 == GBM && DW * GW * 8 == GBN && ROWS % 64 == 0, "tile");
-  static_assert(GBN % 128 == 0, "an MX output's column padding lies within the last tile");
-  __shared__ u32x4_t lds[UNITS > EPI_UNITS ? UNITS : EPI_UNITS];
+  __shared__ u32x4_t lds[2 * STAGE + 2 * ROWS];
   u32x4_t* const sc_lds = lds + 2 * STAGE;
 
+  if (OUT == MXO_FP8) mx_out_padding(p);
   const int nb = gridDim.x, b = blockIdx.x;
   const int L = (b & 7) * (nb >> 3) + (b >> 3);
   if (L >= p.tiles_m * p.tiles_n) return;
@@ -245,17 +375,213 @@ __global__ __launch_bounds__(WM * WN * 64, EU) void mx_gemm_kernel(MxGemmArgs p)
     if (kt + 2 < nk) stage(kt + 2, std::integral_constant<int, 2>{});
     if (kt + 3 < nk) stage(kt + 3, std::integral_constant<int, 3>{});
   }
-  __syncthreads();  // every wave's operand reads are done: the space becomes the staging rows
-  if (OUT == MXO_FP8 && n0 + GBN >= p.N) {
-    // the scales behind the last tile, up to the row's multiple of 16 (the data's
-    // padding, up to a multiple of 128 columns, lies within the tile)
-    const int b0 = (n0 + GBN) / 32, nb = (int)mx_scale_bytes(p.N) - b0;
-    for (int i = tid; i < GBM * nb; i += GW * 64)
-      if (m0 + i / nb < p.M) p.Cs[(int64_t)(m0 + i / nb) * p.ldcs + mx_scale_at(b0 + i % nb)] = 127;
-  }
-  mx_epilogue<EPI, OUT, FI, FJ>(p, acc, reinterpret_cast<f32x4_t*>(lds) + wave * (16 * (WTN / 4 + 1)), m0 + a_row0,
-                                n0 + w_row0, lane);
+  int seg = 0;
+  const bool one_seg = EPI != MXE_GATE_RES || one_segment(p, m0 + a_row0, WTM, seg);
+  auto bias8 = [&](int n, float (&v)[8]) {
+    if (p.bias != nullptr) load8(p.bias + min(n, p.N - 8), v);
+    else zero8(v);
+  };
+  auto gate8 = [&](int n, float (&v)[8]) { load8(p.gate + (int64_t)seg * p.gate_stride + min(n, p.N - 8), v); };
+  mx_epilogue<EPI, OUT, FI, FJ>(p, [&](int i, int j) { return acc[i][j]; }, bias8, gate8, one_seg,
+                                MxTile{m0, n0, m0, n0}, m0 + a_row0, n0 + w_row0, lane);
 }
+
+// One wave per SIMD, K > 384: a workgroup tile as 2 x 2 wave tiles with their accumulators in the
+// AGPRs.  The k loop is generated assembly (gen_mx_gemm.py -> mx_l4_*_body.inc); this C++ part
+// gives it the per-lane addresses and runs the epilogue on the accumulators.  Persistent:
+// XCD x (= blockIdx % 8) owns the tiles [x * per_xcd, (x + 1) * per_xcd), which its workgroups take
+// in turn; the operands of a workgroup's tiles are one stream of stages, so the next tile's
+// first stages arrive under the epilogue.
+template <int FI, int FJ>
+struct MxL4 {
+  static constexpr int GBM = 32 * FJ, GBN = 32 * FI, ROWS = GBM + GBN;
+  static constexpr int NBUF = FJ == 8 ? 2 : FI == 8 ? 3 : 4;  // stage buffers, as generated
+  static constexpr int VEC0 = NBUF * ROWS * 128 + 2 * ROWS * 16;  // bias of two tiles, then gates of two
+  static constexpr int LDS_BYTES = VEC0 + 4 * 1024;
+  static_assert(LDS_BYTES <= 160 * 1024, "LDS");
+};
+#define DITK_MX_L4_START_OPERANDS                                                                                     \
+  [a_lo] "s"(lo32(cur.a)), [a_hi] "s"(hi32(cur.a)), [w_lo] "s"(lo32(cur.w)), [w_hi] "s"(hi32(cur.w)),                 \
+      [sa_lo] "s"(lo32(cur.sa)), [sa_hi] "s"(hi32(cur.sa)), [sw_lo] "s"(lo32(cur.sw)), [sw_hi] "s"(hi32(cur.sw)),     \
+      [ldsw] "s"(ldsw), [scm_a] "s"(scm_a), [scm_w] "s"(scm_w), [saoff] "v"(lv.saoff), [swoff] "v"(lv.swoff),               \
+      [aoff0] "v"(lv.aoff[0]), [aoff1] "v"(lv.aoff[1]), [aoff2] "v"(lv.aoff[2]), [aoff3] "v"(lv.aoff[3]), [aoff4] "v"(lv.aoff[4]),   \
+      [aoff5] "v"(lv.aoff[5]), [aoff6] "v"(lv.aoff[6]), [aoff7] "v"(lv.aoff[7]), [woff0] "v"(lv.woff[0]), [woff1] "v"(lv.woff[1]),   \
+      [woff2] "v"(lv.woff[2]), [woff3] "v"(lv.woff[3]), [woff4] "v"(lv.woff[4]), [woff5] "v"(lv.woff[5]), [woff6] "v"(lv.woff[6]),   \
+      [woff7] "v"(lv.woff[7])
+#define DITK_MX_L4_OPERANDS                                                                                           \
+  DITK_MX_L4_START_OPERANDS, [na_lo] "s"(lo32(nxt.a)), [na_hi] "s"(hi32(nxt.a)), [nw_lo] "s"(lo32(nxt.w)),            \
+      [nw_hi] "s"(hi32(nxt.w)), [nsa_lo] "s"(lo32(nxt.sa)), [nsa_hi] "s"(hi32(nxt.sa)), [nsw_lo] "s"(lo32(nxt.sw)),   \
+      [nsw_hi] "s"(hi32(nxt.sw)), [nk] "s"(nk), [rdx0] "v"(lv.rdx[0]), [rdx1] "v"(lv.rdx[1]), [rdw0] "v"(lv.rdw[0]),           \
+      [rdw1] "v"(lv.rdw[1]), [scx] "v"(lv.scx), [scw] "v"(lv.scw)
+
+template <int EPI, int OUT, int FI, int FJ>
+__global__ __launch_bounds__(256, 1) void mx_gemm_l4(MxGemmArgs p) {
+  using G = MxL4<FI, FJ>;
+  constexpr int GBM = G::GBM, GBN = G::GBN, ROWS = G::ROWS, WTM = 16 * FJ, WTN = 16 * FI;
+  __shared__ u32x4_t lds[G::LDS_BYTES / 16];
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int a_row0 = (wave & 1) * WTM, w_row0 = (wave >> 1) * WTN;
+  auto su = [](uint32_t x) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)x); };
+  auto lo32 = [&](uint64_t x) { return su((uint32_t)x); };
+  auto hi32 = [&](uint64_t x) { return su((uint32_t)(x >> 32)); };
+  const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) u32x4_t*)&lds[0];
+  const uint32_t sc0 = lds0 + G::NBUF * ROWS * 128;
+  // The lane's id anew, so that neither it nor what is computed from it is kept across the k loop,
+  // which has no registers to spare: spilled, it would be read back behind all of a tile's stores
+  // (which share the loads' counter), every store of the tile waited for.
+  auto lane_id = []() {
+    int l;
+    asm volatile("v_mbcnt_lo_u32_b32 %0, -1, 0\n v_mbcnt_hi_u32_b32 %0, -1, %0" : "=v"(l));
+    return l;
+  };
+  const int sa_row = (wave % (GBM / 64)) * 64, sw_row = (wave % (GBN / 64)) * 64;
+  const uint32_t ldsw = su(lds0 + wave * 1024), scm_a = su(sc0 + sa_row * 16), scm_w = su(sc0 + (GBM + sw_row) * 16);
+  const uint32_t nk = su((p.K + 127) / 128);
+  struct Lane {
+    uint32_t rdx[2], rdw[2], scx, scw, aoff[8], woff[8], saoff, swoff;
+  };
+  auto lane_values = [&](int lane) {
+    const int ql = lane & 15, g = lane >> 4;
+    Lane v;
+    // fragment reads: row ql of a 16-row fragment, 16-byte units g and 4 + g of its 128 k,
+    // stored at unit ^ ((row >> 1) & 7) of the 128-byte LDS row
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      const uint32_t part = (uint32_t)(ql * 128 + (((c * 4 + g) ^ ((ql >> 1) & 7)) * 16));
+      v.rdx[c] = lds0 + a_row0 * 128 + part;
+      v.rdw[c] = lds0 + (GBM + w_row0) * 128 + part;
+    }
+    v.scx = sc0 + (a_row0 + ql) * 16 + g * 4;
+    v.scw = sc0 + (GBM + w_row0 + ql) * 16 + g * 4;
+    // DMA instruction d of this wave fills rows 8 (4 d + wave) .. + 7 (1 KiB): lane l -> row l / 8, LDS
+    // unit l % 8 <- k unit (l % 8) ^ ((row >> 1) & 7).  Rows past the matrix (of a matrix of less than a
+    // tile's rows) read its last one.
+#pragma unroll
+    for (int d = 0; d < 8; ++d) {
+      const int row = (d * 4 + wave) * 8 + lane / 8;
+      const uint32_t unit = (uint32_t)(((lane & 7) ^ ((row >> 1) & 7)) * 16);
+      v.aoff[d] = d < FJ ? (uint32_t)min(row, p.M - 1) * (uint32_t)p.lda + unit : 0u;
+      v.woff[d] = d < FI ? (uint32_t)min(row, p.N - 1) * (uint32_t)p.ldw + unit : 0u;
+    }
+    // scale DMA: 64 rows of 16 bytes; a wave has one instruction for A and one for W (at 128 rows
+    // two waves each fetch the same rows)
+    v.saoff = (uint32_t)min(sa_row + lane, p.M - 1) * (uint32_t)p.ldas;
+    v.swoff = (uint32_t)min(sw_row + lane, p.N - 1) * (uint32_t)p.ldws;
+    return v;
+  };
+
+  struct Bases {
+    uint64_t a, w, sa, sw;
+  };
+  auto tile_at = [&](int L) {
+    const int group = L / (p.group_m * p.tiles_n), first_m = group * p.group_m;
+    const int gm = min(p.group_m, p.tiles_m - first_m), pid = L % (p.group_m * p.tiles_n);
+    MxTile t;
+    t.m0 = (first_m + pid % gm) * GBM;
+    t.n0 = pid / gm * GBN;
+    t.mb = min(t.m0, max(0, p.M - GBM));
+    t.nb = min(t.n0, max(0, p.N - GBN));
+    return t;
+  };
+  auto bases = [&](const MxTile& t) {
+    return Bases{(uint64_t)(uintptr_t)(p.A + t.mb * p.lda), (uint64_t)(uintptr_t)(p.W + t.nb * p.ldw),
+                 (uint64_t)(uintptr_t)(p.As + t.mb * p.ldas), (uint64_t)(uintptr_t)(p.Ws + t.nb * p.ldws)};
+  };
+  const int nb = gridDim.x, b = blockIdx.x, ntiles = p.tiles_m * p.tiles_n, per_xcd = (ntiles + 7) / 8;
+  const int thi = min((b & 7) * per_xcd + per_xcd, ntiles);
+  int L = (b & 7) * per_xcd + (b >> 3);
+  if (OUT == MXO_FP8) mx_out_padding(p);
+  if (L >= thi) return;
+  MxTile tile = tile_at(L);
+  Bases cur = bases(tile);
+  {
+  const Lane lv = lane_values(lane_id());
+  if constexpr (FI == 8 && FJ == 8)
+    asm volatile(
+#include "mx_l4_256x256_start.inc"
+        : : DITK_MX_L4_START_OPERANDS : DITK_MX_L4_256X256_CLOBBERS "scc", "memory");
+  else if constexpr (FI == 8 && FJ == 4)
+    asm volatile(
+#include "mx_l4_128x256_start.inc"
+        : : DITK_MX_L4_START_OPERANDS : DITK_MX_L4_128X256_CLOBBERS "scc", "memory");
+  else
+    asm volatile(
+#include "mx_l4_128x128_start.inc"
+        : : DITK_MX_L4_START_OPERANDS : DITK_MX_L4_128X128_CLOBBERS "scc", "memory");
+  }
+  uint32_t buf = 0, scb = 0;  // LDS offsets of the next tile's stage 0 and scale group 0
+  int par = 0;                // this tile's bias and gate in LDS
+  for (;;) {
+    // The tile's bias and gate come through LDS, asked for a tile ahead of their use: loaded behind
+    // the k loop they would wait for the next tile's DMA.  (The buffers alternate: waves may
+    // still be in the last tile's epilogue, but behind the last barrier of the tile before.)
+    int seg = 0;
+    const bool one_seg = EPI != MXE_GATE_RES || one_segment(p, tile.mb, GBM, seg);
+    const int vrow = (wave % (GBN / 64)) * 64;
+    auto fetch = [&](const float* src, int at) {
+      const uint32_t m0v = su(lds0 + G::VEC0 + at * 1024 + vrow * 4), off = (uint32_t)min(tile.nb + vrow + lane_id(), p.N - 1) * 4;
+      asm volatile("s_mov_b32 m0, %0\n s_nop 0\n global_load_lds_dword %1, %2" ::"s"(m0v), "v"(off), "s"(src) : "memory");
+    };
+    uint64_t has_bias = (uint64_t)(uintptr_t)p.bias;  // compared where it is used, as lane_id()
+    asm volatile("" : "+s"(has_bias));
+    if (has_bias) fetch(p.bias, par);
+    if (EPI == MXE_GATE_RES && one_seg) fetch(p.gate + (int64_t)seg * p.gate_stride, 2 + par);
+    const int Ln = L + (nb >> 3);
+    const bool more = Ln < thi;
+    const MxTile next = more ? tile_at(Ln) : tile;
+    const Bases nxt = bases(next);  // behind the last tile: its own first stages once more, read by nobody
+    f32x16_t c[FI * FJ / 4];
+    buf = su(buf);
+    scb = su(scb);
+    const Lane lv = lane_values(lane_id());
+    if constexpr (FI == 8 && FJ == 8)
+      asm volatile(
+#include "mx_l4_256x256_body.inc"
+          : [buf] "+s"(buf), [scb] "+s"(scb), "={a[0:15]}"(c[0]), "={a[16:31]}"(c[1]), "={a[32:47]}"(c[2]),
+            "={a[48:63]}"(c[3]), "={a[64:79]}"(c[4]), "={a[80:95]}"(c[5]), "={a[96:111]}"(c[6]), "={a[112:127]}"(c[7]),
+            "={a[128:143]}"(c[8]), "={a[144:159]}"(c[9]), "={a[160:175]}"(c[10]), "={a[176:191]}"(c[11]),
+            "={a[192:207]}"(c[12]), "={a[208:223]}"(c[13]), "={a[224:239]}"(c[14]), "={a[240:255]}"(c[15])
+          : DITK_MX_L4_OPERANDS : DITK_MX_L4_256X256_CLOBBERS "scc", "memory");
+    else if constexpr (FI == 8 && FJ == 4)
+      asm volatile(
+#include "mx_l4_128x256_body.inc"
+          : [buf] "+s"(buf), [scb] "+s"(scb), "={a[0:15]}"(c[0]), "={a[16:31]}"(c[1]), "={a[32:47]}"(c[2]),
+            "={a[48:63]}"(c[3]), "={a[64:79]}"(c[4]), "={a[80:95]}"(c[5]), "={a[96:111]}"(c[6]), "={a[112:127]}"(c[7])
+          : DITK_MX_L4_OPERANDS : DITK_MX_L4_128X256_CLOBBERS "scc", "memory");
+    else
+      asm volatile(
+#include "mx_l4_128x128_body.inc"
+          : [buf] "+s"(buf), [scb] "+s"(scb), "={a[0:15]}"(c[0]), "={a[16:31]}"(c[1]), "={a[32:47]}"(c[2]),
+            "={a[48:63]}"(c[3])
+          : DITK_MX_L4_OPERANDS : DITK_MX_L4_128X128_CLOBBERS "scc", "memory");
+    auto acc = [&](int i, int j) {
+      const int r = i * FJ + j;
+      const f32x16_t& v = c[r / 4];
+      const int e = r % 4 * 4;
+      return f32x4_t{v[e], v[e + 1], v[e + 2], v[e + 3]};
+    };
+    const int lane = lane_id();
+    const float* vec = reinterpret_cast<const float*>(reinterpret_cast<const char*>(lds) + G::VEC0) - tile.nb;
+    asm volatile("" : "+s"(has_bias));
+    auto bias8 = [&](int n, float (&v)[8]) {
+      if (has_bias) load8(vec + par * 256 + n, v);
+      else zero8(v);
+    };
+    auto gate8 = [&](int n, float (&v)[8]) { load8(vec + (2 + par) * 256 + n, v); };
+    mx_epilogue<EPI, OUT, FI, FJ>(p, acc, bias8, gate8, one_seg, tile, tile.mb + a_row0, tile.nb + w_row0, lane);
+    if (!more) break;
+    par ^= 1;
+    L = Ln;
+    tile = next;
+    cur = nxt;
+  }
+  // the DMAs on their way behind the last tile have to land before the LDS is another workgroup's
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+}
+
+// An output of this size or more is stored past the caches: it would not stay there until the
+// next kernel reads it, as gemm.hip's.
+constexpr int64_t kStreamBytes = 64ll << 20;
 
 // Tile order: groups of m-tiles walked m-fastest, so the tiles running together share
 // operand rows in their XCD's L2.
@@ -273,10 +599,30 @@ int launch(MxGemmArgs p, hipStream_t stream) {
   return ditk_check_launch("ditk_mx_gemm");
 }
 
+template <int EPI, int OUT, int FI, int FJ>
+int launch_l4(MxGemmArgs p, hipStream_t stream) {
+  constexpr int GBM = MxL4<FI, FJ>::GBM, GBN = MxL4<FI, FJ>::GBN;
+  p.tiles_m = (p.M + GBM - 1) / GBM;
+  p.tiles_n = (p.N + GBN - 1) / GBN;
+  p.group_m = mx_group_m(p.K, p.tiles_n);
+  const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n;
+  DITK_REQUIRE(tiles < (1ll << 30), "ditk_mx_gemm: grid too large");
+  // one persistent workgroup per CU (a multiple of 8: the same number per XCD)
+  const int64_t blocks = std::min<int64_t>((tiles + 7) / 8 * 8, std::max(8, ditk_cu_count() / 8 * 8));
+  mx_gemm_l4<EPI, OUT, FI, FJ><<<(unsigned)blocks, 256, 0, stream>>>(p);
+  return ditk_check_launch("ditk_mx_gemm");
+}
+
 template <int EPI, int OUT>
 int launch_tile(const MxGemmArgs& p, hipStream_t stream) {
-  if ((int64_t)((p.M + 255) / 256) * ((p.N + 255) / 256) >= 128) return launch<EPI, OUT, 4, 8, 2, 4, 1>(p, stream);
-  return launch<EPI, OUT, 4, 2, 2, 2, 2>(p, stream);
+  // 32-bit row offsets within a tile
+  const int64_t ld = std::max(std::max(p.lda, p.ldw), std::max(p.ldas, p.ldws));
+  const bool l4 = p.K > 384 && 256 * ld < (1ll << 31);
+  const int64_t t256 = (int64_t)((p.M + 255) / 256) * ((p.N + 255) / 256);
+  if (!l4) return t256 >= 128 ? launch<EPI, OUT, 4, 8, 2, 4, 1>(p, stream) : launch<EPI, OUT, 4, 2, 2, 2, 2>(p, stream);
+  if (t256 >= 192) return launch_l4<EPI, OUT, 8, 8>(p, stream);
+  if ((int64_t)((p.M + 127) / 128) * ((p.N + 255) / 256) >= 128) return launch_l4<EPI, OUT, 8, 4>(p, stream);
+  return launch_l4<EPI, OUT, 4, 4>(p, stream);
 }
 
 }  // namespace
@@ -309,6 +655,7 @@ DITK_EXPORT int ditk_mx_gemm(const void* A, int64_t lda, const void* As, int64_t
                      ((uintptr_t)Cs % 16) == 0,
                  "ditk_mx_gemm: MX output rows need their padding and 16-byte strides");
   }
+  DITK_REQUIRE(ldc < (1 << 22) && ldr < (1 << 22) && ldcs < (1 << 22), "ditk_mx_gemm: output row strides too large");
   DITK_REQUIRE(!res || ((R || M == 0) && ldr % 8 == 0 && ldr >= N && ((uintptr_t)R % 16) == 0),
                "ditk_mx_gemm: residual epilogue needs a 16-byte aligned R with ldr %% 8 == 0");
   DITK_REQUIRE(epilogue != MXE_GATE_RES || (gate && cu_seqlens && nseg > 0 && gate_stride % 4 == 0 &&
@@ -317,7 +664,7 @@ DITK_EXPORT int ditk_mx_gemm(const void* A, int64_t lda, const void* As, int64_t
   if (M == 0) return 0;
   const MxGemmArgs p{(const uint8_t*)A, lda, (const uint8_t*)As, ldas, (const uint8_t*)W, ldw, (const uint8_t*)Ws, ldws,
                      bias, C, ldc, (uint8_t*)Cs, ldcs, (const bf16_t*)R, ldr, gate, gate_stride, cu_seqlens, nseg,
-                     M, N, K, 0, 0, 0};
+                     M, N, K, 0, 0, 0, (int64_t)M * N * (out_kind == MXO_FP8 ? 1 : 2) >= kStreamBytes};
   const bool mx = out_kind == MXO_FP8;
   switch (epilogue) {
     case MXE_BIAS: return mx ? launch_tile<MXE_BIAS, MXO_FP8>(p, stream) : launch_tile<MXE_BIAS, MXO_BF16>(p, stream);
