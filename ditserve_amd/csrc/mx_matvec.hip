@@ -2,15 +2,26 @@
 //
 //   C[m, n] = epilogue( sum_k x[m, k] v[n, k] 2^e[n, k / 32]  + bias[n] )
 //
-// Bound by streaming the weight once, 4.25 bits a value.  A wave takes
-// 16 features at a time: lane (ql = lane % 16, g = lane / 16) loads the 16 bytes of block 4 c + g
-// of weight row ql -- 32 weights under one scale -- which the convert instructions turn
-// into bf16, exactly (an e2m1 value times a power of two), for four MFMAs of 16 features x
-// 16 tokens x 32 k.  The MFMAs' k order is a permutation of the row's (MFMA t takes k 32 g
-// + 8 t .. + 7 of each lane group), the same for both operands.
+// Bound by streaming the weight once, 4.25 bits a value.  A wave takes 16 features at a
+// time: lane (ql = lane % 16, g = lane / 16) loads the 16 bytes of block 4 c + g of weight row
+// ql -- 32 weights under one scale -- which the convert instructions turn into bf16,
+// exactly (an e2m1 value times a power of two), for four MFMAs of 16 features x 16 tokens x 32
+// k.  The MFMAs' k order is a permutation of the row's (MFMA u takes k 32 g + 8 u .. + 7 of each
+// lane group), the same for both operands.
 //
-// The four waves of a workgroup share its features and split K; they join in LDS in a
-// fixed order, which depends on K alone: a row's result does not depend on M.
+// A workgroup keeps its rows of x in LDS and goes through many groups of 16 features.  Its
+// waves split K in chunks of 512 (a lane's four scales of a chunk are one dword) and join in LDS
+// in wave order.  The split depends on K alone: a row's result does not depend on M.
+//
+// What bounds it: 2 x 1536 x 499712 (408 MB) 85 us, 4.8 TB/s, which is what a copy reaches here.  One
+// short matrix takes the launch's 2.6 us, a memory latency for x and the first weights, and its
+// own bytes: 1 x 1536 x 9216 4.7 us, 1 x 5120 x 5120 8.7, 1 x 8960 x 1536 7.1.  There the way of the code
+// into the instruction cache counts too: with x in registers (its operands exchanged
+// between lanes) and four chunks ahead, all unrolled, the large one took 85 us as well but the
+// small one 7.9.
+#include <algorithm>
+#include <type_traits>
+
 #include "mx_common.h"
 
 namespace {
@@ -31,84 +42,191 @@ __device__ __forceinline__ float e8m0_to_f32(uint32_t byte) {
   return byte == 255 ? __uint_as_float(0x7fc00000u) : __uint_as_float(byte << 23);
 }
 
+constexpr int kMaxWaves = 16;
+constexpr int kLds = 160 * 1024;
+constexpr int D = 2;      // chunks of weights a wave has in registers or on their way (3: 0-3% slower, 4: 3-8%)
+// Waves a CU is given where there are groups for them: 12 take 5-45% longer on the large matrices, 20 0-7%,
+// 24 15-24%.
+constexpr int kWavesPerCu = 16;
+
+// A row of x in LDS: whole 128-k steps, 16 units of 16 bytes each, unit 4 u + g of a step holding k
+// 32 g + 8 u .. + 7 (the operand of MFMA u and lane group g), XOR-swizzled by (row / 2) % 8, and
+// 128 bytes more: the units that the lanes of an operand read together lie in different banks
+// (as gemm.hip's operand rows).
+__host__ __device__ inline int x_stride(int K) { return (int)mx_cols(K) * 2 + 128; }
+
+// FJ x 16 tokens, of which a workgroup has x_rows
 template <int EPI, int FJ>
-__global__ __launch_bounds__(256) void mx_matvec_kernel(const bf16_t* __restrict__ x, int64_t ldx,
-                                                        const uint8_t* __restrict__ W, int64_t ldw,
-                                                        const uint8_t* __restrict__ Ws, int64_t ldws,
-                                                        const float* __restrict__ bias, void* Cv, int64_t ldc, int M,
-                                                        int N, int K, const bf16_t* R, int64_t ldr) {
-  __shared__ f32x4_t part[3][FJ][64];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, ql = lane & 15, g = lane >> 4;
-  const int n0 = blockIdx.x * 16, m0 = blockIdx.y * (16 * FJ);
-  const int blocks = K / 32, steps = (blocks + 3) / 4;  // 128-k steps
-  const int row = min(n0 + ql, N - 1);
-  const uint8_t* wp = W + (int64_t)row * ldw + g * 16;
-  const uint8_t* sp = Ws + (int64_t)row * ldws + g * 4;
-  const bf16_t* xp[FJ];
-#pragma unroll
-  for (int j = 0; j < FJ; ++j) xp[j] = x + (int64_t)min(m0 + j * 16 + ql, M - 1) * ldx + g * 32;
-  f32x4_t acc[FJ];
-#pragma unroll
-  for (int j = 0; j < FJ; ++j) acc[j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-  for (int c = wave; c < steps; c += 4) {
-    const u32x4_t w = *reinterpret_cast<const u32x4_t*>(wp + (int64_t)c * 64);
-    const float s = e8m0_to_f32(sp[(c >> 2) * 16 + (c & 3)]);
-    const bool on = c * 4 + g < blocks;  // else padding: zeros, past the end of x
-#pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      const bf16x8_t wf = fp4_to_bf16(w[t], s);
-#pragma unroll
-      for (int j = 0; j < FJ; ++j) {
-        const u32x4_t xr = on ? *reinterpret_cast<const u32x4_t*>(xp[j] + (int64_t)c * 128 + t * 8) : u32x4_t{0, 0, 0, 0};
-        acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wf, __builtin_bit_cast(bf16x8_t, xr), acc[j], 0, 0, 0);
-      }
+__global__ __launch_bounds__(64 * kMaxWaves) void mx_matvec_kernel(const bf16_t* __restrict__ x, int64_t ldx,
+                                                                   const uint8_t* __restrict__ W, int64_t ldw,
+                                                                   const uint8_t* __restrict__ Ws, int64_t ldws,
+                                                                   const float* __restrict__ bias, void* Cv,
+                                                                   int64_t ldc, int M, int N, int K, const bf16_t* R,
+                                                                   int64_t ldr, int x_rows) {
+  extern __shared__ u32x4_t lds[];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
+  const int ql = lane & 15, g = lane >> 4;
+  auto part = reinterpret_cast<f32x4_t(*)[FJ][64]>(lds);  // [2 waves]: the partial sums of two groups in turn
+  char* const xs = reinterpret_cast<char*>(lds + 2 * waves * FJ * 64);
+  const int m0 = blockIdx.y * x_rows, rows = min(x_rows, M - m0), groups = (N + 15) / 16, stride = x_stride(K);
+  const int blocks = K / 32, steps = (blocks + 3) / 4, chunks = (steps + 3) / 4;  // of 32, 128 and 512 k
+  const int each = (chunks + waves - 1) / waves;  // a wave's chunks: wave, wave + waves, ...
+  // this thread's output of a group: token ql of 16 ej, features n .. n + 3
+  const int ej = threadIdx.x >> 6, m = m0 + ej * 16 + ql;
+  const bool has_row = ej < FJ && ej * 16 + ql < rows;
+  u32x4_t w[D][4];
+  uint32_t s[D];
+  f32x4_t b4[D], bcur;
+  u32x2_t r2[D], rcur;
+  // A chunk's weights (past the row's end its last 128 once more) and, with a group's first, its bias
+  // and residual: loads return in order, and asked for later they would wait for the next weights.
+  auto load = [&](int set, int group, int i) {
+    if (i == 0) {
+      const int n = group * 16 + 4 * g;
+      const bool mine = has_row && n < N;
+      b4[set] = mine && bias != nullptr ? *reinterpret_cast<const f32x4_t*>(bias + n) : f32x4_t{0.f, 0.f, 0.f, 0.f};
+      if (EPI == MV_RES)
+        r2[set] = mine ? *reinterpret_cast<const u32x2_t*>(R + (int64_t)m * ldr + n) : u32x2_t{0, 0};
     }
-  }
-  if (wave > 0) {
+    const int row = min(group * 16 + ql, N - 1), chunk = min(wave + i * waves, chunks - 1);
+    s[set] = *reinterpret_cast<const uint32_t*>(Ws + (int64_t)row * ldws + chunk * 16 + g * 4);
+    const uint8_t* wp = W + (int64_t)row * ldw + g * 16;
 #pragma unroll
-    for (int j = 0; j < FJ; ++j) part[wave - 1][j][lane] = acc[j];
-  }
-  __syncthreads();
-  if (wave > 0) return;
-  // this lane: token ql of each 16, features n .. n + 3
-  const int n = n0 + 4 * g;
-  if (n >= N) return;
-  const f32x4_t b4 = bias != nullptr ? *reinterpret_cast<const f32x4_t*>(bias + n) : f32x4_t{0.f, 0.f, 0.f, 0.f};
+    for (int t = 0; t < 4; ++t)
+      w[set][t] = __builtin_nontemporal_load(reinterpret_cast<const u32x4_t*>(wp + min(chunk * 4 + t, steps - 1) * 64));
+  };
+  f32x4_t acc[FJ];
+  const char* xl[FJ];
+  int swz[FJ];
 #pragma unroll
   for (int j = 0; j < FJ; ++j) {
-    const int m = m0 + j * 16 + ql;
-    if (m >= M) continue;
-    f32x4_t y = ((acc[j] + part[0][j][lane]) + (part[1][j][lane] + part[2][j][lane])) + b4;
+    const int r = min(j * 16 + ql, rows - 1);
+    xl[j] = xs + r * stride;
+    swz[j] = (r >> 1) & 7;
+  }
+  auto use = [&](int set, int chunk) {
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      const int c = chunk * 4 + t;
+      if (c >= steps) break;  // the same for the wave
+      const float scale = e8m0_to_f32((s[set] >> (8 * t)) & 255);
+#pragma unroll
+      for (int u = 0; u < 4; ++u) {
+        const bf16x8_t wf = fp4_to_bf16(w[set][t][u], scale);
+#pragma unroll
+        for (int j = 0; j < FJ; ++j)
+          acc[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
+              wf, *reinterpret_cast<const bf16x8_t*>(xl[j] + c * 256 + (((u * 4 + g) ^ swz[j]) * 16)), acc[j], 0, 0, 0);
+      }
+    }
+  };
+  // the waves' sums of a group, joined, and the epilogue
+  auto join = [&](int group, int buf) {
+    const int n = group * 16 + 4 * g;
+#pragma unroll
+    for (int j = 0; j < FJ; ++j) part[buf * waves + wave][j][lane] = acc[j];
+    // LDS only: the next weights stay on their way
+    asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    if (!has_row || n >= N) return;
+    f32x4_t y = part[buf * waves][ej][lane];
+    for (int v = 1; v < waves; ++v) y += part[buf * waves + v][ej][lane];
+    y += bcur;
     if (EPI == MV_F32) {
       *reinterpret_cast<f32x4_t*>(reinterpret_cast<float*>(Cv) + (int64_t)m * ldc + n) = y;
-      continue;
+      return;
     }
     if (EPI == MV_GELU) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) y[e] = gelu_tanh_f(y[e]);
+      for (int k = 0; k < 4; ++k) y[k] = gelu_tanh_f(y[k]);
     } else if (EPI == MV_SILU) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) y[e] = silu_f(y[e]);
+      for (int k = 0; k < 4; ++k) y[k] = silu_f(y[k]);
     } else if (EPI == MV_RES) {
-      const u32x2_t r = *reinterpret_cast<const u32x2_t*>(R + (int64_t)m * ldr + n);
-      y[0] += __uint_as_float(r[0] << 16);
-      y[1] += __uint_as_float(r[0] & 0xffff0000u);
-      y[2] += __uint_as_float(r[1] << 16);
-      y[3] += __uint_as_float(r[1] & 0xffff0000u);
+      y[0] += __uint_as_float(rcur[0] << 16);
+      y[1] += __uint_as_float(rcur[0] & 0xffff0000u);
+      y[2] += __uint_as_float(rcur[1] << 16);
+      y[3] += __uint_as_float(rcur[1] & 0xffff0000u);
     }
     *reinterpret_cast<u32x2_t*>(reinterpret_cast<bf16_t*>(Cv) + (int64_t)m * ldc + n) =
         u32x2_t{pack_bf2(y[0], y[1]), pack_bf2(y[2], y[3])};
+  };
+
+  int group = blockIdx.x, i = 0, buf = 0;
+  int lgroup = group, li = 0;  // the next chunk to ask for
+  auto load_next = [&](int set) {
+    if (lgroup >= groups) return;
+    load(set, lgroup, li);
+    if (++li == each) {
+      li = 0;
+      lgroup += gridDim.x;
+    }
+  };
+#pragma unroll
+  for (int d = 0; d < D - 1; ++d) load_next(d);
+  // x: 512 k of a row per DMA instruction; past K zeros, under which weights count for nothing
+  // (in a loop of their own: between the DMAs the compiler would wait for each)
+  auto x_unit = [&](int p, bool tail) {
+    const int r = p / chunks, c = p % chunks, v = lane ^ ((r >> 1) & 7);  // this lane's unit of the four steps
+    const int k = c * 512 + (v >> 4) * 128 + (v & 3) * 32 + ((v >> 2) & 3) * 8;
+    char* dst = xs + r * stride + c * 1024;
+    if (!tail && k < K)
+      __builtin_amdgcn_global_load_lds(
+          (const __attribute__((address_space(1))) void*)(x + (int64_t)(m0 + r) * ldx + k),
+          (__attribute__((address_space(3))) void*)dst, 16, 0, 0);
+    if (tail && k >= K && c * 4 + (lane >> 4) < steps) *reinterpret_cast<u32x4_t*>(dst + lane * 16) = u32x4_t{0, 0, 0, 0};
+  };
+  for (int p = wave; p < rows * chunks; p += waves) x_unit(p, false);
+  if (K % 128 != 0)
+    for (int p = wave; p < rows * chunks; p += waves) x_unit(p, true);
+  asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+  __syncthreads();
+#pragma unroll
+  for (int j = 0; j < FJ; ++j) acc[j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  // one chunk from `set`; false behind the last
+  auto step = [&](int set) {
+    load_next((set + D - 1) % D);
+    if (i == 0) {
+      bcur = b4[set];
+      rcur = r2[set];
+    }
+    if (wave + i * waves < chunks) use(set, wave + i * waves);
+    if (++i == each) {
+      join(group, buf);
+      buf ^= 1;
+#pragma unroll
+      for (int j = 0; j < FJ; ++j) acc[j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+      i = 0;
+      group += gridDim.x;
+    }
+    return group < groups;
+  };
+  for (;;) {
+    bool more = true;
+#pragma unroll
+    for (int d = 0; d < D; ++d)
+      if (more) more = step(d);
+    if (!more) break;
   }
 }
 
 template <int EPI>
 int launch(const void* x, int64_t ldx, const void* W, int64_t ldw, const void* Ws, int64_t ldws, const float* bias,
            void* C, int64_t ldc, int M, int N, int K, const void* R, int64_t ldr, hipStream_t stream) {
-  const int fj = M <= 16 ? 1 : M <= 32 ? 2 : 4;
-  const dim3 grid((unsigned)((N + 15) / 16), (unsigned)((M + 16 * fj - 1) / (16 * fj)));
-  auto kern = fj == 1 ? mx_matvec_kernel<EPI, 1> : fj == 2 ? mx_matvec_kernel<EPI, 2> : mx_matvec_kernel<EPI, 4>;
-  kern<<<grid, 256, 0, stream>>>((const bf16_t*)x, ldx, (const uint8_t*)W, ldw, (const uint8_t*)Ws, ldws, bias, C, ldc,
-                                 M, N, K, (const bf16_t*)R, ldr);
+  // waves: a chunk of 512 k each up to kMaxWaves, beyond that as even a share as there is
+  const int chunks = (K + 511) / 512, each = (chunks + kMaxWaves - 1) / kMaxWaves, waves = (chunks + each - 1) / each;
+  // the rows of x that fit in LDS, up to 16 (or 32); more rows in as many even passes over the weight
+  auto fit = [&](int fj) { return std::min(16 * fj, (kLds - 2 * waves * fj * 1024) / x_stride(K)); };
+  DITK_REQUIRE(fit(1) > 0, "ditk_mx_matvec: K=%d too long", K);
+  const int fj = waves > 1 && fit(2) > 0 && (M + fit(2) - 1) / fit(2) < (M + fit(1) - 1) / fit(1) ? 2 : 1;
+  const int passes = (M + fit(fj) - 1) / fit(fj), x_rows = (M + passes - 1) / passes;
+  DITK_REQUIRE(passes <= 65535, "ditk_mx_matvec: too many rows");
+  const int groups = (N + 15) / 16, lds = 2 * waves * fj * 1024 + x_rows * x_stride(K);
+  const int per_cu = std::max(1, std::min(kWavesPerCu / waves, kLds / lds));
+  const dim3 grid((unsigned)std::min(groups, std::max(1, ditk_cu_count() * per_cu / passes)), (unsigned)passes);
+  auto kern = fj == 1 ? mx_matvec_kernel<EPI, 1> : mx_matvec_kernel<EPI, 2>;
+  kern<<<grid, 64 * waves, lds, stream>>>((const bf16_t*)x, ldx, (const uint8_t*)W, ldw, (const uint8_t*)Ws, ldws, bias,
+                                          C, ldc, M, N, K, (const bf16_t*)R, ldr, x_rows);
   return ditk_check_launch("ditk_mx_matvec");
 }
 
@@ -120,7 +238,6 @@ DITK_EXPORT int ditk_mx_matvec(const void* x, int64_t ldx, const void* W, int64_
   DITK_REQUIRE(W && Ws && (M == 0 || (x && C)), "ditk_mx_matvec: null operand");
   DITK_REQUIRE(M >= 0 && N > 0 && K > 0, "ditk_mx_matvec: bad shape M=%d N=%d K=%d", M, N, K);
   DITK_REQUIRE(K % 32 == 0 && N % 8 == 0, "ditk_mx_matvec: K=%d must be a multiple of 32, N=%d of 8", K, N);
-  DITK_REQUIRE(M <= 65535 * 64, "ditk_mx_matvec: too many rows");
   DITK_REQUIRE(ldx % 8 == 0 && ldx >= K && ldw % 16 == 0 && ldw >= mx_cols(K) / 2 && ldws % 16 == 0 &&
                    ldws >= mx_scale_bytes(K),
                "ditk_mx_matvec: operand rows need their padding and 16-byte strides");
