@@ -10,7 +10,7 @@ sets, the token fragments four buffers that a stage's FJ columns take in turn.
 
   AGPR a[4 (i FJ + j)..]    acc[i][j]: features 16 i + 4 (lane / 16) + e, token 16 j + lane % 16
   VGPR W[p][i]              W fragments, set p = stage % 2
-  VGPR X[b]                 token fragments, column j in b = j % 4
+  VGPR X[b]                 token fragments, column j in b = j % NX
   VGPR S[q][..]             scales of 4 stages (a byte each), set q = (stage / 4) % 2
   VGPR 4 addresses          this stage's fragment reads
   SGPR s40..s63             loop state
@@ -36,8 +36,7 @@ import sys
 
 # the generated wave tiles: (feature fragments, token fragments, stage buffers, slot of the
 # barrier, slot of W's barrier if it has one of its own)
-VARIANTS = [(8, 8, 2, 40, 8), (8, 4, 3, 8, None), (4, 4, 4, 7, None)]
-NX = 4                   # token fragment buffers
+VARIANTS = [(8, 8, 2, 40, 8), (8, 4, 3, 8, None), (4, 4, 4, 7, None), (4, 2, 4, 4, None)]
 
 
 def name_of(fi, fj):
@@ -45,18 +44,20 @@ def name_of(fi, fj):
 
 
 def configure(fi, fj, nbuf, bar, wbar):
-    global FI, FJ, NBUF, BAR, WBAR, WOFF, BUF, ROWS, ND, WB, XB, SB, AB, LAST_VGPR
+    global FI, FJ, NBUF, BAR, WBAR, NX, WOFF, BUF, ROWS, ND, WB, XB, SB, AB, LAST_VGPR
     FI, FJ, NBUF, BAR, WBAR = fi, fj, nbuf, bar, wbar
     WOFF = 32 * fj * 128
     ROWS = 32 * (fi + fj)
     BUF = ROWS * 128
     ND = fi + fj
+    NX = min(4, fj)                       # token fragment buffers
     WB = 0
     XB = WB + 2 * fi * 8
     SB = XB + NX * 8
     AB = SB + 2 * (fi + fj)      # addresses: x chunk 0, 1, w chunk 0, 1, x and w scales
     LAST_VGPR = AB + 5
-    assert fj % NX == 0 and nbuf * BUF + 2 * ROWS * 16 <= 160 * 1024
+    # (NBUF <= 4: the scales have two buffers)
+    assert fj % NX == 0 and nbuf <= 4 and nbuf * BUF + 2 * ROWS * 16 <= 160 * 1024
 
 
 # loop state
