@@ -47,6 +47,7 @@ struct MxGemmArgs {
   int64_t gate_stride;
   const int32_t* cu;
   int nseg, M, N, K;
+  int m_begin;  // this launch's rows: m_begin .. M - 1
   int tiles_m, tiles_n, group_m;
   bool stream;  // output stored past the caches
 };
@@ -268,7 +269,7 @@ __device__ __forceinline__ void mx_out_padding(const MxGemmArgs& p) {
   const int cols = ((int)mx_cols(p.N) - p.N) / 16, b0 = p.N / 32, sc = (int)mx_scale_bytes(p.N) - b0;
   const int i = threadIdx.x & 31, per = blockDim.x / 32;  // 32 threads a row: at most 6 + 15 stores
   if (cols + sc == 0) return;
-  for (int row = blockIdx.x * per + threadIdx.x / 32; row < p.M; row += gridDim.x * per) {
+  for (int row = p.m_begin + blockIdx.x * per + threadIdx.x / 32; row < p.M; row += gridDim.x * per) {
     if (i < cols)
       *reinterpret_cast<u32x4_t*>(reinterpret_cast<uint8_t*>(p.C) + (int64_t)row * p.ldc + p.N + i * 16) = u32x4_t{0, 0, 0, 0};
     if (i >= 16 && i < 16 + sc) p.Cs[(int64_t)row * p.ldcs + mx_scale_at(b0 + i - 16)] = 127;
@@ -477,7 +478,7 @@ __global__ __launch_bounds__(256, 1) void mx_gemm_l4(MxGemmArgs p) {
     const int group = L / (p.group_m * p.tiles_n), first_m = group * p.group_m;
     const int gm = min(p.group_m, p.tiles_m - first_m), pid = L % (p.group_m * p.tiles_n);
     MxTile t;
-    t.m0 = (first_m + pid % gm) * GBM;
+    t.m0 = p.m_begin + (first_m + pid % gm) * GBM;
     t.n0 = pid / gm * GBN;
     t.mb = min(t.m0, max(0, p.M - GBM));
     t.nb = min(t.n0, max(0, p.N - GBN));
@@ -592,9 +593,10 @@ __global__ __launch_bounds__(256, 1) void mx_gemm_l4(MxGemmArgs p) {
 // next kernel reads it, as gemm.hip's.
 constexpr int64_t kStreamBytes = 64ll << 20;
 
-// Tile order: groups of m-tiles walked m-fastest, so the tiles running together share
-// operand rows in their XCD's L2.
-int mx_group_m(int K, int tiles_n) { return K >= 8192 ? 2 : (tiles_n >= 24 ? 4 : 8); }
+// Tile order: groups of m-tiles walked m-fastest, so that the tiles running together share
+// operand rows in their XCD's L2.  Groups of 2 to 16 are within 3% of each other, 1 loses up to 12%
+// where many n-tiles make a round (65520 x 8960 x 1536) and 32 10-48%.
+int mx_group_m(int K, int tiles_n) { return K >= 4096 || tiles_n >= 24 ? 4 : 8; }
 
 template <int EPI, int OUT, int FI, int FJ, int WM, int WN, int EU>
 int launch(MxGemmArgs p, hipStream_t stream) {
@@ -611,7 +613,7 @@ int launch(MxGemmArgs p, hipStream_t stream) {
 template <int EPI, int OUT, int FI, int FJ>
 int launch_l4(MxGemmArgs p, hipStream_t stream) {
   constexpr int GBM = MxL4<FI, FJ>::GBM, GBN = MxL4<FI, FJ>::GBN;
-  p.tiles_m = (p.M + GBM - 1) / GBM;
+  p.tiles_m = (p.M - p.m_begin + GBM - 1) / GBM;
   p.tiles_n = (p.N + GBN - 1) / GBN;
   p.group_m = mx_group_m(p.K, p.tiles_n);
   const int64_t tiles = (int64_t)p.tiles_m * p.tiles_n;
@@ -622,16 +624,82 @@ int launch_l4(MxGemmArgs p, hipStream_t stream) {
   return ditk_check_launch("ditk_mx_gemm");
 }
 
+// The tiles of mx_gemm_l4 (tokens x features) and their measured time in us, start + rounds x (tile +
+// stage x K / 128) with a round one tile per CU: least squares over 100 products of 16 to 65520 rows with
+// seven weights of the Wan and SD3.5 blocks, operands from memory, 9-11% rms.  The tile it predicts
+// fastest is 0.15% slower than the fastest on average.  A stage of 256 x 256 is 1.07 us for
+// 64 MFMAs of 32 cycles, 0.85 us at 2.4 GHz; the smaller tiles' are bound by their LDS reads and the issue
+// of one wave (64 x 128: 0.36 us for 0.11 of MFMA) but let few rows use more CUs.
+struct MxCfg {
+  int gbm, gbn;
+  float start, tile, stage;
+};
+constexpr int kCfgs = 4;
+constexpr MxCfg kCfg[kCfgs] = {{256, 256, -2.4f, 10.1f, 1.067f}, {128, 256, 0.5f, 4.8f, 0.674f},
+                               {128, 128, 2.1f, 1.8f, 0.469f},   {64, 128, 2.5f, 0.55f, 0.358f}};
+
+float cfg_us(int c, int64_t tiles, int K, int cus) {
+  const int64_t rounds = (tiles + cus - 1) / cus;
+  return kCfg[c].start + (float)rounds * (kCfg[c].tile + kCfg[c].stage * (float)((K + 127) / 128));
+}
+
+// How a product runs: rows [0, rows) on tiles of configuration cfg, the others on `rest` in a second
+// launch, where the last round of tiles would leave most CUs idle and the estimate gains by
+// kSplitGain: 4096 x 5120 x 5120 120 -> 108 us (20% predicted), but 16384 x 1536 x 8960 188 -> 202 us (6%
+// predicted: over several rounds the workgroups drift apart).  Every row is computed the same
+// way whichever tile has it.
+struct MxPlan {
+  int cfg, rows, rest;
+  float us;
+};
+constexpr float kSplitGain = 0.9f;
+MxPlan plan_one(int M, int N, int K, int cus) {
+  MxPlan best{0, M, 0, 1e30f};
+  for (int c = 0; c < kCfgs; ++c) {
+    const int64_t tiles = (int64_t)((M + kCfg[c].gbm - 1) / kCfg[c].gbm) * ((N + kCfg[c].gbn - 1) / kCfg[c].gbn);
+    const float us = cfg_us(c, tiles, K, cus);
+    if (us < best.us) best = MxPlan{c, M, 0, us};
+  }
+  return best;
+}
+MxPlan mx_plan(int M, int N, int K) {
+  const int cus = std::max(8, ditk_cu_count() / 8 * 8);
+  const MxPlan one = plan_one(M, N, K, cus);
+  MxPlan best = one;
+  for (int c = 0; c < kCfgs; ++c) {
+    const int64_t tn = (N + kCfg[c].gbn - 1) / kCfg[c].gbn, tm = (M + kCfg[c].gbm - 1) / kCfg[c].gbm;
+    const int64_t main_m = tm * tn / cus * cus / tn;  // tile rows of the full rounds
+    if (main_m == 0 || main_m >= tm || tm * tn % cus == 0) continue;
+    const int rows = (int)main_m * kCfg[c].gbm;
+    const MxPlan rest = plan_one(M - rows, N, K, cus);
+    const float us = cfg_us(c, main_m * tn, K, cus) + rest.us;
+    if (us < best.us && us < kSplitGain * one.us) best = MxPlan{c, rows, rest.cfg, us};
+  }
+  return best;
+}
+
 template <int EPI, int OUT>
 int launch_tile(const MxGemmArgs& p, hipStream_t stream) {
-  // 32-bit row offsets within a tile
+  // the l4 kernel: its ring of stages within K, and 32-bit row offsets within a tile
   const int64_t ld = std::max(std::max(p.lda, p.ldw), std::max(p.ldas, p.ldws));
-  const bool l4 = p.K > 384 && 256 * ld < (1ll << 31);
-  const int64_t t256 = (int64_t)((p.M + 255) / 256) * ((p.N + 255) / 256);
-  if (!l4) return t256 >= 128 ? launch<EPI, OUT, 4, 8, 2, 4, 1>(p, stream) : launch<EPI, OUT, 4, 2, 2, 2, 2>(p, stream);
-  if (t256 >= 192) return launch_l4<EPI, OUT, 8, 8>(p, stream);
-  if ((int64_t)((p.M + 127) / 128) * ((p.N + 255) / 256) >= 128) return launch_l4<EPI, OUT, 8, 4>(p, stream);
-  return launch_l4<EPI, OUT, 4, 4>(p, stream);
+  if (p.K <= 384 || 256 * ld >= (1ll << 31)) {
+    if ((int64_t)((p.M + 255) / 256) * ((p.N + 255) / 256) >= 128) return launch<EPI, OUT, 4, 8, 2, 4, 1>(p, stream);
+    return launch<EPI, OUT, 4, 2, 2, 2, 2>(p, stream);
+  }
+  auto part = [&](int cfg, int begin, int end) {
+    MxGemmArgs q = p;
+    q.m_begin = begin;
+    q.M = end;
+    switch (cfg) {
+      case 0: return launch_l4<EPI, OUT, 8, 8>(q, stream);
+      case 1: return launch_l4<EPI, OUT, 8, 4>(q, stream);
+      case 2: return launch_l4<EPI, OUT, 4, 4>(q, stream);
+      default: return launch_l4<EPI, OUT, 4, 2>(q, stream);
+    }
+  };
+  const MxPlan plan = mx_plan(p.M, p.N, p.K);
+  const int rc = part(plan.cfg, 0, plan.rows);
+  return rc != 0 || plan.rows == p.M ? rc : part(plan.rest, plan.rows, p.M);
 }
 
 }  // namespace
@@ -673,7 +741,7 @@ DITK_EXPORT int ditk_mx_gemm(const void* A, int64_t lda, const void* As, int64_t
   if (M == 0) return 0;
   const MxGemmArgs p{(const uint8_t*)A, lda, (const uint8_t*)As, ldas, (const uint8_t*)W, ldw, (const uint8_t*)Ws, ldws,
                      bias, C, ldc, (uint8_t*)Cs, ldcs, (const bf16_t*)R, ldr, gate, gate_stride, cu_seqlens, nseg,
-                     M, N, K, 0, 0, 0, (int64_t)M * N * (out_kind == MXO_FP8 ? 1 : 2) >= kStreamBytes};
+                     M, N, K, 0, 0, 0, 0, (int64_t)M * N * (out_kind == MXO_FP8 ? 1 : 2) >= kStreamBytes};
   const bool mx = out_kind == MXO_FP8;
   switch (epilogue) {
     case MXE_BIAS: return mx ? launch_tile<MXE_BIAS, MXO_FP8>(p, stream) : launch_tile<MXE_BIAS, MXO_BF16>(p, stream);

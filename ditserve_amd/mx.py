@@ -118,14 +118,16 @@ class MXTensor:
 
 def _call(device, name, *args):
     """Launch on the current stream of `device`, which need not be the current device."""
-    if device.index == torch.cuda.current_device():
-        return _lib.call(name, *args, ops._stream())
-    with torch.cuda.device(device):
-        return _lib.call(name, *args, ops._stream())
+    index = device.index
+    if index == torch._C._cuda_getDevice():
+        return _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(index))
+    with torch.cuda.device(index):
+        return _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(index))
 
 
-def _one_device(device, **tensors):
-    for name, t in tensors.items():
+def _one_device(device, *tensors):
+    """Refuse operands on another device (pairs of a name and a tensor or None)."""
+    for name, t in tensors:
         if t is not None and t.device != device:
             raise ValueError(f"{name} is on {t.device}, the other operands on {device}")
 
@@ -143,7 +145,7 @@ def _mx_out(out, rows, cols, device, fmt):
     _mx_check(out, "out", fmt)
     if out.shape != (rows, cols):
         raise ValueError(f"out must be [{rows}, {cols}], got {out.shape}")
-    _one_device(device, out=out)
+    _one_device(device, ("out", out))
     return out
 
 
@@ -198,8 +200,9 @@ def norm(x, residual=None, shift=None, scale=None, segments=None, weight=None, b
         raise ValueError(f"x needs blocks of 32 columns, got {D}")
     if kind not in ("ln", "rms"):
         raise ValueError(f"kind must be 'ln' or 'rms', got {kind!r}")
-    _one_device(x.device, residual=residual, shift=shift, scale=scale, weight=weight, bias=bias,
-                residual_out=residual_out, segments=None if segments is None else segments.dev)
+    device = x.device
+    _one_device(device, ("residual", residual), ("shift", shift), ("scale", scale), ("weight", weight), ("bias", bias),
+                ("residual_out", residual_out), ("segments", None if segments is None else segments.dev))
     h, ldr, ldh = None, 0, 0
     if residual is not None:
         _check(residual, "residual", _BF16, 2)
@@ -207,7 +210,7 @@ def norm(x, residual=None, shift=None, scale=None, segments=None, weight=None, b
             raise ValueError(f"residual must be [{T}, {D}], got {tuple(residual.shape)}")
         ldr = _rows(residual, "residual")
         if residual_out is None:
-            h = torch.empty((T, D), dtype=_BF16, device=x.device)
+            h = torch.empty((T, D), dtype=_BF16, device=device)
         else:
             h = residual_out
             _check(h, "residual_out", _BF16, 2)
@@ -234,11 +237,11 @@ def norm(x, residual=None, shift=None, scale=None, segments=None, weight=None, b
     for t, n in ((weight, "weight"), (bias, "bias")):
         if t is not None:
             _vec(t, n, D)
-    y = _mx_out(out, T, D, x.device, "fp8")
+    y = _mx_out(out, T, D, device, "fp8")
     if out is not None or residual_out is not None:
         outs = ([] if out is None else [y.data, y.scales]) + ([] if residual_out is None else [h])
         _apart("norm", outs, (shift, scale, weight, bias), same=(x, residual))
-    _call(x.device, "ditk_mx_norm", _ptr(x), ldx, _ptr(residual), ldr, _ptr(h), ldh, *y._args(), T, D, _ptr(cu), nseg,
+    _call(device, "ditk_mx_norm", _ptr(x), ldx, _ptr(residual), ldr, _ptr(h), ldh, *y._args(), T, D, _ptr(cu), nseg,
           _ptr(shift), _ptr(scale), mod_stride, _ptr(weight), _ptr(bias), float(eps), 0 if kind == "ln" else 1)
     return y if residual is None else (y, h)
 
@@ -288,10 +291,12 @@ def linear(x, w, b=None, epilogue="bias", residual=None, gate=None, segments=Non
         raise ValueError(f"an MX output needs N % 32 == 0 (got N={N})")
     if b is not None:
         _vec(b, "bias", N)
-    _one_device(x.device, w=w, bias=b, residual=residual if res else None, gate=gate if res else None,
-                out=out, segments=None if segments is None else segments.dev)
-    ldr = _residual(residual, M, N) if res else 0
-    gate_stride, cu, nseg = 0, None, 0
+    device = x.device
+    _one_device(device, ("w", w), ("bias", b), ("out", out))
+    ldr, gate_stride, cu, nseg = 0, 0, None, 0
+    if res:
+        ldr = _residual(residual, M, N)
+        _one_device(device, ("residual", residual))
     if epilogue == "gate_res":
         _check(gate, "gate", torch.float32, 2)
         if segments is None or segments.total != M:
@@ -300,17 +305,18 @@ def linear(x, w, b=None, epilogue="bias", residual=None, gate=None, segments=Non
         gate_stride, unit = gate.stride()
         if gate.shape != (nseg, N) or unit != 1 or gate_stride % 4 or gate.data_ptr() % 16:
             raise ValueError(f"gate must be [{nseg}, {N}] with unit column stride and 16-byte aligned rows")
+        _one_device(device, ("gate", gate), ("segments", cu))
     given = out
     if out_fmt:
-        out = _mx_out(out, M, N, x.device, "fp8")
+        out = _mx_out(out, M, N, device, "fp8")
         c, outs = out._args(), (out.data, out.scales)
     else:
-        out = _bf16_out(out, M, N, _BF16, x.device)
+        out = _bf16_out(out, M, N, _BF16, device)
         c, outs = (_ptr(out), out.stride(0), None, 0), (out,)
     if given is not None:
         _apart("linear", outs, (x.data, x.scales, w.data, w.scales, b, gate if res else None),
                same=(residual,) if res else ())
-    _call(x.device, "ditk_mx_gemm", *x._args(), *w._args(), _ptr(b), *c, M, N, K, EPILOGUES[epilogue],
+    _call(device, "ditk_mx_gemm", *x._args(), *w._args(), _ptr(b), *c, M, N, K, EPILOGUES[epilogue],
           1 if out_fmt else 0, _ptr(residual) if res else None, ldr, _ptr(gate) if cu is not None else None,
           gate_stride, _ptr(cu), nseg)
     return out
@@ -345,12 +351,13 @@ def matvec(x, w, b=None, epilogue="bias", residual=None, out=None):
     if b is not None:
         _vec(b, "bias", N)
     res = epilogue == "res"
-    _one_device(x.device, w=w, bias=b, residual=residual if res else None, out=out)
+    device = x.device
+    _one_device(device, ("w", w), ("bias", b), ("residual", residual if res else None), ("out", out))
     ldr = _residual(residual, M, N) if res else 0
     given = out
-    out = _bf16_out(out, M, N, torch.float32 if epilogue == "f32" else _BF16, x.device)
+    out = _bf16_out(out, M, N, torch.float32 if epilogue == "f32" else _BF16, device)
     if given is not None:
         _apart("matvec", (out,), (x, w.data, w.scales, b), same=(residual,) if res else ())
-    _call(x.device, "ditk_mx_matvec", _ptr(x), ldx, *w._args(), _ptr(b), _ptr(out), out.stride(0), M, N, K,
+    _call(device, "ditk_mx_matvec", _ptr(x), ldx, *w._args(), _ptr(b), _ptr(out), out.stride(0), M, N, K,
           EPILOGUES[epilogue], _ptr(residual) if res else None, ldr)
     return out[0] if one else out
