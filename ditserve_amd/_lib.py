@@ -80,6 +80,7 @@ SIGNATURES = {
                              _P, _P, c_int64, _P, _P, c_float, c_int, _P]),
     "ditk_mx_gemm": (c_int, [_P, c_int64, _P, c_int64, _P, c_int64, _P, c_int64, _P, _P, c_int64, _P, c_int64, c_int,
                              c_int, c_int, c_int, c_int, _P, c_int64, _P, c_int64, _P, c_int, _P]),
+    "ditk_mx_gemm_plan": (c_int, [c_int, c_int, c_int, ctypes.POINTER(c_int)]),
     "ditk_mx_matvec": (c_int, [_P, c_int64, _P, c_int64, _P, c_int64, _P, _P, c_int64, c_int, c_int, c_int, c_int, _P,
                                c_int64, _P]),
     "ditk_flash_attn_varlen_noalloc": (c_int, [_P, c_int64, _P, c_int64, _P, c_int64, _P, c_int64, _P, c_int64,

@@ -397,6 +397,140 @@ def test_linear_large_tiles_against_64_bits():
     assert (got - want).norm() <= 2.0 ** -8 / math.sqrt(3) * want.norm()
 
 
+def mx_plan(m, n, k):
+    import ctypes
+    p = (ctypes.c_int * 3)()
+    _lib.call("ditk_mx_gemm_plan", m, n, k, p)
+    return tuple(p)
+
+
+def on_gpu(m):
+    return values(m).to(DEV)
+
+
+# every tile with rows and features that end inside it, one and several tiles a workgroup, K a multiple
+# of its steps of 128, of 512 and of neither, and launches split in two
+@pytest.mark.parametrize("shape,want", [
+    ((100, 1544, 416), (3, 100, 0)), ((63, 9992, 512), (3, 63, 0)), ((1000, 4616, 1056), None),
+    ((520, 4616, 448), (2, 520, 0)), ((333, 8968, 1536), (2, 333, 0)), ((667, 7304, 2432), (1, 667, 0)),
+    ((2600, 4104, 640), None), ((2600, 8968, 512), None), ((4353, 4104, 1568), (0, 3840, 2)),
+    ((4600, 5128, 416), (0, 3072, 1)), ((9000, 2440, 3104), None), ((129, 24, 8960), None), ((300, 40, 14336), None)])
+@pytest.mark.parametrize("epi", ["gate_res", "gelu"])
+def test_linear_tiles(shape, want, epi):
+    M, N, K = shape
+    assert want is None or mx_plan(*shape) == want
+    x, w = mx_random(M, K, M + K), mx_random(N, K, N + K + 1)
+    w.scales.view(torch.uint8).sub_(4)
+    g = gen(M)
+    b = torch.randn(N, generator=g).to(DEV)
+    y, mag = torch.mm(on_gpu(x), on_gpu(w).T) + b.double(), torch.mm(on_gpu(x).abs(), on_gpu(w).abs().T)
+    buf = torch.full((M + 2, N + 24), 7.0, dtype=torch.bfloat16, device=DEV)
+    out = buf[:M, 8:8 + N]
+    if epi == "gate_res":
+        cu = [0, 1, 1, M // 3, M]  # (a segment may end inside a tile)
+        res = torch.randn((M, N), generator=g).to(DEV, torch.bfloat16)
+        gt = torch.randn((4, N), generator=g).to(DEV)
+        mx.linear(x, w, b, epilogue=epi, residual=res, gate=gt, segments=ops.Segments(cu, DEV), out=out)
+        rows = torch.tensor([0] + [2] * (M // 3 - 1) + [3] * (M - M // 3), device=DEV)
+        slope, want64 = gt.double()[rows].abs(), res.double() + y * gt.double()[rows]
+    else:
+        mx.linear(x, w, b, epilogue=epi, out=out)
+        slope, want64 = 1.13, act64(y, epi)
+    # acc_error with the groups' largest products taken as the sum of all
+    acc = (7 * 2.0 ** -13 + (K + 127) // 128 * 17 * 2.0 ** -23) * mag
+    err = (out.double() - want64).abs()
+    assert (err <= BF16_HALF * want64.abs() + slope * (acc + 2.0 ** -20 * y.abs()) + 1e-30).all()
+    # in norm, where errors do not add up: the roundings, and 2^-13 of each product at random
+    norm = (out.double() - want64).norm()
+    assert norm <= BF16_HALF / math.sqrt(3) * want64.norm() + 2.0 ** -13 * 1.13 * (slope * y).norm()
+    assert (buf[M:] == 7).all() and (buf[:, :8] == 7).all() and (buf[:, 8 + N:] == 7).all()
+
+
+@pytest.mark.parametrize("M,N,K", [(1560, 8960, 512), (333, 4640, 1536), (700, 7328, 1056), (100, 1568, 416),
+                                   (4600, 5152, 448)])
+def test_linear_tiles_mx_output(M, N, K):
+    """The MX output of every tile is that of the same product in fp32 -> quantised: compared with 64 bits."""
+    x, w = mx_random(M, K, M + K), mx_random(N, K, N + K + 1)
+    w.scales.view(torch.uint8).sub_(4)
+    b = torch.randn(N, generator=gen(M)).to(DEV)
+    whole, out = poisoned(M, N)
+    mx.linear(x, w, b, epilogue="silu", out_fmt="fp8", out=out)
+    y, mag = torch.mm(on_gpu(x), on_gpu(w).T) + b.double(), torch.mm(on_gpu(x).abs(), on_gpu(w).abs().T)
+    want = act64(y, "silu")
+    s = decode(out)[1][:, :N // 32].to(DEV)
+    off = 1.13 * ((7 * 2.0 ** -13 + (K + 127) // 128 * 17 * 2.0 ** -23) * mag + 2.0 ** -20 * y.abs())
+    err = (on_gpu(out) - want).abs()
+    assert (err <= E4M3_HALF * want.abs() + s.repeat_interleave(32, 1) * 2.0 ** -10 + 1.25 * off).all()
+    amax, ob = want.reshape(M, -1, 32).abs().amax(2), off.reshape(M, -1, 32).amax(2)
+    assert ((amax <= s * 448 + ob) & ((amax > s * 224 - ob) | (s == 2.0 ** -126))).all()
+    check_padding(out)
+    check_poison(whole, M)
+
+
+def random_bytes(rows, cols, fmt="fp8"):
+    """A large MX matrix of random bytes (no NaN codes), scales around 1."""
+    m = mx.MXTensor.empty(rows, cols, DEV, fmt)
+    m.data.view(torch.uint8).random_(0, 120)
+    m.scales.view(torch.uint8).random_(120, 130)
+    if m.data.shape[1] != cols // (2 if fmt == "fp4" else 1):
+        m.data[:, cols // (2 if fmt == "fp4" else 1):] = 0
+    return m
+
+
+def test_offsets_past_32_bits():
+    """Weights, activations and outputs whose last rows lie past 4 GiB."""
+    w = random_bytes(1_060_000, 4096)
+    x = mx_random(3, 4096, 1)
+    got = mx.linear(x, w)
+    assert torch.equal(got[:, -264:], mx.linear(x, w[-264:])) and torch.equal(got[:, :264], mx.linear(x, w[:264]))
+    del w, got
+    a = torch.zeros((2_900_000, 1536), dtype=torch.bfloat16, device=DEV)
+    a[-700:] = token_rows(700, 1536, 2)
+    q = mx.quantize(a)
+    tail = mx.quantize(a[-700:].clone())
+    assert torch.equal(q.data[-700:].view(torch.uint8), tail.data.view(torch.uint8))
+    wt = mx_random(768, 1536, 3)
+    got = mx.linear(q, wt)  # 4.45 GB of output
+    assert torch.equal(got[-700:], mx.linear(tail, wt)) and (got[:700] == 0).all()
+    del got
+    y, h = mx.norm(a, a, out=q, residual_out=a)
+    assert torch.equal(y.data[-700:].view(torch.uint8), mx.norm(h[-700:].clone()).data.view(torch.uint8))
+    del a, y, h, q
+    w4 = random_bytes(2_130_000, 4096, "fp4")
+    v = token_rows(2, 4096, 4)
+    got = mx.matvec(v, w4)
+    assert torch.equal(got[:, -264:], mx.matvec(v, w4[-264:])) and torch.equal(got[:, :264], mx.matvec(v, w4[:264]))
+
+
+def test_linear_wide_row_strides():
+    """Row strides that 256 rows of pass 2^31 bytes (another kernel than the packed rows': the same bits)."""
+    x, w = mx_random(5, 1536, 1), mx_random(40, 1536, 2)
+    stride = (1 << 23) + 16
+    flat = torch.empty(5 * stride, dtype=torch.uint8, device=DEV)
+    data = flat.as_strided((5, 1536), (stride, 1))
+    data.copy_(x.data.view(torch.uint8))
+    wide = mx.MXTensor("fp8", data.view(torch.float8_e4m3fn), x.scales, 1536)
+    assert torch.equal(mx.linear(wide, w), mx.linear(x, w))
+
+
+def test_two_streams_at_once():
+    x, w, w4 = mx_random(700, 1536, 1), mx_random(4608, 1536, 2), mx_random(4608, 1536, 3, "fp4")
+    v = token_rows(3, 1536, 4)
+    want = (mx.linear(x, w), mx.matvec(v, w4))
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = [[], []]
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    for _ in range(20):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append((mx.linear(x, w), mx.matvec(v, w4)))
+    torch.cuda.synchronize()
+    for pairs in got:
+        for a, b in pairs:
+            assert torch.equal(a, want[0]) and torch.equal(b, want[1])
+
+
 def test_linear_nan_stays_in_its_row():
     x, w = token_rows(40, 512, 1), mx_random(64, 512, 2)
     clean = mx.linear(mx.quantize(x), w)
@@ -412,7 +546,9 @@ def test_linear_nan_stays_in_its_row():
 # ---------------------------------------------------------------------------------------------
 
 @pytest.mark.parametrize("M,N,K", [(1, 8, 32), (2, 16, 96), (3, 24, 128), (1, 9216, 1536), (16, 136, 544), (17, 264, 2432),
-                                   (32, 40, 4096), (33, 520, 8960), (64, 64, 160), (100, 72, 1536), (1, 1544, 14336)])
+                                   (32, 40, 4096), (33, 520, 8960), (64, 64, 160), (100, 72, 1536), (1, 1544, 14336),
+                                   (16, 5128, 5120), (11, 4616, 5120), (5, 264, 13824), (3, 40016, 1056),
+                                   (2, 24, 60000)])
 @pytest.mark.parametrize("epi", ["bias", "gelu", "silu", "res", "f32"])
 def test_matvec(M, N, K, epi):
     x, w = strided(token_rows(M, K, M + K)), mx_random(N, K, N + K, "fp4")

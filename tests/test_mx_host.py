@@ -47,7 +47,7 @@ def test_norm_refuses(change, word):
     (dict(W=None), "null"), (dict(A=None), "null"), (dict(M=-1), "shape"), (dict(N=0), "shape"), (dict(K=100), "K=100"),
     (dict(N=60), "N=60"), (dict(lda=96), "padding"), (dict(ldws=0), "padding"), (dict(W=C + 8), "aligned"),
     (dict(out=2), "output"), (dict(epi=4), "epilogue"), (dict(epi=6), "epilogue"), (dict(ldc=60), "ldc"),
-    (dict(ldc=56), "ldc"), (dict(out=1, epi=3, R=F, ldr=64), "bf16"), (dict(out=1, N=72), "N=72"),
+    (dict(ldc=56), "ldc"), (dict(ldc=1 << 22), "strides"), (dict(epi=3, R=F, ldr=1 << 22), "strides"), (dict(out=1, epi=3, R=F, ldr=64), "bf16"), (dict(out=1, N=72), "N=72"),
     (dict(out=1, ldc=128), "MX output"), (dict(out=1, Cs=F, ldc=64, ldcs=16), "MX output"), (dict(epi=3), "residual"),
     (dict(epi=3, R=F, ldr=60), "residual"), (dict(epi=2, R=F, ldr=64), "gate"),
     (dict(epi=2, R=F, ldr=64, gate=G, gs=66, cu=H, nseg=1), "gate")])
@@ -62,6 +62,31 @@ def test_gemm_refuses(change, word):
     (dict(K=81920, ldx=81920, ldw=40960, ldws=2560), "too long")])
 def test_matvec_refuses(change, word):
     refused("ditk_mx_matvec", tuple({**MV, **change}.values()), word)
+
+
+def plan(m, n, k):
+    import ctypes
+    p = (ctypes.c_int * 3)()
+    _lib.call("ditk_mx_gemm_plan", m, n, k, p)
+    return tuple(p)
+
+
+def test_plans():
+    """Few rows on small tiles, many on large ones, a short last round on smaller ones; both parts
+    of a split have rows, the first one whole tile rows."""
+    assert plan(16, 9216, 1536) == (3, 16, 0) and plan(512, 4608, 1536) == (2, 512, 0)
+    assert plan(667, 7296, 2432) == (1, 667, 0) and plan(65520, 1536, 8960) == (0, 65520, 0)
+    assert plan(4096, 5120, 5120) == (0, 3072, 1)
+    assert plan(2600, 4096, 384) == (4, 2600, 0) and plan(130, 96, 128) == (5, 130, 0)
+    heights = (256, 128, 128, 64)
+    for m in (1, 63, 64, 65, 127, 500, 1560, 2560, 4097, 20000, 65520):
+        for n in (8, 96, 1536, 5120, 13824):
+            for k in (416, 1536, 5120, 14336):
+                tile, rows, rest = plan(m, n, k)
+                assert 0 <= tile < 4 and 0 <= rest < 4 and 0 < rows <= m
+                assert rows == m or rows % heights[tile] == 0
+    with pytest.raises(_lib.DitkError):
+        plan(0, 64, 64)
 
 
 def test_no_rows_need_no_pointers():
