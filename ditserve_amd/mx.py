@@ -55,15 +55,17 @@ class MXTensor:
         cols = int(cols)
         if cols <= 0 or cols % 32:
             raise ValueError(f"an MX matrix has blocks of 32 columns, got {cols}")
-        if data.shape[1] != _data_bytes(cols, fmt) or scales.shape != (data.shape[0], _scale_bytes(cols)):
+        (rows, n), (rows_s, n_s) = data.shape, scales.shape
+        if n != _data_bytes(cols, fmt) or n_s != _scale_bytes(cols) or rows != rows_s:
             raise ValueError(f"{cols} {fmt} columns take data [rows, {_data_bytes(cols, fmt)}] and scales "
                              f"[rows, {_scale_bytes(cols)}], got {tuple(data.shape)} and {tuple(scales.shape)}")
         if data.device != scales.device:
             raise ValueError(f"data is on {data.device}, scales on {scales.device}")
-        for t, name in ((data, "data"), (scales, "scales")):
-            st = t.stride()
-            if st[1] != 1 or st[0] % 16 or (t.shape[0] > 1 and st[0] < t.shape[1]) or t.data_ptr() % 16:
-                raise ValueError(f"{name} rows must have unit column stride and be 16-byte aligned, got strides {st}")
+        for t, name, width in ((data, "data", n), (scales, "scales", n_s)):
+            ld, unit = t.stride()
+            if unit != 1 or ld & 15 or (ld < width and rows > 1) or t.data_ptr() & 15:
+                raise ValueError(f"{name} rows must have unit column stride and be 16-byte aligned, got strides "
+                                 f"{t.stride()}")
         self.fmt, self.data, self.scales, self.cols = fmt, data, scales, cols
 
     @classmethod
@@ -73,8 +75,8 @@ class MXTensor:
             raise ValueError(f"an MX matrix is 'fp8' or 'fp4' with blocks of 32 columns, got {fmt!r} and {cols}")
         self = cls.__new__(cls)
         self.fmt, self.cols = fmt, int(cols)
-        self.data = torch.empty((rows, _data_bytes(cols, fmt)), dtype=_DATA_TYPE[fmt], device=device)
-        self.scales = torch.empty((rows, _scale_bytes(cols)), dtype=_E8M0, device=device)
+        self.data = torch.empty(rows, _data_bytes(cols, fmt), dtype=_DATA_TYPE[fmt], device=device)
+        self.scales = torch.empty(rows, _scale_bytes(cols), dtype=_E8M0, device=device)
         return self
 
     @property
@@ -113,7 +115,8 @@ class MXTensor:
         return (v[:, :cols].reshape(rows, cols // 32, 32) * s.unsqueeze(2)).reshape(rows, cols)
 
     def _args(self):
-        return _ptr(self.data), self.data.stride(0), _ptr(self.scales), self.scales.stride(0)
+        d, s = self.data, self.scales
+        return d.data_ptr(), d.stride(0), s.data_ptr(), s.stride(0)
 
 
 def _call(device, name, *args):
@@ -123,6 +126,16 @@ def _call(device, name, *args):
         return _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(index))
     with torch.cuda.device(index):
         return _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(index))
+
+
+def _bf16_rows(t, name):
+    """(rows, columns, row stride, address) of a bf16 row view, or the refusal of what is none."""
+    if t.__class__ is torch.Tensor and t.dtype is _BF16 and t.is_cuda:
+        st = t.stride()
+        if len(st) == 2 and st[1] == 1 and not st[0] & 7 and not t.data_ptr() & 15:
+            return (*t.shape, st[0], t.data_ptr())
+    _check(t, name, _BF16, 2)
+    return (*t.shape, _rows(t, name), t.data_ptr())
 
 
 def _one_device(device, *tensors):
@@ -171,16 +184,14 @@ def quantize(x, fmt="fp8", out=None):
     A block that holds an infinity or NaN becomes NaN (in fp4: by its scale)."""
     if fmt not in FORMATS:
         raise ValueError(f"fmt must be 'fp8' or 'fp4', got {fmt!r}")
-    _check(x, "x", _BF16, 2)
-    T, K = x.shape
-    ldx = _rows(x, "x")
+    T, K, ldx, xp = _bf16_rows(x, "x")
     if K == 0 or K % 32:
         raise ValueError(f"x needs blocks of 32 columns, got {K}")
-    given = out
-    out = _mx_out(out, T, K, x.device, fmt)
+    device, given = x.device, out
+    out = _mx_out(out, T, K, device, fmt)
     if given is not None:
         _apart("quantize", (out.data, out.scales), (x,))
-    _call(x.device, "ditk_mx_quantize", _ptr(x), ldx, *out._args(), T, K, FORMATS[fmt])
+    _call(device, "ditk_mx_quantize", xp, ldx, *out._args(), T, K, FORMATS[fmt])
     return out
 
 
@@ -193,30 +204,27 @@ def norm(x, residual=None, shift=None, scale=None, segments=None, weight=None, b
     ops.adaln's, kind "rms" by default.  Returns the MX matrix, and with a residual
     also s in bf16 (in residual_out if given, which may be x or residual itself);
     the norm is that of the unrounded s."""
-    _check(x, "x", _BF16, 2)
-    T, D = x.shape
-    ldx = _rows(x, "x")
+    T, D, ldx, xp = _bf16_rows(x, "x")
     if D == 0 or D % 32:
         raise ValueError(f"x needs blocks of 32 columns, got {D}")
     if kind not in ("ln", "rms"):
         raise ValueError(f"kind must be 'ln' or 'rms', got {kind!r}")
     device = x.device
-    _one_device(device, ("residual", residual), ("shift", shift), ("scale", scale), ("weight", weight), ("bias", bias),
-                ("residual_out", residual_out), ("segments", None if segments is None else segments.dev))
-    h, ldr, ldh = None, 0, 0
+    h, hp, rp, ldr, ldh = None, None, None, 0, 0
     if residual is not None:
-        _check(residual, "residual", _BF16, 2)
-        if residual.shape != (T, D):
+        rows, cols, ldr, rp = _bf16_rows(residual, "residual")
+        if rows != T or cols != D:
             raise ValueError(f"residual must be [{T}, {D}], got {tuple(residual.shape)}")
-        ldr = _rows(residual, "residual")
+        _one_device(device, ("residual", residual))
         if residual_out is None:
-            h = torch.empty((T, D), dtype=_BF16, device=device)
+            h, ldh = torch.empty(T, D, dtype=_BF16, device=device), D
+            hp = h.data_ptr()
         else:
             h = residual_out
-            _check(h, "residual_out", _BF16, 2)
-            if h.shape != (T, D):
+            rows, cols, ldh, hp = _bf16_rows(h, "residual_out")
+            if rows != T or cols != D:
                 raise ValueError(f"residual_out must be [{T}, {D}], got {tuple(h.shape)}")
-        ldh = _rows(h, "residual_out")
+            _one_device(device, ("residual_out", h))
     elif residual_out is not None:
         raise ValueError("residual_out needs a residual")
     mod_stride, cu, nseg = 0, None, 0
@@ -234,21 +242,23 @@ def norm(x, residual=None, shift=None, scale=None, segments=None, weight=None, b
         if segments.total != T:
             raise ValueError(f"segments cover {segments.total} tokens, x has {T}")
         mod_stride, cu, nseg = shift.stride(0), segments.dev, segments.nseg
+        _one_device(device, ("shift", shift), ("scale", scale), ("segments", cu))
     for t, n in ((weight, "weight"), (bias, "bias")):
         if t is not None:
             _vec(t, n, D)
+            _one_device(device, (n, t))
     y = _mx_out(out, T, D, device, "fp8")
     if out is not None or residual_out is not None:
         outs = ([] if out is None else [y.data, y.scales]) + ([] if residual_out is None else [h])
         _apart("norm", outs, (shift, scale, weight, bias), same=(x, residual))
-    _call(device, "ditk_mx_norm", _ptr(x), ldx, _ptr(residual), ldr, _ptr(h), ldh, *y._args(), T, D, _ptr(cu), nseg,
+    _call(device, "ditk_mx_norm", xp, ldx, rp, ldr, hp, ldh, *y._args(), T, D, _ptr(cu), nseg,
           _ptr(shift), _ptr(scale), mod_stride, _ptr(weight), _ptr(bias), float(eps), 0 if kind == "ln" else 1)
     return y if residual is None else (y, h)
 
 
 def _bf16_out(out, M, N, dtype, device):
     if out is None:
-        return torch.empty((M, N), dtype=dtype, device=device)
+        return torch.empty(M, N, dtype=dtype, device=device)
     _check(out, "out", dtype, 2)
     ldc, unit = out.stride()
     if out.shape != (M, N) or unit != 1 or ldc % 8 or out.data_ptr() % 16:
@@ -277,8 +287,8 @@ def linear(x, w, b=None, epilogue="bias", residual=None, gate=None, segments=Non
     of the sum of magnitudes on random data, far below e4m3's own 2^-4.)"""
     _mx_check(x, "x", "fp8")
     _mx_check(w, "w", "fp8")
-    (M, K), (N, Kw) = x.shape, w.shape
-    if Kw != K:
+    M, K, N = x.data.shape[0], x.cols, w.data.shape[0]
+    if w.cols != K:
         raise ValueError(f"weight is {w.shape}, input has K={K}")
     if N == 0 or N % 8:
         raise ValueError(f"linear needs N % 8 == 0 (got N={N})")
@@ -291,10 +301,11 @@ def linear(x, w, b=None, epilogue="bias", residual=None, gate=None, segments=Non
         raise ValueError(f"epilogue {epilogue!r} writes bf16")
     if out_fmt and N % 32:
         raise ValueError(f"an MX output needs N % 32 == 0 (got N={N})")
+    device = x.data.device
     if b is not None:
         _vec(b, "bias", N)
-    device = x.device
-    _one_device(device, ("w", w), ("bias", b), ("out", out))
+        _one_device(device, ("bias", b))
+    _one_device(device, ("w", w.data), ("out", out))
     ldr, gate_stride, cu, nseg = 0, 0, None, 0
     if res:
         ldr = _residual(residual, M, N)
@@ -333,33 +344,32 @@ def matvec(x, w, b=None, epilogue="bias", residual=None, out=None):
     that fit into LDS (up to 16 or 32): for many rows quantize them and use an fp8
     weight and linear().  A row's result does not depend on the other rows."""
     _mx_check(w, "w", "fp4")
-    _check(x, "x", _BF16)
-    if x.dim() not in (1, 2):
-        raise ValueError(f"x must be [M, K] or [K], got shape {tuple(x.shape)}")
-    one = x.dim() == 1
+    one = isinstance(x, torch.Tensor) and x.dim() == 1
     if one:
         x = x.unsqueeze(0)
         residual = None if residual is None else residual.unsqueeze(0)
         out = None if out is None else out.unsqueeze(0)
-    M, K = x.shape
-    N = w.rows
+    M, K, ldx, xp = _bf16_rows(x, "x")
+    N = w.data.shape[0]
     if w.cols != K:
         raise ValueError(f"weight is {w.shape}, input has K={K}")
     if N == 0 or N % 8:
         raise ValueError(f"matvec needs N % 8 == 0 (got N={N})")
     if epilogue not in EPILOGUES or epilogue == "gate_res":
         raise ValueError(f"unknown epilogue {epilogue!r}")
-    ldx = _rows(x, "x")
+    device = x.device
     if b is not None:
         _vec(b, "bias", N)
-    res = epilogue == "res"
-    device = x.device
-    _one_device(device, ("w", w), ("bias", b), ("residual", residual if res else None), ("out", out))
-    ldr = _residual(residual, M, N) if res else 0
+        _one_device(device, ("bias", b))
+    _one_device(device, ("w", w.data), ("out", out))
+    res, ldr = epilogue == "res", 0
+    if res:
+        ldr = _residual(residual, M, N)
+        _one_device(device, ("residual", residual))
     given = out
     out = _bf16_out(out, M, N, torch.float32 if epilogue == "f32" else _BF16, device)
     if given is not None:
         _apart("matvec", (out,), (x, w.data, w.scales, b), same=(residual,) if res else ())
-    _call(device, "ditk_mx_matvec", _ptr(x), ldx, *w._args(), _ptr(b), _ptr(out), out.stride(0), M, N, K,
+    _call(device, "ditk_mx_matvec", xp, ldx, *w._args(), _ptr(b), _ptr(out), out.stride(0), M, N, K,
           EPILOGUES[epilogue], _ptr(residual) if res else None, ldr)
     return out[0] if one else out
