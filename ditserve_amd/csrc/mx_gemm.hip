@@ -400,7 +400,7 @@ __global__ __launch_bounds__(WM * WN * 64, EU) void mx_gemm_kernel(MxGemmArgs p)
                                 MxTile{m0, n0, m0, n0}, m0 + a_row0, n0 + w_row0, lane);
 }
 
-// One wave per SIMD, K > 384: a workgroup tile as 2 x 2 wave tiles with their accumulators in the
+// One wave per SIMD, K of NBUF stages or more: a workgroup tile as 2 x 2 wave tiles with their accumulators in the
 // AGPRs.  The k loop is generated assembly (gen_mx_gemm.py -> mx_l4_*_body.inc); this C++ part
 // gives it the per-lane addresses and runs the epilogue on the accumulators.  Persistent:
 // XCD x (= blockIdx % 8) owns the tiles [x * per_xcd, (x + 1) * per_xcd), which its workgroups take
@@ -692,13 +692,14 @@ MxPlan mx_plan(int M, int N, int K) {
 }
 
 // The kernels a product can run on (as numbered by ditk_mx_gemm_plan): a configuration of kCfg, or
-// mx_gemm_kernel on 256 x 256 or 64 x 128 tiles, for K up to 384, which the ring of stages of the l4
-// kernel does not fit into, and for row strides that its 32-bit offsets do not reach over 256 rows.
+// mx_gemm_kernel on 256 x 256 or 64 x 128 tiles, for the short K that the l4 kernel's ring of stages
+// does not fit into (2 for 256 x 256 tiles, up to 4 for the others) and for row strides that its 32-bit
+// offsets do not reach over 256 rows.  (65520 x 8960 x 384: 423 us on mx_gemm_kernel, 327 on the l4 one.)
 constexpr int kPlainLarge = kCfgs, kPlainSmall = kCfgs + 1;
 MxPlan mx_plan_any(int M, int N, int K, int64_t ld) {
-  if (K > 384 && 256 * ld < (1ll << 31)) return mx_plan(M, N, K);
-  const bool large = (int64_t)((M + 255) / 256) * ((N + 255) / 256) >= 128;
-  return MxPlan{large ? kPlainLarge : kPlainSmall, M, 0, 0.f};
+  const bool l4 = 256 * ld < (1ll << 31), large = (int64_t)((M + 255) / 256) * ((N + 255) / 256) >= 128;
+  if (l4 && K > 384) return mx_plan(M, N, K);
+  return MxPlan{!large ? kPlainSmall : l4 && K > 128 ? 0 : kPlainLarge, M, 0, 0.f};
 }
 
 template <int EPI, int OUT>

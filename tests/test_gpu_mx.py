@@ -371,7 +371,7 @@ def test_linear_mx_output(M, N, K, epi):
     check_poison(whole, M)
 
 
-@pytest.mark.parametrize("K", [96, 1536, 2432])
+@pytest.mark.parametrize("K", [96, 256, 352, 1536, 2432])
 def test_linear_rows_do_not_depend_on_the_batch(K):
     """Whatever tile a launch takes, a row's result is bitwise the same; and without a bias."""
     M, N = 2600, 4096
@@ -414,7 +414,8 @@ def on_gpu(m):
     ((100, 1544, 416), (3, 100, 0)), ((63, 9992, 512), (3, 63, 0)), ((1000, 4616, 1056), None),
     ((520, 4616, 448), (2, 520, 0)), ((333, 8968, 1536), (2, 333, 0)), ((667, 7304, 2432), (1, 667, 0)),
     ((2600, 4104, 640), None), ((2600, 8968, 512), None), ((4353, 4104, 1568), (0, 3840, 2)),
-    ((4600, 5128, 416), (0, 3072, 1)), ((9000, 2440, 3104), None), ((129, 24, 8960), None), ((300, 40, 14336), None)])
+    ((4600, 5128, 416), (0, 3072, 1)), ((2601, 4104, 384), (0, 2601, 0)), ((5000, 8200, 160), (0, 5000, 0)),
+    ((5000, 8200, 256), (0, 5000, 0)), ((2601, 4104, 128), (4, 2601, 0)), ((700, 4104, 288), (5, 700, 0)), ((9000, 2440, 3104), None), ((129, 24, 8960), None), ((300, 40, 14336), None)])
 @pytest.mark.parametrize("epi", ["gate_res", "gelu"])
 def test_linear_tiles(shape, want, epi):
     M, N, K = shape

@@ -77,7 +77,8 @@ def test_plans():
     assert plan(16, 9216, 1536) == (3, 16, 0) and plan(512, 4608, 1536) == (2, 512, 0)
     assert plan(667, 7296, 2432) == (1, 667, 0) and plan(65520, 1536, 8960) == (0, 65520, 0)
     assert plan(4096, 5120, 5120) == (0, 3072, 1)
-    assert plan(2600, 4096, 384) == (4, 2600, 0) and plan(130, 96, 128) == (5, 130, 0)
+    assert plan(2600, 4096, 384) == (0, 2600, 0) and plan(2600, 4096, 128) == (4, 2600, 0)
+    assert plan(130, 96, 128) == (5, 130, 0)
     heights = (256, 128, 128, 64)
     for m in (1, 63, 64, 65, 127, 500, 1560, 2560, 4097, 20000, 65520):
         for n in (8, 96, 1536, 5120, 13824):
