@@ -2,7 +2,9 @@
 //
 //   C[m, n] = epilogue( sum_k x[m, k] v[n, k] 2^e[n, k / 32]  + bias[n] )
 //
-// Bound by streaming the weight once, 4.25 bits a value.  A wave takes 16 features at a
+// Two kernels, bitwise alike, and a rule between them (launch): one for few rows, one of tiles for more.
+//
+// Bound by streaming the weight once, 4.25 bits a value.  In the first a wave takes 16 features at a
 // time: lane (ql = lane % 16, g = lane / 16) loads the 16 bytes of block 4 c + g of weight row
 // ql -- 32 weights under one scale -- which the convert instructions turn into bf16,
 // exactly (an e2m1 value times a power of two), for four MFMAs of 16 features x 16 tokens x 32
@@ -40,6 +42,29 @@ __device__ __forceinline__ bf16x8_t fp4_to_bf16(uint32_t w, float scale) {
 // e8m0 byte -> fp32 (255: NaN)
 __device__ __forceinline__ float e8m0_to_f32(uint32_t byte) {
   return byte == 255 ? __uint_as_float(0x7fc00000u) : __uint_as_float(byte << 23);
+}
+
+// y (4 consecutive features of a row, before the bias) -> the output, from element `at`
+template <int EPI>
+__device__ __forceinline__ void finish4(f32x4_t y, const f32x4_t& b, const u32x2_t& r, void* Cv, int64_t at) {
+  y += b;
+  if (EPI == MV_F32) {
+    *reinterpret_cast<f32x4_t*>(reinterpret_cast<float*>(Cv) + at) = y;
+    return;
+  }
+  if (EPI == MV_GELU) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) y[k] = gelu_tanh_f(y[k]);
+  } else if (EPI == MV_SILU) {
+#pragma unroll
+    for (int k = 0; k < 4; ++k) y[k] = silu_f(y[k]);
+  } else if (EPI == MV_RES) {
+    y[0] += __uint_as_float(r[0] << 16);
+    y[1] += __uint_as_float(r[0] & 0xffff0000u);
+    y[2] += __uint_as_float(r[1] << 16);
+    y[3] += __uint_as_float(r[1] & 0xffff0000u);
+  }
+  *reinterpret_cast<u32x2_t*>(reinterpret_cast<bf16_t*>(Cv) + at) = u32x2_t{pack_bf2(y[0], y[1]), pack_bf2(y[2], y[3])};
 }
 
 constexpr int kMaxWaves = 16;
@@ -131,25 +156,7 @@ __global__ __launch_bounds__(64 * kMaxWaves) void mx_matvec_kernel(const bf16_t*
     if (!has_row || n >= N) return;
     f32x4_t y = part[buf * waves][ej][lane];
     for (int v = 1; v < waves; ++v) y += part[buf * waves + v][ej][lane];
-    y += bcur;
-    if (EPI == MV_F32) {
-      *reinterpret_cast<f32x4_t*>(reinterpret_cast<float*>(Cv) + (int64_t)m * ldc + n) = y;
-      return;
-    }
-    if (EPI == MV_GELU) {
-#pragma unroll
-      for (int k = 0; k < 4; ++k) y[k] = gelu_tanh_f(y[k]);
-    } else if (EPI == MV_SILU) {
-#pragma unroll
-      for (int k = 0; k < 4; ++k) y[k] = silu_f(y[k]);
-    } else if (EPI == MV_RES) {
-      y[0] += __uint_as_float(rcur[0] << 16);
-      y[1] += __uint_as_float(rcur[0] & 0xffff0000u);
-      y[2] += __uint_as_float(rcur[1] << 16);
-      y[3] += __uint_as_float(rcur[1] & 0xffff0000u);
-    }
-    *reinterpret_cast<u32x2_t*>(reinterpret_cast<bf16_t*>(Cv) + (int64_t)m * ldc + n) =
-        u32x2_t{pack_bf2(y[0], y[1]), pack_bf2(y[2], y[3])};
+    finish4<EPI>(y, bcur, rcur, Cv, (int64_t)m * ldc + n);
   };
 
   int group = blockIdx.x, i = 0, buf = 0;
@@ -210,6 +217,157 @@ __global__ __launch_bounds__(64 * kMaxWaves) void mx_matvec_kernel(const bf16_t*
   }
 }
 
+// More rows than LDS holds, or more features than the first kernel streams well: tiles of 16 FJ tokens x 64 FI
+// features as 4 waves, both operands through LDS in stages of 128 k (x rows of 256 bytes, weight rows
+// of 64, their 16-byte units XOR-swizzled by row) by direct DMA into NBUF stages.  `classes` is
+// the first kernel's number of waves: the stages go through the chunks of its wave 0, then of wave 1,
+// ..., each class's sum added to the total.  The same additions in the same order, bitwise its results.
+//
+// 48 x 8960 x 51200 361 us on the first kernel (7 passes over the weight), 95 here; 1 x 5120 x 131072 97 and
+// 76 (4.7 TB/s).  A tile's stage takes 0.27 + 0.125 FJ us: its way through one wave a SIMD, some 130
+// instructions, the LDS reads and the MFMAs one after the other; more stages ahead (6 or 7) change nothing, two
+// tiles on a CU fill each other's gaps.
+template <int EPI, int FJ, int FI, int NBUF>
+__global__ __launch_bounds__(256) void mx_matvec_wide_kernel(const bf16_t* __restrict__ x, int64_t ldx,
+                                                             const uint8_t* __restrict__ W, int64_t ldw,
+                                                             const uint8_t* __restrict__ Ws, int64_t ldws,
+                                                             const float* __restrict__ bias, void* Cv, int64_t ldc,
+                                                             int M, int N, int K, const bf16_t* R, int64_t ldr,
+                                                             int classes) {
+  constexpr int TN = 64 * FI, XU = 16 * FJ * 16, WU = TN * 4, STAGE = XU + WU;  // 16-byte units of a stage
+  constexpr int DMAS = FJ + FI;                                                         // per wave and stage
+  // and the scales of four chunks of 512 k, 16 bytes a row: two stages ahead of the chunk that is read may lie one
+  // of 128 k and the beginning of the next
+  __shared__ u32x4_t lds[NBUF * STAGE + 4 * TN];
+  u32x4_t* const sc = lds + NBUF * STAGE;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), ql = lane & 15, g = lane >> 4;
+  const int n0 = blockIdx.x * TN, m0 = blockIdx.y * (16 * FJ);
+  const int blocks = K / 32, steps = (blocks + 3) / 4, chunks = (steps + 3) / 4;
+  auto lds_at = [&](const void* q) {
+    return (uint32_t)__builtin_amdgcn_readfirstlane(
+        (int)(uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char*)reinterpret_cast<const char*>(q));
+  };
+  // (as assembly, the waits below its own: for a DMA it sees the compiler would wait at every LDS read)
+  auto dma = [&](const void* src, const void* dst) {
+    asm volatile("s_mov_b32 m0, %0\n s_nop 0\n global_load_lds_dwordx4 %1, off" ::"s"(lds_at(dst)), "v"(src) : "memory", "m0");
+  };
+  // DMA instruction d of this wave: x rows 4 (4 d + wave) .. + 3, weight rows 16 (4 d + wave) .. + 15
+  const bf16_t* xsrc[FJ];
+  int xk[FJ];
+#pragma unroll
+  for (int d = 0; d < FJ; ++d) {
+    const int row = (d * 4 + wave) * 4 + (lane >> 4), v = (lane & 15) ^ (row & 15);
+    xsrc[d] = x + (int64_t)min(m0 + row, M - 1) * ldx;
+    xk[d] = (v & 3) * 32 + (v >> 2) * 8;  // unit 4 u + g: k 32 g + 8 u
+  }
+  const uint8_t* wsrc[FI];
+#pragma unroll
+  for (int d = 0; d < FI; ++d) {
+    const int row = (d * 4 + wave) * 16 + (lane >> 2);
+    wsrc[d] = W + (int64_t)min(n0 + row, N - 1) * ldw + (((lane & 3) ^ (row >> 2)) & 3) * 16;
+  }
+  const uint8_t* ssrc = Ws + (int64_t)min(n0 + wave * 16 * FI + (lane & (16 * FI - 1)), N - 1) * ldws;
+  const uint8_t* zeros = W + K / 2;  // a weight row's padding behind K, where K % 128 != 0
+  // the order of the stages: the chunks of class 0 (c % classes == 0), of class 1, ...
+  struct Place {
+    int cls, chunk, t, n;  // n: chunks begun so far
+  };
+  auto next = [&](Place& p) {
+    if (p.chunk * 4 + ++p.t < steps && p.t < 4) return;
+    p.t = 0;
+    ++p.n;
+    p.chunk += classes;
+    if (p.chunk >= chunks) p.chunk = ++p.cls;
+  };
+  Place fetch{0, 0, 0, 0}, at{0, 0, 0, 0};
+  auto issue = [&](int buf) {
+    if (fetch.cls >= classes) return;
+    u32x4_t* st = lds + buf * STAGE;
+    const int kt = fetch.chunk * 4 + fetch.t;
+    if (fetch.t == 0 && lane < 16 * FI) dma(ssrc + fetch.chunk * 16, sc + (fetch.n & 3) * TN + wave * 16 * FI);
+#pragma unroll
+    for (int d = 0; d < FJ; ++d) {
+      const int k = kt * 128 + xk[d];
+      dma(k < K ? reinterpret_cast<const void*>(xsrc[d] + k) : zeros, st + (d * 4 + wave) * 64);
+    }
+#pragma unroll
+    for (int d = 0; d < FI; ++d) dma(wsrc[d] + kt * 64, st + XU + (d * 4 + wave) * 64);
+    next(fetch);
+  };
+#pragma unroll
+  for (int b = 0; b < NBUF - 1; ++b) issue(b);
+  f32x4_t total[FI][FJ], acc[FI][FJ];
+#pragma unroll
+  for (int i = 0; i < FI; ++i)
+#pragma unroll
+    for (int j = 0; j < FJ; ++j) total[i][j] = acc[i][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+  int buf = 0;
+  for (int s = 0; s < steps; ++s) {
+    // this stage is here (behind it at most NBUF - 2 stages are on their way), and read by
+    // every wave is the one whose buffer is filled next
+    if (s + NBUF - 1 <= steps) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((NBUF - 2) * DMAS) : "memory");
+    else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    // every operand is asked for before the next stage's DMAs and the first use: one LDS latency a stage
+    const u32x4_t* st = lds + buf * STAGE;
+    const uint32_t* s32 = reinterpret_cast<const uint32_t*>(sc + (at.n & 3) * TN);
+    u32x4_t w[FI];
+    uint32_t s4[FI];
+    bf16x8_t xf[4][FJ];
+#pragma unroll
+    for (int i = 0; i < FI; ++i) {
+      const int row = (wave * FI + i) * 16 + ql;
+      s4[i] = s32[row * 4 + g];
+      w[i] = st[XU + row * 4 + ((g ^ (row >> 2)) & 3)];
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+#pragma unroll
+      for (int j = 0; j < FJ; ++j)
+        xf[u][j] = __builtin_bit_cast(bf16x8_t, st[(j * 16 + ql) * 16 + ((u * 4 + g) ^ ql)]);
+    __builtin_amdgcn_sched_barrier(0);
+    issue(buf == 0 ? NBUF - 1 : buf - 1);
+    float scale[FI];
+#pragma unroll
+    for (int i = 0; i < FI; ++i) scale[i] = e8m0_to_f32((s4[i] >> (8 * at.t)) & 255);
+#pragma unroll
+    for (int u = 0; u < 4; ++u)
+#pragma unroll
+      for (int i = 0; i < FI; ++i) {
+        const bf16x8_t wf = fp4_to_bf16(w[i][u], scale[i]);
+#pragma unroll
+        for (int j = 0; j < FJ; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wf, xf[u][j], acc[i][j], 0, 0, 0);
+      }
+    const int cls = at.cls;
+    next(at);
+    if (at.cls != cls) {
+#pragma unroll
+      for (int i = 0; i < FI; ++i)
+#pragma unroll
+        for (int j = 0; j < FJ; ++j) {
+          total[i][j] = cls == 0 ? acc[i][j] : total[i][j] + acc[i][j];
+          acc[i][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+        }
+    }
+    buf = buf + 1 == NBUF ? 0 : buf + 1;
+  }
+#pragma unroll
+  for (int i = 0; i < FI; ++i) {
+    const int n = n0 + (wave * FI + i) * 16 + 4 * g;
+    if (n >= N) continue;
+    const f32x4_t b = bias != nullptr ? *reinterpret_cast<const f32x4_t*>(bias + n) : f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int j = 0; j < FJ; ++j) {
+      const int m = m0 + j * 16 + ql;
+      if (m >= M) continue;
+      u32x2_t r{0, 0};
+      if (EPI == MV_RES) r = *reinterpret_cast<const u32x2_t*>(R + (int64_t)m * ldr + n);
+      finish4<EPI>(total[i][j], b, r, Cv, (int64_t)m * ldc + n);
+    }
+  }
+}
+
 template <int EPI>
 int launch(const void* x, int64_t ldx, const void* W, int64_t ldw, const void* Ws, int64_t ldws, const float* bias,
            void* C, int64_t ldc, int M, int N, int K, const void* R, int64_t ldr, hipStream_t stream) {
@@ -220,9 +378,32 @@ int launch(const void* x, int64_t ldx, const void* W, int64_t ldw, const void* W
   DITK_REQUIRE(fit(1) > 0, "ditk_mx_matvec: K=%d too long", K);
   const int fj = waves > 1 && fit(2) > 0 && (M + fit(2) - 1) / fit(2) < (M + fit(1) - 1) / fit(1) ? 2 : 1;
   const int passes = (M + fit(fj) - 1) / fit(fj), x_rows = (M + passes - 1) / passes;
-  DITK_REQUIRE(passes <= 65535, "ditk_mx_matvec: too many rows");
   const int groups = (N + 15) / 16, lds = 2 * waves * fj * 1024 + x_rows * x_stride(K);
   const int per_cu = std::max(1, std::min(kWavesPerCu / waves, kLds / lds));
+  // Which kernel: the first streams the weight `passes` times, more slowly with fewer than some 12 waves on a CU; a
+  // tile of the wide one takes a 128-k step in 0.27 + 0.125 wj us, however few the tiles are, and many tiles stream
+  // the weight a little more slowly.  In us a 128-k step (measured around it: 16 x 5120 x 9216 18.5 us on the
+  // first, 19.1 on the wide, x 16384 26.9 and 19.8; 48 x 1536 x 5120 11.4 and 10.5; 1 x 1536 x 499712 81 and 88;
+  // 1 x 5120 x 131072 97 and 78; wrong by up to 20% at some, as 64 x 8960 x 5120, 46 and 55):
+  const int tall = (M + 63) / 64, wj = ((M + tall - 1) / tall + 15) / 16;
+  const float weight_us = (float)N / 68000.f;  // 128 k of the weight at 4.6 TB/s
+  const float first_us = weight_us * (float)passes * std::max(1.f, 12.f / (float)(per_cu * waves));
+  const float wide_us = std::max(0.27f + 0.125f * (float)wj, weight_us * 1.08f * (float)tall);
+  if (first_us > wide_us) {
+    // 64 features a tile until there is one of 128 a CU (48 x 1536 x 9216 10.6 and 13.4 us, 48 x 5120 x 65536
+    // 75 and 56)
+    const bool narrow = (int64_t)((N + 127) / 128) * tall <= ditk_cu_count();
+    const dim3 grid((unsigned)(narrow ? (N + 63) / 64 : (N + 127) / 128), (unsigned)tall);
+    DITK_REQUIRE(tall <= 65535, "ditk_mx_matvec: too many rows");
+    auto kern = wj == 1   ? (narrow ? mx_matvec_wide_kernel<EPI, 1, 1, 4> : mx_matvec_wide_kernel<EPI, 1, 2, 4>)
+                : wj == 2 ? (narrow ? mx_matvec_wide_kernel<EPI, 2, 1, 4> : mx_matvec_wide_kernel<EPI, 2, 2, 4>)
+                : wj == 3 ? (narrow ? mx_matvec_wide_kernel<EPI, 3, 1, 3> : mx_matvec_wide_kernel<EPI, 3, 2, 3>)
+                          : (narrow ? mx_matvec_wide_kernel<EPI, 4, 1, 3> : mx_matvec_wide_kernel<EPI, 4, 2, 3>);
+    kern<<<grid, 256, 0, stream>>>((const bf16_t*)x, ldx, (const uint8_t*)W, ldw, (const uint8_t*)Ws, ldws, bias, C, ldc,
+                                   M, N, K, (const bf16_t*)R, ldr, waves);
+    return ditk_check_launch("ditk_mx_matvec");
+  }
+  DITK_REQUIRE(passes <= 65535, "ditk_mx_matvec: too many rows");
   const dim3 grid((unsigned)std::min(groups, std::max(1, ditk_cu_count() * per_cu / passes)), (unsigned)passes);
   auto kern = fj == 1 ? mx_matvec_kernel<EPI, 1> : mx_matvec_kernel<EPI, 2>;
   kern<<<grid, 64 * waves, lds, stream>>>((const bf16_t*)x, ldx, (const uint8_t*)W, ldw, (const uint8_t*)Ws, ldws, bias,

@@ -340,9 +340,9 @@ def matvec(x, w, b=None, epilogue="bias", residual=None, out=None):
 
     x [M, K] (a row view) or [K], b [N] fp32, N % 8 == 0.  Epilogues "bias", "gelu"
     (GELU-tanh), "silu", "res" (residual + y), "f32" (fp32 output); in fp32 with one
-    rounding at the end.  Returns [M, N] (or [N]).  The weight is read once for the rows
-    that fit into LDS (up to 16 or 32): for many rows quantize them and use an fp8
-    weight and linear().  A row's result does not depend on the other rows."""
+    rounding at the end.  Returns [M, N] (or [N]).  The weight is read once for up to 64
+    rows (a smaller one more often, where that is faster): for many rows quantize them and use
+    an fp8 weight and linear().  A row's result does not depend on the other rows."""
     _mx_check(w, "w", "fp4")
     one = isinstance(x, torch.Tensor) and x.dim() == 1
     if one:

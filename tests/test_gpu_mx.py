@@ -585,6 +585,50 @@ def test_matvec_rows_do_not_depend_on_the_batch():
         assert torch.equal(mx.matvec(x[a:a + n], w, epilogue="f32"), whole[a:a + n])
 
 
+# more rows than LDS holds, or more features than the first kernel streams well: the kernel of tiles, 16 to 64
+# rows a tile, 64 or 128 features
+@pytest.mark.parametrize("M,N,K", [(3, 27016, 5120), (2, 33800, 4640), (30, 17000, 1568), (17, 33016, 1056),
+                                   (48, 9000, 8960), (40, 33000, 2432), (64, 9224, 5120), (100, 16648, 1056)])
+@pytest.mark.parametrize("epi", ["gelu", "silu", "res", "f32"])
+def test_matvec_tiles(M, N, K, epi):
+    x, w = strided(token_rows(M, K, M + K)), mx_random(N, K, N + K, "fp4")
+    w.scales.view(torch.uint8).sub_(4)
+    g = gen(M)
+    b = torch.randn(N, generator=g).to(DEV)
+    res = strided(torch.randn((M, N), generator=g).to(DEV, torch.bfloat16)) if epi == "res" else None
+    dt = torch.float32 if epi == "f32" else torch.bfloat16
+    buf = torch.full((M + 2, N + 24), 7.0, dtype=dt, device=DEV)
+    out = buf[:M, 8:8 + N]
+    assert mx.matvec(x, w, b, epilogue=epi, residual=res, out=out) is out
+    assert (buf[M:] == 7).all() and (buf[:, :8] == 7).all() and (buf[:, 8 + N:] == 7).all()
+    # a row's bits are those of the product of few rows and features, which the other kernel computes
+    for m in sorted({0, min(15, M - 1), min(16, M - 1), M // 2, M - 1}):
+        for n in (0, N // 2 // 8 * 8, N - 1000):
+            r = None if res is None else res[m:m + 1, n:n + 1000]
+            few = mx.matvec(x[m:m + 1], w[n:n + 1000], b[n:n + 1000], epilogue=epi, residual=r)
+            assert torch.equal(few, out[m:m + 1, n:n + 1000]), (m, n)
+    # and 64 bits: exact products, K + 8 additions in fp32
+    r = None if res is None else res[:, N - 1000:]
+    y, mag = product64(x, w[N - 1000:], b[N - 1000:])
+    want = act64(y, epi, r)
+    off = 1.13 * ((K + 8) * 2.0 ** -24 * mag + 2.0 ** -20 * y.abs())
+    bound = off + 1e-30 if epi == "f32" else BF16_HALF * want.abs() + off + 1e-30
+    err = (out[:, N - 1000:].cpu().double() - want).abs()
+    assert (err <= bound).all(), float((err / bound).max())
+
+
+def test_matvec_tiles_non_finite():
+    # 16 rows of a long K: a NaN block and a NaN row stay where they are, also in rows that end inside a 128-column step
+    x, w = token_rows(16, 8736, 1), token_rows(16392, 8736, 2)
+    w[16000, 8730] = math.nan
+    x[7, 8735] = math.nan
+    got = mx.matvec(x, mx.quantize(w, "fp4"), epilogue="f32").isnan().cpu()
+    hit = torch.zeros((16, 16392), dtype=torch.bool)
+    hit[7] = True
+    hit[:, 16000] = True
+    assert torch.equal(got, hit)
+
+
 def test_matvec_non_finite():
     x, w = token_rows(3, 256, 1), token_rows(24, 256, 2)
     w[5, 40] = math.nan
