@@ -218,38 +218,59 @@ __global__ __launch_bounds__(64 * kMaxWaves) void mx_matvec_kernel(const bf16_t*
 }
 
 // More rows than LDS holds, or more features than the first kernel streams well: tiles of 16 FJ tokens x 64 FI
-// features as 4 waves, both operands through LDS in stages of 128 k (x rows of 256 bytes, weight rows
-// of 64, their 16-byte units XOR-swizzled by row) by direct DMA into NBUF stages.  `classes` is
-// the first kernel's number of waves: the stages go through the chunks of its wave 0, then of wave 1,
-// ..., each class's sum added to the total.  The same additions in the same order, bitwise its results.
+// features, both operands through LDS in stages of 128 k (x rows of 256 bytes, weight rows of 64,
+// their 16-byte units XOR-swizzled by row) by direct DMA into NBUF stages.  G groups of 4 waves share
+// the k: `classes` is the first kernel's number of waves, class c its wave c's chunks, and a
+// round is a class for each group, each with stages of its own; the classes' sums are added in
+// order.  The same additions in the same order: bitwise the first kernel's results.
 //
-// 48 x 8960 x 51200 361 us on the first kernel (7 passes over the weight), 95 here; 1 x 5120 x 131072 97 and
-// 76 (4.7 TB/s).  A tile's stage takes 0.27 + 0.125 FJ us: its way through one wave a SIMD, some 130
-// instructions, the LDS reads and the MFMAs one after the other; more stages ahead (6 or 7) change nothing, two
-// tiles on a CU fill each other's gaps.
-template <int EPI, int FJ, int FI, int NBUF>
-__global__ __launch_bounds__(256) void mx_matvec_wide_kernel(const bf16_t* __restrict__ x, int64_t ldx,
-                                                             const uint8_t* __restrict__ W, int64_t ldw,
-                                                             const uint8_t* __restrict__ Ws, int64_t ldws,
-                                                             const float* __restrict__ bias, void* Cv, int64_t ldc,
-                                                             int M, int N, int K, const bf16_t* R, int64_t ldr,
-                                                             int classes) {
-  constexpr int TN = 64 * FI, XU = 16 * FJ * 16, WU = TN * 4, STAGE = XU + WU;  // 16-byte units of a stage
-  constexpr int DMAS = FJ + FI;                                                         // per wave and stage
-  // and the scales of four chunks of 512 k, 16 bytes a row: two stages ahead of the chunk that is read may lie one
-  // of 128 k and the beginning of the next
-  __shared__ u32x4_t lds[NBUF * STAGE + 4 * TN];
-  u32x4_t* const sc = lds + NBUF * STAGE;
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), ql = lane & 15, g = lane >> 4;
+// 48 x 8960 x 51200 361 us on the first kernel (7 passes over the weight), 80 here; 1 x 5120 x 131072 97 and
+// 76 (4.7 TB/s).  A tile's stage takes 0.3 us for the instructions of one wave a SIMD and 0.12 for
+// each 16 tokens' LDS reads and MFMAs behind one another; more stages ahead (6, 7) change nothing.  Where tiles
+// are few, two groups a tile take 0.6 of that; four 1.2 of what two take.
+template <int EPI, int FJ, int FI, int NBUF, int G>
+__global__ __launch_bounds__(256 * G) void mx_matvec_wide_kernel(const bf16_t* __restrict__ x, int64_t ldx,
+                                                                 const uint8_t* __restrict__ W, int64_t ldw,
+                                                                 const uint8_t* __restrict__ Ws, int64_t ldws,
+                                                                 const float* __restrict__ bias, void* Cv, int64_t ldc,
+                                                                 int M, int N, int K, const bf16_t* R, int64_t ldr,
+                                                                 int classes) {
+  constexpr int TN = 64 * FI, XU = 16 * FJ * 16, STAGE = XU + TN * 4;  // 16-byte units of a stage
+  constexpr int DMAS = FJ + FI;                                        // per wave and stage
+  // a group's stages, and the scales of four chunks of 512 k, 16 bytes a row: two stages ahead of the chunk that
+  // is read may lie one of 128 k and the beginning of the next
+  constexpr int GROUP = NBUF * STAGE + 4 * TN;
+  __shared__ u32x4_t lds[G * GROUP];
+  __shared__ f32x4_t part[G > 1 ? G - 1 : 1][G > 1 ? FI * FJ : 1][G > 1 ? 256 : 1];
+  const int lane = threadIdx.x & 63, ql = lane & 15, g = lane >> 4;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6) & 3;
+  const int q = G == 1 ? 0 : __builtin_amdgcn_readfirstlane(threadIdx.x >> 8);
+  u32x4_t* const ring = lds + q * GROUP;
+  u32x4_t* const sc = ring + NBUF * STAGE;
   const int n0 = blockIdx.x * TN, m0 = blockIdx.y * (16 * FJ);
   const int blocks = K / 32, steps = (blocks + 3) / 4, chunks = (steps + 3) / 4;
-  auto lds_at = [&](const void* q) {
+  // the 128-k steps of a class; a round takes as many stages as the longest of its G classes
+  auto steps_of = [&](int c) {
+    if (c >= classes) return 0;
+    return ((chunks - 1 - c) / classes + 1) * 4 - ((chunks - 1) % classes == c ? chunks * 4 - steps : 0);
+  };
+  auto stages_of = [&](int r) {
+    int s = steps_of(r * G);
+#pragma unroll
+    for (int c = 1; c < G; ++c) s = max(s, steps_of(r * G + c));
+    return s;
+  };
+  const int rounds = (classes + G - 1) / G;
+  int left = 0;  // stages not yet computed
+  for (int r = 0; r < rounds; ++r) left += stages_of(r);
+  auto lds_at = [&](const void* at) {
     return (uint32_t)__builtin_amdgcn_readfirstlane(
-        (int)(uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char*)reinterpret_cast<const char*>(q));
+        (int)(uint32_t)(uintptr_t)(__attribute__((address_space(3))) const char*)reinterpret_cast<const char*>(at));
   };
   // (as assembly, the waits below its own: for a DMA it sees the compiler would wait at every LDS read)
   auto dma = [&](const void* src, const void* dst) {
-    asm volatile("s_mov_b32 m0, %0\n s_nop 0\n global_load_lds_dwordx4 %1, off" ::"s"(lds_at(dst)), "v"(src) : "memory", "m0");
+    asm volatile("s_mov_b32 m0, %0\n s_nop 0\n global_load_lds_dwordx4 %1, off" ::"s"(lds_at(dst)), "v"(src)
+                 : "memory", "m0");
   };
   // DMA instruction d of this wave: x rows 4 (4 d + wave) .. + 3, weight rows 16 (4 d + wave) .. + 15
   const bf16_t* xsrc[FJ];
@@ -268,23 +289,18 @@ __global__ __launch_bounds__(256) void mx_matvec_wide_kernel(const bf16_t* __res
   }
   const uint8_t* ssrc = Ws + (int64_t)min(n0 + wave * 16 * FI + (lane & (16 * FI - 1)), N - 1) * ldws;
   const uint8_t* zeros = W + K / 2;  // a weight row's padding behind K, where K % 128 != 0
-  // the order of the stages: the chunks of class 0 (c % classes == 0), of class 1, ...
-  struct Place {
-    int cls, chunk, t, n;  // n: chunks begun so far
-  };
-  auto next = [&](Place& p) {
-    if (p.chunk * 4 + ++p.t < steps && p.t < 4) return;
-    p.t = 0;
-    ++p.n;
-    p.chunk += classes;
-    if (p.chunk >= chunks) p.chunk = ++p.cls;
-  };
-  Place fetch{0, 0, 0, 0}, at{0, 0, 0, 0};
-  auto issue = [&](int buf) {
-    if (fetch.cls >= classes) return;
-    u32x4_t* st = lds + buf * STAGE;
-    const int kt = fetch.chunk * 4 + fetch.t;
-    if (fetch.t == 0 && lane < 16 * FI) dma(ssrc + fetch.chunk * 16, sc + (fetch.n & 3) * TN + wave * 16 * FI);
+  // A stage: step i of this group's class of round r.  Behind the class's end its last step is loaded again
+  // (and not used): every stage is the same number of DMAs.
+  int fr = 0, fi = 0, fn = stages_of(0), fbuf = 0, fchunk = 0;  // the next to load
+  auto issue = [&]() {
+    if (fr >= rounds) return;
+    const int c = min(fr * G + q, classes - 1), chunk = min(c + (fi >> 2) * classes, chunks - 1);
+    const int kt = min(chunk * 4 + (fi & 3), steps - 1);
+    u32x4_t* st = ring + fbuf * STAGE;
+    if ((fi & 3) == 0) {
+      if (lane < 16 * FI) dma(ssrc + chunk * 16, sc + (fchunk & 3) * TN + wave * 16 * FI);
+      ++fchunk;
+    }
 #pragma unroll
     for (int d = 0; d < FJ; ++d) {
       const int k = kt * 128 + xk[d];
@@ -292,66 +308,90 @@ __global__ __launch_bounds__(256) void mx_matvec_wide_kernel(const bf16_t* __res
     }
 #pragma unroll
     for (int d = 0; d < FI; ++d) dma(wsrc[d] + kt * 64, st + XU + (d * 4 + wave) * 64);
-    next(fetch);
+    fbuf = fbuf + 1 == NBUF ? 0 : fbuf + 1;
+    if (++fi == fn) {
+      fi = 0;
+      fn = stages_of(++fr);
+    }
   };
 #pragma unroll
-  for (int b = 0; b < NBUF - 1; ++b) issue(b);
-  f32x4_t total[FI][FJ], acc[FI][FJ];
+  for (int b = 0; b < NBUF - 1; ++b) issue();
+  f32x4_t total[FI][FJ];
+  int buf = 0, chunk = -1;
+  for (int r = 0; r < rounds; ++r) {
+    f32x4_t acc[FI][FJ];
 #pragma unroll
-  for (int i = 0; i < FI; ++i)
+    for (int i = 0; i < FI; ++i)
 #pragma unroll
-    for (int j = 0; j < FJ; ++j) total[i][j] = acc[i][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-  int buf = 0;
-  for (int s = 0; s < steps; ++s) {
-    // this stage is here (behind it at most NBUF - 2 stages are on their way), and read by
-    // every wave is the one whose buffer is filled next
-    if (s + NBUF - 1 <= steps) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((NBUF - 2) * DMAS) : "memory");
-    else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-    // every operand is asked for before the next stage's DMAs and the first use: one LDS latency a stage
-    const u32x4_t* st = lds + buf * STAGE;
-    const uint32_t* s32 = reinterpret_cast<const uint32_t*>(sc + (at.n & 3) * TN);
-    u32x4_t w[FI];
-    uint32_t s4[FI];
-    bf16x8_t xf[4][FJ];
-#pragma unroll
-    for (int i = 0; i < FI; ++i) {
-      const int row = (wave * FI + i) * 16 + ql;
-      s4[i] = s32[row * 4 + g];
-      w[i] = st[XU + row * 4 + ((g ^ (row >> 2)) & 3)];
-    }
-#pragma unroll
-    for (int u = 0; u < 4; ++u)
-#pragma unroll
-      for (int j = 0; j < FJ; ++j)
-        xf[u][j] = __builtin_bit_cast(bf16x8_t, st[(j * 16 + ql) * 16 + ((u * 4 + g) ^ ql)]);
-    __builtin_amdgcn_sched_barrier(0);
-    issue(buf == 0 ? NBUF - 1 : buf - 1);
-    float scale[FI];
-#pragma unroll
-    for (int i = 0; i < FI; ++i) scale[i] = e8m0_to_f32((s4[i] >> (8 * at.t)) & 255);
-#pragma unroll
-    for (int u = 0; u < 4; ++u)
+      for (int j = 0; j < FJ; ++j) acc[i][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    const int mine = steps_of(r * G + q), n = stages_of(r);
+    for (int s = 0; s < n; ++s, --left) {
+      // this stage is here (behind it at most NBUF - 2 stages are on their way), and read by every wave is the
+      // one whose buffer is filled next
+      if (left >= NBUF - 1) asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"((NBUF - 2) * DMAS) : "memory");
+      else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+      const int t = s & 3;
+      if (t == 0) ++chunk;
+      // every operand is asked for before the next stage's DMAs and the first use: one LDS latency a stage
+      const u32x4_t* st = ring + buf * STAGE;
+      const uint32_t* s32 = reinterpret_cast<const uint32_t*>(sc + (chunk & 3) * TN);
+      u32x4_t w[FI];
+      uint32_t s4[FI];
+      bf16x8_t xf[4][FJ];
 #pragma unroll
       for (int i = 0; i < FI; ++i) {
-        const bf16x8_t wf = fp4_to_bf16(w[i][u], scale[i]);
-#pragma unroll
-        for (int j = 0; j < FJ; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wf, xf[u][j], acc[i][j], 0, 0, 0);
+        const int row = (wave * FI + i) * 16 + ql;
+        s4[i] = s32[row * 4 + g];
+        w[i] = st[XU + row * 4 + ((g ^ (row >> 2)) & 3)];
       }
-    const int cls = at.cls;
-    next(at);
-    if (at.cls != cls) {
 #pragma unroll
-      for (int i = 0; i < FI; ++i)
+      for (int u = 0; u < 4; ++u)
 #pragma unroll
-        for (int j = 0; j < FJ; ++j) {
-          total[i][j] = cls == 0 ? acc[i][j] : total[i][j] + acc[i][j];
-          acc[i][j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+        for (int j = 0; j < FJ; ++j)
+          xf[u][j] = __builtin_bit_cast(bf16x8_t, st[(j * 16 + ql) * 16 + ((u * 4 + g) ^ ql)]);
+      __builtin_amdgcn_sched_barrier(0);
+      issue();
+      buf = buf + 1 == NBUF ? 0 : buf + 1;
+      if (G > 1 && s >= mine) continue;  // the same for the wave
+      float scale[FI];
+#pragma unroll
+      for (int i = 0; i < FI; ++i) scale[i] = e8m0_to_f32((s4[i] >> (8 * t)) & 255);
+#pragma unroll
+      for (int u = 0; u < 4; ++u)
+#pragma unroll
+        for (int i = 0; i < FI; ++i) {
+          const bf16x8_t wf = fp4_to_bf16(w[i][u], scale[i]);
+#pragma unroll
+          for (int j = 0; j < FJ; ++j)
+            acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(wf, xf[u][j], acc[i][j], 0, 0, 0);
         }
     }
-    buf = buf + 1 == NBUF ? 0 : buf + 1;
+    // the round's classes in order, in group 0 (its next write of `part` lies behind the next stage's barrier)
+    if (G > 1) {
+      if (q > 0) {
+#pragma unroll
+        for (int i = 0; i < FI; ++i)
+#pragma unroll
+          for (int j = 0; j < FJ; ++j) part[q - 1][i * FJ + j][wave * 64 + lane] = acc[i][j];
+      }
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+      if (q > 0) continue;
+    }
+#pragma unroll
+    for (int i = 0; i < FI; ++i)
+#pragma unroll
+      for (int j = 0; j < FJ; ++j) {
+        total[i][j] = r == 0 ? acc[i][j] : total[i][j] + acc[i][j];
+#pragma unroll
+        for (int c = 1; c < G; ++c)
+          if (r * G + c < classes) total[i][j] += part[c - 1][i * FJ + j][wave * 64 + lane];
+      }
   }
+  if (q > 0) return;
 #pragma unroll
   for (int i = 0; i < FI; ++i) {
     const int n = n0 + (wave * FI + i) * 16 + 4 * g;
@@ -376,34 +416,33 @@ int launch(const void* x, int64_t ldx, const void* W, int64_t ldw, const void* W
   // the rows of x that fit in LDS, up to 16 (or 32); more rows in as many even passes over the weight
   auto fit = [&](int fj) { return std::min(16 * fj, (kLds - 2 * waves * fj * 1024) / x_stride(K)); };
   DITK_REQUIRE(fit(1) > 0, "ditk_mx_matvec: K=%d too long", K);
-  const int fj = waves > 1 && fit(2) > 0 && (M + fit(2) - 1) / fit(2) < (M + fit(1) - 1) / fit(1) ? 2 : 1;
-  const int passes = (M + fit(fj) - 1) / fit(fj), x_rows = (M + passes - 1) / passes;
+  const int fj = waves > 1 && fit(2) > 0 && (M - 1) / fit(2) < (M - 1) / fit(1) ? 2 : 1;
+  const int passes = (M - 1) / fit(fj) + 1;
+  DITK_REQUIRE(passes <= 65535, "ditk_mx_matvec: too many rows");  // and no more tiles
+  const int x_rows = (M + passes - 1) / passes;
   const int groups = (N + 15) / 16, lds = 2 * waves * fj * 1024 + x_rows * x_stride(K);
   const int per_cu = std::max(1, std::min(kWavesPerCu / waves, kLds / lds));
-  // Which kernel: the first streams the weight `passes` times, more slowly with fewer than some 12 waves on a CU; a
-  // tile of the wide one takes a 128-k step in 0.27 + 0.125 wj us, however few the tiles are, and many tiles stream
-  // the weight a little more slowly.  In us a 128-k step (measured around it: 16 x 5120 x 9216 18.5 us on the
-  // first, 19.1 on the wide, x 16384 26.9 and 19.8; 48 x 1536 x 5120 11.4 and 10.5; 1 x 1536 x 499712 81 and 88;
-  // 1 x 5120 x 131072 97 and 78; wrong by up to 20% at some, as 64 x 8960 x 5120, 46 and 55):
-  const int tall = (M + 63) / 64, wj = ((M + tall - 1) / tall + 15) / 16;
-  const float weight_us = (float)N / 68000.f;  // 128 k of the weight at 4.6 TB/s
-  const float first_us = weight_us * (float)passes * std::max(1.f, 12.f / (float)(per_cu * waves));
-  const float wide_us = std::max(0.27f + 0.125f * (float)wj, weight_us * 1.08f * (float)tall);
-  if (first_us > wide_us) {
-    // 64 features a tile until there is one of 128 a CU (48 x 1536 x 9216 10.6 and 13.4 us, 48 x 5120 x 65536
-    // 75 and 56)
-    const bool narrow = (int64_t)((N + 127) / 128) * tall <= ditk_cu_count();
+  // Which kernel, in us beyond the launch.  The first streams the weight `passes` times, more slowly with fewer than
+  // some 12 waves on a CU.  Tiles take a time for each 128 k, however few they are: of 64 features and two
+  // groups up to one tile a CU, beyond that of 128 and one.  (16 x 5120 x 9216 18.5 us on the first kernel and
+  // 16.7 on tiles, x 5120 12.6 and 16.4; 48 x 8960 x 5120 44 and 33, 48 x 5120 x 5120 18.6 and 22; 1 x 1536 x 499712
+  // 81 and 88, 1 x 5120 x 131072 97 and 76; wrong by 8% at 64 x 5120 x 5120, 28 and 26.)
+  const int steps = (K + 127) / 128, tall = (M + 63) / 64, wj = ((M + tall - 1) / tall + 15) / 16;
+  const bool narrow = (int64_t)((N + 63) / 64) * tall <= ditk_cu_count();
+  const float weight = (float)N / 68000.f;  // 128 k of the weight at 4.6 TB/s
+  const float first = 3.f + (float)steps * weight * (float)passes * std::max(1.f, 12.f / (float)(per_cu * waves));
+  const float tiles = narrow ? 4.5f + (float)steps * (0.22f + 0.065f * (float)wj)
+                             : 3.2f + (float)steps * std::max(0.3f + 0.12f * (float)wj, weight * 1.05f * (float)tall);
+  if (tiles < first) {
     const dim3 grid((unsigned)(narrow ? (N + 63) / 64 : (N + 127) / 128), (unsigned)tall);
-    DITK_REQUIRE(tall <= 65535, "ditk_mx_matvec: too many rows");
-    auto kern = wj == 1   ? (narrow ? mx_matvec_wide_kernel<EPI, 1, 1, 4> : mx_matvec_wide_kernel<EPI, 1, 2, 4>)
-                : wj == 2 ? (narrow ? mx_matvec_wide_kernel<EPI, 2, 1, 4> : mx_matvec_wide_kernel<EPI, 2, 2, 4>)
-                : wj == 3 ? (narrow ? mx_matvec_wide_kernel<EPI, 3, 1, 3> : mx_matvec_wide_kernel<EPI, 3, 2, 3>)
-                          : (narrow ? mx_matvec_wide_kernel<EPI, 4, 1, 3> : mx_matvec_wide_kernel<EPI, 4, 2, 3>);
-    kern<<<grid, 256, 0, stream>>>((const bf16_t*)x, ldx, (const uint8_t*)W, ldw, (const uint8_t*)Ws, ldws, bias, C, ldc,
-                                   M, N, K, (const bf16_t*)R, ldr, waves);
+    auto kern = wj == 1   ? (narrow ? mx_matvec_wide_kernel<EPI, 1, 1, 4, 2> : mx_matvec_wide_kernel<EPI, 1, 2, 4, 1>)
+                : wj == 2 ? (narrow ? mx_matvec_wide_kernel<EPI, 2, 1, 4, 2> : mx_matvec_wide_kernel<EPI, 2, 2, 4, 1>)
+                : wj == 3 ? (narrow ? mx_matvec_wide_kernel<EPI, 3, 1, 3, 2> : mx_matvec_wide_kernel<EPI, 3, 2, 3, 1>)
+                          : (narrow ? mx_matvec_wide_kernel<EPI, 4, 1, 3, 2> : mx_matvec_wide_kernel<EPI, 4, 2, 3, 1>);
+    kern<<<grid, narrow ? 512 : 256, 0, stream>>>((const bf16_t*)x, ldx, (const uint8_t*)W, ldw, (const uint8_t*)Ws, ldws,
+                                                  bias, C, ldc, M, N, K, (const bf16_t*)R, ldr, waves);
     return ditk_check_launch("ditk_mx_matvec");
   }
-  DITK_REQUIRE(passes <= 65535, "ditk_mx_matvec: too many rows");
   const dim3 grid((unsigned)std::min(groups, std::max(1, ditk_cu_count() * per_cu / passes)), (unsigned)passes);
   auto kern = fj == 1 ? mx_matvec_kernel<EPI, 1> : mx_matvec_kernel<EPI, 2>;
   kern<<<grid, 64 * waves, lds, stream>>>((const bf16_t*)x, ldx, (const uint8_t*)W, ldw, (const uint8_t*)Ws, ldws, bias,

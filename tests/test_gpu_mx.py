@@ -586,9 +586,10 @@ def test_matvec_rows_do_not_depend_on_the_batch():
 
 
 # more rows than LDS holds, or more features than the first kernel streams well: the kernel of tiles, 16 to 64
-# rows a tile, 64 or 128 features
+# rows a tile, 64 features (two groups of waves) or 128
 @pytest.mark.parametrize("M,N,K", [(3, 27016, 5120), (2, 33800, 4640), (30, 17000, 1568), (17, 33016, 1056),
-                                   (48, 9000, 8960), (40, 33000, 2432), (64, 9224, 5120), (100, 16648, 1056)])
+                                   (48, 9000, 8960), (40, 33000, 2432), (64, 9224, 5120), (100, 16648, 1056),
+                                   (11, 10008, 13856), (25, 9000, 8928), (64, 16000, 480)])
 @pytest.mark.parametrize("epi", ["gelu", "silu", "res", "f32"])
 def test_matvec_tiles(M, N, K, epi):
     x, w = strided(token_rows(M, K, M + K)), mx_random(N, K, N + K, "fp4")
@@ -618,15 +619,16 @@ def test_matvec_tiles(M, N, K, epi):
 
 
 def test_matvec_tiles_non_finite():
-    # 16 rows of a long K: a NaN block and a NaN row stay where they are, also in rows that end inside a 128-column step
+    # 16 rows of a long K, both tiles: a NaN block and a NaN row stay where they are, also in rows that end inside a 128-column step
     x, w = token_rows(16, 8736, 1), token_rows(16392, 8736, 2)
     w[16000, 8730] = math.nan
     x[7, 8735] = math.nan
-    got = mx.matvec(x, mx.quantize(w, "fp4"), epilogue="f32").isnan().cpu()
+    w4 = mx.quantize(w, "fp4")
     hit = torch.zeros((16, 16392), dtype=torch.bool)
     hit[7] = True
     hit[:, 16000] = True
-    assert torch.equal(got, hit)
+    assert torch.equal(mx.matvec(x, w4, epilogue="f32").isnan().cpu(), hit)
+    assert torch.equal(mx.matvec(x, w4[200:], epilogue="f32").isnan().cpu(), hit[:, 200:])
 
 
 def test_matvec_non_finite():

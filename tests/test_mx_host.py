@@ -58,7 +58,7 @@ def test_gemm_refuses(change, word):
 @pytest.mark.parametrize("change,word", [
     (dict(Ws=None), "null"), (dict(x=None), "null"), (dict(N=0), "shape"), (dict(K=48), "K=48"), (dict(N=4), "N=4"),
     (dict(ldw=48), "padding"), (dict(ldx=88), "padding"), (dict(x=A + 4), "aligned"), (dict(ldc=68), "ldc"),
-    (dict(epi=2), "epilogue"), (dict(epi=3), "residual"), (dict(M=65536 * 32), "rows"),
+    (dict(epi=2), "epilogue"), (dict(epi=3), "residual"), (dict(M=65536 * 32), "rows"), (dict(M=2**31 - 1), "rows"),
     (dict(K=81920, ldx=81920, ldw=40960, ldws=2560), "too long")])
 def test_matvec_refuses(change, word):
     refused("ditk_mx_matvec", tuple({**MV, **change}.values()), word)
