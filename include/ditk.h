@@ -428,7 +428,8 @@ int ditk_mx_gemm(const void* A, int64_t lda, const void* As, int64_t ldas, const
 /*
  * How ditk_mx_gemm runs an M x N x K product (unpadded strides), host only: rows
  * [0, plan[1]) on tile plan[0], the others on plan[2] (0: 256 x 256, 1: 128 x 256,
- * 2: 128 x 128, 3: 64 x 128, one wave per SIMD; 4, 5: 256 x 256 and 64 x 128, for short K).
+ * 2: 128 x 128, 3: 64 x 128, one wave per SIMD; 4, 5: 256 x 256 and 64 x 128, for short K;
+ * 6, 7: few rows, waves of 16 x 16 and 32 x 32).  For bf16 outputs; an MX output may differ.
  */
 int ditk_mx_gemm_plan(int M, int N, int K, int* plan);
 

@@ -411,10 +411,10 @@ def on_gpu(m):
 # every tile with rows and features that end inside it, one and several tiles a workgroup, K a multiple
 # of its steps of 128, of 512 and of neither, and launches split in two
 @pytest.mark.parametrize("shape,want", [
-    ((100, 1544, 416), (3, 100, 0)), ((63, 9992, 512), (3, 63, 0)), ((1000, 4616, 1056), None),
+    ((100, 4104, 416), (3, 100, 0)), ((63, 9992, 512), (3, 63, 0)), ((1000, 4616, 1056), None),
     ((520, 4616, 448), (2, 520, 0)), ((333, 8968, 1536), (2, 333, 0)), ((667, 7304, 2432), (1, 667, 0)),
-    ((2600, 4104, 640), None), ((2600, 8968, 512), None), ((4353, 4104, 1568), (0, 3840, 2)),
-    ((4600, 5128, 416), (0, 3072, 1)), ((2601, 4104, 384), (0, 2601, 0)), ((5000, 8200, 160), (0, 5000, 0)),
+    ((2600, 4104, 640), None), ((2600, 8968, 512), (0, 1792, 1)), ((4353, 4104, 1568), (0, 3840, 2)),
+    ((4600, 5128, 416), None), ((2601, 4104, 384), (0, 2601, 0)), ((5000, 8200, 160), (0, 5000, 0)),
     ((5000, 8200, 256), (0, 5000, 0)), ((2601, 4104, 128), (4, 2601, 0)), ((700, 4104, 288), (5, 700, 0)), ((9000, 2440, 3104), None), ((129, 24, 8960), None), ((300, 40, 14336), None)])
 @pytest.mark.parametrize("epi", ["gate_res", "gelu"])
 def test_linear_tiles(shape, want, epi):
@@ -445,6 +445,47 @@ def test_linear_tiles(shape, want, epi):
     norm = (out.double() - want64).norm()
     assert norm <= BF16_HALF / math.sqrt(3) * want64.norm() + 2.0 ** -13 * 1.13 * (slope * y).norm()
     assert (buf[M:] == 7).all() and (buf[:, :8] == 7).all() and (buf[:, 8 + N:] == 7).all()
+
+
+# Few rows, by single waves: bitwise the rows of a product of many, which the tiles compute (and the tests above
+# hold against 64 bits); rows and features that end inside a wave's, K of whole and broken chunks
+@pytest.mark.parametrize("M,N,K,want", [(1, 4128, 1568, 6), (9, 5152, 5088, 7), (5, 1568, 96, 6), (16, 9216, 1536, 6), (16, 1568, 14336, 6),
+                                        (19, 4128, 416, 7), (40, 1568, 8960, 7), (100, 1568, 512, 7),
+                                        (64, 1568, 544, 6), (33, 1544, 288, 6), (99, 1544, 288, 7), (1, 1544, 32, 6)])
+def test_linear_rows_by_waves(M, N, K, want):
+    assert mx_plan(M, N, K) == (want, M, 0) and mx_plan(800, N, K)[0] < 6
+    x, w = mx_random(M, K, M + K), mx_random(N, K, N + K + 1)
+    w.scales.view(torch.uint8).sub_(4)
+    many = mx.MXTensor.empty(800, K, DEV)
+    at = torch.arange(800, device=DEV) % M
+    many.data.view(torch.uint8).copy_(x.data.view(torch.uint8)[at])
+    many.scales.view(torch.uint8).copy_(x.scales.view(torch.uint8)[at])
+    g = gen(M)
+    b, gt = torch.randn(N, generator=g).to(DEV), torch.randn((4, N), generator=g).to(DEV)
+    res = strided(torch.randn((M, N), generator=g).to(DEV, torch.bfloat16))
+    more = torch.zeros((800, N), dtype=torch.bfloat16, device=DEV)
+    more[:M] = res
+    for epi in ("bias", "gelu", "silu", "res", "gate_res"):
+        few, all_ = {}, {}
+        if "res" in epi:
+            few, all_ = dict(residual=res), dict(residual=more)
+        if epi == "gate_res":
+            cu = [0, (M + 1) // 2, (M + 1) // 2, M]  # an empty segment; the other rows of `many` are the last
+            few.update(gate=gt, segments=ops.Segments(cu + [M], DEV))
+            all_.update(gate=gt, segments=ops.Segments(cu + [800], DEV))
+        buf = torch.full((M + 2, N + 24), 7.0, dtype=torch.bfloat16, device=DEV)
+        out = buf[:M, 8:8 + N]
+        mx.linear(x, w, b, epilogue=epi, out=out, **few)
+        assert torch.equal(out, mx.linear(many, w, b, epilogue=epi, **all_)[:M]), epi
+        assert (buf[M:] == 7).all() and (buf[:, :8] == 7).all() and (buf[:, 8 + N:] == 7).all()
+        if N % 32 == 0 and not few:
+            whole, q = poisoned(M, N)
+            mx.linear(x, w, b, epilogue=epi, out_fmt="fp8", out=q)
+            ref = mx.linear(many, w, b, epilogue=epi, out_fmt="fp8")
+            assert torch.equal(q.data.view(torch.uint8), ref.data[:M].view(torch.uint8))
+            assert torch.equal(q.scales.view(torch.uint8), ref.scales[:M].view(torch.uint8))
+            check_padding(q)
+            check_poison(whole, M)
 
 
 @pytest.mark.parametrize("M,N,K", [(1560, 8960, 512), (333, 4640, 1536), (700, 7328, 1056), (100, 1568, 416),
@@ -511,6 +552,16 @@ def test_linear_wide_row_strides():
     data = flat.as_strided((5, 1536), (stride, 1))
     data.copy_(x.data.view(torch.uint8))
     wide = mx.MXTensor("fp8", data.view(torch.float8_e4m3fn), x.scales, 1536)
+    assert torch.equal(mx.linear(wide, w), mx.linear(x, w))
+
+
+def test_linear_wide_row_strides_of_many_rows():
+    x, w = mx_random(300, 512, 1), mx_random(4104, 512, 2)
+    stride = (1 << 23) + 16
+    flat = torch.empty(300 * stride, dtype=torch.uint8, device=DEV)
+    data = flat.as_strided((300, 512), (stride, 1))
+    data.copy_(x.data.view(torch.uint8))
+    wide = mx.MXTensor("fp8", data.view(torch.float8_e4m3fn), x.scales, 512)
     assert torch.equal(mx.linear(wide, w), mx.linear(x, w))
 
 

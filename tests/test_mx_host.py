@@ -72,20 +72,23 @@ def plan(m, n, k):
 
 
 def test_plans():
-    """Few rows on small tiles, many on large ones, a short last round on smaller ones; both parts
-    of a split have rows, the first one whole tile rows."""
-    assert plan(16, 9216, 1536) == (3, 16, 0) and plan(512, 4608, 1536) == (2, 512, 0)
+    """Few rows by single waves, then on small tiles, many on large ones, a short last round on smaller
+    ones; both parts of a split have rows, the first one whole tile rows."""
+    assert plan(16, 9216, 1536) == (6, 16, 0) and plan(100, 1544, 416) == (7, 100, 0)
+    assert plan(130, 96, 128) == (6, 130, 0) and plan(128, 1536, 5120) == (7, 128, 0)
+    assert plan(64, 9216, 1536) == (3, 64, 0) and plan(512, 4608, 1536) == (2, 512, 0)
     assert plan(667, 7296, 2432) == (1, 667, 0) and plan(65520, 1536, 8960) == (0, 65520, 0)
-    assert plan(4096, 5120, 5120) == (0, 3072, 1)
+    assert plan(2600, 8968, 512) == (0, 1792, 1)
     assert plan(2600, 4096, 384) == (0, 2600, 0) and plan(2600, 4096, 128) == (4, 2600, 0)
-    assert plan(130, 96, 128) == (5, 130, 0)
+    assert plan(700, 4104, 288) == (5, 700, 0)
     heights = (256, 128, 128, 64)
     for m in (1, 63, 64, 65, 127, 500, 1560, 2560, 4097, 20000, 65520):
         for n in (8, 96, 1536, 5120, 13824):
             for k in (416, 1536, 5120, 14336):
                 tile, rows, rest = plan(m, n, k)
-                assert 0 <= tile < 4 and 0 <= rest < 4 and 0 < rows <= m
+                assert tile in (0, 1, 2, 3, 6, 7) and 0 <= rest < 4 and 0 < rows <= m
                 assert rows == m or rows % heights[tile] == 0
+    assert plan(2**31 - 1, 8, 32)[0] not in (6, 7) and plan(8, 2**31 - 8, 32)[0] not in (6, 7)  # their grids
     with pytest.raises(_lib.DitkError):
         plan(0, 64, 64)
 
