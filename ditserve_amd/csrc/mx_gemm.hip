@@ -948,11 +948,17 @@ DITK_EXPORT int ditk_mx_gemm(const void* A, int64_t lda, const void* As, int64_t
   }
 }
 
-DITK_EXPORT int ditk_mx_gemm_plan(int M, int N, int K, int* plan) {
-  DITK_REQUIRE(plan && M > 0 && N > 0 && N % 8 == 0 && K > 0 && K % 32 == 0, "ditk_mx_gemm_plan: bad arguments");
-  const MxPlan p = mx_plan_any(M, N, K, mx_cols(K), false);
+DITK_EXPORT int ditk_mx_gemm_plan_for(int M, int N, int K, int64_t row_stride, int out_kind, int* plan) {
+  DITK_REQUIRE(plan && M > 0 && N > 0 && N % 8 == 0 && K > 0 && K % 32 == 0 && row_stride >= mx_cols(K) &&
+                   (out_kind == MXO_BF16 || (out_kind == MXO_FP8 && N % 32 == 0)),
+               "ditk_mx_gemm_plan: bad arguments");
+  const MxPlan p = mx_plan_any(M, N, K, row_stride, out_kind == MXO_FP8);
   plan[0] = p.cfg;
   plan[1] = p.rows;
   plan[2] = p.rest;
   return 0;
+}
+
+DITK_EXPORT int ditk_mx_gemm_plan(int M, int N, int K, int* plan) {
+  return ditk_mx_gemm_plan_for(M, N, K, K > 0 ? mx_cols(K) : 0, MXO_BF16, plan);
 }

@@ -434,6 +434,12 @@ int ditk_mx_gemm(const void* A, int64_t lda, const void* As, int64_t ldas, const
 int ditk_mx_gemm_plan(int M, int N, int K, int* plan);
 
 /*
+ * The same for any call: row_stride is the largest row stride of A and W, in bytes (at least
+ * K rounded up to 128), out_kind as ditk_mx_gemm's.
+ */
+int ditk_mx_gemm_plan_for(int M, int N, int K, int64_t row_stride, int out_kind, int* plan);
+
+/*
  * C = epilogue(x W^T + bias) of bf16 rows x [M, K] and an fp4 MX matrix W [N, K],
  * K % 32 == 0, N % 8 == 0, for few rows: the weight is read once for up to 64 rows
  * (a smaller one more often, where that is faster).  A row has to fit into LDS: K up to about

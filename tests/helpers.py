@@ -55,3 +55,15 @@ def attn_items(tq, tk, nseg, heads, equal=False, joint=False):
     """Queries per work item (128 or 256) of an attention launch: host only."""
     from ditserve_amd import _lib
     return _lib.load().ditk_attn_item_queries(tq, tk, nseg, heads, equal, joint)
+
+
+def mx_gemm_plan(m, n, k, ld=None, mx_out=False, name="ditk_mx_gemm_plan_for"):
+    """(kernel, rows, rest) ditk_mx_gemm takes for an m x n x k product whose operands' longest row stride is ld
+    bytes: host only."""
+    import ctypes
+
+    from ditserve_amd import _lib
+    plan = (ctypes.c_int * 3)()
+    more = (ld or (k + 127) // 128 * 128, int(mx_out)) if name.endswith("for") else ()
+    _lib.call(name, m, n, k, *more, plan)
+    return tuple(plan)

@@ -2,7 +2,8 @@
 import pytest
 import torch
 
-from ditserve_amd import mx
+from ditserve_amd import mx, ops
+from tests.helpers import mx_gemm_plan
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -34,3 +35,120 @@ def test_more_rows_than_one_launch_dimension_holds(op, cols):
         for i in range(0, parts.shape[0], 1024):
             assert (parts[i:i + 1024] == ref).all(), i
         assert torch.equal(got[whole:], ref[:rows - whole])
+
+
+# ---------------------------------------------------------------------------------------------
+# linear: the kernels by shape and stride, each asserted
+# ---------------------------------------------------------------------------------------------
+
+def decode(m):
+    """(values over the scales, scales of each value) of an fp8 MX matrix in 64 bits, from its bytes, on the GPU."""
+    data, scales = (t.long() for t in raw(m))
+    e, f, sign = data >> 3 & 15, (data & 7).double() / 8, 1 - 2 * (data >> 7).double()
+    v = sign * torch.where(e > 0, (1 + f) * torch.exp2((e - 7).double()), f * 2.0 ** -6)
+    place = [16 * (i // 16) + 4 * (i % 4) + (i % 16) // 4 for i in range(m.cols // 32)]  # block i's byte
+    return v[:, :m.cols], torch.exp2((scales[:, place] - 127).double()).repeat_interleave(32, 1)
+
+
+def operand(rows, cols, seed, sub=0, pad=0):
+    """MX rows of random values (scales lowered by 2^sub); pad: bytes behind each row of both tensors."""
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    x = torch.randn((rows, cols), generator=g, device=DEV) * torch.exp(torch.randn((rows, 1), generator=g, device=DEV))
+    q = mx.quantize(x.to(torch.bfloat16))
+    raw(q)[1].sub_(sub)
+    return q if not pad else in_rows(q, q.data.shape[1] + pad, q.scales.shape[1] + pad)
+
+
+def in_rows(q, data_stride, scale_stride):
+    """The same matrix with row strides of its own."""
+    parts = []
+    for t, stride in zip(raw(q), (data_stride, scale_stride)):
+        view = torch.empty(t.shape[0] * stride, dtype=torch.uint8, device=DEV).as_strided(t.shape, (stride, 1))
+        parts.append(view.copy_(t))
+    return mx.MXTensor("fp8", parts[0].view(torch.float8_e4m3fn), parts[1].view(torch.float8_e8m0fnu), q.cols)
+
+
+def gated(M, N, seed):
+    """Residual, gate and segments: an empty one, and ends inside tiles."""
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    cu = [0, 1, 1, M // 3, M]
+    return dict(epilogue="gate_res", residual=torch.randn((M, N), generator=g, device=DEV).to(torch.bfloat16),
+                gate=torch.randn((4, N), generator=g, device=DEV), segments=ops.Segments(cu, DEV))
+
+
+def same(a, b):
+    if isinstance(a, mx.MXTensor):
+        return all(torch.equal(x, y) for x, y in zip(raw(a), raw(b)))
+    return torch.equal(a.view(torch.int16), b.view(torch.int16))
+
+
+WIDE = (1 << 23) + 16  # 256 rows of it pass 2^31 bytes
+
+
+@pytest.mark.parametrize("mx_out", [False, True])
+@pytest.mark.parametrize("M,N,K,wide,kernel", [(333, 1568, 1056, "x", 5), (1560, 320, 2464, "x", 5), (1300, 1568, 608, "w", 5),
+                                               (4200, 2016, 1056, "w", 4), (4353, 2016, 672, "w", 4)])
+def test_linear_wide_strides_of_long_k(M, N, K, wide, kernel, mx_out):
+    """More than four stages of 128 k (both scale buffers) in the kernels with 64-bit addresses, bitwise the packed
+    product's results, which other kernels compute."""
+    x, w = operand(M, K, M + K), operand(N, K, N + K, 4)
+    b = torch.randn(N, generator=torch.Generator(device=DEV).manual_seed(M), device=DEV)
+    kw = dict(epilogue="gelu", out_fmt="fp8") if mx_out else gated(M, N, K)
+    assert mx_gemm_plan(M, N, K, WIDE, mx_out) == (kernel, M, 0) and mx_gemm_plan(M, N, K, mx_out=mx_out)[0] not in (4, 5)
+    want = mx.linear(x, w, b, **kw)
+    wx, ww = (in_rows(q, WIDE, q.scales.shape[1] + 32) if name == wide else q for q, name in ((x, "x"), (w, "w")))
+    assert same(mx.linear(wx, ww, b, **kw), want)
+
+
+@pytest.mark.parametrize("M,N,K,plan", [
+    (9000, 120, 1536, (3, 9000, 0)), (5000, 120, 448, (3, 5000, 0)), (5000, 96, 448, (3, 5000, 0)),
+    (20000, 64, 1536, (2, 20000, 0)), (20000, 8, 2432, (2, 20000, 0)), (20000, 96, 672, (2, 20000, 0)),
+    (40000, 200, 1536, (0, 40000, 0)), (70000, 200, 416, (0, 65536, 3)), (33000, 160, 160, (0, 33000, 0)),
+    (25000, 200, 416, (1, 25000, 0)), (18000, 224, 672, (1, 18000, 0))])
+def test_linear_tiles_wider_than_the_matrix(M, N, K, plan):
+    """Tiles of the one-wave-per-SIMD kernel that reach past N: weight rows, scales, bias and gate behind the last
+    feature are not read, outputs behind it not written.  Against 64 bits, and bitwise against a few of the
+    rows alone, which single waves compute."""
+    assert mx_gemm_plan(M, N, K) == plan
+    x, w = operand(M, K, M + K, pad=64), operand(N, K, N + K, 4, pad=32)
+    b = torch.randn(N, generator=torch.Generator(device=DEV).manual_seed(M), device=DEV)
+    kw = gated(M, N, K)
+    buf = torch.full((M + 2, N + 24), 7.0, dtype=torch.bfloat16, device=DEV)
+    out = mx.linear(x, w, b, out=buf[:M, 8:8 + N], **kw)
+    assert (buf[M:] == 7).all() and (buf[:, :8] == 7).all() and (buf[:, 8 + N:] == 7).all()
+    (xv, xs), (wv, ws) = decode(x), decode(w)
+    y = torch.mm(xv * xs, (wv * ws).T) + b.double()
+    # Of the products of 8 consecutive k the instruction keeps 13 bits below the largest sum of two factors' exponents, a
+    # subnormal factor's being that of 2^-6: 8 * 2^-13 of it a group, taken as the sum of all; and 17 additions
+    # with 24 bits for each 128 k.
+    least = [torch.where(v == 0, 0.0, v.abs().clamp_min(2.0 ** -6)) * s for v, s in ((xv, xs), (wv, ws))]
+    acc = (8 * 2.0 ** -13 + (K + 127) // 128 * 17 * 2.0 ** -23) * torch.mm(least[0], least[1].T)
+    seg = torch.bucketize(torch.arange(M, device=DEV), torch.tensor(kw["segments"].cu[1:], device=DEV), right=True)
+    gate = kw["gate"].double()[seg]
+    want = kw["residual"].double() + y * gate
+    err = (out.double() - want).abs()
+    assert (err <= 2.0 ** -8 * want.abs() + gate.abs() * (acc + 2.0 ** -22 * y.abs())).all()
+    # in norm, where errors do not add up: uniform roundings to bf16, and 2^-15 of the magnitudes (1.6e-5 on random data)
+    mag = torch.mm((xv * xs).abs(), (wv * ws).abs().T)
+    assert (out.double() - want).norm() <= 2.0 ** -8 / 3 ** 0.5 * want.norm() + 2.0 ** -15 * (gate * mag).norm()
+    rows = [0, 1, M // 3 - 1, M // 3, M // 2, M - 17]
+    few = {i: mx.linear(x[i:i + 1], w, b) for i in rows}
+    all_ = mx.linear(x, w, b)
+    for i in rows:
+        assert mx_gemm_plan(1, N, K)[0] in (6, 7) and same(all_[i:i + 1], few[i])
+    if N % 32 == 0:
+        whole = mx.MXTensor.empty(M + 2, N, DEV)
+        for t in raw(whole):
+            t.fill_(0xAA)
+        got = mx.linear(x, w, b, epilogue="silu", out_fmt="fp8", out=whole[:M])
+        assert all((t[M:] == 0xAA).all() for t in raw(whole))
+        data, scales = raw(got)
+        assert (data[:, N:] == 0).all()
+        pad = [i for i in range(scales.shape[1]) if 16 * (i // 16) + 4 * (i % 4) + (i % 16) // 4 >= N // 32]
+        assert (scales[:, pad] == 127).all()
+        v, s = decode(got)
+        z = y * torch.sigmoid(y)
+        off = 1.13 * (acc + 2.0 ** -20 * y.abs())  # SiLU's slope is up to 1.1
+        assert ((v * s - z).abs() <= 2.0 ** -4 * z.abs() + s * 2.0 ** -10 + 1.25 * off).all()
+        for i in rows:
+            assert same(got[i:i + 1], mx.linear(x[i:i + 1], w, b, epilogue="silu", out_fmt="fp8"))
