@@ -361,8 +361,11 @@ __global__ __launch_bounds__(WM * WN * 64, EU) void mx_gemm_kernel(MxGemmArgs p)
   uint32_t sw[FI], sx[FJ];
   auto stage = [&](int kt, auto sel) {
     constexpr int S = decltype(sel)::value;
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __builtin_amdgcn_s_barrier();  // stage kt is here for every wave; the other buffer is read out
+    // stage kt is here for every wave, and the other buffer is read out: this wave's reads of it have landed too (the
+    // MFMAs that wait for them are not held before the barrier by anything)
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
     if (kt + 1 < nk) issue(kt + 1);
     if (S == 0) {
       const uint32_t* s32 = reinterpret_cast<const uint32_t*>(sc_lds + ((kt >> 2) & 1) * ROWS);
