@@ -12,26 +12,28 @@ namespace {
 constexpr int kRowsPerBlock = 4;  // 4 waves, one row (or 512 columns of one) each
 constexpr int kMaxChunks = 12;    // 16-byte chunks per lane -> D <= 64 * 8 * 12 = 6144
 
-// A grid's first dimension holds less than 2^32 threads (more wrap around, and no error is reported): workgroups past
-// 2^22 of 256 go on in the second, and those past the last row return.
-constexpr int64_t kGridX = 1ll << 22, kMaxBlocks = kGridX * 65535;
-dim3 row_grid(int64_t blocks) {
-  return dim3((unsigned)(blocks < kGridX ? blocks : kGridX), (unsigned)((blocks + kGridX - 1) / kGridX));
-}
-// this wave's number among the grid's
-__device__ __forceinline__ int64_t wave_id() {
-  return ((int64_t)blockIdx.y * gridDim.x + blockIdx.x) * kRowsPerBlock + (threadIdx.x >> 6);
+// A grid's first dimension holds less than 2^32 threads (more wrap around, and no error is reported): it takes the
+// rows of 2^24 waves at most, `rows` of them, and the second dimension the next.
+struct RowGrid {
+  dim3 grid;
+  int rows;
+};
+constexpr int kMaxGridY = 65535;
+RowGrid row_grid(int T, int waves_per_row) {
+  const int most = (1 << 24) / waves_per_row, rows = T < most ? T : most;
+  const int waves = rows * waves_per_row;
+  return RowGrid{dim3((unsigned)((waves + kRowsPerBlock - 1) / kRowsPerBlock), (unsigned)((T - 1) / rows + 1)), rows};
 }
 
 template <int FMT>
 __global__ __launch_bounds__(256) void mx_quantise_kernel(const bf16_t* __restrict__ x, int64_t ldx,
                                                           uint8_t* __restrict__ data, int64_t ldd,
-                                                          uint8_t* __restrict__ scales, int64_t lds, int64_t units,
+                                                          uint8_t* __restrict__ scales, int64_t lds, int T, int rows,
                                                           int per_row, int nchunk) {
-  const int64_t u = wave_id();
-  if (u >= units) return;
-  const int64_t row = u / per_row;
-  const int c = (int)(u % per_row) * 64 + (threadIdx.x & 63);
+  const uint32_t u = blockIdx.x * kRowsPerBlock + (threadIdx.x >> 6), part = u / (uint32_t)per_row;
+  const int64_t row = (int64_t)blockIdx.y * rows + part;
+  if (part >= (uint32_t)rows || row >= T) return;
+  const int c = (int)(u - part * (uint32_t)per_row) * 64 + (threadIdx.x & 63);
   const u32x4_t raw = c < nchunk ? *reinterpret_cast<const u32x4_t*>(x + row * ldx + c * 8) : u32x4_t{0, 0, 0, 0};
   float v[8];
   unpack8(raw, v);
@@ -46,7 +48,8 @@ __global__ __launch_bounds__(256) void mx_norm_kernel(
     int64_t ldd, uint8_t* __restrict__ scales, int64_t lds, int T, int D, const int32_t* __restrict__ cu, int nseg,
     const float* __restrict__ shift, const float* __restrict__ scale, int64_t mod_stride, const float* __restrict__ w,
     const float* __restrict__ b, float eps) {
-  const int64_t at = wave_id();
+  // (whole workgroups in the first dimension: its rows are a multiple of theirs, or all)
+  const int64_t at = (int64_t)blockIdx.y * (1 << 24) + blockIdx.x * kRowsPerBlock + (threadIdx.x >> 6);
   if (at >= T) return;
   const int row = (int)at;
   const int lane = threadIdx.x & 63;
@@ -168,11 +171,11 @@ DITK_EXPORT int ditk_mx_quantize(const void* x, int64_t ldx, void* data, int64_t
   DITK_REQUIRE(ldx % 8 == 0 && ldx >= K && ((uintptr_t)x % 16) == 0, "ditk_mx_quantize: x rows must be 16-byte aligned");
   if (T == 0) return 0;
   const int per_row = (K + 511) / 512;
-  const int64_t units = (int64_t)T * per_row, blocks = (units + kRowsPerBlock - 1) / kRowsPerBlock;
-  DITK_REQUIRE(blocks <= kMaxBlocks, "ditk_mx_quantize: too many rows");
+  const RowGrid g = row_grid(T, per_row);
+  DITK_REQUIRE(g.grid.y <= kMaxGridY, "ditk_mx_quantize: too many rows");
   auto kern = fmt == MX_FP8 ? mx_quantise_kernel<MX_FP8> : mx_quantise_kernel<MX_FP4>;
-  kern<<<row_grid(blocks), 256, 0, stream>>>((const bf16_t*)x, ldx, (uint8_t*)data, ldd, (uint8_t*)scales, lds, units,
-                                             per_row, K / 8);
+  kern<<<g.grid, 256, 0, stream>>>((const bf16_t*)x, ldx, (uint8_t*)data, ldd, (uint8_t*)scales, lds, T, g.rows, per_row,
+                                   K / 8);
   return ditk_check_launch("ditk_mx_quantize");
 }
 
@@ -196,7 +199,7 @@ DITK_EXPORT int ditk_mx_norm(const void* x, int64_t ldx, const void* residual, i
                    ((uintptr_t)bias % 16) == 0,
                "ditk_mx_norm: vectors must be 16-byte aligned");
   if (T == 0) return 0;
-  const dim3 grid = row_grid(((int64_t)T + kRowsPerBlock - 1) / kRowsPerBlock);
+  const dim3 grid = row_grid(T, 1).grid;
 #define DITK_MXN(K, NCV)                                                                                         \
   mx_norm_kernel<K, NCV><<<grid, 256, 0, stream>>>((const bf16_t*)x, ldx, (const bf16_t*)residual, ldr, (bf16_t*)h, \
                                                    ldh, (uint8_t*)data, ldd, (uint8_t*)scales, lds, T, D, cu_seqlens, \
