@@ -19,6 +19,10 @@ enum MxFmt : int { MX_FP8 = 0, MX_FP4 = 1 };
 typedef __attribute__((__vector_size__(8 * sizeof(int)))) int i32x8_t;
 typedef __attribute__((__vector_size__(2 * sizeof(short)))) short s16x2_t;
 
+// The longest row, and the most rows of a product's output: column and row numbers of whole tiles past the last one
+// stay below 2^31.
+constexpr int kMxMaxCols = 1 << 30, kMxMaxRows = 0x70000000;
+
 // columns a row of K holds with its padding, and bytes of its scales
 __host__ __device__ inline int64_t mx_cols(int64_t K) { return (K + 127) / 128 * 128; }
 __host__ __device__ inline int64_t mx_scale_bytes(int64_t K) { return (K + 511) / 512 * 16; }

@@ -622,7 +622,7 @@ int launch(MxGemmArgs p, hipStream_t stream) {
   p.tiles_n = (p.N + GBN - 1) / GBN;
   p.group_m = mx_group_m(p.K, p.tiles_n);
   const int64_t blocks = ((int64_t)p.tiles_m * p.tiles_n + 7) / 8 * 8;
-  DITK_REQUIRE(blocks < (1ll << 31), "ditk_mx_gemm: grid too large");
+  DITK_REQUIRE(blocks * (WM * WN * 64) < (1ll << 32), "ditk_mx_gemm: grid too large");
   mx_gemm_kernel<EPI, OUT, FI, FJ, WM, WN, EU><<<(unsigned)blocks, WM * WN * 64, 0, stream>>>(p);
   return ditk_check_launch("ditk_mx_gemm");
 }
@@ -805,7 +805,7 @@ constexpr MxCfg kCfg[kCfgs] = {{256, 256, -2.4f, 10.1f, 1.067f}, {128, 256, 0.5f
 
 float cfg_us(int c, int64_t tiles, int K, int cus) {
   const int64_t rounds = (tiles + cus - 1) / cus;
-  return kCfg[c].start + (float)rounds * (kCfg[c].tile + kCfg[c].stage * (float)((K + 127) / 128));
+  return kCfg[c].start + (float)rounds * (kCfg[c].tile + kCfg[c].stage * (float)((K - 1) / 128 + 1));
 }
 
 // How a product runs: rows [0, rows) on tiles of configuration cfg, the others on `rest` in a second
@@ -821,7 +821,7 @@ constexpr float kSplitGain = 0.9f;
 MxPlan plan_one(int M, int N, int K, int cus) {
   MxPlan best{0, M, 0, 1e30f};
   for (int c = 0; c < kCfgs; ++c) {
-    const int64_t tiles = (int64_t)((M + kCfg[c].gbm - 1) / kCfg[c].gbm) * ((N + kCfg[c].gbn - 1) / kCfg[c].gbn);
+    const int64_t tiles = ((int64_t)(M - 1) / kCfg[c].gbm + 1) * ((N - 1) / kCfg[c].gbn + 1);
     const float us = cfg_us(c, tiles, K, cus);
     if (us < best.us) best = MxPlan{c, M, 0, us};
   }
@@ -832,7 +832,7 @@ MxPlan mx_plan(int M, int N, int K) {
   const MxPlan one = plan_one(M, N, K, cus);
   MxPlan best = one;
   for (int c = 0; c < kCfgs; ++c) {
-    const int64_t tn = (N + kCfg[c].gbn - 1) / kCfg[c].gbn, tm = (M + kCfg[c].gbm - 1) / kCfg[c].gbm;
+    const int64_t tn = (N - 1) / kCfg[c].gbn + 1, tm = (M - 1) / kCfg[c].gbm + 1;
     const int64_t main_m = tm * tn / cus * cus / tn;  // tile rows of the full rounds
     if (main_m == 0 || main_m >= tm || tm * tn % cus == 0) continue;
     const int rows = (int)main_m * kCfg[c].gbm;
@@ -864,7 +864,7 @@ constexpr RowsCfg kRowsCfg[3] = {{16, 16, 2.1f, 0.02f, 0.55f, 0.132f},
                                  {32, 32, 2.8f, 0.02f, 0.9f, 0.24f}};
 float rows_us(const RowsCfg& c, int M, int N, int K, int cus) {
   const int64_t waves = (int64_t)((M - 1) / c.gbm + 1) * ((N - 1) / c.gbn + 1), rounds = (waves + cus - 1) / cus;
-  const float steps = (float)((K + 127) / 128);
+  const float steps = (float)((K - 1) / 128 + 1);
   // (more rounds than this are the tiles' business, and their grid is not checked)
   return rounds > 8 ? 1e30f : c.start + c.step * steps + (float)rounds * (c.wave + c.stage * steps);
 }
@@ -872,9 +872,9 @@ MxPlan mx_plan_any(int M, int N, int K, int64_t ld, bool mx_out) {
   const int cus = ditk_cu_count();
   const float r16 = rows_us(kRowsCfg[mx_out ? 1 : 0], M, N, K, cus), r32 = rows_us(kRowsCfg[2], M, N, K, cus);
   const float rows = std::min(r16, r32);
-  if (rows < 1e30f && rows < mx_plan(M, N, K).us + kCold * (float)((K + 127) / 128))
+  if (rows < 1e30f && rows < mx_plan(M, N, K).us + kCold * (float)((K - 1) / 128 + 1))
     return MxPlan{r16 <= r32 ? kRows16 : kRows32, M, 0, rows};
-  const bool l4 = 256 * ld < (1ll << 31), large = (int64_t)((M + 255) / 256) * ((N + 255) / 256) >= 128;
+  const bool l4 = 256 * ld < (1ll << 31), large = ((int64_t)(M - 1) / 256 + 1) * ((N - 1) / 256 + 1) >= 128;
   if (l4 && K > 384) return mx_plan(M, N, K);
   return MxPlan{!large ? kPlainSmall : l4 && K > 128 ? 0 : kPlainLarge, M, 0, 0.f};
 }
@@ -912,6 +912,7 @@ DITK_EXPORT int ditk_mx_gemm(const void* A, int64_t lda, const void* As, int64_t
   DITK_REQUIRE(W && Ws && (M == 0 || (A && As && C)), "ditk_mx_gemm: null operand");
   DITK_REQUIRE(M >= 0 && N > 0 && K > 0, "ditk_mx_gemm: bad shape M=%d N=%d K=%d", M, N, K);
   DITK_REQUIRE(K % 32 == 0 && N % 8 == 0, "ditk_mx_gemm: K=%d must be a multiple of 32, N=%d of 8", K, N);
+  DITK_REQUIRE(M <= kMxMaxRows && K <= kMxMaxCols, "ditk_mx_gemm: too many rows (M=%d) or K=%d too long", M, K);
   DITK_REQUIRE(lda % 16 == 0 && ldw % 16 == 0 && lda >= mx_cols(K) && ldw >= mx_cols(K) && ldas % 16 == 0 &&
                    ldws % 16 == 0 && ldas >= mx_scale_bytes(K) && ldws >= mx_scale_bytes(K),
                "ditk_mx_gemm: operand rows need their padding and 16-byte strides");

@@ -154,6 +154,7 @@ int mx_out_check(const char* what, const void* data, int64_t ldd, const void* sc
                  int fmt) {
   DITK_REQUIRE(T == 0 || (data && scales), "%s: null MX output", what);
   DITK_REQUIRE(K > 0 && K % 32 == 0, "%s: %d columns are not blocks of 32", what, K);
+  DITK_REQUIRE(K <= kMxMaxCols, "%s: %d columns are too long", what, K);
   DITK_REQUIRE(ldd % 16 == 0 && ldd >= mx_cols(K) >> (fmt == MX_FP4) && lds % 16 == 0 && lds >= mx_scale_bytes(K),
                "%s: MX rows need their padding and 16-byte strides", what);
   DITK_REQUIRE(((uintptr_t)data % 16) == 0 && ((uintptr_t)scales % 16) == 0,

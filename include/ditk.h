@@ -393,7 +393,7 @@ int ditk_flash_attn_varlen_noalloc(const void* q, int64_t ldq, const void* k, in
  * data, scales = MX of x [T, K] bf16, K % 32 == 0: per block
  * e = max(ceil(log2(amax / vmax)), -126), vmax 448 (fp8) or 6 (fp4), values
  * rounded to nearest even.  A block with an infinity or NaN gets the scale NaN
- * (and, in fp8, NaN values).
+ * (and, in fp8, NaN values).  K up to 2^30.
  */
 int ditk_mx_quantize(const void* x, int64_t ldx, void* data, int64_t ldd, void* scales, int64_t lds, int T, int K,
                      int fmt, ditk_stream_t stream);
@@ -413,12 +413,12 @@ int ditk_mx_norm(const void* x, int64_t ldx, const void* residual, int64_t ldr, 
 /*
  * C = epilogue(A W^T + bias) of fp8 MX matrices A [M, K] and W [N, K], K % 32 == 0,
  * N % 8 == 0; fp32 accumulators (the matrix instruction's own sums keep 13 bits below the
- * largest of 8 products), one rounding at the end.  epilogue 0 bias, 1 GELU-tanh, 2 R + y * gate[seg], 3 R + y, 5 SiLU (as ditk_gemm's, which also
- * rounds before the activation or residual).  out_kind 0: C bf16 [M, N], ldc in
- * elements, ldc % 8 == 0, may be R itself.  out_kind 1 (epilogues 0, 1, 5; N % 32 ==
- * 0): C, Cs the fp8 MX matrix of the result, padding included.  Output and residual row
- * strides below 2^22.  Every row is computed the same way whatever M is and wherever it
- * sits.
+ * largest of 8 products), one rounding at the end.  epilogue 0 bias, 1 GELU-tanh,
+ * 2 R + y * gate[seg], 3 R + y, 5 SiLU (as ditk_gemm's, which also rounds before the
+ * activation or residual).  out_kind 0: C bf16 [M, N], ldc in elements, ldc % 8 == 0, may
+ * be R itself.  out_kind 1 (epilogues 0, 1, 5; N % 32 == 0): C, Cs the fp8 MX matrix of the
+ * result, padding included.  Output and residual row strides below 2^22, M up to 1.8e9, K up
+ * to 2^30.  Every row is computed the same way whatever M is and wherever it sits.
  */
 int ditk_mx_gemm(const void* A, int64_t lda, const void* As, int64_t ldas, const void* W, int64_t ldw, const void* Ws,
                  int64_t ldws, const float* bias, void* C, int64_t ldc, void* Cs, int64_t ldcs, int M, int N, int K,

@@ -47,3 +47,33 @@ def test_plan_refusals():
     for bad in (dict(m=0), dict(n=12), dict(k=40), dict(ld=96), dict(n=24, mx_out=True)):
         with pytest.raises(_lib.DitkError, match="bad arguments"):
             mx_gemm_plan(**{**dict(m=4, n=64, k=128), **bad})
+
+
+HOST = dict(A=0x10000, lda=128, As=0x20000, ldas=16, W=0x30000, ldw=128, Ws=0x40000, ldws=16, bias=None, C=0x50000,
+            ldc=64, Cs=None, ldcs=0, M=4, N=64, K=96, epi=0, out=0, R=None, ldr=0, gate=None, gs=0, cu=None, nseg=0,
+            stream=None)  # addresses only
+
+
+@pytest.mark.parametrize("change,word", [(dict(M=2**31 - 1), "rows"), (dict(M=2**31 - 2**28 + 1), "rows"),
+                                         (dict(K=2**31 - 32, lda=1 << 31, ldw=1 << 31, ldas=1 << 26, ldws=1 << 26), "long"),
+                                         (dict(K=2**30 + 32, lda=1 << 31, ldw=1 << 31, ldas=1 << 26, ldws=1 << 26), "long")])
+def test_product_refuses_sizes_near_2_31(change, word):
+    lib = _lib.load()
+    assert lib.ditk_mx_gemm(*{**HOST, **change}.values()) == 1
+    assert word in lib.ditk_last_error().decode(), lib.ditk_last_error()
+
+
+@pytest.mark.parametrize("K", [2**31 - 32, 2**30 + 32])
+def test_quantize_refuses_rows_near_2_31(K):
+    lib = _lib.load()
+    assert lib.ditk_mx_quantize(0x10000, 1 << 31, 0x20000, 1 << 31, 0x30000, 1 << 26, 1, K, 0, None) == 1
+    assert "too long" in lib.ditk_last_error().decode(), lib.ditk_last_error()
+
+
+def test_plans_near_2_31():
+    """Row, feature and column counts are multiplied and rounded up past 31 bits."""
+    for m, n, k in ((2**31 - 1, 8, 512), (2**31 - 1, 264, 32), (8, 2**31 - 8, 512), (2**31 - 1, 2**31 - 8, 1536)):
+        assert mx_gemm_plan(m, n, k)[0] not in (6, 7), (m, n, k)
+    assert mx_gemm_plan(2**31 - 1, 264, 32) == (4, 2**31 - 1, 0)
+    # the longest rows: no fewer steps than those of half the length
+    assert mx_gemm_plan(16, 64, 2**31 - 32)[0] == mx_gemm_plan(16, 64, 2**30)[0]
