@@ -517,19 +517,19 @@ __global__ __launch_bounds__(256, 1) void mx_gemm_l4(MxGemmArgs p) {
   if constexpr (FI == 8 && FJ == 8)
     asm volatile(
 #include "mx_l4_256x256_start.inc"
-        : : DITK_MX_L4_START_OPERANDS : DITK_MX_L4_256X256_CLOBBERS "scc", "memory");
+        : : DITK_MX_L4_START_OPERANDS : DITK_MX_L4_256X256_CLOBBERS "m0", "scc", "memory");
   else if constexpr (FI == 8 && FJ == 4)
     asm volatile(
 #include "mx_l4_128x256_start.inc"
-        : : DITK_MX_L4_START_OPERANDS : DITK_MX_L4_128X256_CLOBBERS "scc", "memory");
+        : : DITK_MX_L4_START_OPERANDS : DITK_MX_L4_128X256_CLOBBERS "m0", "scc", "memory");
   else if constexpr (FI == 4 && FJ == 4)
     asm volatile(
 #include "mx_l4_128x128_start.inc"
-        : : DITK_MX_L4_START_OPERANDS : DITK_MX_L4_128X128_CLOBBERS "scc", "memory");
+        : : DITK_MX_L4_START_OPERANDS : DITK_MX_L4_128X128_CLOBBERS "m0", "scc", "memory");
   else
     asm volatile(
 #include "mx_l4_64x128_start.inc"
-        : : DITK_MX_L4_START_OPERANDS : DITK_MX_L4_64X128_CLOBBERS "scc", "memory");
+        : : DITK_MX_L4_START_OPERANDS : DITK_MX_L4_64X128_CLOBBERS "m0", "scc", "memory");
   }
   uint32_t buf = 0, scb = 0;  // LDS offsets of the next tile's stage 0 and scale group 0
   int par = 0;                // this tile's bias and gate in LDS
@@ -542,7 +542,8 @@ __global__ __launch_bounds__(256, 1) void mx_gemm_l4(MxGemmArgs p) {
     const int vrow = (wave % (GBN / 64)) * 64;
     auto fetch = [&](const float* src, int at) {
       const uint32_t m0v = su(lds0 + G::VEC0 + at * 1024 + vrow * 4), off = (uint32_t)min(tile.nb + vrow + lane_id(), p.N - 1) * 4;
-      asm volatile("s_mov_b32 m0, %0\n s_nop 0\n global_load_lds_dword %1, %2" ::"s"(m0v), "v"(off), "s"(src) : "memory");
+      asm volatile("s_mov_b32 m0, %0\n s_nop 0\n global_load_lds_dword %1, %2" ::"s"(m0v), "v"(off), "s"(src)
+                   : "m0", "memory");
     };
     uint64_t has_bias = (uint64_t)(uintptr_t)p.bias;  // compared where it is used, as lane_id()
     asm volatile("" : "+s"(has_bias));
@@ -563,24 +564,24 @@ __global__ __launch_bounds__(256, 1) void mx_gemm_l4(MxGemmArgs p) {
             "=&{a[48:63]}"(c[3]), "=&{a[64:79]}"(c[4]), "=&{a[80:95]}"(c[5]), "=&{a[96:111]}"(c[6]), "=&{a[112:127]}"(c[7]),
             "=&{a[128:143]}"(c[8]), "=&{a[144:159]}"(c[9]), "=&{a[160:175]}"(c[10]), "=&{a[176:191]}"(c[11]),
             "=&{a[192:207]}"(c[12]), "=&{a[208:223]}"(c[13]), "=&{a[224:239]}"(c[14]), "=&{a[240:255]}"(c[15])
-          : DITK_MX_L4_OPERANDS : DITK_MX_L4_256X256_CLOBBERS "scc", "memory");
+          : DITK_MX_L4_OPERANDS : DITK_MX_L4_256X256_CLOBBERS "m0", "scc", "memory");
     else if constexpr (FI == 8 && FJ == 4)
       asm volatile(
 #include "mx_l4_128x256_body.inc"
           : [buf] "+&s"(buf), [scb] "+&s"(scb), "=&{a[0:15]}"(c[0]), "=&{a[16:31]}"(c[1]), "=&{a[32:47]}"(c[2]),
             "=&{a[48:63]}"(c[3]), "=&{a[64:79]}"(c[4]), "=&{a[80:95]}"(c[5]), "=&{a[96:111]}"(c[6]), "=&{a[112:127]}"(c[7])
-          : DITK_MX_L4_OPERANDS : DITK_MX_L4_128X256_CLOBBERS "scc", "memory");
+          : DITK_MX_L4_OPERANDS : DITK_MX_L4_128X256_CLOBBERS "m0", "scc", "memory");
     else if constexpr (FI == 4 && FJ == 4)
       asm volatile(
 #include "mx_l4_128x128_body.inc"
           : [buf] "+&s"(buf), [scb] "+&s"(scb), "=&{a[0:15]}"(c[0]), "=&{a[16:31]}"(c[1]), "=&{a[32:47]}"(c[2]),
             "=&{a[48:63]}"(c[3])
-          : DITK_MX_L4_OPERANDS : DITK_MX_L4_128X128_CLOBBERS "scc", "memory");
+          : DITK_MX_L4_OPERANDS : DITK_MX_L4_128X128_CLOBBERS "m0", "scc", "memory");
     else
       asm volatile(
 #include "mx_l4_64x128_body.inc"
           : [buf] "+&s"(buf), [scb] "+&s"(scb), "=&{a[0:15]}"(c[0]), "=&{a[16:31]}"(c[1])
-          : DITK_MX_L4_OPERANDS : DITK_MX_L4_64X128_CLOBBERS "scc", "memory");
+          : DITK_MX_L4_OPERANDS : DITK_MX_L4_64X128_CLOBBERS "m0", "scc", "memory");
     auto acc = [&](int i, int j) {
       const int r = i * FJ + j;
       const f32x16_t& v = c[r / 4];
