@@ -110,8 +110,8 @@ class MXTensor:
         else:
             table = torch.tensor([0, 0.5, 1, 1.5, 2, 3, 4, 6], device=self.device)
             table = torch.cat([table, -table])
-            v = torch.stack([table[(self.data & 15).long()], table[(self.data >> 4).long()]], 2).reshape(rows, -1)
-        s = self.scales.float().reshape(rows, -1, 4, 4).transpose(2, 3).reshape(rows, -1)[:, :cols // 32]
+            v = torch.stack([table[(self.data & 15).long()], table[(self.data >> 4).long()]], 2).flatten(1)
+        s = self.scales.float().unflatten(1, (-1, 4, 4)).transpose(2, 3).flatten(1)[:, :cols // 32]
         return (v[:, :cols].reshape(rows, cols // 32, 32) * s.unsqueeze(2)).reshape(rows, cols)
 
     def _args(self):
