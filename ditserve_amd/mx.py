@@ -260,6 +260,7 @@ def _bf16_out(out, M, N, dtype, device):
     if out is None:
         return torch.empty(M, N, dtype=dtype, device=device)
     _check(out, "out", dtype, 2)
+    _one_device(device, ("out", out))
     ldc, unit = out.stride()
     if out.shape != (M, N) or unit != 1 or ldc % 8 or out.data_ptr() % 16:
         raise ValueError("out must be [M, N], unit column stride, leading dim % 8 == 0, 16-byte aligned")
@@ -305,7 +306,7 @@ def linear(x, w, b=None, epilogue="bias", residual=None, gate=None, segments=Non
     if b is not None:
         _vec(b, "bias", N)
         _one_device(device, ("bias", b))
-    _one_device(device, ("w", w.data), ("out", out))
+    _one_device(device, ("w", w.data))
     ldr, gate_stride, cu, nseg = 0, 0, None, 0
     if res:
         ldr = _residual(residual, M, N)
@@ -347,8 +348,7 @@ def matvec(x, w, b=None, epilogue="bias", residual=None, out=None):
     one = isinstance(x, torch.Tensor) and x.dim() == 1
     if one:
         x = x.unsqueeze(0)
-        residual = None if residual is None else residual.unsqueeze(0)
-        out = None if out is None else out.unsqueeze(0)
+        residual, out = (t.unsqueeze(0) if isinstance(t, torch.Tensor) else t for t in (residual, out))
     M, K, ldx, xp = _bf16_rows(x, "x")
     N = w.data.shape[0]
     if w.cols != K:
@@ -361,7 +361,7 @@ def matvec(x, w, b=None, epilogue="bias", residual=None, out=None):
     if b is not None:
         _vec(b, "bias", N)
         _one_device(device, ("bias", b))
-    _one_device(device, ("w", w.data), ("out", out))
+    _one_device(device, ("w", w.data))
     res, ldr = epilogue == "res", 0
     if res:
         ldr = _residual(residual, M, N)

@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from ditserve_amd import mx
+from ditserve_amd import mx, ops
 
 
 def random_matrix(rows, cols, fmt):
@@ -35,3 +35,41 @@ def test_dequantize(rows, cols, fmt):
             v = e4m3(data[r][c]) if fmt == "fp8" else e2m1(data[r][c // 2] >> 4 * (c % 2) & 15)
             b = c // 32
             assert got[r, c].item() == v * 2.0 ** (scales[r][b // 16 * 16 + b % 4 * 4 + b % 16 // 4] - 127)
+
+
+@pytest.fixture
+def host(monkeypatch):
+    """The Python checks on CPU tensors: the device check is left out, and a launch is an error."""
+    def check(t, name, dtype=None, dims=None):
+        if not isinstance(t, torch.Tensor) or (dtype is not None and t.dtype != dtype) or (dims is not None and t.dim() != dims):
+            raise ValueError(name)
+
+    def launched(*args):
+        raise AssertionError("launched")
+    monkeypatch.setattr(mx, "_check", check)
+    monkeypatch.setattr(ops, "_check", check)
+    monkeypatch.setattr(mx, "_call", launched)
+
+
+@pytest.mark.parametrize("out", [[1.0], "out", 3, (torch.zeros(1), torch.zeros(1))])
+def test_outputs_that_are_no_tensors_are_refused(host, out):
+    x, v = torch.zeros((4, 64), dtype=torch.bfloat16), torch.zeros(64, dtype=torch.bfloat16)
+    q, w, w4 = (mx.MXTensor.empty(n, 64, "cpu", f) for n, f in ((4, "fp8"), (32, "fp8"), (32, "fp4")))
+    for call in (lambda: mx.quantize(x, out=out), lambda: mx.norm(x, out=out), lambda: mx.norm(x, x, residual_out=out),
+                 lambda: mx.linear(q, w, out=out), lambda: mx.linear(q, w, out=out, out_fmt="fp8"),
+                 lambda: mx.matvec(x, w4, out=out), lambda: mx.matvec(v, w4, out=out),
+                 lambda: mx.matvec(v, w4, epilogue="res", residual=out),
+                 lambda: mx.linear(q, w, epilogue="res", residual=out)):
+        with pytest.raises(ValueError):
+            call()
+
+
+def test_outputs_of_the_other_kind_are_refused(host):
+    q, w, w4 = (mx.MXTensor.empty(n, 64, "cpu", f) for n, f in ((4, "fp8"), (32, "fp8"), (32, "fp4")))
+    x = torch.zeros((4, 64), dtype=torch.bfloat16)
+    for call in (lambda: mx.linear(q, w, out=mx.MXTensor.empty(4, 32, "cpu")),
+                 lambda: mx.linear(q, w, out_fmt="fp8", out=torch.zeros((4, 32), dtype=torch.bfloat16)),
+                 lambda: mx.matvec(x, w4, out=mx.MXTensor.empty(4, 32, "cpu")),
+                 lambda: mx.matvec(x[0], w4, out=mx.MXTensor.empty(4, 32, "cpu"))):
+        with pytest.raises(ValueError):
+            call()
