@@ -162,6 +162,17 @@ def _mx_out(out, rows, cols, device, fmt):
     return out
 
 
+def _beside(a, b):
+    """Whether two row views of one row stride hold different columns of a buffer."""
+    if a.dim() != 2 or b.dim() != 2:
+        return False
+    line = a.stride(0) * a.element_size()
+    if line <= 0 or b.stride(0) * b.element_size() != line:
+        return False
+    first, width = (b.data_ptr() - a.data_ptr()) % line, b.shape[1] * b.element_size()
+    return a.shape[1] * a.element_size() <= first and first + width <= line
+
+
 def _apart(fn, outs, operands, same=()):
     """Refuse outputs that share memory with an operand or with each other.  same:
     operands that an output may be as a whole (written where they are read)."""
@@ -172,6 +183,8 @@ def _apart(fn, outs, operands, same=()):
                 continue
             if any(u is s for s in same) and t.data_ptr() == u.data_ptr() and t.stride() == u.stride() \
                     and t.dtype == u.dtype and t.shape == u.shape:
+                continue
+            if _beside(t, u):
                 continue
             raise ValueError(f"{fn}: an output overlaps an operand or another output")
 

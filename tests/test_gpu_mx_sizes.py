@@ -152,3 +152,21 @@ def test_linear_tiles_wider_than_the_matrix(M, N, K, plan):
         assert ((v * s - z).abs() <= 2.0 ** -4 * z.abs() + s * 2.0 ** -10 + 1.25 * off).all()
         for i in rows:
             assert same(got[i:i + 1], mx.linear(x[i:i + 1], w, b, epilogue="silu", out_fmt="fp8"))
+
+
+def test_outputs_beside_their_operands():
+    """Operands and outputs that are column ranges of one buffer."""
+    g = torch.Generator(device=DEV).manual_seed(5)
+    M, N = 333, 512
+    wide = torch.randn((M + 1, 6 * N), generator=g, device=DEV).to(torch.bfloat16)
+    part = [wide[:M, i * N:(i + 1) * N] for i in range(6)]
+    kept = [p.clone() for p in part]
+    want, h = mx.norm(kept[0], kept[1])
+    got, h2 = mx.norm(part[0], part[1], residual_out=part[2])
+    assert same(got, want) and torch.equal(part[2], h) and h2 is part[2]
+    w, w4 = operand(N, N, 6), mx.quantize(kept[0].repeat(2, 1)[:N], "fp4")
+    mx.linear(got, w, epilogue="res", residual=part[1], out=wide[1:, 3 * N:4 * N])
+    assert torch.equal(wide[1:, 3 * N:4 * N], mx.linear(got, w, epilogue="res", residual=kept[1]))
+    mx.matvec(part[0][:40], w4, epilogue="res", residual=part[1][:40], out=wide[:40, 4 * N:5 * N])
+    assert torch.equal(wide[:40, 4 * N:5 * N], mx.matvec(kept[0][:40], w4, epilogue="res", residual=kept[1][:40]))
+    assert all(torch.equal(part[i], kept[i]) for i in (0, 1, 5))

@@ -73,3 +73,27 @@ def test_outputs_of_the_other_kind_are_refused(host):
                  lambda: mx.matvec(x[0], w4, out=mx.MXTensor.empty(4, 32, "cpu"))):
         with pytest.raises(ValueError):
             call()
+
+
+def test_outputs_beside_their_operands_in_one_buffer(host):
+    """Column ranges of one buffer share an extent but no byte: they are no overlap."""
+    wide = torch.zeros((9, 320), dtype=torch.bfloat16)
+    left, right, middle = wide[:8, :64], wide[:8, 64:128], wide[:8, 32:96]
+    q, w, w4 = (mx.MXTensor.empty(n, 64, "cpu", f) for n, f in ((8, "fp8"), (32, "fp8"), (32, "fp4")))
+    for call in (lambda: mx.norm(left, right, residual_out=wide[:8, 128:192]),
+                 lambda: mx.norm(left, right, residual_out=wide[1:, 128:192]),
+                 lambda: mx.norm(left, left, residual_out=right),
+                 lambda: mx.linear(q, w, epilogue="res", residual=wide[1:, :32], out=wide[:8, 32:64]),
+                 lambda: mx.linear(q, w, epilogue="res", residual=wide[:8, 32:64], out=wide[1:, :32]),
+                 lambda: mx.matvec(left, w4, out=wide[1:, 288:]), lambda: mx.matvec(wide[:8, 256:], w4, out=wide[:8, :32])):
+        with pytest.raises(AssertionError, match="launched"):
+            call()
+    # shared columns overlap, also across the end of a line and with another stride
+    flat = wide.view(-1)
+    across = flat[288:288 + 8 * 320].view(8, 320)[:, :64]  # columns 288 .. 319 and 0 .. 31 of the next row
+    for call in (lambda: mx.norm(left, right, residual_out=middle), lambda: mx.norm(left, right, residual_out=wide[1:, :64]),
+                 lambda: mx.matvec(left, w4, out=wide[:8, 56:88]), lambda: mx.matvec(across, w4, out=wide[:8, :32]),
+                 lambda: mx.matvec(across, w4, out=wide[:8, 288:]),
+                 lambda: mx.matvec(left[:4], w4, out=torch.as_strided(wide, (4, 32), (640, 1), 32))):
+        with pytest.raises(ValueError, match="overlaps"):
+            call()
