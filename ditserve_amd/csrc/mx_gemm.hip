@@ -18,12 +18,13 @@
 // whatever M is, wherever its row sits and whichever tile computed it.  Few rows go without
 // LDS to single waves (mx_gemm_rows).
 //
-// What the instruction adds: the products of 8 consecutive k over a common exponent, the largest of
-// their factors' exponent sums, below which it keeps 13 bits and cuts the others off (measured: 1 +
-// 2^-13 is exact within 8 k, 1 + 2^-14 is 1); the sums of 8 and the accumulator with 24 bits.  A product loses at
-// most 2^-13 of the largest of its 8, where e4m3 has already rounded each factor by up to 2^-4; on random data
-// the result is off by 1.6e-5 of the sum of the products' magnitudes.  (Its bf16 counterpart adds exactly at half the
-// rate.)
+// What the instruction adds: the products of 8 consecutive k over a common exponent E, the largest sum of two
+// nonzero factors' exponents, below which it keeps 13 bits and cuts the others off (measured: 1 + 2^-13 is exact
+// within 8 k, 1 + 2^-14 is 1); the sums of 8 and the accumulator with 24 bits.  A product loses less than 2^(E - 13).
+// Of factors that are normal numbers that is at most 2^-13 of the largest product of the 8; a subnormal factor (below
+// 2^-6 of its scale) counts with the exponent -6, so 448 x 2^-9 = 0.875 hides what a product of 4 would.  e4m3 has already
+// rounded a factor by up to 2^-4 of it, and by 2^-10 of its scale where it is subnormal; on random data the result is
+// off by 1.6e-5 of the sum of the products' magnitudes.  (Its bf16 counterpart adds exactly at half the rate.)
 //
 // What bounds it, on one MI355X: 65520 x 1536 x 8960 takes 631 us (2.86 PFLOP/s; 654 with the gated residual),
 // the matrix pipes busy 70% of the cycles at a clock that their power holds at 1.68 GHz.  The k loop
