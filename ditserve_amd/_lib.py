@@ -84,6 +84,7 @@ SIGNATURES = {
     "ditk_mx_gemm_plan_for": (c_int, [c_int, c_int, c_int, c_int64, c_int, ctypes.POINTER(c_int)]),
     "ditk_mx_matvec": (c_int, [_P, c_int64, _P, c_int64, _P, c_int64, _P, _P, c_int64, c_int, c_int, c_int, c_int, _P,
                                c_int64, _P]),
+    "ditk_mx_matvec_plan": (c_int, [c_int, c_int, c_int, ctypes.POINTER(c_int)]),
     "ditk_flash_attn_varlen_noalloc": (c_int, [_P, c_int64, _P, c_int64, _P, c_int64, _P, c_int64, _P, c_int64,
                                                _P, _P, c_int, c_int, c_int, c_int, c_int, c_float, _P]),
 }

@@ -2,7 +2,7 @@
 //
 //   C[m, n] = epilogue( sum_k x[m, k] v[n, k] 2^e[n, k / 32]  + bias[n] )
 //
-// Two kernels, bitwise alike, and a rule between them (launch): one for few rows, one of tiles for more.
+// Two kernels, bitwise alike, and a rule between them (mv_plan): one for few rows, one of tiles for more.
 //
 // Bound by streaming the weight once, 4.25 bits a value.  In the first a wave takes 16 features at a
 // time: lane (ql = lane % 16, g = lane / 16) loads the 16 bytes of block 4 c + g of weight row
@@ -408,45 +408,65 @@ __global__ __launch_bounds__(256 * G) void mx_matvec_wide_kernel(const bf16_t* _
   }
 }
 
-template <int EPI>
-int launch(const void* x, int64_t ldx, const void* W, int64_t ldw, const void* Ws, int64_t ldws, const float* bias,
-           void* C, int64_t ldc, int M, int N, int K, const void* R, int64_t ldr, hipStream_t stream) {
+// Which kernel, in us beyond the launch.  The first streams the weight `passes` times, more slowly with fewer than
+// some 12 waves on a CU.  Tiles take a time for each 128 k, however few they are: of 64 features and two
+// groups up to one tile a CU, beyond that of 128 and one.  (16 x 5120 x 9216 18.5 us on the first kernel and
+// 16.7 on tiles, x 5120 12.6 and 16.4; 48 x 8960 x 5120 44 and 33, 48 x 5120 x 5120 18.6 and 22; 1 x 1536 x 499712
+// 81 and 88, 1 x 5120 x 131072 97 and 76; wrong by 8% at 64 x 5120 x 5120, 28 and 26.)
+enum MvKernel : int { MV_STREAM = 0, MV_TILES64 = 1, MV_TILES128 = 2 };
+struct MvPlan {
+  MvKernel kernel;
+  int fj;      // 16-token fragments of a workgroup
+  int passes;  // over the weight, each of `rows` tokens but the last
+  int rows;
+  int waves;  // of the first kernel's workgroups: the classes of k
+  int lds, per_cu;
+};
+
+int mv_plan(int M, int N, int K, MvPlan& p) {
   // waves: a chunk of 512 k each up to kMaxWaves, beyond that as even a share as there is
-  const int chunks = (K + 511) / 512, each = (chunks + kMaxWaves - 1) / kMaxWaves, waves = (chunks + each - 1) / each;
+  const int chunks = (K - 1) / 512 + 1, each = (chunks + kMaxWaves - 1) / kMaxWaves, waves = (chunks + each - 1) / each;
+  DITK_REQUIRE(K <= kLds / 2, "ditk_mx_matvec: K=%d too long", K);
   // the rows of x that fit in LDS, up to 16 (or 32); more rows in as many even passes over the weight
   auto fit = [&](int fj) { return std::min(16 * fj, (kLds - 2 * waves * fj * 1024) / x_stride(K)); };
   DITK_REQUIRE(fit(1) > 0, "ditk_mx_matvec: K=%d too long", K);
   const int fj = waves > 1 && fit(2) > 0 && (M - 1) / fit(2) < (M - 1) / fit(1) ? 2 : 1;
   const int passes = (M - 1) / fit(fj) + 1;
   DITK_REQUIRE(passes <= 65535, "ditk_mx_matvec: too many rows");  // and no more tiles
-  const int x_rows = (M + passes - 1) / passes;
-  const int groups = (N + 15) / 16, lds = 2 * waves * fj * 1024 + x_rows * x_stride(K);
+  const int x_rows = (M + passes - 1) / passes, lds = 2 * waves * fj * 1024 + x_rows * x_stride(K);
   const int per_cu = std::max(1, std::min(kWavesPerCu / waves, kLds / lds));
-  // Which kernel, in us beyond the launch.  The first streams the weight `passes` times, more slowly with fewer than
-  // some 12 waves on a CU.  Tiles take a time for each 128 k, however few they are: of 64 features and two
-  // groups up to one tile a CU, beyond that of 128 and one.  (16 x 5120 x 9216 18.5 us on the first kernel and
-  // 16.7 on tiles, x 5120 12.6 and 16.4; 48 x 8960 x 5120 44 and 33, 48 x 5120 x 5120 18.6 and 22; 1 x 1536 x 499712
-  // 81 and 88, 1 x 5120 x 131072 97 and 76; wrong by 8% at 64 x 5120 x 5120, 28 and 26.)
   const int steps = (K + 127) / 128, tall = (M + 63) / 64, wj = ((M + tall - 1) / tall + 15) / 16;
-  const bool narrow = (int64_t)((N + 63) / 64) * tall <= ditk_cu_count();
+  const bool narrow = (int64_t)((N - 1) / 64 + 1) * tall <= ditk_cu_count();
   const float weight = (float)N / 68000.f;  // 128 k of the weight at 4.6 TB/s
   const float first = 3.f + (float)steps * weight * (float)passes * std::max(1.f, 12.f / (float)(per_cu * waves));
   const float tiles = narrow ? 4.5f + (float)steps * (0.22f + 0.065f * (float)wj)
                              : 3.2f + (float)steps * std::max(0.3f + 0.12f * (float)wj, weight * 1.05f * (float)tall);
-  if (tiles < first) {
-    const dim3 grid((unsigned)(narrow ? (N + 63) / 64 : (N + 127) / 128), (unsigned)tall);
-    auto kern = wj == 1   ? (narrow ? mx_matvec_wide_kernel<EPI, 1, 1, 4, 2> : mx_matvec_wide_kernel<EPI, 1, 2, 4, 1>)
-                : wj == 2 ? (narrow ? mx_matvec_wide_kernel<EPI, 2, 1, 4, 2> : mx_matvec_wide_kernel<EPI, 2, 2, 4, 1>)
-                : wj == 3 ? (narrow ? mx_matvec_wide_kernel<EPI, 3, 1, 3, 2> : mx_matvec_wide_kernel<EPI, 3, 2, 3, 1>)
-                          : (narrow ? mx_matvec_wide_kernel<EPI, 4, 1, 3, 2> : mx_matvec_wide_kernel<EPI, 4, 2, 3, 1>);
+  if (tiles < first) p = MvPlan{narrow ? MV_TILES64 : MV_TILES128, wj, tall, 16 * wj, waves, 0, 0};
+  else p = MvPlan{MV_STREAM, fj, passes, x_rows, waves, lds, per_cu};
+  return 0;
+}
+
+template <int EPI>
+int launch(const void* x, int64_t ldx, const void* W, int64_t ldw, const void* Ws, int64_t ldws, const float* bias,
+           void* C, int64_t ldc, int M, int N, int K, const void* R, int64_t ldr, hipStream_t stream) {
+  MvPlan p;
+  if (int rc = mv_plan(M, N, K, p)) return rc;
+  if (p.kernel != MV_STREAM) {
+    const bool narrow = p.kernel == MV_TILES64;
+    const dim3 grid((unsigned)(narrow ? (N - 1) / 64 + 1 : (N - 1) / 128 + 1), (unsigned)p.passes);
+    auto kern = p.fj == 1   ? (narrow ? mx_matvec_wide_kernel<EPI, 1, 1, 4, 2> : mx_matvec_wide_kernel<EPI, 1, 2, 4, 1>)
+                : p.fj == 2 ? (narrow ? mx_matvec_wide_kernel<EPI, 2, 1, 4, 2> : mx_matvec_wide_kernel<EPI, 2, 2, 4, 1>)
+                : p.fj == 3 ? (narrow ? mx_matvec_wide_kernel<EPI, 3, 1, 3, 2> : mx_matvec_wide_kernel<EPI, 3, 2, 3, 1>)
+                            : (narrow ? mx_matvec_wide_kernel<EPI, 4, 1, 3, 2> : mx_matvec_wide_kernel<EPI, 4, 2, 3, 1>);
     kern<<<grid, narrow ? 512 : 256, 0, stream>>>((const bf16_t*)x, ldx, (const uint8_t*)W, ldw, (const uint8_t*)Ws, ldws,
-                                                  bias, C, ldc, M, N, K, (const bf16_t*)R, ldr, waves);
+                                                  bias, C, ldc, M, N, K, (const bf16_t*)R, ldr, p.waves);
     return ditk_check_launch("ditk_mx_matvec");
   }
-  const dim3 grid((unsigned)std::min(groups, std::max(1, ditk_cu_count() * per_cu / passes)), (unsigned)passes);
-  auto kern = fj == 1 ? mx_matvec_kernel<EPI, 1> : mx_matvec_kernel<EPI, 2>;
-  kern<<<grid, 64 * waves, lds, stream>>>((const bf16_t*)x, ldx, (const uint8_t*)W, ldw, (const uint8_t*)Ws, ldws, bias,
-                                          C, ldc, M, N, K, (const bf16_t*)R, ldr, x_rows);
+  const int groups = (N - 1) / 16 + 1;
+  const dim3 grid((unsigned)std::min(groups, std::max(1, ditk_cu_count() * p.per_cu / p.passes)), (unsigned)p.passes);
+  auto kern = p.fj == 1 ? mx_matvec_kernel<EPI, 1> : mx_matvec_kernel<EPI, 2>;
+  kern<<<grid, 64 * p.waves, p.lds, stream>>>((const bf16_t*)x, ldx, (const uint8_t*)W, ldw, (const uint8_t*)Ws, ldws,
+                                              bias, C, ldc, M, N, K, (const bf16_t*)R, ldr, p.rows);
   return ditk_check_launch("ditk_mx_matvec");
 }
 
@@ -476,4 +496,14 @@ DITK_EXPORT int ditk_mx_matvec(const void* x, int64_t ldx, const void* W, int64_
     case MV_SILU: return launch<MV_SILU>(x, ldx, W, ldw, Ws, ldws, bias, C, ldc, M, N, K, R, ldr, stream);
     default: ditk_set_error("ditk_mx_matvec: unknown epilogue %d", epilogue); return 1;
   }
+}
+
+DITK_EXPORT int ditk_mx_matvec_plan(int M, int N, int K, int* plan) {
+  DITK_REQUIRE(plan && M > 0 && N > 0 && N % 8 == 0 && K > 0 && K % 32 == 0, "ditk_mx_matvec_plan: bad arguments");
+  MvPlan p;
+  if (int rc = mv_plan(M, N, K, p)) return rc;
+  plan[0] = p.kernel;
+  plan[1] = p.fj;
+  plan[2] = p.passes;
+  return 0;
 }

@@ -452,6 +452,13 @@ int ditk_mx_matvec(const void* x, int64_t ldx, const void* W, int64_t ldw, const
                    const float* bias, void* C, int64_t ldc, int M, int N, int K, int epilogue, const void* R,
                    int64_t ldr, ditk_stream_t stream);
 
+/*
+ * How ditk_mx_matvec runs an M x N x K product, host only: plan[0] 0 the kernel that
+ * streams the weight past rows held in LDS, 1 tiles of 64 features, 2 tiles of 128;
+ * plan[1] the 16-row fragments of a workgroup; plan[2] its passes over the weight.
+ */
+int ditk_mx_matvec_plan(int M, int N, int K, int* plan);
+
 #ifdef __cplusplus
 }
 #endif

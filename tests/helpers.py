@@ -67,3 +67,13 @@ def mx_gemm_plan(m, n, k, ld=None, mx_out=False, name="ditk_mx_gemm_plan_for"):
     more = (ld or (k + 127) // 128 * 128, int(mx_out)) if name.endswith("for") else ()
     _lib.call(name, m, n, k, *more, plan)
     return tuple(plan)
+
+
+def mx_matvec_plan(m, n, k):
+    """(kernel, 16-row fragments, passes) of an m x n x k ditk_mx_matvec: host only."""
+    import ctypes
+
+    from ditserve_amd import _lib
+    plan = (ctypes.c_int * 3)()
+    _lib.call("ditk_mx_matvec_plan", m, n, k, plan)
+    return tuple(plan)

@@ -9,6 +9,7 @@ import pytest
 import torch
 
 from ditserve_amd import mx
+from tests.helpers import mx_gemm_plan, mx_matvec_plan
 
 pytestmark = pytest.mark.gpu
 DEV = "cuda"
@@ -81,3 +82,70 @@ def test_what_is_lost_can_pass_the_largest_product():
     assert lost(pairs) == 7 * 1.75 * 2.0 ** -12 > 7 * 2.0 ** -13 * 0.875
     # the same beside a product of normal factors of that size are not
     assert lost([(1.75, 0.5)] + pairs[1:]) == 0
+
+
+# ---------------------------------------------------------------------------------------------
+# sums that fp32 holds exactly: a stretch of k that is left out, or counted twice, shows in every output
+# ---------------------------------------------------------------------------------------------
+
+def whole_numbers(rows, cols, seed, fmt):
+    """An MX matrix of small whole numbers under scales of 1, 2 and 4, and its values."""
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    v = torch.randint(-3, 4, (rows, cols), generator=g, device=DEV).double()  # e2m1 and e4m3 hold them
+    s = torch.randint(0, 3, (rows, cols // 32), generator=g, device=DEV)
+    m = mx.MXTensor.empty(rows, cols, DEV, fmt)
+    data, scales = m.data.view(torch.uint8), m.scales.view(torch.uint8)
+    data.zero_()
+    scales.fill_(127)
+    if fmt == "fp8":
+        data[:, :cols] = v.float().to(torch.float8_e4m3fn).view(torch.uint8)
+    else:
+        code = torch.tensor([0, 2, 4, 5], device=DEV)[v.abs().long()] + 8 * (v < 0)
+        data[:, :cols // 2] = (code[:, 0::2] + 16 * code[:, 1::2]).to(torch.uint8)
+    b = torch.arange(cols // 32, device=DEV)
+    scales[:, b // 16 * 16 + b % 4 * 4 + b % 16 // 4] = (127 + s).to(torch.uint8)
+    return m, v * torch.exp2(s.double()).repeat_interleave(32, 1)
+
+
+@pytest.mark.parametrize("shape,plan", [
+    ((1, 1544, 14336), (0, 1, 1)), ((9, 1544, 14336), (0, 1, 3)), ((2, 24, 60000), (0, 1, 2)), ((1, 24, 65408), (0, 1, 1)),
+    ((17, 264, 8224), (0, 1, 3)), ((32, 136, 1568), (0, 2, 1)), ((100, 72, 1536), (0, 2, 4)), ((5, 40, 32), (0, 1, 1)),
+    ((11, 10008, 13856), (1, 1, 1)), ((25, 9000, 8928), (1, 2, 1)), ((48, 9000, 8960), (1, 3, 1)), ((64, 9224, 5120), (1, 4, 1)),
+    ((40, 9000, 60000), (1, 3, 1)), ((3, 27016, 5120), (2, 1, 1)), ((30, 17000, 1568), (2, 2, 1)),
+    ((40, 33000, 2432), (2, 3, 1)), ((100, 16648, 1056), (2, 4, 2))])
+def test_matvec_of_whole_numbers(shape, plan):
+    """|x| <= 4 and |w| <= 12: sums below 48 K < 2^24, exact in any order."""
+    M, N, K = shape
+    assert mx_matvec_plan(*shape) == plan and 48 * K < 2 ** 24
+    g = torch.Generator(device=DEV).manual_seed(K)
+    x = torch.randint(-4, 5, (M, K), generator=g, device=DEV).to(torch.bfloat16)
+    w, wv = whole_numbers(N, K, N, "fp4")
+    b = torch.randint(-9, 10, (N,), generator=g, device=DEV).float()
+    r = torch.randint(-99, 100, (M, N), generator=g, device=DEV).to(torch.bfloat16)
+    want = torch.mm(x.double(), wv.T) + b.double()
+    assert torch.equal(mx.matvec(x, w, b, epilogue="f32").double(), want)
+    assert torch.equal(mx.matvec(x, w, b), want.float().to(torch.bfloat16))
+    assert torch.equal(mx.matvec(x, w, b, epilogue="res", residual=r), (want + r.double()).float().to(torch.bfloat16))
+
+
+@pytest.mark.parametrize("shape,wide,plan", [
+    ((16, 512, 14336), False, (6, 16, 0)), ((96, 1536, 14336), False, (7, 96, 0)), ((70, 5128, 14368), False, (7, 70, 0)),
+    ((512, 2440, 8960), False, (3, 512, 0)), ((700, 4104, 14336), False, (2, 700, 0)), ((1000, 2440, 14368), False, (2, 1000, 0)),
+    ((667, 7304, 8992), False, (1, 667, 0)), ((2600, 4104, 14336), False, (0, 2600, 0)), ((2600, 8968, 512), False, (0, 1792, 1)),
+    ((512, 2440, 8960), True, (5, 512, 0)), ((2600, 4104, 14368), True, (4, 2600, 0)), ((700, 4104, 288), False, (5, 700, 0))])
+def test_linear_of_whole_numbers(shape, wide, plan):
+    """Whole numbers up to 3 under a scale for their block: products of 8 k lie within 13 bits; |x|, |w| <= 12: sums
+    below 144 K < 2^24."""
+    M, N, K = shape
+    stride = (1 << 23) + 16
+    assert mx_gemm_plan(M, N, K, stride if wide else None) == plan and 144 * K < 2 ** 24
+    (x, xv), (w, wv) = whole_numbers(M, K, M, "fp8"), whole_numbers(N, K, N, "fp8")
+    if wide:
+        rows = torch.empty(M * stride, dtype=torch.uint8, device=DEV).as_strided(x.data.shape, (stride, 1))
+        x = mx.MXTensor("fp8", rows.copy_(x.data.view(torch.uint8)).view(torch.float8_e4m3fn), x.scales, K)
+    g = torch.Generator(device=DEV).manual_seed(K)
+    b = torch.randint(-9, 10, (N,), generator=g, device=DEV).float()
+    r = torch.randint(-99, 100, (M, N), generator=g, device=DEV).to(torch.bfloat16)
+    want = torch.mm(xv, wv.T) + b.double()
+    assert torch.equal(mx.linear(x, w, b), want.float().to(torch.bfloat16))
+    assert torch.equal(mx.linear(x, w, b, epilogue="res", residual=r), (want + r.double()).float().to(torch.bfloat16))

@@ -2,7 +2,7 @@
 import pytest
 
 from ditserve_amd import _lib
-from tests.helpers import mx_gemm_plan
+from tests.helpers import mx_gemm_plan, mx_matvec_plan
 
 if not _lib.LIB_PATH.exists():
     pytest.skip("libditk.so not built (run python -m ditserve_amd.build)", allow_module_level=True)
@@ -77,3 +77,25 @@ def test_plans_near_2_31():
     assert mx_gemm_plan(2**31 - 1, 264, 32) == (4, 2**31 - 1, 0)
     # the longest rows: no fewer steps than those of half the length
     assert mx_gemm_plan(16, 64, 2**31 - 32)[0] == mx_gemm_plan(16, 64, 2**30)[0]
+
+
+@pytest.mark.parametrize("shape,want", [
+    # few rows past the weight: one or two fragments of 16 rows, more rows in more passes
+    ((1, 9216, 1536), (0, 1, 1)), ((2, 499712, 1536), (0, 1, 1)), ((17, 264, 2432), (0, 2, 1)), ((100, 72, 1536), (0, 2, 4)),
+    ((33, 520, 8960), (0, 1, 5)), ((2, 24, 60000), (0, 1, 2)), ((1, 24, 65408), (0, 1, 1)),
+    # tiles of 64 features, 1 to 4 fragments
+    ((11, 10008, 13856), (1, 1, 1)), ((25, 9000, 8928), (1, 2, 1)), ((48, 9000, 8960), (1, 3, 1)),
+    ((64, 9224, 5120), (1, 4, 1)), ((64, 16000, 480), (1, 4, 1)),
+    # and of 128
+    ((3, 27016, 5120), (2, 1, 1)), ((2, 33800, 4640), (2, 1, 1)), ((30, 17000, 1568), (2, 2, 1)),
+    ((17, 33016, 1056), (2, 2, 1)), ((40, 33000, 2432), (2, 3, 1)), ((100, 16648, 1056), (2, 4, 2))])
+def test_plans_of_matvec(shape, want):
+    assert mx_matvec_plan(*shape) == want
+    # what one row of a few features runs on, which others are compared with bitwise
+    assert mx_matvec_plan(1, 1000, shape[2])[0] == 0
+
+
+def test_matvec_plan_refusals():
+    for bad in ((0, 64, 128), (1, 12, 128), (1, 64, 40), (1, 64, 65440), (1, 64, 2**31 - 32), (65536 * 32, 64, 128)):
+        with pytest.raises(_lib.DitkError):
+            mx_matvec_plan(*bad)
