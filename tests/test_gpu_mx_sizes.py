@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from ditserve_amd import mx, ops
+from ditserve_amd import _lib, mx, ops
 from tests.helpers import mx_gemm_plan
 
 pytestmark = pytest.mark.gpu
@@ -170,3 +170,113 @@ def test_outputs_beside_their_operands():
     mx.matvec(part[0][:40], w4, epilogue="res", residual=part[1][:40], out=wide[:40, 4 * N:5 * N])
     assert torch.equal(wide[:40, 4 * N:5 * N], mx.matvec(kept[0][:40], w4, epilogue="res", residual=kept[1][:40]))
     assert all(torch.equal(part[i], kept[i]) for i in (0, 1, 5))
+
+
+def mx_rows_in(rows, cols, extra=2):
+    """An MX output inside wider rows, every byte of the buffers 0xAA."""
+    d, s = (cols + 127) // 128 * 128, (cols + 511) // 512 * 16
+    bufs = [torch.full((rows + extra, n + 48), 0xAA, dtype=torch.uint8, device=DEV) for n in (d, s)]
+    views = [b[:rows, 16:16 + n] for b, n in zip(bufs, (d, s))]
+    return bufs, mx.MXTensor("fp8", views[0].view(torch.float8_e4m3fn), views[1].view(torch.float8_e8m0fnu), cols)
+
+
+def untouched(bufs, rows):
+    return all((b[rows:] == 0xAA).all() and (b[:rows, :16] == 0xAA).all() and (b[:rows, -32:] == 0xAA).all() for b in bufs)
+
+
+# every kernel (few rows, the tiles, the two with 64-bit addresses, a split launch)
+KERNELS = [((16, 1536, 1536), (6, 16, 0)), ((100, 1568, 416), (7, 100, 0)), ((333, 4640, 1536), (3, 333, 0)),
+           ((520, 4640, 448), (2, 520, 0)), ((700, 7328, 1056), (1, 700, 0)), ((1560, 8960, 512), (0, 1560, 0)),
+           ((4600, 5152, 448), (0, 3072, 1)), ((700, 4128, 288), (5, 700, 0)), ((2601, 4128, 96), (4, 2601, 0))]
+
+
+@pytest.mark.parametrize("shape,plan", KERNELS)
+def test_mx_outputs_in_wider_rows(shape, plan):
+    M, N, K = shape
+    assert mx_gemm_plan(*shape, mx_out=True) == plan
+    x, w = operand(M, K, 1), operand(N, K, 2, 4, pad=16)
+    bufs, out = mx_rows_in(M, N)
+    assert same(mx.linear(x, w, epilogue="gelu", out_fmt="fp8", out=out), mx.linear(x, w, epilogue="gelu", out_fmt="fp8"))
+    assert untouched(bufs, M)
+
+
+@pytest.mark.parametrize("rows,cols", [(5, 96), (67, 2432), (300, 6144)])
+def test_row_operators_in_wider_rows(rows, cols):
+    g = torch.Generator(device=DEV).manual_seed(rows)
+    x, r = (torch.randn((rows, cols), generator=g, device=DEV).to(torch.bfloat16) for _ in range(2))
+    bufs, out = mx_rows_in(rows, cols)
+    assert same(mx.quantize(x, out=out), mx.quantize(x)) and untouched(bufs, rows)
+    want, h = mx.norm(x, r)
+    bufs, out = mx_rows_in(rows, cols)
+    wide = torch.full((rows + 2, cols + 24), 7.0, dtype=torch.bfloat16, device=DEV)
+    got, h2 = mx.norm(x, r, out=out, residual_out=wide[:rows, 8:8 + cols])
+    assert same(got, want) and torch.equal(h2, h) and untouched(bufs, rows)
+    assert (wide[rows:] == 7).all() and (wide[:, :8] == 7).all() and (wide[:, 8 + cols:] == 7).all()
+
+
+@pytest.mark.parametrize("shape,plan", KERNELS)
+def test_non_finite_values_stay_in_their_row_and_feature(shape, plan):
+    """An operand block of NaN makes its row or feature NaN and no other; a NaN or infinity of the residual, bias or
+    gate its own outputs; in an MX output the block of 32."""
+    M, N, K = shape
+    assert mx_gemm_plan(*shape) == mx_gemm_plan(*shape, mx_out=True) == plan
+    x, w = operand(M, K, 1), operand(N, K, 2, 4)
+    kw = gated(M, N, 3)
+    b = torch.randn(N, generator=torch.Generator(device=DEV).manual_seed(4), device=DEV)
+    clean, clean_mx = mx.linear(x, w, b, **kw), mx.linear(x, w, b, out_fmt="fp8")
+    row, feature, last = M // 2, N // 3, K // 32 - 1
+    byte = last // 16 * 16 + last % 4 * 4 + last % 16 // 4
+    raw(x)[1][row, byte] = 255
+    raw(w)[1][feature, byte] = 255
+    b[N - 1] = float("inf")
+    kw["residual"][M - 1, 5] = float("nan")
+    kw["gate"][3, 9] = float("nan")
+    hit = torch.zeros((M, N), dtype=torch.bool, device=DEV)
+    hit[row] = hit[:, feature] = hit[:, N - 1] = True
+    own = hit.clone()
+    own[M - 1, 5] = own[M // 3:, 9] = True
+    got = mx.linear(x, w, b, **kw)
+    assert torch.equal(~got.isfinite(), own) and torch.equal(got[~own], clean[~own])
+    data, scales = raw(mx.linear(x, w, b, out_fmt="fp8"))
+    blocks = hit.view(M, N // 32, 32).any(2)
+    place = [16 * (i // 16) + 4 * (i % 4) + (i % 16) // 4 for i in range(N // 32)]
+    assert torch.equal(scales[:, place] == 255, blocks)
+    keep = ~blocks.repeat_interleave(32, 1)
+    assert torch.equal(data[:, :N][keep], raw(clean_mx)[0][:, :N][keep])
+
+
+@pytest.mark.parametrize("shape,plan", KERNELS)
+def test_gate_of_one_segment_and_of_each_row(shape, plan):
+    """One segment for all rows, and segments of one row: the tiles' gate by LDS and by row."""
+    M, N, K = shape
+    x, w = operand(M, K, 1), operand(N, K, 2, 4)
+    g = torch.Generator(device=DEV).manual_seed(5)
+    r = torch.randn((M, N), generator=g, device=DEV).to(torch.bfloat16)
+    gate = torch.randn((1, N), generator=g, device=DEV)
+    one = mx.linear(x, w, epilogue="gate_res", residual=r, gate=gate, segments=ops.Segments([0, M], DEV))
+    each = mx.linear(x, w, epilogue="gate_res", residual=r, gate=gate.expand(M, N), segments=ops.Segments(range(M + 1), DEV))
+    assert same(one, each)
+    # and the ungated one under a gate of 1
+    ones = mx.linear(x, w, epilogue="gate_res", residual=r, gate=torch.ones_like(gate), segments=ops.Segments([0, M], DEV))
+    assert same(ones, mx.linear(x, w, epilogue="res", residual=r))
+
+
+@pytest.mark.parametrize("shape,plan", [((300, 4640, 1536), (3, 300, 0)), ((1560, 8960, 512), (0, 1560, 0)),
+                                        ((100, 1568, 416), (7, 100, 0)), ((700, 4128, 288), (5, 700, 0))])
+def test_widest_output_and_residual_rows(shape, plan):
+    """Rows of 2^22 - 8 elements, the longest that a tile's 32-bit offsets are used with, are written and read where
+    they are; longer ones are refused."""
+    M, N, K = shape
+    assert mx_gemm_plan(*shape) == plan
+    x, w, kw = operand(M, K, 1), operand(N, K, 2, 4), gated(M, N, 3)
+    want = mx.linear(x, w, **kw)
+    stride = (1 << 22) - 8
+    flat = torch.empty(M * stride, dtype=torch.bfloat16, device=DEV)
+    res = flat.as_strided((M, N), (stride, 1)).copy_(kw["residual"])
+    out = flat.as_strided((M, N), (stride, 1), N).fill_(7.0)
+    behind = flat.as_strided((M, 64), (stride, 1), 2 * N).fill_(7.0)
+    assert mx.linear(x, w, **{**kw, "residual": res}, out=out) is out
+    assert same(out, want) and torch.equal(res, kw["residual"]) and (behind == 7).all()
+    over = flat.as_strided((M - 1, N), (stride + 8, 1))
+    with pytest.raises(_lib.DitkError, match="strides too large"):
+        mx.linear(x[:M - 1], w, out=over)
