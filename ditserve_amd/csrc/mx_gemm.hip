@@ -26,11 +26,11 @@
 // rounded a factor by up to 2^-4 of it, and by 2^-10 of its scale where it is subnormal; on random data the result is
 // off by 1.6e-5 of the sum of the products' magnitudes.  (Its bf16 counterpart adds exactly at half the rate.)
 //
-// What bounds it, on one MI355X: 65520 x 1536 x 8960 takes 631 us (2.86 PFLOP/s; 654 with the gated residual),
-// the matrix pipes busy 70% of the cycles at a clock that their power holds at 1.68 GHz.  The k loop
+// What bounds it, on one MI355X (M x N x K): 65520 x 1536 x 8960 takes 631 us (2.86 PFLOP/s; 654-692 with the gated
+// residual), the matrix pipes busy 70% of the cycles at a clock that their power holds at 1.68 GHz.  The k loop
 // without an epilogue does 3.0-3.1 PFLOP/s, a loop of these MFMAs on random registers alone 3.3 (4.5 on
-// zeros).  At K = 1536 the epilogue's stores count: 65520 x 1536 x 1536 130 us for 105 without them (201 MB),
-// 32760 x 5120 x 5120 582-617 us (2.8-2.95 PFLOP/s).
+// zeros).  At K = 1536 the epilogue counts: 65520 x 1536 x 1536 130 us for 105 without its stores (201 MB), 65520 x
+// 8960 x 1536 774 us with a bias, 866 with GELU, 973 with GELU and an MX output; 32760 x 5120 x 5120 582-617 us.
 #include <algorithm>
 #include <type_traits>
 

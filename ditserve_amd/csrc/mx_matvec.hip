@@ -224,7 +224,7 @@ __global__ __launch_bounds__(64 * kMaxWaves) void mx_matvec_kernel(const bf16_t*
 // round is a class for each group, each with stages of its own; the classes' sums are added in
 // order.  The same additions in the same order: bitwise the first kernel's results.
 //
-// 48 x 8960 x 51200 361 us on the first kernel (7 passes over the weight), 80 here; 1 x 5120 x 131072 97 and
+// 48 x 8960 x 51200 361 us on the first kernel (6 passes over the weight), 80 here; 1 x 5120 x 131072 97 and
 // 76 (4.7 TB/s).  A tile's stage takes 0.3 us for the instructions of one wave a SIMD and 0.12 for
 // each 16 tokens' LDS reads and MFMAs behind one another; more stages ahead (6, 7) change nothing.  Where tiles
 // are few, two groups a tile take 0.6 of that; four 1.2 of what two take.

@@ -442,8 +442,9 @@ int ditk_mx_gemm_plan_for(int M, int N, int K, int64_t row_stride, int out_kind,
 /*
  * C = epilogue(x W^T + bias) of bf16 rows x [M, K] and an fp4 MX matrix W [N, K],
  * K % 32 == 0, N % 8 == 0, for few rows: the weight is read once for up to 64 rows
- * (a smaller one more often, where that is faster).  A row has to fit into LDS: K up to about
- * 65000.  The columns of W behind K, up to the next multiple of 128, have to be zero.
+ * (a smaller one more often, where that is faster).  A row has to fit into LDS: K up to
+ * 65408.  The columns of W behind K, up to the next multiple of 128, have to be zero; a
+ * weight of 2^128 or more counts as infinite.
  * fp32 accumulation, one rounding at the end.  epilogue 0 bias, 1 GELU-tanh, 3 R + y,
  * 4 fp32 output, 5 SiLU.  ldc, ldr in elements, multiples of 8; C may be R itself.
  * Every row is computed the same way whatever M is.
