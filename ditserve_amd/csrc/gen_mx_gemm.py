@@ -383,7 +383,7 @@ def clobbers():
     for v in VARIANTS:
         configure(*v)
         regs = [f"v{i}" for i in range(LAST_VGPR + 1)] + [f"s{i}" for i in SGPRS]
-        rows = [", ".join(f'"{r}"' for r in regs[i:i + 16]) for i in range(0, len(regs), 16)]
+        rows = [", ".join(f'"{r}"' for r in regs[i:i + 14]) for i in range(0, len(regs), 14)]
         out.append(f"#define DITK_{name_of(FI, FJ).upper()}_CLOBBERS \\\n" + "".join(f"  {r}, \\\n" for r in rows))
     return "\n".join(out) + "\n"
 

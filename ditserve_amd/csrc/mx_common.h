@@ -49,8 +49,8 @@ __device__ __forceinline__ uint32_t quad_max(uint32_t v) {
 }
 
 // Quantises 8 consecutive values per lane, four lanes of which hold one block of 32: a
-// quad, or (GROUPS) the lanes l % 16 + 16 g.  Returns the block's scale byte and the values' bytes (fp8: q[0..1], fp4: q[0]).
-// The largest magnitude keeps an infinity or a NaN: such a block gets the scale NaN, and NaN
+// quad, or (GROUPS) the lanes l % 16 + 16 g.  Returns the block's scale byte and the values' bytes (fp8: q[0..1], fp4:
+// q[0]).  The largest magnitude keeps an infinity or a NaN: such a block gets the scale NaN, and NaN
 // values in fp8.
 template <int FMT, bool GROUPS = false>
 __device__ __forceinline__ uint32_t mx_quantise8(const float (&v)[8], uint32_t (&q)[2]) {

@@ -22,9 +22,10 @@
 // nonzero factors' exponents, below which it keeps 13 bits and cuts the others off (measured: 1 + 2^-13 is exact
 // within 8 k, 1 + 2^-14 is 1); the sums of 8 and the accumulator with 24 bits.  A product loses less than 2^(E - 13).
 // Of factors that are normal numbers that is at most 2^-13 of the largest product of the 8; a subnormal factor (below
-// 2^-6 of its scale) counts with the exponent -6, so 448 x 2^-9 = 0.875 hides what a product of 4 would.  e4m3 has already
-// rounded a factor by up to 2^-4 of it, and by 2^-10 of its scale where it is subnormal; on random data the result is
-// off by 1.6e-5 of the sum of the products' magnitudes.  (Its bf16 counterpart adds exactly at half the rate.)
+// 2^-6 of its scale) counts with the exponent -6, so 448 x 2^-9 = 0.875 hides what a product of 4 would.  e4m3 has
+// already rounded a factor by up to 2^-4 of it, and by 2^-10 of its scale where it is subnormal; on random data the
+// result is off by 1.6e-5 of the sum of the products' magnitudes.  (Its bf16 counterpart adds exactly, at half the
+// rate.)
 //
 // What bounds it, on one MI355X (M x N x K): 65520 x 1536 x 8960 takes 631 us (2.86 PFLOP/s; 654-692 with the gated
 // residual), the matrix pipes busy 70% of the cycles at a clock that their power holds at 1.68 GHz.  The k loop
@@ -128,7 +129,8 @@ __device__ __forceinline__ void mx_epilogue(const MxGemmArgs& p, const Acc& acc,
   };
   auto desc = [&](const void* base, int64_t row_bytes) {
     return __builtin_amdgcn_make_buffer_rsrc(
-        uniform(reinterpret_cast<const char*>(base) + (base != nullptr ? m * row_bytes : 0)), 0, 0x7fffffff, 0x00020000);
+        uniform(reinterpret_cast<const char*>(base) + (base != nullptr ? m * row_bytes : 0)), 0, 0x7fffffff,
+        0x00020000);
   };
   const uint32_t ldc = (uint32_t)p.ldc * (OUT == MXO_FP8 ? 1 : 2), ldr = (uint32_t)p.ldr * 2, ldcs = (uint32_t)p.ldcs;
   const __amdgpu_buffer_rsrc_t cdesc = desc(p.C, ldc), rdesc = desc(kRes ? p.R : nullptr, ldr),
@@ -224,9 +226,11 @@ __device__ __forceinline__ void mx_epilogue(const MxGemmArgs& p, const Acc& acc,
         store(line[0], t + ql, nb, 1);
       }
       const int col = n + g * 32;
-      __builtin_amdgcn_raw_buffer_store_b8(
-          (uint8_t)(scales >> (8 * g)), sdesc,
-          g < NF && row_ok(t + ql) && col_ok(col) ? (uint32_t)(t + ql) * ldcs + (uint32_t)mx_scale_at(col >> 5) : kOut, 0, 0);
+      __builtin_amdgcn_raw_buffer_store_b8((uint8_t)(scales >> (8 * g)), sdesc,
+                                           g < NF && row_ok(t + ql) && col_ok(col)
+                                               ? (uint32_t)(t + ql) * ldcs + (uint32_t)mx_scale_at(col >> 5)
+                                               : kOut,
+                                           0, 0);
     } else {
 #pragma unroll
       for (int f = 0; f < NF; f += 2) {
@@ -286,7 +290,8 @@ __device__ __forceinline__ void mx_out_padding(const MxGemmArgs& p) {
   if (cols + sc == 0) return;
   for (int row = p.m_begin + blockIdx.x * per + threadIdx.x / 32; row < p.M; row += gridDim.x * per) {
     if (i < cols)
-      *reinterpret_cast<u32x4_t*>(reinterpret_cast<uint8_t*>(p.C) + (int64_t)row * p.ldc + p.N + i * 16) = u32x4_t{0, 0, 0, 0};
+      *reinterpret_cast<u32x4_t*>(reinterpret_cast<uint8_t*>(p.C) + (int64_t)row * p.ldc + p.N + i * 16) =
+          u32x4_t{0, 0, 0, 0};
     if (i >= 16 && i < 16 + sc) p.Cs[(int64_t)row * p.ldcs + mx_scale_at(b0 + i - 16)] = 127;
   }
 }
@@ -422,15 +427,15 @@ struct MxL4 {
 #define DITK_MX_L4_START_OPERANDS                                                                                     \
   [a_lo] "s"(lo32(cur.a)), [a_hi] "s"(hi32(cur.a)), [w_lo] "s"(lo32(cur.w)), [w_hi] "s"(hi32(cur.w)),                 \
       [sa_lo] "s"(lo32(cur.sa)), [sa_hi] "s"(hi32(cur.sa)), [sw_lo] "s"(lo32(cur.sw)), [sw_hi] "s"(hi32(cur.sw)),     \
-      [ldsw] "s"(ldsw), [scm_a] "s"(scm_a), [scm_w] "s"(scm_w), [saoff] "v"(lv.saoff), [swoff] "v"(lv.swoff),               \
-      [aoff0] "v"(lv.aoff[0]), [aoff1] "v"(lv.aoff[1]), [aoff2] "v"(lv.aoff[2]), [aoff3] "v"(lv.aoff[3]), [aoff4] "v"(lv.aoff[4]),   \
-      [aoff5] "v"(lv.aoff[5]), [aoff6] "v"(lv.aoff[6]), [aoff7] "v"(lv.aoff[7]), [woff0] "v"(lv.woff[0]), [woff1] "v"(lv.woff[1]),   \
-      [woff2] "v"(lv.woff[2]), [woff3] "v"(lv.woff[3]), [woff4] "v"(lv.woff[4]), [woff5] "v"(lv.woff[5]), [woff6] "v"(lv.woff[6]),   \
-      [woff7] "v"(lv.woff[7])
+      [ldsw] "s"(ldsw), [scm_a] "s"(scm_a), [scm_w] "s"(scm_w), [saoff] "v"(lv.saoff), [swoff] "v"(lv.swoff),         \
+      [aoff0] "v"(lv.aoff[0]), [aoff1] "v"(lv.aoff[1]), [aoff2] "v"(lv.aoff[2]), [aoff3] "v"(lv.aoff[3]),             \
+      [aoff4] "v"(lv.aoff[4]), [aoff5] "v"(lv.aoff[5]), [aoff6] "v"(lv.aoff[6]), [aoff7] "v"(lv.aoff[7]),             \
+      [woff0] "v"(lv.woff[0]), [woff1] "v"(lv.woff[1]), [woff2] "v"(lv.woff[2]), [woff3] "v"(lv.woff[3]),             \
+      [woff4] "v"(lv.woff[4]), [woff5] "v"(lv.woff[5]), [woff6] "v"(lv.woff[6]), [woff7] "v"(lv.woff[7])
 #define DITK_MX_L4_OPERANDS                                                                                           \
   DITK_MX_L4_START_OPERANDS, [na_lo] "s"(lo32(nxt.a)), [na_hi] "s"(hi32(nxt.a)), [nw_lo] "s"(lo32(nxt.w)),            \
       [nw_hi] "s"(hi32(nxt.w)), [nsa_lo] "s"(lo32(nxt.sa)), [nsa_hi] "s"(hi32(nxt.sa)), [nsw_lo] "s"(lo32(nxt.sw)),   \
-      [nsw_hi] "s"(hi32(nxt.sw)), [nk] "s"(nk), [rdx0] "v"(lv.rdx[0]), [rdx1] "v"(lv.rdx[1]), [rdw0] "v"(lv.rdw[0]),           \
+      [nsw_hi] "s"(hi32(nxt.sw)), [nk] "s"(nk), [rdx0] "v"(lv.rdx[0]), [rdx1] "v"(lv.rdx[1]), [rdw0] "v"(lv.rdw[0]),  \
       [rdw1] "v"(lv.rdw[1]), [scx] "v"(lv.scx), [scw] "v"(lv.scw)
 
 template <int EPI, int OUT, int FI, int FJ>
@@ -542,7 +547,8 @@ __global__ __launch_bounds__(256, 1) void mx_gemm_l4(MxGemmArgs p) {
     const bool one_seg = EPI != MXE_GATE_RES || one_segment(p, tile.mb, GBM, seg);
     const int vrow = (wave % (GBN / 64)) * 64;
     auto fetch = [&](const float* src, int at) {
-      const uint32_t m0v = su(lds0 + G::VEC0 + at * 1024 + vrow * 4), off = (uint32_t)min(tile.nb + vrow + lane_id(), p.N - 1) * 4;
+      const uint32_t m0v = su(lds0 + G::VEC0 + at * 1024 + vrow * 4),
+                     off = (uint32_t)min(tile.nb + vrow + lane_id(), p.N - 1) * 4;
       asm volatile("s_mov_b32 m0, %0\n s_nop 0\n global_load_lds_dword %1, %2" ::"s"(m0v), "v"(off), "s"(src)
                    : "m0", "memory");
     };
@@ -562,15 +568,17 @@ __global__ __launch_bounds__(256, 1) void mx_gemm_l4(MxGemmArgs p) {
       asm volatile(
 #include "mx_l4_256x256_body.inc"
           : [buf] "+&s"(buf), [scb] "+&s"(scb), "=&{a[0:15]}"(c[0]), "=&{a[16:31]}"(c[1]), "=&{a[32:47]}"(c[2]),
-            "=&{a[48:63]}"(c[3]), "=&{a[64:79]}"(c[4]), "=&{a[80:95]}"(c[5]), "=&{a[96:111]}"(c[6]), "=&{a[112:127]}"(c[7]),
-            "=&{a[128:143]}"(c[8]), "=&{a[144:159]}"(c[9]), "=&{a[160:175]}"(c[10]), "=&{a[176:191]}"(c[11]),
+            "=&{a[48:63]}"(c[3]), "=&{a[64:79]}"(c[4]), "=&{a[80:95]}"(c[5]), "=&{a[96:111]}"(c[6]),
+            "=&{a[112:127]}"(c[7]), "=&{a[128:143]}"(c[8]), "=&{a[144:159]}"(c[9]), "=&{a[160:175]}"(c[10]),
+            "=&{a[176:191]}"(c[11]),
             "=&{a[192:207]}"(c[12]), "=&{a[208:223]}"(c[13]), "=&{a[224:239]}"(c[14]), "=&{a[240:255]}"(c[15])
           : DITK_MX_L4_OPERANDS : DITK_MX_L4_256X256_CLOBBERS "m0", "scc", "memory");
     else if constexpr (FI == 8 && FJ == 4)
       asm volatile(
 #include "mx_l4_128x256_body.inc"
           : [buf] "+&s"(buf), [scb] "+&s"(scb), "=&{a[0:15]}"(c[0]), "=&{a[16:31]}"(c[1]), "=&{a[32:47]}"(c[2]),
-            "=&{a[48:63]}"(c[3]), "=&{a[64:79]}"(c[4]), "=&{a[80:95]}"(c[5]), "=&{a[96:111]}"(c[6]), "=&{a[112:127]}"(c[7])
+            "=&{a[48:63]}"(c[3]), "=&{a[64:79]}"(c[4]), "=&{a[80:95]}"(c[5]), "=&{a[96:111]}"(c[6]),
+            "=&{a[112:127]}"(c[7])
           : DITK_MX_L4_OPERANDS : DITK_MX_L4_128X256_CLOBBERS "m0", "scc", "memory");
     else if constexpr (FI == 4 && FJ == 4)
       asm volatile(
@@ -898,7 +906,8 @@ int launch_plan(const MxGemmArgs& p, hipStream_t stream) {
       default: return launch<EPI, OUT, 4, 2, 2, 2, 2>(q, stream);
     }
   };
-  const MxPlan plan = mx_plan_any(p.M, p.N, p.K, std::max(std::max(p.lda, p.ldw), std::max(p.ldas, p.ldws)), OUT == MXO_FP8);
+  const int64_t ld = std::max(std::max(p.lda, p.ldw), std::max(p.ldas, p.ldws));
+  const MxPlan plan = mx_plan_any(p.M, p.N, p.K, ld, OUT == MXO_FP8);
   const int rc = part(plan.cfg, 0, plan.rows);
   return rc != 0 || plan.rows == p.M ? rc : part(plan.rest, plan.rows, p.M);
 }

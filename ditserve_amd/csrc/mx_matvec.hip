@@ -181,7 +181,8 @@ __global__ __launch_bounds__(64 * kMaxWaves) void mx_matvec_kernel(const bf16_t*
       __builtin_amdgcn_global_load_lds(
           (const __attribute__((address_space(1))) void*)(x + (int64_t)(m0 + r) * ldx + k),
           (__attribute__((address_space(3))) void*)dst, 16, 0, 0);
-    if (tail && k >= K && c * 4 + (lane >> 4) < steps) *reinterpret_cast<u32x4_t*>(dst + lane * 16) = u32x4_t{0, 0, 0, 0};
+    if (tail && k >= K && c * 4 + (lane >> 4) < steps)
+      *reinterpret_cast<u32x4_t*>(dst + lane * 16) = u32x4_t{0, 0, 0, 0};
   };
   for (int p = wave; p < rows * chunks; p += waves) x_unit(p, false);
   if (K % 128 != 0)
@@ -454,12 +455,14 @@ int launch(const void* x, int64_t ldx, const void* W, int64_t ldw, const void* W
   if (p.kernel != MV_STREAM) {
     const bool narrow = p.kernel == MV_TILES64;
     const dim3 grid((unsigned)(narrow ? (N - 1) / 64 + 1 : (N - 1) / 128 + 1), (unsigned)p.passes);
-    auto kern = p.fj == 1   ? (narrow ? mx_matvec_wide_kernel<EPI, 1, 1, 4, 2> : mx_matvec_wide_kernel<EPI, 1, 2, 4, 1>)
-                : p.fj == 2 ? (narrow ? mx_matvec_wide_kernel<EPI, 2, 1, 4, 2> : mx_matvec_wide_kernel<EPI, 2, 2, 4, 1>)
-                : p.fj == 3 ? (narrow ? mx_matvec_wide_kernel<EPI, 3, 1, 3, 2> : mx_matvec_wide_kernel<EPI, 3, 2, 3, 1>)
-                            : (narrow ? mx_matvec_wide_kernel<EPI, 4, 1, 3, 2> : mx_matvec_wide_kernel<EPI, 4, 2, 3, 1>);
-    kern<<<grid, narrow ? 512 : 256, 0, stream>>>((const bf16_t*)x, ldx, (const uint8_t*)W, ldw, (const uint8_t*)Ws, ldws,
-                                                  bias, C, ldc, M, N, K, (const bf16_t*)R, ldr, p.waves);
+    using Kernel = decltype(&mx_matvec_wide_kernel<EPI, 1, 1, 4, 2>);
+    const Kernel tiles64[] = {mx_matvec_wide_kernel<EPI, 1, 1, 4, 2>, mx_matvec_wide_kernel<EPI, 2, 1, 4, 2>,
+                              mx_matvec_wide_kernel<EPI, 3, 1, 3, 2>, mx_matvec_wide_kernel<EPI, 4, 1, 3, 2>};
+    const Kernel tiles128[] = {mx_matvec_wide_kernel<EPI, 1, 2, 4, 1>, mx_matvec_wide_kernel<EPI, 2, 2, 4, 1>,
+                               mx_matvec_wide_kernel<EPI, 3, 2, 3, 1>, mx_matvec_wide_kernel<EPI, 4, 2, 3, 1>};
+    const Kernel kern = (narrow ? tiles64 : tiles128)[p.fj - 1];
+    kern<<<grid, narrow ? 512 : 256, 0, stream>>>((const bf16_t*)x, ldx, (const uint8_t*)W, ldw, (const uint8_t*)Ws,
+                                                  ldws, bias, C, ldc, M, N, K, (const bf16_t*)R, ldr, p.waves);
     return ditk_check_launch("ditk_mx_matvec");
   }
   const int groups = (N - 1) / 16 + 1;

@@ -169,14 +169,15 @@ DITK_EXPORT int ditk_mx_quantize(const void* x, int64_t ldx, void* data, int64_t
   DITK_REQUIRE(T >= 0 && (T == 0 || x), "ditk_mx_quantize: bad rows");
   DITK_REQUIRE(fmt == MX_FP8 || fmt == MX_FP4, "ditk_mx_quantize: unknown format %d", fmt);
   if (int rc = mx_out_check("ditk_mx_quantize", data, ldd, scales, lds, T, K, fmt)) return rc;
-  DITK_REQUIRE(ldx % 8 == 0 && ldx >= K && ((uintptr_t)x % 16) == 0, "ditk_mx_quantize: x rows must be 16-byte aligned");
+  DITK_REQUIRE(ldx % 8 == 0 && ldx >= K && ((uintptr_t)x % 16) == 0,
+               "ditk_mx_quantize: x rows must be 16-byte aligned");
   if (T == 0) return 0;
   const int per_row = (K + 511) / 512;
   const RowGrid g = row_grid(T, per_row);
   DITK_REQUIRE(g.grid.y <= kMaxGridY, "ditk_mx_quantize: too many rows");
   auto kern = fmt == MX_FP8 ? mx_quantise_kernel<MX_FP8> : mx_quantise_kernel<MX_FP4>;
-  kern<<<g.grid, 256, 0, stream>>>((const bf16_t*)x, ldx, (uint8_t*)data, ldd, (uint8_t*)scales, lds, T, g.rows, per_row,
-                                   K / 8);
+  kern<<<g.grid, 256, 0, stream>>>((const bf16_t*)x, ldx, (uint8_t*)data, ldd, (uint8_t*)scales, lds, T, g.rows,
+                                   per_row, K / 8);
   return ditk_check_launch("ditk_mx_quantize");
 }
 
