@@ -187,7 +187,8 @@ def untouched(bufs, rows):
 # every kernel (few rows, the tiles, the two with 64-bit addresses, a split launch)
 KERNELS = [((16, 1536, 1536), (6, 16, 0)), ((100, 1568, 416), (7, 100, 0)), ((333, 4640, 1536), (3, 333, 0)),
            ((520, 4640, 448), (2, 520, 0)), ((700, 7328, 1056), (1, 700, 0)), ((1560, 8960, 512), (0, 1560, 0)),
-           ((4600, 5152, 448), (0, 3072, 1)), ((700, 4128, 288), (5, 700, 0)), ((2601, 4128, 96), (4, 2601, 0))]
+           ((4353, 4128, 448), (0, 3840, 2)), ((2600, 8960, 512), (0, 1792, 1)), ((700, 4128, 288), (5, 700, 0)),
+           ((2601, 4128, 96), (4, 2601, 0))]
 
 
 @pytest.mark.parametrize("shape,plan", KERNELS)

@@ -16,7 +16,7 @@ WIDE = (1 << 23) + 16  # 256 rows of it pass 2^31 bytes
     # tiles wider than the matrix
     ((9000, 120, 1536), (3, 9000, 0)), ((20000, 64, 1536), (2, 20000, 0)), ((40000, 200, 1536), (0, 40000, 0)),
     # split launches
-    ((1000, 4616, 1056), (1, 1000, 0)), ((2600, 4104, 640), (0, 2600, 0)), ((4600, 5128, 416), (0, 3072, 1)),
+    ((1000, 4616, 1056), (1, 1000, 0)), ((2600, 4104, 640), (0, 2600, 0)), ((2600, 8968, 512), (0, 1792, 1)),
     ((9000, 2440, 3104), (0, 6400, 1)), ((70000, 200, 1536), (0, 65536, 3))])
 def test_plans_of_bf16_outputs(shape, want):
     assert mx_gemm_plan(*shape) == want
@@ -26,7 +26,7 @@ def test_plans_of_bf16_outputs(shape, want):
 
 @pytest.mark.parametrize("shape,want", [
     ((1560, 8960, 512), (0, 1560, 0)), ((333, 4640, 1536), (3, 333, 0)), ((700, 7328, 1056), (1, 700, 0)),
-    ((100, 1568, 416), (7, 100, 0)), ((4600, 5152, 448), (0, 3072, 1)), ((20000, 96, 672), (2, 20000, 0)),
+    ((100, 1568, 416), (7, 100, 0)), ((4353, 4128, 448), (0, 3840, 2)), ((20000, 96, 672), (2, 20000, 0)),
     ((16, 1536, 1536), (6, 16, 0))])
 def test_plans_of_mx_outputs(shape, want):
     assert mx_gemm_plan(*shape, mx_out=True) == want
