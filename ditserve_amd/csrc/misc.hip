@@ -296,6 +296,7 @@ DITK_EXPORT int ditk_joint_copy(void* img, int64_t ld_img, void* txt, int64_t ld
   DITK_REQUIRE(width % 8 == 0 && ld_img % 8 == 0 && ld_txt % 8 == 0 && ld_joint % 8 == 0,
                "ditk_joint_copy: widths must be multiples of 8");
   DITK_REQUIRE(direction == 0 || direction == 1, "ditk_joint_copy: direction must be 0 or 1");
+  DITK_REQUIRE(total < 1 << 26, "ditk_joint_copy: too many rows (%d)", total);  // 2^32 threads
   if (total == 0) return 0;
   joint_copy_kernel<<<total, 64, 0, stream>>>((bf16_t*)img, ld_img, (bf16_t*)txt, ld_txt, (bf16_t*)joint,
                                               ld_joint, cu_img, cu_txt, nseg, total, width, direction);

@@ -390,6 +390,10 @@ __global__ __launch_bounds__(256) void qk_norm_multi_kernel(QkNormJobs jobs) {
 }  // namespace
 
 namespace {
+// A grid's first dimension holds less than 2^32 threads (more wrap around, and no error is reported).
+constexpr int64_t kMaxBlocks = (1ll << 32) / 256;
+int64_t row_blocks(int T) { return ((int64_t)T + kRowsPerBlock - 1) / kRowsPerBlock; }
+
 int adaln_check(const void* x, int64_t ldx, void* y, int64_t ldy, int T, int D, const int32_t* cu_seqlens, int nseg,
                 const float* shift, const float* scale, int64_t mod_stride, const float* weight, const float* bias,
                 int norm_kind) {
@@ -418,7 +422,9 @@ DITK_EXPORT int ditk_adaln(const void* x, int64_t ldx, void* y, int64_t ldy, int
                              norm_kind);
   if (rc) return rc;
   if (T == 0) return 0;
-  dim3 grid((T + kRowsPerBlock - 1) / kRowsPerBlock);
+  const int64_t blocks = row_blocks(T);
+  DITK_REQUIRE(blocks < kMaxBlocks, "ditk_adaln: too many rows (%d)", T);
+  const dim3 grid((unsigned)blocks);
   const int nc = (D / 8 + 63) / 64;
   const bool aff = shift == nullptr && (weight != nullptr || bias != nullptr);
 #define DITK_ADALN(K, NCV)                                                                                     \
@@ -469,9 +475,9 @@ DITK_EXPORT int ditk_adaln_multi(const ditk_adaln_job* jobs, int njobs, hipStrea
     a.job[j] = AdalnJob{(const bf16_t*)p.x, p.ldx, (bf16_t*)p.y, p.ldy, p.cu_seqlens, p.shift, p.scale,
                         p.mod_stride, p.weight, p.bias, p.T, p.D, p.nseg, p.eps};
     a.block0[j] = (int)blocks;
-    blocks += (p.T + kRowsPerBlock - 1) / kRowsPerBlock;
+    blocks += row_blocks(p.T);
   }
-  DITK_REQUIRE(blocks < (1ll << 31), "ditk_adaln_multi: too many rows");
+  DITK_REQUIRE(blocks < kMaxBlocks, "ditk_adaln_multi: too many rows");
   a.block0[njobs] = (int)blocks;
   if (blocks == 0) return 0;
   const dim3 grid((unsigned)blocks);
@@ -545,7 +551,9 @@ int qk_norm_rope_launch(const void* q, int64_t ldq, const void* k, int64_t ldk, 
                                max_pos, cu_seqlens, grids, nseg, t_pairs, h_pairs);
   if (rc) return rc;
   if (T == 0) return 0;
-  dim3 grid((T + kRowsPerBlock - 1) / kRowsPerBlock);
+  const int64_t blocks = row_blocks(T);
+  DITK_REQUIRE(blocks < kMaxBlocks, "ditk_qk_norm_rope: too many rows (%d)", T);
+  const dim3 grid((unsigned)blocks);
   const int nc = (D / 8 + 63) / 64;
 #define DITK_QKN(G, NCV)                                                                                  \
   qk_norm_rope_kernel<G, NCV><<<grid, 256, 0, stream>>>((const bf16_t*)q, ldq, (const bf16_t*)k, ldk,    \
@@ -598,9 +606,9 @@ DITK_EXPORT int ditk_qk_norm_multi(const ditk_qk_norm_job* jobs, int njobs, hipS
     group = gj;
     a.job[j] = p;
     a.block0[j] = (int)blocks;
-    blocks += (p.T + kRowsPerBlock - 1) / kRowsPerBlock;
+    blocks += row_blocks(p.T);
   }
-  DITK_REQUIRE(blocks < (1ll << 31), "ditk_qk_norm_multi: too many rows");
+  DITK_REQUIRE(blocks < kMaxBlocks, "ditk_qk_norm_multi: too many rows");
   a.block0[njobs] = (int)blocks;
   if (blocks == 0) return 0;
   const dim3 grid((unsigned)blocks);
