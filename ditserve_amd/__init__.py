@@ -6,4 +6,4 @@ ops raise if the library is not built.
 """
 __version__ = "0.1.0"
 
-from . import mx, ops  # noqa: F401
+from . import kv, mx, ops  # noqa: F401

@@ -460,6 +460,53 @@ int ditk_mx_matvec(const void* x, int64_t ldx, const void* W, int64_t ldw, const
  */
 int ditk_mx_matvec_plan(int M, int N, int K, int* plan);
 
+/*
+ * Paged key-value caches.  A cache of `pages` pages of `page` slots (16, 32, 64, 128 or 256) holds
+ * keys and values [page][head_dim] bf16 (head_dim 64 or 128), contiguous, for each (page, key head),
+ * with a page stride *_ps and a head stride *_hs (elements, multiples of 8); weights (fp32, may be
+ * NULL) one for each (page, key head, slot).  Slot i of sequence b is slot i % page of page
+ * table[b * ldt + i / page]; the table's rows hold `width` pages and lengths[b] slots are filled.
+ * A length outside [0, min(width * page, max_len)] is clamped; a page outside [0, pages) is neither
+ * read nor written and its slots count as absent; either sets *status (pinned host memory) to 1.
+ * No reference counterpart: the reference's models attend over whole videos.
+ *
+ * ditk_kv_append: row i of segment b of k and v [T, kv_heads * head_dim] goes to slot lengths[b] + i
+ * (cu_seqlens NULL: one row a sequence); new_lengths[b] = lengths[b] + its rows (another array).
+ */
+int ditk_kv_append(const void* k, int64_t ldk, const void* v, int64_t ldv, void* k_cache, int64_t k_ps, int64_t k_hs,
+                   void* v_cache, int64_t v_ps, int64_t v_hs, float* weights, int64_t w_ps, int64_t w_hs, int pages,
+                   int page, const int32_t* table, int64_t ldt, int width, const int32_t* lengths,
+                   int32_t* new_lengths, const int32_t* cu_seqlens, int batch, int T, int kv_heads, int head_dim,
+                   int32_t* status, ditk_stream_t stream);
+
+/* Bytes of the workspace of ditk_kv_attn (most: the smaller of width * page and max_len; weights: whether it has any). */
+int64_t ditk_kv_attn_workspace(int batch, int heads, int head_dim, int most, int weights);
+
+/*
+ * Attention of one query row of each sequence (q [batch, heads * head_dim], heads a multiple of
+ * kv_heads) over its slots: o [batch, heads * head_dim] bf16, lse [batch][heads] fp32 natural log
+ * (may be NULL).  weights not NULL: the probabilities of each slot, summed over the query heads of
+ * its key head, are written there (add != 0: added).  workspace: 16-byte aligned, this call's alone.
+ */
+int ditk_kv_attn(const void* q, int64_t ldq, const void* k_cache, int64_t k_ps, int64_t k_hs, const void* v_cache,
+                 int64_t v_ps, int64_t v_hs, float* weights, int64_t w_ps, int64_t w_hs, int add, int pages, int page,
+                 const int32_t* table, int64_t ldt, int width, const int32_t* lengths, int max_len, void* o,
+                 int64_t ldo, float* lse, void* workspace, int64_t workspace_bytes, int batch, int heads, int kv_heads,
+                 int head_dim, float softmax_scale, int32_t* status, ditk_stream_t stream);
+
+/*
+ * Of each (sequence, key head) the last `recent` slots and those of the others with the largest
+ * weights (ties: the lowest slot; NaN counts as -inf), min(length, keep) in all, copied in their
+ * order, with their weights, into the first slots of out_table's pages (other pages than
+ * table's; out_width * page >= min(keep, width * page, max_len)).  slots: workspace of
+ * batch * kv_heads * keep ints.
+ */
+int ditk_kv_evict(void* k_cache, int64_t k_ps, int64_t k_hs, void* v_cache, int64_t v_ps, int64_t v_hs,
+                  float* weights, int64_t w_ps, int64_t w_hs, int pages, int page, const int32_t* table, int64_t ldt,
+                  int width, const int32_t* lengths, int max_len, const int32_t* out_table, int64_t ldo, int out_width,
+                  int32_t* new_lengths, int keep, int recent, int32_t* slots, int batch, int kv_heads, int head_dim,
+                  int32_t* status, ditk_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

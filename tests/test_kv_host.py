@@ -1,0 +1,86 @@
+"""Refusals of the paged cache's entry points: on the host, before any launch (no GPU)."""
+import pytest
+import torch
+
+from ditserve_amd import _lib, kv
+
+if not _lib.LIB_PATH.exists():
+    pytest.skip("libditk.so not built (run python -m ditserve_amd.build)", allow_module_level=True)
+
+A, B, C, D, E, F, G, H = (0x10000 * i for i in range(1, 9))  # addresses only: nothing is launched
+
+
+def refused(name, args, word):
+    lib = _lib.load()
+    assert getattr(lib, name)(*args) == 1
+    assert word in lib.ditk_last_error().decode(), lib.ditk_last_error()
+
+
+CACHE = dict(k=A, k_ps=2 * 16 * 64, k_hs=16 * 64, v=B, v_ps=2 * 16 * 64, v_hs=16 * 64, w=None, w_ps=32, w_hs=16)
+PAGES = dict(pages=8, page=16, table=C, ldt=4, width=4, lengths=D)
+APPEND = dict(new_k=E, ldk=128, new_v=F, ldv=128, **CACHE, **PAGES, new=G, cu=None, batch=2, T=2, hk=2, d=64, status=H,
+              stream=None)
+ATTN = dict(q=E, ldq=256, **CACHE, add=0, **PAGES, max_len=64, o=F, ldo=256, lse=None, space=None, size=0, batch=2, heads=4,
+            hk=2, d=64, scale=0.1, status=H, stream=None)
+EVICT = dict(**{**CACHE, "w": E}, **PAGES, max_len=64, out_table=F, ldo=2, out_width=2, new=G, keep=32, recent=4, slots=A,
+             batch=2, hk=2, d=64, status=H, stream=None)
+
+COMMON = [
+    (dict(batch=-1), "sequences"), (dict(batch=65536), "sequences"), (dict(hk=0), "key head"), (dict(d=96), "head_dim"),
+    (dict(page=8), "slots"), (dict(page=48), "slots"), (dict(pages=0), "no pages"), (dict(table=None), "null table"),
+    (dict(lengths=None), "null table"), (dict(status=None), "null table"), (dict(ldt=3), "page table"),
+    (dict(width=-1), "page table"), (dict(width=2**26, ldt=2**26), "page table"), (dict(k=None), "null cache"),
+    (dict(v=None), "null cache"), (dict(k=A + 8), "aligned"), (dict(v_hs=1028), "aligned"), (dict(k_ps=-2048), "aligned")]
+
+
+@pytest.mark.parametrize("change,word", COMMON + [
+    (dict(new_k=None), "rows"), (dict(T=-1), "rows"), (dict(T=3), "3 rows for 2"), (dict(ldk=120), "aligned"),
+    (dict(ldv=132), "aligned"), (dict(new_v=F + 2), "aligned"), (dict(new=None), "lengths")])
+def test_append_refuses(change, word):
+    refused("ditk_kv_append", tuple({**APPEND, **change}.values()), word)
+
+
+@pytest.mark.parametrize("change,word", COMMON + [
+    (dict(heads=5), "query heads"), (dict(heads=0), "query heads"), (dict(q=None), "null"), (dict(o=None), "null"),
+    (dict(ldq=252), "aligned"), (dict(o=F + 8), "aligned"), (dict(max_len=-1), "max_len"), (dict(scale=0.0), "scale"),
+    (dict(scale=float("nan")), "scale"), (dict(w=G), "workspace"),
+    (dict(width=4096, ldt=4096, max_len=65536, space=G, size=64), "workspace")])
+def test_attn_refuses(change, word):
+    refused("ditk_kv_attn", tuple({**ATTN, **change}.values()), word)
+
+
+@pytest.mark.parametrize("change,word", COMMON + [
+    (dict(w=None), "no weights"), (dict(keep=0), "keep"), (dict(recent=-1), "recent"), (dict(recent=33), "recent"),
+    (dict(max_len=-1), "max_len"), (dict(out_table=None), "null table"), (dict(out_width=1), "32 stay"),
+    (dict(new=None), "null output"), (dict(slots=None), "null output")])
+def test_evict_refuses(change, word):
+    refused("ditk_kv_evict", tuple({**EVICT, **change}.values()), word)
+
+
+def test_nothing_to_do():
+    """No sequences: no launch."""
+    lib = _lib.load()
+    none = dict(batch=0, table=None, lengths=None)
+    assert lib.ditk_kv_append(*{**APPEND, **none, "T": 0, "new": None}.values()) == 0
+    assert lib.ditk_kv_attn(*{**ATTN, **none}.values()) == 0
+    assert lib.ditk_kv_evict(*{**EVICT, **none, "new": None}.values()) == 0
+
+
+def test_workspace_grows_with_what_it_holds():
+    size = _lib.load().ditk_kv_attn_workspace
+    assert size(4, 8, 128, 64, 0) == 0 and size(0, 8, 128, 1 << 20, 1) == 0
+    assert size(4, 8, 128, 1 << 20, 0) < size(4, 8, 128, 1 << 20, 1)
+    # a float for each query head and slot, past 32 bits
+    assert size(64, 128, 128, 1 << 20, 1) > 64 * 128 * (1 << 20) * 4
+
+
+def test_cpu_tensors_are_refused():
+    k = torch.zeros((4, 2, 16, 64), dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="cuda"):
+        kv.PagedCache(k, k)
+    with pytest.raises(ValueError, match="PagedCache"):
+        kv.append(k, k, k, k, k)
+    with pytest.raises(ValueError, match="PagedCache"):
+        kv.decode_attn(k, k, k, k, 2)
+    with pytest.raises(ValueError, match="PagedCache"):
+        kv.evict(k, k, k, k, 2)
