@@ -12,6 +12,8 @@ varlen flash kernel (bf16, head_dim 64/128, non-causal, no dropout).
    :448-486): ``flash_attn_varlen_func(q, k, v, cu_q, cu_k, max_q, max_k,
    dropout_p=0.0, causal=False) -> out`` on packed [T, H, D] tensors with int32
    device cu_seqlens.  No host synchronisation: cu tables stay on the device.
+   ``causal_attn_varlen_func`` is the same with the causal mask and grouped query
+   heads, for prompts (the reference has no such call).
 
 Device cu_seqlens tables from callers are checked on the GPU before any kernel
 reads them (ops.Segments.from_device): an invalid table is clamped into bounds
@@ -129,6 +131,23 @@ def flash_attn_varlen_func(q, k, v, cu_q, cu_k, max_q, max_k, dropout_p=0.0, cau
     seg_q, seg_k = ops.Segments.pair_from_device(cu_q.to(torch.int32), tq, cu_k.to(torch.int32), k.shape[0])
     out = ops.flash_attn_varlen(q.reshape(tq, h * d), k.reshape(k.shape[0], h * d),
                                 v.reshape(v.shape[0], h * d).contiguous(), seg_q, seg_k, h, d)
+    return out.view(tq, h, d)
+
+
+def causal_attn_varlen_func(q, k, v, cu_q, cu_k, max_q, max_k, softmax_scale=None):
+    """flash_attn_varlen_func with the causal mask and query heads in groups: q [Tq, H, D],
+    k/v [Tk, Hk, D] bf16, H a multiple of Hk.  A segment's queries are the last of its
+    keys: query i of nq sees the keys j <= i + nk - nq (ops.flash_attn_causal)."""
+    if q.dim() != 3 or k.dim() != 3 or v.dim() != 3:
+        raise ValueError("q, k, v must be [T, H, D]")
+    (tq, h, d), (tk, hk, _) = q.shape, k.shape
+    if k.shape[2] != d or v.shape != k.shape:
+        raise ValueError(f"k and v must be [Tk, Hk, {d}], got {tuple(k.shape)} and {tuple(v.shape)}")
+    if cu_q.numel() != cu_k.numel():
+        raise ValueError("cu_seqlens_q and cu_seqlens_k must have the same length")
+    seg_q, seg_k = ops.Segments.pair_from_device(cu_q.to(torch.int32), tq, cu_k.to(torch.int32), tk)
+    out = ops.flash_attn_causal(q.reshape(tq, h * d), k.reshape(tk, hk * d), v.reshape(tk, hk * d), seg_q, seg_k, h, hk,
+                                d, softmax_scale)
     return out.view(tq, h, d)
 
 

@@ -1,4 +1,4 @@
-// Varlen block-diagonal flash attention (forward, non-causal), bf16 MFMA.
+// Varlen block-diagonal flash attention (forward; causal with grouped heads, further down), bf16 MFMA.
 //
 // Packed layout: Q [Tq, ldq], K [Tk, ldk] with head h at columns [h*HD, h*HD+HD);
 // segment m's queries [cu_q[m], cu_q[m+1]) attend only to keys
@@ -137,6 +137,10 @@ __device__ __forceinline__ int padded_key_start(const int32_t* __restrict__ cu, 
       [otxt_hi] "s"(su((uint32_t)(otxt >> 32))), [qa0lo] "a"((uint32_t)qa[0]), [qa0hi] "a"((uint32_t)(qa[0] >> 32)), \
       [qa1lo] "a"((uint32_t)qa[1]), [qa1hi] "a"((uint32_t)(qa[1] >> 32)), [krow0] "a"(krow_of[0]),                  \
       [krow1] "a"(krow_of[1]), [krow2] "a"(krow_of[2]), [krow3] "a"(krow_of[3])
+// Causal (plain q): how many keys each lane's queries see, less 8 (lane / 32), and the
+// first key tile that is not whole to every query of the wave
+#define DITK_ATTN_ASM_OPERANDS_CAUSAL                                                                               \
+  DITK_ATTN_ASM_OPERANDS, [vlim0] "v"(vlim[0]), [vlim1] "v"(vlim[1]), [kdiag] "s"(su(kdiag))
 // Row r, head h of segment m of an operand lies at base + h * hs + m * sa + r * ld
 // (elements).  Packed rows: hs = head_dim, sa = 0.  A [batch, heads, rows, head_dim]
 // tensor read in place: hs and ld its head and row strides, sa = batch stride -
@@ -145,15 +149,16 @@ struct RowLayout {
   int64_t hs, sa;
 };
 constexpr int kXcdChunk = 32;  // most work items per XCD chunk (one per CU of an XCD)
-template <int HD, bool PRE, bool JOINT, int QB>
+template <int HD, bool PRE, bool JOINT, int QB, bool CAUSAL = false>
 __global__ __launch_bounds__(256, 1) void flash_fwd_asm(
     const bf16_t* __restrict__ Q, int64_t ldq, const bf16_t* __restrict__ Kp, int64_t ldk,
     const bf16_t* __restrict__ Vt, int64_t vt_ld, int64_t vt_hs, bf16_t* __restrict__ O, int64_t ldo,
     float* __restrict__ lse, int64_t lse_ld, const int32_t* __restrict__ cu_q,
     const int32_t* __restrict__ cu_k, int nseg, int heads, int np, int chunk, bool stream_out, float scale_log2, RowLayout ql, RowLayout kl,
     const bf16_t* __restrict__ Qb = nullptr, const bf16_t* __restrict__ Kb = nullptr, bf16_t* __restrict__ Ob = nullptr,
-    const int32_t* __restrict__ cu_a = nullptr, const int32_t* __restrict__ cu_b = nullptr) {
+    const int32_t* __restrict__ cu_a = nullptr, const int32_t* __restrict__ cu_b = nullptr, int group = 1) {
   static_assert(!JOINT || (PRE && HD == 64), "joint sources: pre-scaled head_dim 64");
+  static_assert(!CAUSAL || !PRE, "causal: plain q");
   constexpr int NW = 4, BM = 128 * QB;  // QB 32-query blocks per wave
   constexpr int ND = HD / 32;  // DMA instructions per wave and operand per tile
   __shared__ u32x4_t Ks[2][BN * HD / 8];
@@ -169,10 +174,30 @@ __global__ __launch_bounds__(256, 1) void flash_fwd_asm(
   // evenly over the XCDs, and the items running on one XCD at a time are tiles of
   // the same (segment, head), sharing its K and Vt in that XCD's L2.  The grid is
   // a multiple of 8 chunks; items past the last exit.
+  //
+  // Causal items differ in length, and the longest come first: a segment's last tile
+  // of every head, then the tile before it (np = 1).  With a multiple of 8 heads an XCD
+  // has consecutive heads of its own, which share keys.
   const int b = blockIdx.x;
   const int j = b >> 3;
-  int t = ((j / chunk) * 8 + (b & 7)) * chunk + j % chunk;
+  int t = CAUSAL ? b : ((j / chunk) * 8 + (b & 7)) * chunk + j % chunk;
   int seg = -1, head = 0, npass = 0;
+  if constexpr (CAUSAL) {
+    for (int m = 0, prev = cu_q[0]; m < nseg; ++m) {
+      const int next = cu_q[m + 1];
+      const int ntile = (next - prev + BM - 1) / BM;
+      if (t < ntile * heads) {
+        seg = m;
+        npass = 1;
+        head = t % heads;
+        t = ntile - 1 - t / heads;
+        if ((heads & 7) == 0) head = (head & 7) * (heads >> 3) + (head >> 3);
+        break;
+      }
+      t -= ntile * heads;
+      prev = next;
+    }
+  } else
   for (int m = 0, prev = cu_q[0]; m < nseg; ++m) {
     const int next = cu_q[m + 1];
     const int ntile = (next - prev + BM - 1) / BM;
@@ -196,13 +221,26 @@ __global__ __launch_bounds__(256, 1) void flash_fwd_asm(
   const int qrow1 = qrow0 + 32;
   const int k_beg = cu_k[seg], k_len = max(cu_k[seg + 1] - k_beg, 0);
   // nkt == 0 (no keys): the body stores zero rows and lse = -inf, issuing no DMA
-  const int nkt = (k_len + BN - 1) / BN;
-  const int valid_last = k_len - (nkt - 1) * BN;
+  int nkt = (k_len + BN - 1) / BN;
+  int valid_last = k_len - (nkt - 1) * BN;
+  // causal: query q0 + i of the segment sees the keys below i + 1 + (keys - queries), a row
+  // past the end as many as the last
+  const int kv_head = CAUSAL ? head / group : head;
+  int vlim[2] = {0, 0}, kdiag = 0, valid_rows = valid_last;
+  if constexpr (CAUSAL) {
+    const int ahead = k_len - q_end + 1;
+    nkt = min(nkt, max(min(cu_q[seg] + t * BM + BM, q_end) - 1 + ahead + BN - 1, 0) / BN);
+    valid_rows = min(k_len - (nkt - 1) * BN, BN);  // keys of the last tile that there are
+    valid_last = BN;                               // ... all of which the masks look at
+    kdiag = max(min(__builtin_amdgcn_readfirstlane(qrow0 - l32), q_end - 1) + ahead, 0) / BN;
+    vlim[0] = min(qrow0 + ahead, k_len) - 8 * hh;
+    vlim[1] = min(qrow1 + ahead, k_len) - 8 * hh;
+  }
   const int pk = padded_key_start(cu_k, seg);
   // Q rows past the segment end read its last row (their outputs are not stored);
   // the body forms each lane's 64-bit row address from qbase, its row and ldq
   const uint64_t qbase = (uint64_t)(uintptr_t)(Q + head * ql.hs + seg * ql.sa);
-  uint64_t kdma = (uint64_t)(uintptr_t)(Kp + head * kl.hs + seg * kl.sa + (int64_t)k_beg * ldk);
+  uint64_t kdma = (uint64_t)(uintptr_t)(Kp + kv_head * kl.hs + seg * kl.sa + (int64_t)k_beg * ldk);
   // joint: row j of the segment is row a0 + j of the "a" (image) operands while
   // j < len_a, else row b0 + j - len_a of the "b" (text) operands
   int len_a = 0, qseg = 0;
@@ -222,7 +260,7 @@ __global__ __launch_bounds__(256, 1) void flash_fwd_asm(
       qa[qb] = (uint64_t)(uintptr_t)(src + (int64_t)head * HD + hh * 8);
     }
   }
-  const uint64_t vdma = (uint64_t)(uintptr_t)(Vt + (int64_t)head * vt_hs + pk);
+  const uint64_t vdma = (uint64_t)(uintptr_t)(Vt + (int64_t)kv_head * vt_hs + pk);
   const uint32_t ktile = (uint32_t)(BN * ldk * 2);
   const uint32_t ldkb = (uint32_t)(ldk * 2);
   // LDS read bases (bytes within a stage): K rows permuted by kperm, 16-byte
@@ -252,7 +290,7 @@ __global__ __launch_bounds__(256, 1) void flash_fwd_asm(
     const uint32_t krow = (uint32_t)(r8 * 8 + lrow);
     const uint32_t kcolb = (uint32_t)(grp * 64 + ((r8 & 1) ? lsw1 : lsw0)) * 2;
     koff[i] = krow * ldkb + kcolb;
-    koffl[i] = min(krow, (uint32_t)(valid_last - 1)) * ldkb + kcolb;
+    koffl[i] = min(krow, (uint32_t)(valid_rows - 1)) * ldkb + kcolb;
     if constexpr (JOINT) krow_of[i] = krow;
     voff[i] = (uint32_t)((int64_t)(g * 8 + lrow) * vt_ld + ((g & 1) ? lsw1 : lsw0)) * 2;
   }
@@ -268,7 +306,23 @@ __global__ __launch_bounds__(256, 1) void flash_fwd_asm(
   auto su64 = [&](uint64_t x) { return ((uint64_t)su((uint32_t)(x >> 32)) << 32) | su((uint32_t)x); };
   const float sc = __builtin_bit_cast(float, su(__builtin_bit_cast(uint32_t, scale_log2)));
   (void)sc;
-  if constexpr (HD == 128 && !PRE && QB == 2) {
+  if constexpr (CAUSAL && HD == 128 && QB == 2) {
+    asm volatile(
+#include "attn_d128c_body.inc"
+        : : DITK_ATTN_ASM_OPERANDS_CAUSAL : DITK_D128_CLOBBERS "vcc", "scc", "memory");
+  } else if constexpr (CAUSAL && HD == 128 && QB == 1) {
+    asm volatile(
+#include "attn_d128cq1_body.inc"
+        : : DITK_ATTN_ASM_OPERANDS_CAUSAL : DITK_D128_CLOBBERS "vcc", "scc", "memory");
+  } else if constexpr (CAUSAL && HD == 64 && QB == 2) {
+    asm volatile(
+#include "attn_d64c_body.inc"
+        : : DITK_ATTN_ASM_OPERANDS_CAUSAL : DITK_D64_CLOBBERS "vcc", "scc", "memory");
+  } else if constexpr (CAUSAL && HD == 64 && QB == 1) {
+    asm volatile(
+#include "attn_d64cq1_body.inc"
+        : : DITK_ATTN_ASM_OPERANDS_CAUSAL : DITK_D64_CLOBBERS "vcc", "scc", "memory");
+  } else if constexpr (HD == 128 && !PRE && QB == 2) {
     asm volatile(
 #include "attn_d128_body.inc"
         : : DITK_ATTN_ASM_OPERANDS : DITK_D128_CLOBBERS "vcc", "scc", "memory");
@@ -460,6 +514,11 @@ int item_queries(int Tq, int nseg, int heads, int np, bool equal) {
   return most * heads <= ncu ? 128 : 256;
 }
 
+// Queries per work item of a causal launch: 128 when 256-query items would not fill the CUs
+int causal_item_queries(int Tq, int Tk, int nseg, int heads) {
+  return (int64_t)((Tq + 255) / 256) * heads < 2 * ditk_cu_count() ? 128 : 256;
+}
+
 // shared checks and launch of both attention entry points; sl2 = the factor that
 // takes q.k to log2 units inside the kernel (unused when pre); equal = the
 // segments are known to have Tq / nseg queries each
@@ -508,7 +567,7 @@ int flash_launch(const void* q, int64_t ldq, const void* k, int64_t ldk, const v
   kern<<<(unsigned)nblocks, 256, 0, stream>>>((const bf16_t*)q, ldq, (const bf16_t*)k, ldk, (const bf16_t*)vt, vt_ld,
                                               hs, (bf16_t*)o, ldo, lse, lse_ld, cu_q, cu_k, nseg, heads, np, chunk,
                                               stream_out, sl2, ql, kl, (const bf16_t*)q2, (const bf16_t*)kb,
-                                              (bf16_t*)ob, cu_a, cu_b);
+                                              (bf16_t*)ob, cu_a, cu_b, 1);
   return ditk_check_launch("ditk_flash_attn_varlen");
 }
 }  // namespace
@@ -542,6 +601,38 @@ DITK_EXPORT int ditk_joint_attn_q_prescaled(const void* q_a, const void* q_b, in
   return flash_launch(q_a, ldq, k_a, ldk, vt, vt_ld, o_a, ldo, nullptr, 0, cu_joint, cu_joint, nseg, T_joint, heads,
                       head_dim, 1.0f, true, RowLayout{head_dim, 0}, RowLayout{head_dim, 0}, stream, false, q_b, k_b, o_b,
                       cu_a, cu_b);
+}
+
+DITK_EXPORT int ditk_flash_attn_causal(const void* q, int64_t ldq, const void* k, int64_t ldk, const void* vt,
+                                       int64_t vt_ld, void* o, int64_t ldo, float* lse, int64_t lse_ld,
+                                       const int32_t* cu_q, const int32_t* cu_k, int nseg, int Tq, int Tk, int heads,
+                                       int kv_heads, int head_dim, float softmax_scale, hipStream_t stream) {
+  const char* what = "ditk_flash_attn_causal";
+  DITK_REQUIRE(softmax_scale >= 1e-30f && softmax_scale <= 1e30f, "%s: softmax_scale must be in 1e-30..1e30", what);
+  DITK_REQUIRE(cu_q && cu_k && (Tq == 0 || (q && o)) && (Tk == 0 || (k && vt)), "%s: null tensor", what);
+  DITK_REQUIRE(head_dim == 64 || head_dim == 128, "%s: head_dim must be 64 or 128, got %d", what, head_dim);
+  DITK_REQUIRE(nseg > 0 && Tq >= 0 && Tk >= 0 && Tq < (1 << 30) && Tk < (1 << 30), "%s: bad sizes", what);
+  DITK_REQUIRE(heads > 0 && kv_heads > 0 && heads % kv_heads == 0, "%s: %d query heads for %d key heads", what, heads,
+               kv_heads);
+  DITK_REQUIRE(ldq % 8 == 0 && ldk % 8 == 0 && ldo % 8 == 0 && vt_ld % 8 == 0 && vt_ld >= ditk_vt_columns(Tk, nseg),
+               "%s: leading dims must be multiples of 8, vt_ld at least ditk_vt_columns", what);
+  DITK_REQUIRE(((uintptr_t)q % 16) == 0 && ((uintptr_t)k % 16) == 0 && ((uintptr_t)vt % 16) == 0 &&
+                   ((uintptr_t)o % 16) == 0, "%s: misaligned tensor", what);
+  // the kernel addresses a 64-row K tile, HD Vt rows, and a row's bytes, with 32 bits
+  DITK_REQUIRE(ldq >= 0 && ldk >= 0 && ldo >= 0 && ldq < (1ll << 30) && ldo < (1ll << 30) && ldk < (1ll << 23) &&
+                   vt_ld < (1ll << 23), "%s: rows too long for 32-bit lane offsets", what);
+  if (Tq == 0) return 0;
+  const int qb = causal_item_queries(Tq, Tk, nseg, heads) / 128;
+  const int64_t nblocks = ((int64_t)(Tq + 128 * qb - 1) / (128 * qb) + nseg) * heads;
+  DITK_REQUIRE(nblocks < (1ll << 24), "%s: grid too large", what);
+  const bool stream_out = (int64_t)Tq * heads * head_dim * 2 >= (64ll << 20);
+  auto kern = head_dim == 128 ? (qb == 2 ? flash_fwd_asm<128, false, false, 2, true> : flash_fwd_asm<128, false, false, 1, true>)
+                              : (qb == 2 ? flash_fwd_asm<64, false, false, 2, true> : flash_fwd_asm<64, false, false, 1, true>);
+  kern<<<(unsigned)nblocks, 256, 0, stream>>>(
+      (const bf16_t*)q, ldq, (const bf16_t*)k, ldk, (const bf16_t*)vt, vt_ld, (int64_t)head_dim * vt_ld, (bf16_t*)o, ldo,
+      lse, lse_ld, cu_q, cu_k, nseg, heads, 1, 1, stream_out, softmax_scale * 1.4426950408889634f, RowLayout{head_dim, 0},
+      RowLayout{head_dim, 0}, nullptr, nullptr, nullptr, nullptr, nullptr, heads / kv_heads);
+  return ditk_check_launch(what);
 }
 
 DITK_EXPORT int ditk_attn_item_queries(int Tq, int Tk, int nseg, int heads, int equal, int joint) {

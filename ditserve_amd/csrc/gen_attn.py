@@ -45,7 +45,8 @@ v_accvgpr_write, an s_nop between an M0 write and the DMA that reads it.
 
 Usage: python gen_attn.py [dir/any]  (writes attn_d128_body.inc, attn_d128p_body.inc,
 attn_d64_body.inc, attn_d64p_body.inc, attn_d64j_body.inc and their
-*_clobbers.h into that directory, default beside this file)
+*_clobbers.h, and attn_d128c_body.inc and attn_d64c_body.inc, into that directory,
+default beside this file)
 """
 import os
 import sys
@@ -57,7 +58,7 @@ P_SET = (128, 160)
 BN = 64
 
 
-def configure(hd, pre=False, joint=False, qb=2):
+def configure(hd, pre=False, joint=False, qb=2, causal=False):
     """Head dim 128 or 64: NC 16-wide chunks of the head dim (K fragments per key
     half), DT 32-row d tiles of O^T, NF Vt fragments per tile (4 key groups x DT),
     ND DMA instructions per wave and operand per tile; AGPRs: O^T, then Q, the K
@@ -85,14 +86,22 @@ def configure(hd, pre=False, joint=False, qb=2):
     per key tile for the same fragment reads, so the reads are issued further ahead
     (a longer ring, from the registers the second block leaves free).  A query's
     arithmetic does not depend on it: rescales are decided for 64 queries, the blocks
-    of a wave or of a pair of one-block waves (flag_queries)."""
+    of a wave or of a pair of one-block waves (flag_queries).
+
+    causal (plain q, one query tile per work item): this lane's query of block qb sees the
+    keys below %[vlim{qb}] + 8 (lane / 32) only.  The wrapper ends the key loop behind the
+    last key that a query of the workgroup sees, and from tile %[kdiag] on, the first that
+    is not seen whole by every query of the wave, a tile's scores are set to -inf where they
+    are not seen, out of line, once they are complete (mask_scores).  The tile that holds a
+    segment's last key is such a tile for every wave, so no row sums are masked."""
     global QB, BM, KRING, KA, VRING, VA
     QB, BM = qb, 128 * qb
     KRING, KA, VRING, VA = (3, 2, 6, 4) if qb == 2 else (6, 4, 10, 8)
     global HD, NC, DT, NF, ND, KSTAGE_BYTES, VSTAGE_BYTES, O_A, Q_A, KF_A, VF_A, LAST_AGPR
-    global PRE, TMP, RING, DTMP, RS0, RS1, NEGM, NEGB, LRUN, KOFF, LAST_VGPR, EPI_T, EPI_L, JOINT
+    global PRE, TMP, RING, DTMP, RS0, RS1, NEGM, NEGB, LRUN, KOFF, LAST_VGPR, EPI_T, EPI_L, JOINT, CAUSAL
     assert pre or not joint
-    HD, PRE, JOINT = hd, pre, joint
+    assert not (causal and pre)
+    HD, PRE, JOINT, CAUSAL = hd, pre, joint, causal
     TMP = 192
     if pre:
         RING, DTMP = 2, 196
@@ -511,6 +520,26 @@ def scale_o(g, qb, alpha):
             g(f"v_accvgpr_write_b32 {ar(a)}, {vr(DTMP)}")
 
 
+def mask_scores(g, s_set, tile=None):
+    """Causal: scores of key tile `tile` (a scalar register; None: tile 0) in S set s_set become
+    -inf where this lane's query does not see the key.  Register v of key half kk holds key
+    32 kk + 16 (v / 8) + 8 (lane / 32) + v % 8."""
+    g.nops(20)  # the scores' MFMAs must have landed
+    if tile is not None:
+        g(f"s_lshl_b32 {s_(S_T1)}, {s_(tile)}, 6")
+    g(f"v_mov_b32 {vr(DTMP + 3)}, 0xff800000")
+    for qb in range(QB):
+        lim = f"%[vlim{qb}]"
+        if tile is not None:
+            g(f"v_subrev_u32 {vr(DTMP + 2)}, {s_(S_T1)}, {lim}")
+            lim = vr(DTMP + 2)
+        for kk in range(2):
+            for v in range(16):
+                r = vr(s_reg(s_set, qb, kk, v))
+                g(f"v_cmp_lt_i32 vcc, {kk * 32 + (v // 8) * 16 + v % 8}, {lim}")
+                g(f"v_cndmask_b32 {r}, {vr(DTMP + 3)}, {r}, vcc")
+
+
 def softmax_tile(g, s_set, p_set, qb, kks, rs_dst, masked=False):
     """Recompute P for the given key halves of query block qb from the raw scores
     and the running m (pre: from S = q.k - m); rs_dst += sum (masked: keys >=
@@ -695,6 +724,13 @@ def tile(g, a):
     g.label(after_check)
     for qb in range(QB):
         g(f"v_add_f32 {vr(LRUN + qb)}, {vr(LRUN + qb)}, {vr(DTMP + qb)}")
+    mask = masked = None
+    if CAUSAL:
+        mask, masked = g.new_label("mask"), g.new_label("masked")
+        g(f"s_add_u32 {s_(S_T0)}, {s_(S_KT)}, 1")
+        g(f"s_cmp_ge_u32 {s_(S_T0)}, %[kdiag]")
+        g(f"s_cbranch_scc1 {mask}")
+        g.label(masked)
     # phase 2: O += Vt(kt) P(kt) || P(kt+1) keys 0..31 from set b.  The wait
     # covers the VALU reads of the S(kt+1) results of the last MFMAs (already
     # three MFMAs old) and the MFMA reads of the P(kt) just packed.
@@ -712,7 +748,14 @@ def tile(g, a):
     for c in range(KA):
         k_read(g, c, 0, a)
         k_read(g, c, 1, a)
-    return resc, after_check
+    return resc, after_check, mask, masked
+
+
+def mask_block(g, a, mask, back):
+    """Out-of-line mask of tile kt + 1's scores (in set 1 - a, not yet read)."""
+    g.label(mask)
+    mask_scores(g, 1 - a, S_T0)
+    g(f"s_branch {back}")
 
 
 def rescale_block(g, a, resc, back):
@@ -760,7 +803,7 @@ def last_tile(g, a):
     # S MFMAs), K(0) and K(1) (no wave reads K any more: all passed the last
     # tile barrier), and, when this tile's Vt is in stage 1, Vt(0) into stage 0
     nopf = g.new_label("noprefetch")
-    multi = not JOINT  # joint work items are one query tile (one pass)
+    multi = not (JOINT or CAUSAL)  # their work items are one query tile (one pass)
     if multi:
         last_tile_prefetch(g, a, nopf)
     g.label(nopf)
@@ -770,8 +813,9 @@ def last_tile(g, a):
     recompute = g.new_label("lastrecompute")
     common = g.new_label("lastpv")
     reuse_back = g.new_label("lastreuseback")
-    g(f"s_cmp_eq_u32 {s_(S_VALID)}, {BN}")
-    g(f"s_cbranch_scc0 {recompute}")
+    if not CAUSAL:
+        g(f"s_cmp_eq_u32 {s_(S_VALID)}, {BN}")
+        g(f"s_cbranch_scc0 {recompute}")
     g(f"s_cmp_eq_u32 {s_(S_NKT1)}, 0")
     g(f"s_cbranch_scc1 {recompute}")
     for it in make_items(g, pair_list(1), a, a, RS1):
@@ -790,23 +834,25 @@ def last_tile(g, a):
     g.label(recompute)
     for qb in range(QB):
         g(f"v_mov_b32 {vr(RS0 + qb)}, 0")
-    g(f"s_cmp_eq_u32 {s_(S_VALID)}, {BN}")
-    g(f"s_cbranch_scc1 {full}")
-    for qb in range(QB):
-        softmax_tile(g, a, a, qb, (0, 1), RS0, masked=True)
-    g(f"s_branch {done_rs}")
-    g.label(full)
+    if not CAUSAL:
+        g(f"s_cmp_eq_u32 {s_(S_VALID)}, {BN}")
+        g(f"s_cbranch_scc1 {full}")
+        for qb in range(QB):
+            softmax_tile(g, a, a, qb, (0, 1), RS0, masked=True)
+        g(f"s_branch {done_rs}")
+        g.label(full)
     for qb in range(QB):
         softmax_tile(g, a, a, qb, (0, 1), RS0, masked=False)
     g.label(done_rs)
     _, clear = flag_queries(g, RS0)
     g(f"{clear} {checked}")
     # rescale against the exact tile max (masked sums)
-    g(f"s_cmp_eq_u32 {s_(S_VALID)}, {BN}")
-    g(f"s_cbranch_scc1 {resc}")
-    exact_rescale(g, a, a, (0, 1), masked=True)
-    g(f"s_branch {checked}")
-    g.label(resc)
+    if not CAUSAL:
+        g(f"s_cmp_eq_u32 {s_(S_VALID)}, {BN}")
+        g(f"s_cbranch_scc1 {resc}")
+        exact_rescale(g, a, a, (0, 1), masked=True)
+        g(f"s_branch {checked}")
+        g.label(resc)
     exact_rescale(g, a, a, (0, 1), masked=False)
     g.label(checked)
     for qb in range(QB):
@@ -931,9 +977,17 @@ def pass_start(g):
         k_read(g, c, 1, 0)
     s_phase(g, 0, kstage=0, first=True)
     g.nops(20)
+    if CAUSAL:
+        seen = g.new_label("tile0seen")
+        g("s_cmp_lg_u32 %[kdiag], 0")
+        g(f"s_cbranch_scc1 {seen}")
+        mask_scores(g, 0)
+        g.label(seen)
     # m = exact max of tile 0 (pre: S(0) -= m, and the -m blocks)
     for qb in range(QB):
         row_max_to(g, 0, qb, DTMP + 1, DTMP + 2, DTMP + 3)
+        if CAUSAL:  # a query that sees no key: m stays finite, so that its probabilities are 0
+            g(f"v_max_f32 {vr(DTMP + 1)}, 0xff7fffff, {vr(DTMP + 1)}")
         if PRE:
             for kk in range(2):
                 for v in range(16):
@@ -1129,15 +1183,18 @@ def generate():
     for it in items:
         it()
     g.label(loop)
-    ra, ba = tile(g, 0)
+    ra, ba, *ma = tile(g, 0)
     g(f"s_cmp_ge_u32 {s_(S_KT)}, {s_(S_NKT1)}")
     g(f"s_cbranch_scc1 {last_b}")
-    rb, bb = tile(g, 1)
+    rb, bb, *mb = tile(g, 1)
     g(f"s_cmp_lt_u32 {s_(S_KT)}, {s_(S_NKT1)}")
     g(f"s_cbranch_scc1 {loop}")
     g(f"s_branch {last_a}")
     rescale_block(g, 0, ra, ba)
     rescale_block(g, 1, rb, bb)
+    if CAUSAL:
+        mask_block(g, 0, *ma)
+        mask_block(g, 1, *mb)
     g.label(last_a)
     last_tile(g, 0)
     g(f"s_branch {fin}")
@@ -1179,12 +1236,12 @@ def clobbers(hd, pre=False, joint=False):
             f"#define DITK_D{name.upper()}_CLOBBERS \\\n" + "".join(f"  {r}, \\\n" for r in rows) + "\n")
 
 
-def write_body(path, hd, pre=False, joint=False, qb=2):
-    configure(hd, pre, joint, qb)
+def write_body(path, hd, pre=False, joint=False, qb=2, causal=False):
+    configure(hd, pre, joint, qb, causal)
     lines = generate()
     with open(path, "w") as f:
         f.write(f"// Generated by gen_attn.py -- the instruction body of flash_fwd_asm<{hd}, {str(pre).lower()}, "
-                f"{str(joint).lower()}, {qb}>.\n")
+                f"{str(joint).lower()}, {qb}{', true' if causal else ''}>.\n")
         for line in lines:
             esc = line.replace("\\", "\\\\").replace('"', '\\"')
             f.write(f'"{esc}\\n"\n')
@@ -1200,6 +1257,9 @@ def main(argv):
             write_body(os.path.join(out, f"attn_{name}{'' if qb == 2 else 'q1'}_body.inc"), hd, pre, joint, qb)
         with open(os.path.join(out, f"attn_{name}_clobbers.h"), "w") as f:
             f.write(clobbers(hd, pre, joint))
+    for hd in (128, 64):  # causal: the registers of the plain body
+        for qb in (2, 1):
+            write_body(os.path.join(out, f"attn_d{hd}c{'' if qb == 2 else 'q1'}_body.inc"), hd, qb=qb, causal=True)
     return 0
 
 

@@ -25,8 +25,8 @@ import math
 import torch
 
 from . import _lib, ops
-from .mx import _apart, _call, _one_device
-from .ops import _check, _ptr, _rows
+from .mx import _apart
+from .ops import _call, _check, _one_device, _ptr, _rows
 
 PAGES = (16, 32, 64, 128, 256)
 HEAD_DIMS = (64, 128)

@@ -15,8 +15,8 @@ counterpart: its products are in fp16 or bf16.
 """
 import torch
 
-from . import _lib, ops
-from .ops import EPILOGUES, _check, _extent, _meet, _ptr, _rows, _vec
+from . import ops
+from .ops import EPILOGUES, _beside, _call, _check, _extent, _meet, _one_device, _ptr, _rows, _vec
 
 FORMATS = {"fp8": 0, "fp4": 1}
 _BF16, _E4M3, _E8M0 = torch.bfloat16, torch.float8_e4m3fn, torch.float8_e8m0fnu
@@ -119,15 +119,6 @@ class MXTensor:
         return d.data_ptr(), d.stride(0), s.data_ptr(), s.stride(0)
 
 
-def _call(device, name, *args):
-    """Launch on the current stream of `device`, which need not be the current device."""
-    index = device.index
-    if index == torch._C._cuda_getDevice():
-        return _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(index))
-    with torch.cuda.device(index):
-        return _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(index))
-
-
 def _bf16_rows(t, name):
     """(rows, columns, row stride, address) of a bf16 row view, or the refusal of what is none."""
     if t.__class__ is torch.Tensor and t.dtype is _BF16 and t.is_cuda:
@@ -136,13 +127,6 @@ def _bf16_rows(t, name):
             return (*t.shape, st[0], t.data_ptr())
     _check(t, name, _BF16, 2)
     return (*t.shape, _rows(t, name), t.data_ptr())
-
-
-def _one_device(device, *tensors):
-    """Refuse operands on another device (pairs of a name and a tensor or None)."""
-    for name, t in tensors:
-        if t is not None and t.device != device:
-            raise ValueError(f"{name} is on {t.device}, the other operands on {device}")
 
 
 def _mx_check(m, name, fmt=None):
@@ -160,17 +144,6 @@ def _mx_out(out, rows, cols, device, fmt):
         raise ValueError(f"out must be [{rows}, {cols}], got {out.shape}")
     _one_device(device, ("out", out))
     return out
-
-
-def _beside(a, b):
-    """Whether two row views of one row stride hold different columns of a buffer."""
-    if a.dim() != 2 or b.dim() != 2:
-        return False
-    line = a.stride(0) * a.element_size()
-    if line <= 0 or b.stride(0) * b.element_size() != line:
-        return False
-    first, width = (b.data_ptr() - a.data_ptr()) % line, b.shape[1] * b.element_size()
-    return a.shape[1] * a.element_size() <= first and first + width <= line
 
 
 def _apart(fn, outs, operands, same=()):

@@ -38,6 +38,22 @@ def _check(t, name, dtype=None, dims=None):
         raise ValueError(f"{name} must be {dims}-D, got shape {tuple(t.shape)}")
 
 
+def _call(device, name, *args):
+    """Launch on the current stream of `device`, which need not be the current device."""
+    index = device.index
+    if index == torch._C._cuda_getDevice():
+        return _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(index))
+    with torch.cuda.device(index):
+        return _lib.call(name, *args, torch._C._cuda_getCurrentRawStream(index))
+
+
+def _one_device(device, *tensors):
+    """Refuse operands on another device (pairs of a name and a tensor or None)."""
+    for name, t in tensors:
+        if t is not None and t.device != device:
+            raise ValueError(f"{name} is on {t.device}, the other operands on {device}")
+
+
 def to_device(data, dtype, device):
     """Small host table -> device tensor without stalling the host: the values go
     through pinned memory and a non-blocking copy on the current stream (a
@@ -505,6 +521,17 @@ def _overlap(a, b):
     return _meet(_extent(a), _extent(b))
 
 
+def _beside(a, b):
+    """Whether two row views of one row stride hold different columns of a buffer."""
+    if a.dim() != 2 or b.dim() != 2:
+        return False
+    line = a.stride(0) * a.element_size()
+    if line <= 0 or b.stride(0) * b.element_size() != line:
+        return False
+    first, width = (b.data_ptr() - a.data_ptr()) % line, b.shape[1] * b.element_size()
+    return a.shape[1] * a.element_size() <= first and first + width <= line
+
+
 def _disjoint_jobs(fn, jobs_io):
     """jobs_io: per job (outputs, operands).  The jobs of one launch run
     concurrently, so no job's output may overlap another job's operands or
@@ -639,6 +666,57 @@ def flash_attn_varlen(q, k, v, seg_q, seg_k, heads, head_dim, softmax_scale=None
     scale = 1.0 / math.sqrt(head_dim) if softmax_scale is None else float(softmax_scale)
     _lib.call("ditk_flash_attn_varlen", _ptr(q), ldq, kp, ldk, _ptr(vt), vt.shape[2], _ptr(out), ldo,
               _ptr(lse), Tq, _ptr(seg_q.dev), _ptr(seg_k.dev), seg_q.nseg, Tq, heads, head_dim, scale, _stream())
+    return (out, lse) if return_lse else out
+
+
+def flash_attn_causal(q, k, v, seg_q, seg_k, heads, kv_heads, head_dim, softmax_scale=None, return_lse=False,
+                      out=None):
+    """Causal attention of packed prompts, with query heads in groups.
+
+    q [Tq, heads * head_dim], k / v [Tk, kv_heads * head_dim] bf16 row views (columns of one fused
+    projection, for instance), head_dim 64 or 128; query head h reads key head
+    h // (heads / kv_heads).  Segment m has as many keys as seg_k says; its queries are the last of
+    them: query i of nq sees the keys j <= i + nk - nq (with earlier keys in front, the next part of
+    a prompt; a query that sees none gives zeros and an lse of -inf).  Returns out
+    [Tq, heads * head_dim] (and lse [heads, Tq] fp32, natural log, when return_lse).  A segment's
+    result does not depend on what it is packed with.  Values must be finite: an infinity or NaN
+    may also reach queries of the same 256 that do not see it."""
+    if heads <= 0 or kv_heads <= 0 or heads % kv_heads:
+        raise ValueError(f"heads must be a multiple of kv_heads, got {heads} and {kv_heads}")
+    if head_dim not in (64, 128):
+        raise ValueError(f"head_dim must be 64 or 128, got {head_dim}")
+    for t, n, h in ((q, "q", heads), (k, "k", kv_heads), (v, "v", kv_heads)):
+        _check(t, n, _BF16, 2)
+        if t.shape[1] != h * head_dim:
+            raise ValueError(f"{n} must have {h * head_dim} columns, got {t.shape[1]}")
+    Tq, Tk, device = q.shape[0], k.shape[0], q.device
+    if v.shape[0] != Tk:
+        raise ValueError(f"k and v must have the same rows, got {Tk} and {v.shape[0]}")
+    if seg_q.nseg != seg_k.nseg:
+        raise ValueError("cu_seqlens_q and cu_seqlens_k must describe the same number of segments")
+    if seg_q.total != Tq or seg_k.total != Tk:
+        raise ValueError("cu_seqlens totals must match the packed token counts")
+    _one_device(device, ("k", k), ("v", v), ("seg_q", seg_q.dev), ("seg_k", seg_k.dev))
+    ldq, ldk, ldv = _rows(q, "q"), _rows(k, "k"), _rows(v, "v")
+    if out is None:
+        out, ldo = torch.empty((Tq, heads * head_dim), dtype=_BF16, device=device), heads * head_dim
+    else:
+        _check(out, "out", _BF16, 2)
+        _one_device(device, ("out", out))
+        if out.shape != q.shape:
+            raise ValueError(f"out must be {tuple(q.shape)}, got {tuple(out.shape)}")
+        ldo = _rows(out, "out")
+        for t, n in ((q, "q"), (k, "k"), (v, "v")):
+            if _overlap(out, t) and not _beside(out, t):
+                raise ValueError(f"out overlaps {n}")
+    scale = 1.0 / math.sqrt(head_dim) if softmax_scale is None else float(softmax_scale)
+    lse = torch.empty((heads, Tq), dtype=torch.float32, device=device) if return_lse else None
+    if Tq:
+        cols = vt_columns(Tk, seg_k.nseg)
+        vt = torch.empty((kv_heads, head_dim, cols), dtype=_BF16, device=device)
+        _call(device, "ditk_transpose_v", _ptr(v), ldv, _ptr(vt), cols, Tk, kv_heads, head_dim, _ptr(seg_k.dev), seg_k.nseg)
+        _call(device, "ditk_flash_attn_causal", _ptr(q), ldq, _ptr(k), ldk, _ptr(vt), cols, _ptr(out), ldo, _ptr(lse), Tq,
+              _ptr(seg_q.dev), _ptr(seg_k.dev), seg_q.nseg, Tq, Tk, heads, kv_heads, head_dim, scale)
     return (out, lse) if return_lse else out
 
 

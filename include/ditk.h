@@ -461,6 +461,18 @@ int ditk_mx_matvec(const void* x, int64_t ldx, const void* W, int64_t ldw, const
 int ditk_mx_matvec_plan(int M, int N, int K, int* plan);
 
 /*
+ * Causal attention of packed prompts with grouped heads (heads a multiple of kv_heads: query head h
+ * reads key head h / (heads / kv_heads)).  A segment's queries are the last of its keys: query i of
+ * nq sees the keys j <= i + nk - nq; one that sees none gives zeros and lse -inf.  vt:
+ * ditk_transpose_v's of the kv_heads value heads; the rest as ditk_flash_attn_varlen.
+ * No reference counterpart: the reference's attention is non-causal with one key head a query head.
+ */
+int ditk_flash_attn_causal(const void* q, int64_t ldq, const void* k, int64_t ldk, const void* vt, int64_t vt_ld,
+                           void* o, int64_t ldo, float* lse, int64_t lse_ld, const int32_t* cu_q,
+                           const int32_t* cu_k, int nseg, int Tq, int Tk, int heads, int kv_heads, int head_dim,
+                           float softmax_scale, ditk_stream_t stream);
+
+/*
  * Paged key-value caches.  A cache of `pages` pages of `page` slots (16, 32, 64, 128 or 256) holds
  * keys and values [page][head_dim] bf16 (head_dim 64 or 128), contiguous, for each (page, key head),
  * with a page stride *_ps and a head stride *_hs (elements, multiples of 8); weights (fp32, may be
