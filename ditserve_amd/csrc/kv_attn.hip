@@ -15,20 +15,24 @@
 
 namespace {
 
-constexpr int kMinChunk = 256, kMaxChunks = 128;
+constexpr int kMaxChunks = 512;
 
-// slots of a chunk of a sequence of n: at most kMaxChunks of them, whole 32-slot tiles for four waves
+// slots of a chunk of a sequence of n, whole 32-slot tiles
 __host__ __device__ inline int chunk_slots(int n) {
-  const int64_t least = ((int64_t)n + kMaxChunks - 1) / kMaxChunks;
-  const int c = (int)((least + 127) / 128 * 128);
-  return c < kMinChunk ? kMinChunk : c;
+  if (n <= 1024) return 64;
+  if (n <= 8192) return 128;
+  if (n <= 65536) return 256;
+  if (n <= 512 * kMaxChunks) return 512;
+  return (int)(((int64_t)n + kMaxChunks * 128 - 1) / (kMaxChunks * 128) * 128);
 }
 __host__ __device__ inline int chunks_of(int n) { return n == 0 ? 1 : (n - 1) / chunk_slots(n) + 1; }
 
-// the most chunks of any sequence up to `most` slots (fewer are possible past a change of the chunk's length)
+// the most chunks of any sequence up to `most` slots
 int chunks_bound(int most) {
-  const int c = most / kMinChunk + (most % kMinChunk != 0);
-  return c < 1 ? 1 : c > kMaxChunks ? kMaxChunks : c;
+  int c = chunks_of(most);
+  for (int n : {1024, 8192, 65536, 512 * kMaxChunks})
+    if (n < most && chunks_of(n) > c) c = chunks_of(n);
+  return most > 512 * kMaxChunks ? kMaxChunks : c;
 }
 
 struct Args {
@@ -45,7 +49,7 @@ struct Args {
   float* ml;      // [batch * heads][nchunk][2]
   float* score;   // [batch * heads][ld_score], or null
   int64_t ld_score;
-  int heads, group, nchunk;
+  int heads, group, nchunk, batch, hgroups;  // hgroups: (key head, 16 of its query heads) pairs
   float scale2;   // softmax scale times log2 e
 };
 
@@ -65,233 +69,283 @@ __device__ __forceinline__ float group_sumf(float v) {
 
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 
+// A wave takes one chunk of one (sequence, key head, 16 query heads) after another; units go round the waves in
+// order: a sequence's chunks, and for each its heads, which lie side by side in a page.
 template <int HD, bool SCORES>
-__global__ __launch_bounds__(256) void kv_attn_kernel(Args a) {
+__global__ __launch_bounds__(256, 3) void kv_attn_kernel(Args a) {
   constexpr int NC = HD / 32, ND = HD / 16, CH = HD / 8, RPL = 64 / CH;  // RPL: rows of V a load of the wave covers
-  constexpr int OP = HD + 4;                                           // floats of a row of O in LDS
-  __shared__ __align__(16) char lds[4 * 16 * OP * 4];
-  __shared__ float stat[2][4][16];
-  static_assert(sizeof(lds) >= 4 * 32 * HD * 2, "V tiles");
-  const int b = blockIdx.z, tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
-  const int groups = (a.group + 15) / 16, kvh = blockIdx.y / groups, g0 = (blockIdx.y % groups) * 16;
-  const int chunk = blockIdx.x;
-  const int n = kv_length(a.t, b, tid == 0 && chunk == 0 && blockIdx.y == 0);
-  if (chunk >= chunks_of(n)) return;
-  const int csl = chunk_slots(n), s0 = chunk * csl, s1 = min(n, s0 + csl), last = max(n - 1, 0);
+  __shared__ __align__(16) char lds[4 * 32 * HD * 2];
+  __shared__ int sums[4];
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
   const int col = lane & 15, quad = lane >> 4;
-  const int nq = min(a.group - g0, 16), head0 = kvh * a.group + g0;  // query heads of this workgroup
   const int pl = a.t.page_log2, low = (1 << pl) - 1;
-
-  bf16x8_t q[NC];
-  {
-    const bf16_t* qr = a.q + b * a.ldq + (int64_t)(head0 + min(col, nq - 1)) * HD + quad * 8;
-#pragma unroll
-    for (int c = 0; c < NC; ++c) q[c] = *reinterpret_cast<const bf16x8_t*>(qr + c * 32);
-  }
-  f32x4_t o[ND];
-#pragma unroll
-  for (int j = 0; j < ND; ++j) o[j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-  float m = -INFINITY, l = 0.f;
   char* vt = lds + wave * (32 * HD * 2);
 
-  for (int t0 = s0 + wave * 32; t0 < s1; t0 += 128) {
-    // the tile's two halves of 16 slots lie in one page each; slots past the last read it
-    const int e0 = min(t0, last), e1 = min(t0 + 16, last);
-    bool ok0, ok1;
-    const int p0 = kv_page(a.t, b, e0, ok0, true), p1 = kv_page(a.t, b, e1, ok1, true);
-    const bf16_t* kb0 = a.k.p + p0 * a.k.ps + kvh * a.k.hs;
-    const bf16_t* kb1 = a.k.p + p1 * a.k.ps + kvh * a.k.hs;
-    const bf16_t* vb0 = a.v.p + p0 * a.v.ps + kvh * a.v.hs;
-    const bf16_t* vb1 = a.v.p + p1 * a.v.ps + kvh * a.v.hs;
-    bf16x8_t k[2][NC];
+  // chunks before thread t's sequences [t per, t per + per)
+  const int per = (a.batch + 255) / 256;
+  int mine = 0;
+  for (int i = 0; i < per; ++i)
+    if (tid * per + i < a.batch) mine += chunks_of(kv_length(a.t, tid * per + i, blockIdx.x == 0));
+  int incl = mine;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int slot = min(t0 + 8 * (col >> 2) + 4 * i + (col & 3), last);
-      const bf16_t* kr = (col < 8 ? kb0 : kb1) + (int64_t)(slot & low) * HD + quad * 8;
+  for (int off = 1; off < 64; off <<= 1) {
+    const int o = __shfl_up(incl, off, 64);
+    if (lane >= off) incl += o;
+  }
+  if (lane == 63) sums[wave] = incl;
+  __syncthreads();
+  // every wave keeps all 256 sums: lane l those of threads l, 64 + l, 128 + l, 192 + l
+  __shared__ int ends[256];
+  for (int w = 0; w < wave; ++w) incl += sums[w];
+  ends[tid] = incl;
+  __syncthreads();
+  int end[4];
 #pragma unroll
-      for (int c = 0; c < NC; ++c) k[i][c] = *reinterpret_cast<const bf16x8_t*>(kr + c * 32);
+  for (int i = 0; i < 4; ++i) end[i] = ends[i * 64 + lane];
+  const int units = __builtin_amdgcn_readlane(end[3], 63) * a.hgroups;
+
+  for (int u = blockIdx.x * 4 + wave; u < units; u += gridDim.x * 4) {
+    const int c = u / a.hgroups, hg = u - c * a.hgroups;
+    // the thread whose sequences hold chunk c, then the sequence
+    int th = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) th += __popcll(__ballot(end[i] <= c));
+    int b = th * per, chunk = c - (th ? ends[th - 1] : 0);
+    int n = kv_length(a.t, b, false), nch = chunks_of(n);
+    while (chunk >= nch && b + 1 < a.batch) {
+      chunk -= nch;
+      n = kv_length(a.t, ++b, false);
+      nch = chunks_of(n);
     }
-    u32x4_t v[32 / RPL];
+    b = __builtin_amdgcn_readfirstlane(b);
+    n = __builtin_amdgcn_readfirstlane(n);
+    chunk = __builtin_amdgcn_readfirstlane(min(chunk, a.nchunk - 1));
+    const int groups = (a.group + 15) / 16, kvh = hg / groups, g0 = (hg - kvh * groups) * 16;
+    const int csl = chunk_slots(n), s0 = chunk * csl, s1 = min(n, s0 + csl), last = max(n - 1, 0);
+    const int nq = min(a.group - g0, 16), head0 = kvh * a.group + g0;  // query heads of this unit
+
+    bf16x8_t q[NC];
+    {
+      const bf16_t* qr = a.q + b * a.ldq + (int64_t)(head0 + min(col, nq - 1)) * HD + quad * 8;
 #pragma unroll
-    for (int i = 0; i < 32 / RPL; ++i) {
-      const int row = i * RPL + lane / CH, slot = min(t0 + row, last);
-      v[i] = *reinterpret_cast<const u32x4_t*>((i * RPL < 16 ? vb0 : vb1) + (int64_t)(slot & low) * HD + (lane % CH) * 8);
+      for (int i = 0; i < NC; ++i) q[i] = *reinterpret_cast<const bf16x8_t*>(qr + i * 32);
     }
-    // values of absent slots may be anything: they count as 0
-    const int n0 = ok0 ? min(s1 - t0, 16) : 0, n1 = ok1 ? s1 - t0 - 16 : 0;
-    const bool whole = n0 == 16 && n1 >= 16;
-    if (!whole) {
+    f32x4_t o[ND];
 #pragma unroll
-      for (int i = 0; i < 32 / RPL; ++i) {
-        const int row = i * RPL + lane / CH;
-        if (i * RPL < 16 ? row >= n0 : row - 16 >= n1) v[i] = u32x4_t{0, 0, 0, 0};
-      }
-    }
-    f32x4_t s[2];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      s[i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int c = 0; c < NC; ++c) s[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k[i][c], q[c], s[i], 0, 0, 0);
-    }
-    float x[8], top = -INFINITY;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      x[e] = s[e >> 2][e & 3] * a.scale2;
-      const int row = quad * 8 + e;
-      if (!whole && (row < 16 ? row >= n0 : row - 16 >= n1)) x[e] = -INFINITY;
-      top = fmaxf(top, x[e]);
-    }
-    if (SCORES) {
-      if (col < nq) {
-        float* sr = a.score + ((int64_t)b * a.heads + head0 + col) * a.ld_score + t0 + quad * 8;
-        *reinterpret_cast<f32x4_t*>(sr) = f32x4_t{x[0], x[1], x[2], x[3]};
-        *reinterpret_cast<f32x4_t*>(sr + 4) = f32x4_t{x[4], x[5], x[6], x[7]};
-      }
-    }
-    const float mn = fmaxf(m, group_maxf(top));
-    if (__any(mn > m)) {
-      const float al = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
-      l *= al;
-#pragma unroll
-      for (int j = 0; j < ND; ++j)
-#pragma unroll
-        for (int r = 0; r < 4; ++r) o[j][r] *= al;
-      m = mn;
-    }
-    const float base = m == -INFINITY ? 0.f : m;
-    bf16x8_t hi, lo;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      const float p = __builtin_amdgcn_exp2f(x[e] - base);
-      l += p;
-      // hi cut off, so that lo is not negative, and lo not 0 unless p is: an infinite value stays one
-      const float cut = __uint_as_float(__float_as_uint(p) & 0xffff0000u);
-      hi[e] = __builtin_bit_cast(__bf16, (uint16_t)(__float_as_uint(p) >> 16));
-      lo[e] = (__bf16)fmaxf(p - cut, fminf(p, 1.17549435e-38f));
-    }
-#pragma unroll
-    for (int i = 0; i < 32 / RPL; ++i) {
-      const int row = i * RPL + lane / CH, ch = lane % CH;
-      *reinterpret_cast<u32x4_t*>(vt + row * (HD * 2) + (((ch >> 1) ^ v_swizzle<HD>(row)) * 32) + (ch & 1) * 16) = v[i];
-    }
-    // lane i of a quad reads 8 bytes of row i / 4 and gets 4 rows of column i
-#pragma unroll
-    for (int j = 0; j < ND; ++j) {
-      s16x4 w[2];
+    for (int j = 0; j < ND; ++j) o[j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    float m = -INFINITY, l = 0.f;
+
+    for (int t0 = s0; t0 < s1; t0 += 32) {
+      // the tile's two halves of 16 slots lie in one page each; slots past the last read it
+      const int e0 = min(t0, last), e1 = min(t0 + 16, last);
+      bool ok0, ok1;
+      const int p0 = kv_page(a.t, b, e0, ok0, true), p1 = kv_page(a.t, b, e1, ok1, true);
+      const bf16_t* kb0 = a.k.p + p0 * a.k.ps + kvh * a.k.hs;
+      const bf16_t* kb1 = a.k.p + p1 * a.k.ps + kvh * a.k.hs;
+      const bf16_t* vb0 = a.v.p + p0 * a.v.ps + kvh * a.v.hs;
+      const bf16_t* vb1 = a.v.p + p1 * a.v.ps + kvh * a.v.hs;
+      bf16x8_t k[2][NC];
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const int row = quad * 8 + 4 * i + (col >> 2);
-        const char* p = vt + row * (HD * 2) + ((j ^ v_swizzle<HD>(row)) * 32) + (col & 3) * 8;
-        w[i] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p);
+        const int slot = min(t0 + 8 * (col >> 2) + 4 * i + (col & 3), last);
+        const bf16_t* kr = (col < 8 ? kb0 : kb1) + (int64_t)(slot & low) * HD + quad * 8;
+#pragma unroll
+        for (int c = 0; c < NC; ++c) k[i][c] = *reinterpret_cast<const bf16x8_t*>(kr + c * 32);
       }
-      union { s16x4 h[2]; bf16x8_t f; } f;
-      f.h[0] = w[0];
-      f.h[1] = w[1];
-      o[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f.f, hi, o[j], 0, 0, 0);
-      o[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f.f, lo, o[j], 0, 0, 0);
+      u32x4_t v[32 / RPL];
+#pragma unroll
+      for (int i = 0; i < 32 / RPL; ++i) {
+        const int row = i * RPL + lane / CH, slot = min(t0 + row, last);
+        v[i] = *reinterpret_cast<const u32x4_t*>((i * RPL < 16 ? vb0 : vb1) + (int64_t)(slot & low) * HD + (lane % CH) * 8);
+      }
+      // values of absent slots may be anything: they count as 0
+      const int n0 = ok0 ? min(s1 - t0, 16) : 0, n1 = ok1 ? s1 - t0 - 16 : 0;
+      const bool whole = n0 == 16 && n1 >= 16;
+      if (!whole) {
+#pragma unroll
+        for (int i = 0; i < 32 / RPL; ++i) {
+          const int row = i * RPL + lane / CH;
+          if (i * RPL < 16 ? row >= n0 : row - 16 >= n1) v[i] = u32x4_t{0, 0, 0, 0};
+        }
+      }
+      f32x4_t s[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        s[i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int c = 0; c < NC; ++c) s[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k[i][c], q[c], s[i], 0, 0, 0);
+      }
+      float x[8], top = -INFINITY;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        x[e] = s[e >> 2][e & 3] * a.scale2;
+        const int row = quad * 8 + e;
+        if (!whole && (row < 16 ? row >= n0 : row - 16 >= n1)) x[e] = -INFINITY;
+        top = fmaxf(top, x[e]);
+      }
+      if (SCORES) {
+        if (col < nq) {
+          float* sr = a.score + ((int64_t)b * a.heads + head0 + col) * a.ld_score + t0 + quad * 8;
+          *reinterpret_cast<f32x4_t*>(sr) = f32x4_t{x[0], x[1], x[2], x[3]};
+          *reinterpret_cast<f32x4_t*>(sr + 4) = f32x4_t{x[4], x[5], x[6], x[7]};
+        }
+      }
+      const float mn = fmaxf(m, group_maxf(top));
+      if (__any(mn > m)) {
+        const float al = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
+        l *= al;
+#pragma unroll
+        for (int j = 0; j < ND; ++j)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) o[j][r] *= al;
+        m = mn;
+      }
+      const float base = m == -INFINITY ? 0.f : m;
+      bf16x8_t hi, lo;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float p = __builtin_amdgcn_exp2f(x[e] - base);
+        l += p;
+        // hi cut off, so that lo is not negative, and lo not 0 unless p is: an infinite value stays one
+        const float cut = __uint_as_float(__float_as_uint(p) & 0xffff0000u);
+        hi[e] = __builtin_bit_cast(__bf16, (uint16_t)(__float_as_uint(p) >> 16));
+        lo[e] = (__bf16)fmaxf(p - cut, fminf(p, 1.17549435e-38f));
+      }
+#pragma unroll
+      for (int i = 0; i < 32 / RPL; ++i) {
+        const int row = i * RPL + lane / CH, ch = lane % CH;
+        *reinterpret_cast<u32x4_t*>(vt + row * (HD * 2) + (((ch >> 1) ^ v_swizzle<HD>(row)) * 32) + (ch & 1) * 16) = v[i];
+      }
+      // lane i of a quad reads 8 bytes of row i / 4 and gets 4 rows of column i
+#pragma unroll
+      for (int j = 0; j < ND; ++j) {
+        s16x4 w[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int row = quad * 8 + 4 * i + (col >> 2);
+          const char* p = vt + row * (HD * 2) + ((j ^ v_swizzle<HD>(row)) * 32) + (col & 3) * 8;
+          w[i] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p);
+        }
+        union { s16x4 h[2]; bf16x8_t f; } f;
+        f.h[0] = w[0];
+        f.h[1] = w[1];
+        o[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f.f, hi, o[j], 0, 0, 0);
+        o[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f.f, lo, o[j], 0, 0, 0);
+      }
     }
-  }
 
-  // the four waves' parts, in order
-  l = group_sumf(l);
-  if (quad == 0) {
-    stat[0][wave][col] = m;
-    stat[1][wave][col] = l;
-  }
-  __syncthreads();
-  const float top = fmaxf(fmaxf(stat[0][0][col], stat[0][1][col]), fmaxf(stat[0][2][col], stat[0][3][col]));
-  // (a part without a finite score is 0, or NaN and stays it)
-  const float f = m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - top);
-  float* ob = reinterpret_cast<float*>(lds) + wave * 16 * OP;
+    // lane: dims 16 j + 4 quad .. + 3 of query head `col`
+    l = group_sumf(l);
+    if (col < nq) {
+      const int64_t row = (int64_t)b * a.heads + head0 + col;
+      if (nch == 1) {
+        const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
+        bf16_t* ob = a.o + b * a.ldo + (int64_t)(head0 + col) * HD + quad * 4;
 #pragma unroll
-  for (int j = 0; j < ND; ++j) {
-    f32x4_t x = o[j];
+        for (int j = 0; j < ND; ++j)
+          *reinterpret_cast<u32x2_t*>(ob + j * 16) = u32x2_t{pack_bf2(o[j][0] * inv, o[j][1] * inv),
+                                                            pack_bf2(o[j][2] * inv, o[j][3] * inv)};
+        if (quad == 0) {
+          const float e = l > 0.f || l != l ? m + __builtin_amdgcn_logf(l) : -INFINITY;
+          if (a.lse != nullptr) a.lse[row] = e * 0.6931471805599453f;
+          if (SCORES) a.lse2[row] = e;
+        }
+      } else {
+        float* pb = a.part + (row * a.nchunk + chunk) * HD + quad * 4;
 #pragma unroll
-    for (int r = 0; r < 4; ++r) x[r] *= f;
-    *reinterpret_cast<f32x4_t*>(ob + col * OP + j * 16 + quad * 4) = x;
-  }
-  __syncthreads();
-  const int nch = chunks_of(n);
-  for (int i = tid; i < nq * (HD / 4); i += 256) {
-    const int r = i / (HD / 4), d = (i % (HD / 4)) * 4;
-    float mt = -INFINITY, lt = 0.f;
-#pragma unroll
-    for (int w = 0; w < 4; ++w) mt = fmaxf(mt, stat[0][w][r]);
-    f32x4_t x = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int w = 0; w < 4; ++w) {
-      const float mw = stat[0][w][r];
-      lt += stat[1][w][r] * (mw == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(mw - mt));
-      x += *reinterpret_cast<const f32x4_t*>(reinterpret_cast<const float*>(lds) + (w * 16 + r) * OP + d);
-    }
-    const int64_t row = (int64_t)b * a.heads + head0 + r;
-    if (nch == 1) {
-      const float inv = lt > 0.f || lt != lt ? 1.f / lt : 0.f;
-      *reinterpret_cast<u32x2_t*>(a.o + b * a.ldo + (int64_t)(head0 + r) * HD + d) =
-          u32x2_t{pack_bf2(x[0] * inv, x[1] * inv), pack_bf2(x[2] * inv, x[3] * inv)};
-      if (d == 0) {
-        const float e = lt > 0.f || lt != lt ? mt + __builtin_amdgcn_logf(lt) : -INFINITY;
-        if (a.lse != nullptr) a.lse[row] = e * 0.6931471805599453f;
-        if (SCORES) a.lse2[row] = e;
-      }
-    } else {
-      *reinterpret_cast<f32x4_t*>(a.part + (row * a.nchunk + chunk) * HD + d) = x;
-      if (d == 0) {
-        a.ml[(row * a.nchunk + chunk) * 2] = mt;
-        a.ml[(row * a.nchunk + chunk) * 2 + 1] = lt;
+        for (int j = 0; j < ND; ++j) *reinterpret_cast<f32x4_t*>(pb + j * 16) = o[j];
+        if (quad == 0) {
+          a.ml[(row * a.nchunk + chunk) * 2] = m;
+          a.ml[(row * a.nchunk + chunk) * 2 + 1] = l;
+        }
       }
     }
   }
 }
 
-// Joins the chunks of one query head: a wave a row.
+// Joins the chunks of one query head.  HD / 4 threads add up every SUB-th chunk, 16 bytes each, and the SUB sums are
+// added in order: the order goes by the row's own chunks alone.  (A part without a finite score is 0, or NaN and stays it.)
 template <int HD, bool SCORES>
-__global__ __launch_bounds__(64) void kv_join_kernel(Args a) {
-  constexpr int V = HD / 64;
-  const int head = blockIdx.x, b = blockIdx.y, lane = threadIdx.x;
-  const int n = kv_length(a.t, b, false), nch = chunks_of(n);
+__global__ __launch_bounds__(256) void kv_join_kernel(Args a) {
+  constexpr int TPR = HD / 4, SUB = 256 / TPR;
+  __shared__ float f[kMaxChunks];
+  __shared__ float red[2][4];
+  __shared__ __align__(16) float acc[SUB][HD];
+  const int head = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int nch = chunks_of(kv_length(a.t, b, false));
   if (nch == 1) return;
   const int64_t row = (int64_t)b * a.heads + head;
   const float* ml = a.ml + row * a.nchunk * 2;
-  float top = -INFINITY;
-  for (int c = lane; c < nch; c += 64) top = fmaxf(top, ml[2 * c]);
-  top = wave_max<64>(top);
-  float x[V] = {}, lt = 0.f;
-  const float* part = a.part + row * a.nchunk * HD + lane * V;
-  for (int c = 0; c < nch; ++c) {
-    const float mc = ml[2 * c], f = mc == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(mc - top);
-    lt = fmaf(ml[2 * c + 1], f, lt);
+  float mc[kMaxChunks / 256], lc[kMaxChunks / 256], top = -INFINITY;
 #pragma unroll
-    for (int i = 0; i < V; ++i) x[i] = fmaf(part[(int64_t)c * HD + i], f, x[i]);
+  for (int i = 0; i < kMaxChunks / 256; ++i) {
+    const int c = i * 256 + tid;
+    mc[i] = c < nch ? ml[2 * c] : -INFINITY;
+    lc[i] = c < nch ? ml[2 * c + 1] : 0.f;
+    top = fmaxf(top, mc[i]);
   }
-  const float inv = lt > 0.f || lt != lt ? 1.f / lt : 0.f;
-  bf16_t* o = a.o + b * a.ldo + (int64_t)head * HD + lane * V;
+  top = wave_max<64>(top);
+  if (lane == 0) red[0][wave] = top;
+  __syncthreads();
+  top = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
+  float lt = 0.f;
 #pragma unroll
-  for (int i = 0; i < V; ++i) o[i] = f2bf(x[i] * inv);
-  if (lane == 0) {
-    const float e = lt > 0.f || lt != lt ? top + __builtin_amdgcn_logf(lt) : -INFINITY;
-    if (a.lse != nullptr) a.lse[row] = e * 0.6931471805599453f;
-    if (SCORES) a.lse2[row] = e;
+  for (int i = 0; i < kMaxChunks / 256; ++i) {
+    const float fc = mc[i] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(mc[i] - top);
+    f[i * 256 + tid] = fc;
+    lt = fmaf(lc[i], fc, lt);
+  }
+  lt = wave_sum<64>(lt);
+  if (lane == 0) red[1][wave] = lt;
+  __syncthreads();
+  lt = red[1][0] + red[1][1] + red[1][2] + red[1][3];
+  const int sub = tid / TPR, d = (tid % TPR) * 4;
+  const float* part = a.part + row * a.nchunk * HD + d;
+  f32x4_t x = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 8
+  for (int c = sub; c < nch; c += SUB) {
+    const f32x4_t y = *reinterpret_cast<const f32x4_t*>(part + (int64_t)c * HD);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) x[r] = fmaf(y[r], f[c], x[r]);
+  }
+  *reinterpret_cast<f32x4_t*>(&acc[sub][d]) = x;
+  __syncthreads();
+  if (tid < TPR) {
+    f32x4_t y = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < SUB; ++i) y += *reinterpret_cast<const f32x4_t*>(&acc[i][d]);
+    const float inv = lt > 0.f || lt != lt ? 1.f / lt : 0.f;
+    *reinterpret_cast<u32x2_t*>(a.o + b * a.ldo + (int64_t)head * HD + d) =
+        u32x2_t{pack_bf2(y[0] * inv, y[1] * inv), pack_bf2(y[2] * inv, y[3] * inv)};
+    if (tid == 0) {
+      const float e = lt > 0.f || lt != lt ? top + __builtin_amdgcn_logf(lt) : -INFINITY;
+      if (a.lse != nullptr) a.lse[row] = e * 0.6931471805599453f;
+      if (SCORES) a.lse2[row] = e;
+    }
   }
 }
 
-// weights of a key head's slots: the probabilities summed over its query heads, in their order
+// Weights of a key head's slots: the probabilities summed over its query heads, in their order.  Four slots a thread.
 __global__ __launch_bounds__(256) void kv_weights_kernel(Args a, int add) {
-  const int b = blockIdx.z, kvh = blockIdx.y, i = blockIdx.x * 256 + threadIdx.x;
+  const int b = blockIdx.z, kvh = blockIdx.y, i = (blockIdx.x * 256 + threadIdx.x) * 4;
   const int n = kv_length(a.t, b, false);
   if (i >= n) return;
   bool ok;
   const int p = kv_page(a.t, b, i, ok, false);
   if (!ok) return;
   const int64_t row0 = (int64_t)b * a.heads + (int64_t)kvh * a.group;
-  float sum = 0.f;
+  f32x4_t sum = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
   for (int g = 0; g < a.group; ++g) {
     const float e = a.lse2[row0 + g];
-    sum += e == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(a.score[(row0 + g) * a.ld_score + i] - e);
+    const f32x4_t s = *reinterpret_cast<const f32x4_t*>(a.score + (row0 + g) * a.ld_score + i);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) sum[r] += e == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(s[r] - e);
   }
   float* w = a.w.p + p * a.w.ps + kvh * a.w.hs + (i & ((1 << a.t.page_log2) - 1));
-  *w = add ? *w + sum : sum;
+#pragma unroll
+  for (int r = 0; r < 4; ++r)
+    if (i + r < n) w[r] = add ? w[r] + sum[r] : sum[r];
 }
 
 // floats of the workspace's parts, each a multiple of 4
@@ -361,9 +415,12 @@ DITK_EXPORT int ditk_kv_attn(const void* q, int64_t ldq, const void* k_cache, in
   a.group = heads / kv_heads;
   a.nchunk = chunks_bound(most);
   a.scale2 = softmax_scale * 1.4426950408889634f;
-  const int groups = (a.group + 15) / 16;
-  DITK_REQUIRE(kv_heads * groups <= 65535, "%s: too many heads", what);
-  const dim3 grid((unsigned)a.nchunk, (unsigned)(kv_heads * groups), (unsigned)batch);
+  a.batch = batch;
+  a.hgroups = kv_heads * ((a.group + 15) / 16);
+  const int64_t units = (int64_t)batch * a.nchunk * a.hgroups, wgs = (units + 3) / 4;
+  DITK_REQUIRE(units < (1ll << 30), "%s: too many sequences, heads and chunks", what);
+  const int most_wgs = 3 * ditk_cu_count();
+  const dim3 grid((unsigned)(wgs < most_wgs ? wgs : most_wgs));
   const bool s = weights != nullptr;
   auto kern = head_dim == 128 ? (s ? kv_attn_kernel<128, true> : kv_attn_kernel<128, false>)
                               : (s ? kv_attn_kernel<64, true> : kv_attn_kernel<64, false>);
@@ -372,11 +429,11 @@ DITK_EXPORT int ditk_kv_attn(const void* q, int64_t ldq, const void* k_cache, in
   if (a.nchunk > 1) {
     auto join = head_dim == 128 ? (s ? kv_join_kernel<128, true> : kv_join_kernel<128, false>)
                                 : (s ? kv_join_kernel<64, true> : kv_join_kernel<64, false>);
-    join<<<dim3((unsigned)heads, (unsigned)batch), 64, 0, stream>>>(a);
+    join<<<dim3((unsigned)heads, (unsigned)batch), 256, 0, stream>>>(a);
     if (int rc = ditk_check_launch(what)) return rc;
   }
   if (s && most > 0) {
-    kv_weights_kernel<<<dim3((unsigned)((most + 255) / 256), (unsigned)kv_heads, (unsigned)batch), 256, 0, stream>>>(a, add);
+    kv_weights_kernel<<<dim3((unsigned)((most + 1023) / 1024), (unsigned)kv_heads, (unsigned)batch), 256, 0, stream>>>(a, add);
     if (int rc = ditk_check_launch(what)) return rc;
   }
   return 0;
