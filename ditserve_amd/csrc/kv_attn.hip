@@ -15,7 +15,7 @@
 
 namespace {
 
-constexpr int kMaxChunks = 512;
+constexpr int kMaxChunks = 512, kShortChunks = 8;
 
 // slots of a chunk of a sequence of n, whole 32-slot tiles
 __host__ __device__ inline int chunk_slots(int n) {
@@ -69,77 +69,40 @@ __device__ __forceinline__ float group_sumf(float v) {
 
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 
-// A wave takes one chunk of one (sequence, key head, 16 query heads) after another; units go round the waves in
-// order: a sequence's chunks, and for each its heads, which lie side by side in a page.
+// What a wave gathers of one chunk: lane (quad, col) holds dims 16 j + 4 quad .. + 3 of query head `col`'s sums of
+// p v, its m and its l.
 template <int HD, bool SCORES>
-__global__ __launch_bounds__(256, 3) void kv_attn_kernel(Args a) {
-  constexpr int NC = HD / 32, ND = HD / 16, CH = HD / 8, RPL = 64 / CH;  // RPL: rows of V a load of the wave covers
-  __shared__ __align__(16) char lds[4 * 32 * HD * 2];
-  __shared__ int sums[4];
-  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
-  const int col = lane & 15, quad = lane >> 4;
-  const int pl = a.t.page_log2, low = (1 << pl) - 1;
-  char* vt = lds + wave * (32 * HD * 2);
+struct Chunk {
+  static constexpr int NC = HD / 32, ND = HD / 16, CH = HD / 8, RPL = 64 / CH;  // RPL: rows of V a load of the wave covers
+  f32x4_t o[ND];
+  float m, l;
 
-  // chunks before thread t's sequences [t per, t per + per)
-  const int per = (a.batch + 255) / 256;
-  int mine = 0;
-  for (int i = 0; i < per; ++i)
-    if (tid * per + i < a.batch) mine += chunks_of(kv_length(a.t, tid * per + i, blockIdx.x == 0));
-  int incl = mine;
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) {
-    const int o = __shfl_up(incl, off, 64);
-    if (lane >= off) incl += o;
-  }
-  if (lane == 63) sums[wave] = incl;
-  __syncthreads();
-  // every wave keeps all 256 sums: lane l those of threads l, 64 + l, 128 + l, 192 + l
-  __shared__ int ends[256];
-  for (int w = 0; w < wave; ++w) incl += sums[w];
-  ends[tid] = incl;
-  __syncthreads();
-  int end[4];
-#pragma unroll
-  for (int i = 0; i < 4; ++i) end[i] = ends[i * 64 + lane];
-  const int units = __builtin_amdgcn_readlane(end[3], 63) * a.hgroups;
-
-  for (int u = blockIdx.x * 4 + wave; u < units; u += gridDim.x * 4) {
-    const int c = u / a.hgroups, hg = u - c * a.hgroups;
-    // the thread whose sequences hold chunk c, then the sequence
-    int th = 0;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) th += __popcll(__ballot(end[i] <= c));
-    int b = th * per, chunk = c - (th ? ends[th - 1] : 0);
-    int n = kv_length(a.t, b, false), nch = chunks_of(n);
-    while (chunk >= nch && b + 1 < a.batch) {
-      chunk -= nch;
-      n = kv_length(a.t, ++b, false);
-      nch = chunks_of(n);
-    }
-    b = __builtin_amdgcn_readfirstlane(b);
-    n = __builtin_amdgcn_readfirstlane(n);
-    chunk = __builtin_amdgcn_readfirstlane(min(chunk, a.nchunk - 1));
-    const int groups = (a.group + 15) / 16, kvh = hg / groups, g0 = (hg - kvh * groups) * 16;
-    const int csl = chunk_slots(n), s0 = chunk * csl, s1 = min(n, s0 + csl), last = max(n - 1, 0);
-    const int nq = min(a.group - g0, 16), head0 = kvh * a.group + g0;  // query heads of this unit
-
+  // slots [s0, s1) of sequence b (n slots) and key head kvh, for nq query heads from head0 on; vt: 32 HD bf16 of LDS
+  __device__ __forceinline__ void run(const Args& a, int b, int n, int s0, int s1, int kvh, int head0, int nq, char* vt) {
+    const int lane = threadIdx.x & 63, col = lane & 15, quad = lane >> 4;
+    const int pl = a.t.page_log2, low = (1 << pl) - 1, last = max(n - 1, 0);
     bf16x8_t q[NC];
-    {
-      const bf16_t* qr = a.q + b * a.ldq + (int64_t)(head0 + min(col, nq - 1)) * HD + quad * 8;
+    const bf16_t* qr = a.q + b * a.ldq + (int64_t)(head0 + min(col, nq - 1)) * HD + quad * 8;
 #pragma unroll
-      for (int i = 0; i < NC; ++i) q[i] = *reinterpret_cast<const bf16x8_t*>(qr + i * 32);
-    }
-    f32x4_t o[ND];
+    for (int i = 0; i < NC; ++i) q[i] = *reinterpret_cast<const bf16x8_t*>(qr + i * 32);
 #pragma unroll
     for (int j = 0; j < ND; ++j) o[j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-    float m = -INFINITY, l = 0.f;
-
+    m = -INFINITY;
+    l = 0.f;
+    int page = 0, first = 0;
     for (int t0 = s0; t0 < s1; t0 += 32) {
+      // pages of the next 1024 slots, one a lane
+      if (((t0 - s0) & 1023) == 0) {
+        first = t0 >> pl;
+        const int i = min(first + lane, last >> pl), p = a.t.table[b * a.t.ldt + i];
+        page = (unsigned)p < (unsigned)a.t.pages ? p : -1;
+        if (page < 0 && (first + lane) << pl < s1) *a.t.status = 1;
+      }
       // the tile's two halves of 16 slots lie in one page each; slots past the last read it
-      const int e0 = min(t0, last), e1 = min(t0 + 16, last);
-      bool ok0, ok1;
-      const int p0 = kv_page(a.t, b, e0, ok0, true), p1 = kv_page(a.t, b, e1, ok1, true);
+      const int g0 = __builtin_amdgcn_readlane(page, (min(t0, last) >> pl) - first);
+      const int g1 = __builtin_amdgcn_readlane(page, (min(t0 + 16, last) >> pl) - first);
+      const bool ok0 = g0 >= 0, ok1 = g1 >= 0;
+      const int p0 = max(g0, 0), p1 = max(g1, 0);
       const bf16_t* kb0 = a.k.p + p0 * a.k.ps + kvh * a.k.hs;
       const bf16_t* kb1 = a.k.p + p1 * a.k.ps + kvh * a.k.hs;
       const bf16_t* vb0 = a.v.p + p0 * a.v.ps + kvh * a.v.hs;
@@ -233,33 +196,145 @@ __global__ __launch_bounds__(256, 3) void kv_attn_kernel(Args a) {
         o[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f.f, lo, o[j], 0, 0, 0);
       }
     }
-
-    // lane: dims 16 j + 4 quad .. + 3 of query head `col`
     l = group_sumf(l);
+  }
+};
+
+// 1 / l, 0 for a row without slots
+__device__ __forceinline__ float inverse(float l) { return l > 0.f || l != l ? 1.f / l : 0.f; }
+__device__ __forceinline__ void store_lse(const Args& a, int64_t row, float m, float l, bool scores) {
+  const float e = l > 0.f || l != l ? m + __builtin_amdgcn_logf(l) : -INFINITY;
+  if (a.lse != nullptr) a.lse[row] = e * 0.6931471805599453f;
+  if (scores) a.lse2[row] = e;
+}
+
+// A wave takes one chunk of one (sequence, key head, 16 query heads) after another; units go round the waves in
+// order: a sequence's chunks, and for each its heads, which lie side by side in a page.
+template <int HD, bool SCORES>
+__global__ __launch_bounds__(256, 3) void kv_attn_kernel(Args a) {
+  using C = Chunk<HD, SCORES>;
+  __shared__ __align__(16) char lds[4 * 32 * HD * 2];
+  __shared__ int sums[4], ends[256], lens[256];
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+  const int col = lane & 15, quad = lane >> 4;
+
+  // chunks up to and with thread t's sequences, [t per, t per + per)
+  const int per = (a.batch + 255) / 256;
+  int incl = 0;
+  for (int i = 0; i < per; ++i)
+    if (tid * per + i < a.batch) {
+      const int n = kv_length(a.t, tid * per + i, blockIdx.x == 0);
+      if (i == 0) lens[tid] = n;
+      incl += chunks_of(n);
+    }
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) {
+    const int o = __shfl_up(incl, off, 64);
+    if (lane >= off) incl += o;
+  }
+  if (lane == 63) sums[wave] = incl;
+  __syncthreads();
+  for (int w = 0; w < wave; ++w) incl += sums[w];
+  ends[tid] = incl;
+  __syncthreads();
+  int end[4];  // (every wave keeps all of them)
+#pragma unroll
+  for (int i = 0; i < 4; ++i) end[i] = ends[i * 64 + lane];
+  const int units = __builtin_amdgcn_readlane(end[3], 63) * a.hgroups, groups = (a.group + 15) / 16;
+
+  for (int u = blockIdx.x * 4 + wave; u < units; u += gridDim.x * 4) {
+    const int c = u / a.hgroups, hg = u - c * a.hgroups;
+    // the thread whose sequences hold chunk c, then the sequence
+    int th = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) th += __popcll(__ballot(end[i] <= c));
+    int b = th * per, chunk = c - (th ? ends[th - 1] : 0), n = lens[th], nch = chunks_of(n);
+    while (chunk >= nch && b + 1 < a.batch) {
+      chunk -= nch;
+      n = kv_length(a.t, ++b, false);
+      nch = chunks_of(n);
+    }
+    b = __builtin_amdgcn_readfirstlane(b);
+    n = __builtin_amdgcn_readfirstlane(n);
+    chunk = __builtin_amdgcn_readfirstlane(min(chunk, a.nchunk - 1));
+    const int kvh = hg / groups, g0 = (hg - kvh * groups) * 16;
+    const int csl = chunk_slots(n), s0 = chunk * csl, s1 = min(n, s0 + csl);
+    const int nq = min(a.group - g0, 16), head0 = kvh * a.group + g0;  // query heads of this unit
+    C x;
+    x.run(a, b, n, s0, s1, kvh, head0, nq, lds + wave * (32 * HD * 2));
     if (col < nq) {
       const int64_t row = (int64_t)b * a.heads + head0 + col;
       if (nch == 1) {
-        const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
+        const float inv = inverse(x.l);
         bf16_t* ob = a.o + b * a.ldo + (int64_t)(head0 + col) * HD + quad * 4;
 #pragma unroll
-        for (int j = 0; j < ND; ++j)
-          *reinterpret_cast<u32x2_t*>(ob + j * 16) = u32x2_t{pack_bf2(o[j][0] * inv, o[j][1] * inv),
-                                                            pack_bf2(o[j][2] * inv, o[j][3] * inv)};
-        if (quad == 0) {
-          const float e = l > 0.f || l != l ? m + __builtin_amdgcn_logf(l) : -INFINITY;
-          if (a.lse != nullptr) a.lse[row] = e * 0.6931471805599453f;
-          if (SCORES) a.lse2[row] = e;
-        }
+        for (int j = 0; j < C::ND; ++j)
+          *reinterpret_cast<u32x2_t*>(ob + j * 16) = u32x2_t{pack_bf2(x.o[j][0] * inv, x.o[j][1] * inv),
+                                                            pack_bf2(x.o[j][2] * inv, x.o[j][3] * inv)};
+        if (quad == 0) store_lse(a, row, x.m, x.l, SCORES);
       } else {
         float* pb = a.part + (row * a.nchunk + chunk) * HD + quad * 4;
 #pragma unroll
-        for (int j = 0; j < ND; ++j) *reinterpret_cast<f32x4_t*>(pb + j * 16) = o[j];
-        if (quad == 0) {
-          a.ml[(row * a.nchunk + chunk) * 2] = m;
-          a.ml[(row * a.nchunk + chunk) * 2 + 1] = l;
-        }
+        for (int j = 0; j < C::ND; ++j) *reinterpret_cast<f32x4_t*>(pb + j * 16) = x.o[j];
+        if (quad == 0) *reinterpret_cast<u32x2_t*>(a.ml + (row * a.nchunk + chunk) * 2) =
+            u32x2_t{__float_as_uint(x.m), __float_as_uint(x.l)};
       }
     }
+  }
+}
+
+// Sequences of up to 8 chunks in one launch: eight waves take a chunk each of a (sequence, key head, 16 query heads) and
+// join them through LDS, by the join kernel's operations in its order.
+template <int HD, bool SCORES>
+__global__ __launch_bounds__(512) void kv_attn_short_kernel(Args a) {
+  using C = Chunk<HD, SCORES>;
+  constexpr int OP = HD + 4;  // floats of a row of LDS
+  __shared__ __align__(16) char lds[8 * 16 * OP * 4];
+  __shared__ float stat[2][16][8];
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
+  const int col = lane & 15, quad = lane >> 4, groups = (a.group + 15) / 16;
+  const int b = blockIdx.x / a.hgroups, hg = blockIdx.x - b * a.hgroups;
+  const int kvh = hg / groups, g0 = (hg - kvh * groups) * 16;
+  const int n = kv_length(a.t, b, hg == 0 && tid == 0), csl = chunk_slots(n), nch = chunks_of(n);
+  const int s0 = min(wave * csl, n), s1 = min(n, s0 + csl);
+  const int nq = min(a.group - g0, 16), head0 = kvh * a.group + g0;
+  C x;
+  x.run(a, b, n, s0, s1, kvh, head0, nq, lds + wave * (16 * OP * 4));
+  if (quad == 0) {
+    stat[0][col][wave] = x.m;
+    stat[1][col][wave] = x.l;
+  }
+  // (a wave's rows lie where its values were, which it has read)
+  float* ob = reinterpret_cast<float*>(lds) + (wave * 16 + col) * OP + quad * 4;
+#pragma unroll
+  for (int j = 0; j < C::ND; ++j) *reinterpret_cast<f32x4_t*>(ob + j * 16) = x.o[j];
+  __syncthreads();
+  for (int i = tid; i < nq * (HD / 4); i += 512) {
+#pragma clang fp contract(off)  // products rounded, then added, as where the join reads them
+    const int r = i / (HD / 4), d = (i % (HD / 4)) * 4;
+    float m[8], f[8], top = -INFINITY;
+#pragma unroll
+    for (int c = 0; c < 8; ++c) {
+      m[c] = stat[0][r][c];
+      top = fmaxf(top, m[c]);
+    }
+    float l[8];
+    f32x4_t y = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int c = 0; c < 8; ++c) {
+      f[c] = m[c] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[c] - top);
+      if (nch == 1) f[c] = 1.f;
+      l[c] = stat[1][r][c] * f[c];
+      const f32x4_t z = *reinterpret_cast<const f32x4_t*>(reinterpret_cast<const float*>(lds) + (c * 16 + r) * OP + d);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) y[e] += z[e] * f[c];
+    }
+    // wave_sum's order of eight lanes
+    const float lt = ((l[0] + l[4]) + (l[2] + l[6])) + ((l[1] + l[5]) + (l[3] + l[7]));
+    const float inv = inverse(lt);
+    *reinterpret_cast<u32x2_t*>(a.o + b * a.ldo + (int64_t)(head0 + r) * HD + d) =
+        u32x2_t{pack_bf2(y[0] * inv, y[1] * inv), pack_bf2(y[2] * inv, y[3] * inv)};
+    if (d == 0) store_lse(a, (int64_t)b * a.heads + head0 + r, top, lt, SCORES);
   }
 }
 
@@ -293,7 +368,7 @@ __global__ __launch_bounds__(256) void kv_join_kernel(Args a) {
   for (int i = 0; i < kMaxChunks / 256; ++i) {
     const float fc = mc[i] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(mc[i] - top);
     f[i * 256 + tid] = fc;
-    lt = fmaf(lc[i], fc, lt);
+    lt += lc[i] * fc;
   }
   lt = wave_sum<64>(lt);
   if (lane == 0) red[1][wave] = lt;
@@ -306,7 +381,7 @@ __global__ __launch_bounds__(256) void kv_join_kernel(Args a) {
   for (int c = sub; c < nch; c += SUB) {
     const f32x4_t y = *reinterpret_cast<const f32x4_t*>(part + (int64_t)c * HD);
 #pragma unroll
-    for (int r = 0; r < 4; ++r) x[r] = fmaf(y[r], f[c], x[r]);
+    for (int r = 0; r < 4; ++r) x[r] += y[r] * f[c];
   }
   *reinterpret_cast<f32x4_t*>(&acc[sub][d]) = x;
   __syncthreads();
@@ -314,14 +389,10 @@ __global__ __launch_bounds__(256) void kv_join_kernel(Args a) {
     f32x4_t y = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < SUB; ++i) y += *reinterpret_cast<const f32x4_t*>(&acc[i][d]);
-    const float inv = lt > 0.f || lt != lt ? 1.f / lt : 0.f;
+    const float inv = inverse(lt);
     *reinterpret_cast<u32x2_t*>(a.o + b * a.ldo + (int64_t)head * HD + d) =
         u32x2_t{pack_bf2(y[0] * inv, y[1] * inv), pack_bf2(y[2] * inv, y[3] * inv)};
-    if (tid == 0) {
-      const float e = lt > 0.f || lt != lt ? top + __builtin_amdgcn_logf(lt) : -INFINITY;
-      if (a.lse != nullptr) a.lse[row] = e * 0.6931471805599453f;
-      if (SCORES) a.lse2[row] = e;
-    }
+    if (tid == 0) store_lse(a, row, top, lt, SCORES);
   }
 }
 
@@ -356,7 +427,7 @@ struct Space {
 Space space_of(int batch, int heads, int head_dim, int most, bool weights) {
   const int64_t rows = (int64_t)batch * heads, nc = chunks_bound(most);
   Space s{};
-  if (nc > 1) {
+  if (nc > kShortChunks) {
     s.part = rows * nc * head_dim;
     s.ml = (rows * nc * 2 + 3) & ~(int64_t)3;
   }
@@ -418,15 +489,19 @@ DITK_EXPORT int ditk_kv_attn(const void* q, int64_t ldq, const void* k_cache, in
   a.batch = batch;
   a.hgroups = kv_heads * ((a.group + 15) / 16);
   const int64_t units = (int64_t)batch * a.nchunk * a.hgroups, wgs = (units + 3) / 4;
-  DITK_REQUIRE(units < (1ll << 30), "%s: too many sequences, heads and chunks", what);
-  const int most_wgs = 3 * ditk_cu_count();
-  const dim3 grid((unsigned)(wgs < most_wgs ? wgs : most_wgs));
+  DITK_REQUIRE((int64_t)batch * heads < (1 << 22) && units < (1ll << 30), "%s: too many sequences, heads and chunks", what);
   const bool s = weights != nullptr;
-  auto kern = head_dim == 128 ? (s ? kv_attn_kernel<128, true> : kv_attn_kernel<128, false>)
-                              : (s ? kv_attn_kernel<64, true> : kv_attn_kernel<64, false>);
-  kern<<<grid, 256, 0, stream>>>(a);
-  if (int rc = ditk_check_launch(what)) return rc;
-  if (a.nchunk > 1) {
+  if (a.nchunk <= kShortChunks) {
+    auto kern = head_dim == 128 ? (s ? kv_attn_short_kernel<128, true> : kv_attn_short_kernel<128, false>)
+                                : (s ? kv_attn_short_kernel<64, true> : kv_attn_short_kernel<64, false>);
+    kern<<<(unsigned)(batch * a.hgroups), 512, 0, stream>>>(a);
+    if (int rc = ditk_check_launch(what)) return rc;
+  } else {
+    const int most_wgs = 3 * ditk_cu_count();
+    auto kern = head_dim == 128 ? (s ? kv_attn_kernel<128, true> : kv_attn_kernel<128, false>)
+                                : (s ? kv_attn_kernel<64, true> : kv_attn_kernel<64, false>);
+    kern<<<(unsigned)(wgs < most_wgs ? wgs : most_wgs), 256, 0, stream>>>(a);
+    if (int rc = ditk_check_launch(what)) return rc;
     auto join = head_dim == 128 ? (s ? kv_join_kernel<128, true> : kv_join_kernel<128, false>)
                                 : (s ? kv_join_kernel<64, true> : kv_join_kernel<64, false>);
     join<<<dim3((unsigned)heads, (unsigned)batch), 256, 0, stream>>>(a);

@@ -151,8 +151,9 @@ def _cache_check(cache):
 
 def _table(t, name, batch, device):
     """(address, row stride, pages of a row) of a page table [batch, pages]."""
-    _check(t, name, torch.int32, 2)
-    _one_device(device, (name, t))
+    if t.__class__ is not torch.Tensor or t.dtype is not torch.int32 or t.dim() != 2 or t.device != device:
+        _check(t, name, torch.int32, 2)
+        _one_device(device, (name, t))
     rows, width = t.shape
     st, unit = t.stride()
     if rows != batch or (width > 1 and unit != 1) or (rows > 1 and st < width):
@@ -162,20 +163,41 @@ def _table(t, name, batch, device):
 
 
 def _lengths(t, device):
-    _check(t, "lengths", torch.int32, 1)
-    _one_device(device, ("lengths", t))
+    if t.__class__ is not torch.Tensor or t.dtype is not torch.int32 or t.dim() != 1 or t.device != device:
+        _check(t, "lengths", torch.int32, 1)
+        _one_device(device, ("lengths", t))
     if t.shape[0] > 1 and t.stride(0) != 1:
         raise ValueError("lengths must be contiguous")
     return t.shape[0]
 
 
+def _outside(fn, cache, *tensors):
+    """Refuse rows and tables that lie between a cache's first and last byte."""
+    spans = []
+    for c in (cache.k, cache.v, cache.weights):
+        if c is not None:
+            (pages, heads, page), (ps, hs) = c.shape[:3], c.stride()[:2]
+            first, size = c.data_ptr(), c.element_size()
+            spans.append((first, first + ((pages - 1) * ps + (heads - 1) * hs + page * (c.shape[3] if size == 2 else 1)) * size))
+    for t in tensors:
+        if t is not None:
+            first = t.data_ptr()
+            rows = t.shape[0]
+            last = first + ((rows - 1) * t.stride(0) + (t.shape[1] if t.dim() == 2 else 1)) * t.element_size() if rows else first
+            for a, b in spans:
+                if first < b and a < last:
+                    raise ValueError(f"{fn}: an operand lies in the cache")
+
+
 def _rows_of(t, name, rows, cols, device):
-    _check(t, name, _BF16, 2)
-    _one_device(device, (name, t))
-    if t.shape[1] != cols or (rows is not None and t.shape[0] != rows):
+    if t.__class__ is not torch.Tensor or t.dtype is not _BF16 or t.dim() != 2 or t.device != device:
+        _check(t, name, _BF16, 2)
+        _one_device(device, (name, t))
+    n, wide = t.shape
+    if wide != cols or (rows is not None and n != rows):
         raise ValueError(f"{name} must be [{'rows' if rows is None else rows}, {cols}], got {tuple(t.shape)}")
     ld = _rows(t, name)
-    if t.shape[0] > 1 and ld < cols:
+    if n > 1 and ld < cols:
         raise ValueError(f"{name}'s rows overlap: strides {t.stride()}")
     return ld
 
@@ -205,9 +227,7 @@ def append(cache, k, v, table, lengths, segments=None):
     status = _status(device)
     status.poll()
     new = torch.empty(batch, dtype=torch.int32, device=device)
-    for t in (cache.k, cache.v, cache.weights):  # (which may share a buffer of their own)
-        if t is not None:
-            _apart("append", (t,), (k, v, table, lengths, cu))
+    _outside("append", cache, k, v, table, lengths, cu)
     _call(device, "ditk_kv_append", _ptr(k), ldk, _ptr(v), ldv, *cache._kv(), *cache._weights(), cache.pages, cache.page,
           tp, ldt, width, _ptr(lengths), _ptr(new), _ptr(cu), batch, T, hk, d, _ptr(status.host))
     return new
@@ -248,7 +268,8 @@ def decode_attn(q, cache, table, lengths, heads, softmax_scale=None, max_len=Non
         out, ldo = torch.empty((batch, heads * d), dtype=_BF16, device=device), heads * d
     else:
         ldo = _rows_of(out, "out", batch, heads * d, device)
-        _apart("decode_attn", (out,), (cache.k, cache.v, cache.weights, q, table, lengths))
+        _outside("decode_attn", cache, out)
+        _apart("decode_attn", (out,), (q, table, lengths))
     status = _status(device)
     status.poll()
     lse = torch.empty((batch, heads), dtype=torch.float32, device=device) if return_lse else None

@@ -9,6 +9,7 @@ stream without synchronising.  There is no CPU or PyTorch fallback.
 import array
 import ctypes
 import math
+import operator
 
 import torch
 
@@ -105,8 +106,8 @@ class Segments:
 
     def __init__(self, cu, device, dev=None):
         """dev: the table already on the device (else it is uploaded here)."""
-        self.cu = [int(x) for x in cu]
-        if not self.cu or self.cu[0] != 0 or any(b < a for a, b in zip(self.cu, self.cu[1:])):
+        self.cu = list(map(int, cu))
+        if not self.cu or self.cu[0] != 0 or any(map(operator.lt, self.cu[1:], self.cu)):
             raise ValueError(f"cu_seqlens must start at 0 and be nondecreasing, got {self.cu}")
         self.dev = dev if dev is not None else to_device(self.cu, torch.int32, device)
         self._nseg, self._total = len(self.cu) - 1, self.cu[-1]

@@ -44,7 +44,8 @@ def test_append_refuses(change, word):
     (dict(heads=5), "query heads"), (dict(heads=0), "query heads"), (dict(q=None), "null"), (dict(o=None), "null"),
     (dict(ldq=252), "aligned"), (dict(o=F + 8), "aligned"), (dict(max_len=-1), "max_len"), (dict(scale=0.0), "scale"),
     (dict(scale=float("nan")), "scale"), (dict(w=G), "workspace"),
-    (dict(width=4096, ldt=4096, max_len=65536, space=G, size=64), "workspace")])
+    (dict(width=4096, ldt=4096, max_len=65536, space=G, size=64), "workspace"),
+    (dict(batch=65535, heads=128, ldq=8192, ldo=8192), "too many")])
 def test_attn_refuses(change, word):
     refused("ditk_kv_attn", tuple({**ATTN, **change}.values()), word)
 
