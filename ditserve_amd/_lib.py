@@ -94,7 +94,9 @@ SIGNATURES = {
                              c_int, _P, c_int64, c_int, _P, c_int, _P, c_int64, _P, _P, c_int64, c_int, c_int, c_int,
                              c_int, c_float, _P, _P]),
     "ditk_kv_evict": (c_int, [_P, c_int64, c_int64, _P, c_int64, c_int64, _P, c_int64, c_int64, c_int, c_int, _P, c_int64,
-                              c_int, _P, c_int, _P, c_int64, c_int, _P, c_int, c_int, _P, c_int, c_int, c_int, _P, _P]),
+                              c_int, _P, c_int, _P, c_int64, c_int, _P, c_int, c_int, _P, c_int64, c_int, c_int, c_int, _P,
+                              _P]),
+    "ditk_kv_evict_workspace": (c_int64, [c_int, c_int, c_int, c_int]),
     "ditk_flash_attn_varlen_noalloc": (c_int, [_P, c_int64, _P, c_int64, _P, c_int64, _P, c_int64, _P, c_int64,
                                                _P, _P, c_int, c_int, c_int, c_int, c_int, c_float, _P]),
 }

@@ -75,81 +75,275 @@ __device__ __forceinline__ uint32_t order_of(float f) {
   return u & 0x80000000u ? ~u : u | 0x80000000u;
 }
 
-__device__ __forceinline__ float weight_at(const KvPages& t, const KvWeights& w, int b, int h, int i) {
-  bool ok;
-  const int p = kv_page(t, b, i, ok, true);
-  return ok ? w.p[p * w.ps + h * w.hs + (i & ((1 << t.page_log2) - 1))] : -INFINITY;
+// The slots that stay, ascending, of a (sequence, key head): of its `old` slots before the recent ones those above a
+// threshold weight, and the lowest of those at it.  The threshold is the want-th largest of the weights' 32-bit order
+// (order_of), found 11, 11 and 10 bits at a time by counting digits in LDS, the largest first.
+//
+// A workgroup of 1024 threads keeps KPT weights a thread in registers; wave w has KPT * 64 slots from its part's start +
+// w * KPT * 64 on, 64 consecutive ones in each register, so ballots give the places in the list.  Rows that one
+// workgroup holds take one launch (kv_select_kernel).  Longer ones are cut into parts of 1024 * KPT slots and take four,
+// each of every part: counts of the first digit; that digit from all parts' counts, and counts of the second; the same
+// for the third; the threshold and the list (kv_count_kernel, kv_list_kernel).  Counts have a place for each part, so
+// that nothing has to be cleared and no order matters.
+constexpr int kBins = 2048;
+constexpr int kShift[3] = {21, 10, 0};
+
+struct Row {
+  int n, m, r, old, want;  // slots, slots that stay, recent and older ones, and how many of these stay
+  bool sort;               // whether weights decide
+};
+__device__ __forceinline__ Row row_of(const KvPages& t, int b, int keep, int recent, bool tell) {
+  Row x;
+  x.n = kv_length(t, b, tell);
+  x.m = min(x.n, keep);
+  x.r = min(recent, x.m);
+  x.old = x.n - x.r;
+  x.want = x.m - x.r;
+  x.sort = x.n > x.m && x.want > 0;
+  return x;
 }
 
-// The slots that stay, ascending: one workgroup per (key head, sequence).  The threshold is the (m - recent)-th largest
-// weight of the others, found 8 bits at a time; of the slots that hold just it, the lowest stay.
-__global__ __launch_bounds__(1024) void kv_select_kernel(KvPages t, KvWeights w, int keep, int recent,
-                                                         int32_t* __restrict__ slots, int32_t* __restrict__ new_lengths) {
-  __shared__ uint32_t hist[256];
-  __shared__ uint32_t pick[2];      // the digit, and how many of it are wanted
-  __shared__ int above[16], ties[16];
-  const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, wave = tid >> 6, lane = tid & 63;
-  const int n = kv_length(t, b, tid == 0), m = min(n, keep), r = min(recent, m), old = n - r;
-  int32_t* out = slots + ((int64_t)b * gridDim.x + h) * keep;
-  if (h == 0 && tid == 0) new_lengths[b] = m;
-  uint32_t want = (uint32_t)(m - r), top = 0, mask = 0;
-  if (n > m && want > 0) {
-    for (int shift = 24; shift >= 0; shift -= 8) {
-      if (tid < 256) hist[tid] = 0;
-      __syncthreads();
-      for (int i = tid; i < old; i += 1024) {
-        const uint32_t u = order_of(weight_at(t, w, b, h, i));
-        if ((u & mask) == top) atomicAdd(&hist[(u >> shift) & 255], 1u);
-      }
-      __syncthreads();
-      if (tid == 0) {
-        uint32_t left = want;
-        int d = 255;
-        while (d > 0 && hist[d] < left) left -= hist[d--];
-        pick[0] = (uint32_t)d;
-        pick[1] = left;
-      }
-      __syncthreads();
-      top |= pick[0] << shift;
-      mask |= 0xffu << shift;
-      want = pick[1];
-      __syncthreads();
-    }
-  }
-  // now: slots above `top` stay, and the first `want` that equal it.  Wave w takes a part of the slots.
-  const bool all = n <= m, none = !all && m == r;
-  const int part = ((old + 15) / 16 + 63) & ~63, i0 = min(wave * part, old), i1 = min(i0 + part, old);
-  int na = 0, nt = 0;
-  for (int i = i0 + lane; i < i1; i += 64) {
-    const uint32_t u = all || none ? 0u : order_of(weight_at(t, w, b, h, i));
-    na += all || (!none && u > top);
-    nt += !all && !none && u == top;
-  }
+template <int KPT>
+__device__ __forceinline__ void load_keys(const KvPages& t, const KvWeights& w, int b, int h, int first, int old,
+                                          uint32_t (&key)[KPT]) {
+  const int base = first + (threadIdx.x >> 6) * (KPT * 64) + (threadIdx.x & 63);
+  int page[KPT];
 #pragma unroll
-  for (int off = 32; off > 0; off >>= 1) {
-    na += __shfl_xor(na, off, 64);
-    nt += __shfl_xor(nt, off, 64);
+  for (int i = 0; i < KPT; ++i) page[i] = base + i * 64 < old ? t.table[b * t.ldt + ((base + i * 64) >> t.page_log2)] : 0;
+#pragma unroll
+  for (int i = 0; i < KPT; ++i) {
+    const int at = base + i * 64;
+    const bool ok = (unsigned)page[i] < (unsigned)t.pages;
+    if (!ok) *t.status = 1;
+    key[i] = order_of(at < old && ok ? w.p[page[i] * w.ps + h * w.hs + (at & ((1 << t.page_log2) - 1))] : -INFINITY);
   }
-  if (lane == 0) above[wave] = na, ties[wave] = nt;
+}
+
+// counts[d] += keys of this workgroup that have digit d and agree with `top` where `mask` says
+template <int KPT>
+__device__ __forceinline__ void count_digits(const uint32_t (&key)[KPT], int first, int old, uint32_t top, uint32_t mask,
+                                             int shift, int* counts) {
+  const int lane = threadIdx.x & 63, base = first + (threadIdx.x >> 6) * (KPT * 64) + lane;
+#pragma unroll
+  for (int i = 0; i < KPT; ++i) {
+    const bool in = base + i * 64 < old && (key[i] & mask) == top;
+    const int d = (int)(key[i] >> shift) & (kBins - 1) & (int)(~mask >> shift);
+    // lanes that share the first one's digit count as one
+    const uint64_t any = __ballot(in);
+    if (any == 0) continue;
+    const int lead = __builtin_ctzll(any), d0 = __builtin_amdgcn_readlane(d, lead);
+    const uint64_t same = __ballot(in && d == d0);
+    if (lane == lead) atomicAdd(&counts[d0], __popcll(same));
+    else if (in && d != d0) atomicAdd(&counts[d], 1);
+  }
+}
+
+// the digit of the want-th largest, and how many of its keys are wanted: counts in LDS, two a thread
+__device__ __forceinline__ void find_digit(const int* counts, int& want, int& digit, int (*sums)[16], int* pick) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int hi = kBins - 1 - 2 * tid, v0 = counts[hi], v1 = counts[hi - 1];
+  int incl = v0 + v1;
+#pragma unroll
+  for (int off = 1; off < 64; off <<= 1) {
+    const int o = __shfl_up(incl, off, 64);
+    if (lane >= off) incl += o;
+  }
+  if (lane == 63) sums[0][wave] = incl;
   __syncthreads();
-  int at = 0, tie = 0;  // slots that stay, and equal ones, before this wave's part
-  for (int i = 0; i < wave; ++i) {
-    at += above[i];
-    tie += ties[i];
+  for (int i = 0; i < wave; ++i) incl += sums[0][i];
+  const int before = incl - v0 - v1;
+  if (before < want && want <= incl) {
+    pick[0] = before + v0 >= want ? hi : hi - 1;
+    pick[1] = before + v0 >= want ? want - before : want - before - v0;
   }
-  at += min(tie, (int)want) * (all || none ? 0 : 1);
-  for (int i = i0; i < i1; i += 64) {
-    const bool in = i + lane < i1;
-    const uint32_t u = all || none || !in ? 0u : order_of(weight_at(t, w, b, h, i + lane));
-    const bool eq = in && !all && !none && u == top;
-    const uint64_t eqs = __ballot(eq), before = (1ull << lane) - 1;
-    const bool stay = in && (all || (!none && u > top) || (eq && tie + __popcll(eqs & before) < (int)want));
+  __syncthreads();
+  digit = pick[0];
+  want = pick[1];
+  __syncthreads();
+}
+
+// Writes this workgroup's slots that stay: those above `top`, and those equal to it while fewer than `want` of them came
+// before.  at, tie: slots that stay, and equal ones, in the parts before.
+template <int KPT>
+__device__ __forceinline__ void write_list(const uint32_t (&key)[KPT], const Row& x, int first, uint32_t top, int want, int at,
+                                           int tie, int (*sums)[16], int32_t* out) {
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, base = first + wave * (KPT * 64);
+  const bool all = x.n <= x.m;
+  if (!all && !x.sort) return;
+  int na = 0, nt = 0;
+#pragma unroll
+  for (int i = 0; i < KPT; ++i) {
+    const bool in = base + i * 64 + lane < x.old;
+    na += __popcll(__ballot(in && (all || key[i] > top)));
+    nt += __popcll(__ballot(in && !all && key[i] == top));
+  }
+  if (lane == 0) sums[0][wave] = na, sums[1][wave] = nt;
+  __syncthreads();
+  for (int i = 0; i < wave; ++i) {
+    at += sums[0][i];
+    tie += sums[1][i];
+  }
+  at += min(tie, want);
+  const uint64_t before = (1ull << lane) - 1;
+#pragma unroll
+  for (int i = 0; i < KPT; ++i) {
+    const int slot = base + i * 64 + lane;
+    const bool in = slot < x.old, eq = in && !all && key[i] == top;
+    const uint64_t eqs = __ballot(eq);
+    const bool stay = in && (all || key[i] > top || (eq && tie + __popcll(eqs & before) < want));
     const uint64_t stays = __ballot(stay);
-    if (stay) out[at + __popcll(stays & before)] = i + lane;
+    if (stay) out[at + __popcll(stays & before)] = slot;
     at += __popcll(stays);
     tie += __popcll(eqs);
   }
-  for (int i = tid; i < r; i += 1024) out[m - r + i] = old + i;
+}
+
+template <int KPT>
+__global__ __launch_bounds__(1024) void kv_select_kernel(KvPages t, KvWeights w, int keep, int recent,
+                                                         int32_t* __restrict__ slots, int32_t* __restrict__ new_lengths) {
+  __shared__ int counts[3][kBins];
+  __shared__ int sums[2][16], pick[2];
+  const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x;
+  const Row x = row_of(t, b, keep, recent, tid == 0);
+  int32_t* out = slots + ((int64_t)b * gridDim.x + h) * keep;
+  if (h == 0 && tid == 0) new_lengths[b] = x.m;
+  for (int i = tid; i < x.r; i += 1024) out[x.m - x.r + i] = x.old + i;
+  uint32_t key[KPT], top = 0, mask = 0;
+  int want = x.want;
+  if (x.sort) {
+    for (int i = tid; i < 3 * kBins; i += 1024) counts[0][i] = 0;
+    load_keys<KPT>(t, w, b, h, 0, x.old, key);
+    __syncthreads();
+#pragma unroll
+    for (int k = 0; k < 3; ++k) {
+      count_digits<KPT>(key, 0, x.old, top, mask, kShift[k], counts[k]);
+      __syncthreads();
+      int d;
+      find_digit(counts[k], want, d, sums, pick);
+      top |= (uint32_t)d << kShift[k];
+      mask = ~0u << kShift[k];
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < KPT; ++i) key[i] = 0;
+  }
+  write_list<KPT>(key, x, 0, top, want, 0, 0, sums, out);
+}
+
+// what the launches for long rows keep of a row
+struct Counts {
+  int* digits;  // [rows][parts][3][kBins]
+  int* above;   // [rows][parts][2]: keys above the first digit, and at it but above the second
+  int* pick;    // [rows][2][2]: digits found, and how many are wanted of what agrees with them
+  int parts;
+};
+
+// counts of digit PASS of a part; PASS > 0: finds the digit before it first
+template <int KPT, int PASS>
+__global__ __launch_bounds__(1024) void kv_count_kernel(KvPages t, KvWeights w, int keep, int recent, Counts c) {
+  __shared__ int counts[kBins];
+  __shared__ int sums[2][16], pick[2];
+  const int part = blockIdx.x, h = blockIdx.y, b = blockIdx.z, tid = threadIdx.x;
+  const Row x = row_of(t, b, keep, recent, false);
+  const int first = part * (KPT * 1024);
+  if (!x.sort || first >= x.old) return;
+  const int64_t row = (int64_t)b * gridDim.y + h;
+  const int parts = (x.old - 1) / (KPT * 1024) + 1;
+  uint32_t key[KPT], top = 0, mask = 0;
+  load_keys<KPT>(t, w, b, h, first, x.old, key);
+  if (PASS > 0) {
+    int v[2] = {0, 0};
+    for (int p = 0; p < parts; ++p)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) v[i] += c.digits[((row * c.parts + p) * 3 + PASS - 1) * kBins + i * 1024 + tid];
+    counts[tid] = v[0];
+    counts[1024 + tid] = v[1];
+    __syncthreads();
+    int want = x.want, d;
+    if (PASS == 2) {
+      top = (uint32_t)c.pick[row * 4] << kShift[0];
+      want = c.pick[row * 4 + 1];
+    }
+    find_digit(counts, want, d, sums, pick);
+    top |= (uint32_t)d << kShift[PASS - 1];
+    if (part == 0 && tid == 0) {
+      c.pick[row * 4 + 2 * (PASS - 1)] = d;
+      c.pick[row * 4 + 2 * (PASS - 1) + 1] = want;
+    }
+    // this part's keys above, among those that agree with the digits before
+    const uint32_t agree = PASS == 1 ? 0u : ~0u << kShift[0];
+    mask = ~0u << kShift[PASS - 1];
+    int na = 0;
+#pragma unroll
+    for (int i = 0; i < KPT; ++i) {
+      const bool in = first + (tid >> 6) * (KPT * 64) + i * 64 + (tid & 63) < x.old && (key[i] & agree) == (top & agree);
+      na += __popcll(__ballot(in && (key[i] & mask) > top));
+    }
+    if ((tid & 63) == 0) sums[1][tid >> 6] = na;
+    __syncthreads();
+    if (tid == 0) {
+      int all = 0;
+      for (int i = 0; i < 16; ++i) all += sums[1][i];
+      c.above[(row * c.parts + part) * 2 + PASS - 1] = all;
+    }
+  }
+  counts[tid] = counts[1024 + tid] = 0;
+  __syncthreads();
+  count_digits<KPT>(key, first, x.old, top, mask, kShift[PASS], counts);
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < 2; ++i) c.digits[((row * c.parts + part) * 3 + PASS) * kBins + i * 1024 + tid] = counts[i * 1024 + tid];
+}
+
+template <int KPT>
+__global__ __launch_bounds__(1024) void kv_list_kernel(KvPages t, KvWeights w, int keep, int recent, Counts c,
+                                                       int32_t* __restrict__ slots, int32_t* __restrict__ new_lengths) {
+  __shared__ int counts[kBins];
+  __shared__ int sums[2][16], pick[2], before[2];
+  const int part = blockIdx.x, h = blockIdx.y, b = blockIdx.z, tid = threadIdx.x;
+  const Row x = row_of(t, b, keep, recent, part == 0 && tid == 0);
+  const int64_t row = (int64_t)b * gridDim.y + h;
+  int32_t* out = slots + row * keep;
+  if (part == 0 && h == 0 && tid == 0) new_lengths[b] = x.m;
+  for (int i = part * 1024 + tid; i < x.r; i += gridDim.x * 1024) out[x.m - x.r + i] = x.old + i;
+  const int first = part * (KPT * 1024);
+  if (first >= x.old) return;
+  uint32_t key[KPT], top = 0;
+  int want = x.want, at = first, tie = 0;  // (all stay: every slot before)
+  if (x.sort) {
+    const int parts = (x.old - 1) / (KPT * 1024) + 1;
+    load_keys<KPT>(t, w, b, h, first, x.old, key);
+    int v[2] = {0, 0}, mine[2] = {0, 0};  // all parts' counts of the last digit, and those of the parts before
+    for (int p = 0; p < parts; ++p) {
+      if (p == part) mine[0] = v[0], mine[1] = v[1];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) v[i] += c.digits[((row * c.parts + p) * 3 + 2) * kBins + i * 1024 + tid];
+    }
+    counts[tid] = v[0];
+    counts[1024 + tid] = v[1];
+    if (tid < 2) before[tid] = 0;
+    __syncthreads();
+    want = c.pick[row * 4 + 3];
+    int d;
+    find_digit(counts, want, d, sums, pick);
+    top = (uint32_t)c.pick[row * 4] << kShift[0] | (uint32_t)c.pick[row * 4 + 2] << kShift[1] | (uint32_t)d;
+    int na = 0;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int bin = i * 1024 + tid;
+      if (bin > d) na += mine[i];
+      if (bin == d) before[1] = mine[i];
+    }
+    for (int p = tid; p < part; p += 1024) na += c.above[(row * c.parts + p) * 2] + c.above[(row * c.parts + p) * 2 + 1];
+    if (na) atomicAdd(&before[0], na);  // (whole numbers: no order matters)
+    __syncthreads();
+    at = before[0];
+    tie = before[1];
+  } else {
+#pragma unroll
+    for (int i = 0; i < KPT; ++i) key[i] = 0;
+  }
+  write_list<KPT>(key, x, first, top, want, at, tie, sums, out);
 }
 
 // Copies the slots that stay into the pages of `to`: 16 slots of a (key head, sequence) a workgroup, 16 bytes a thread.
@@ -209,11 +403,32 @@ DITK_EXPORT int ditk_kv_append(const void* k, int64_t ldk, const void* v, int64_
   return ditk_check_launch(what);
 }
 
+namespace {
+// launches of the selection: rows of up to 1024 * kpt slots by one workgroup each (parts 1), longer ones in parts
+struct SelectPlan {
+  int kpt, parts;
+};
+SelectPlan select_plan(int most) {
+  for (int kpt : {1, 4, 8, 32})
+    if (most <= 1024 * kpt) return {kpt, 1};
+  const int kpt = most <= 16 * 8192 ? 8 : 32;
+  return {kpt, (most - 1) / (1024 * kpt) + 1};
+}
+}  // namespace
+
+DITK_EXPORT int64_t ditk_kv_evict_workspace(int batch, int kv_heads, int most, int keep) {
+  if (batch <= 0 || kv_heads <= 0 || most < 0 || most >= (1 << 30) || keep <= 0) return 0;
+  const int64_t rows = (int64_t)batch * kv_heads;
+  const SelectPlan pl = select_plan(most);
+  return 4 * (rows * keep + (pl.parts > 1 ? rows * ((int64_t)pl.parts * (3 * kBins + 2) + 4) : 0));
+}
+
 DITK_EXPORT int ditk_kv_evict(void* k_cache, int64_t k_ps, int64_t k_hs, void* v_cache, int64_t v_ps, int64_t v_hs,
                               float* weights, int64_t w_ps, int64_t w_hs, int pages, int page, const int32_t* table,
                               int64_t ldt, int width, const int32_t* lengths, int max_len, const int32_t* out_table,
-                              int64_t ldo, int out_width, int32_t* new_lengths, int keep, int recent, int32_t* slots,
-                              int batch, int kv_heads, int head_dim, int32_t* status, hipStream_t stream) {
+                              int64_t ldo, int out_width, int32_t* new_lengths, int keep, int recent, void* workspace,
+                              int64_t workspace_bytes, int batch, int kv_heads, int head_dim, int32_t* status,
+                              hipStream_t stream) {
   const char* what = "ditk_kv_evict";
   if (int rc = kv_check_pages(what, table, lengths, status, batch, width, ldt, pages, page, kv_heads, head_dim)) return rc;
   if (int rc = kv_check_pages(what, out_table, lengths, status, batch, out_width, ldo, pages, page, kv_heads, head_dim)) return rc;
@@ -222,17 +437,45 @@ DITK_EXPORT int ditk_kv_evict(void* k_cache, int64_t k_ps, int64_t k_hs, void* v
   DITK_REQUIRE(weights != nullptr, "%s: the cache has no weights", what);
   DITK_REQUIRE(keep > 0 && recent >= 0 && recent <= keep && max_len >= 0, "%s: bad keep %d, recent %d or max_len %d",
                what, keep, recent, max_len);
-  DITK_REQUIRE(batch == 0 || (new_lengths && slots), "%s: null output or workspace", what);
   if (batch == 0) return 0;
   const int most = width * page < max_len ? width * page : max_len, m = most < keep ? most : keep;
+  DITK_REQUIRE(new_lengths && workspace && ((uintptr_t)workspace % 16) == 0 &&
+                   workspace_bytes >= ditk_kv_evict_workspace(batch, kv_heads, most, keep),
+               "%s: null output, or a workspace below %lld bytes", what,
+               (long long)ditk_kv_evict_workspace(batch, kv_heads, most, keep));
   DITK_REQUIRE((int64_t)out_width * page >= m, "%s: the new pages hold %lld slots, %d stay", what,
                (long long)out_width * page, m);
   const KvPages t{table, ldt, lengths, pages, log2_of(page), most, status};
   const KvPages to{out_table, ldo, lengths, pages, log2_of(page), out_width * page, status};
   const KvTensor kc{(bf16_t*)k_cache, k_ps, k_hs}, vc{(bf16_t*)v_cache, v_ps, v_hs};
   const KvWeights w{weights, w_ps, w_hs};
-  kv_select_kernel<<<dim3(kv_heads, batch), 1024, 0, stream>>>(t, w, keep, recent, slots, new_lengths);
-  if (int rc = ditk_check_launch(what)) return rc;
+  const int64_t rows = (int64_t)batch * kv_heads;
+  const SelectPlan pl = select_plan(most);
+  int32_t* slots = (int32_t*)workspace;
+  if (pl.parts == 1) {
+    auto kern = pl.kpt == 1 ? kv_select_kernel<1> : pl.kpt == 4 ? kv_select_kernel<4>
+                : pl.kpt == 8 ? kv_select_kernel<8> : kv_select_kernel<32>;
+    kern<<<dim3(kv_heads, batch), 1024, 0, stream>>>(t, w, keep, recent, slots, new_lengths);
+    if (int rc = ditk_check_launch(what)) return rc;
+  } else {
+    Counts c;
+    c.digits = slots + rows * keep;
+    c.above = c.digits + rows * pl.parts * 3 * kBins;
+    c.pick = c.above + rows * pl.parts * 2;
+    c.parts = pl.parts;
+    const dim3 grid(pl.parts, kv_heads, batch);
+    const bool few = pl.kpt == 8;
+    auto count0 = few ? kv_count_kernel<8, 0> : kv_count_kernel<32, 0>;
+    auto count1 = few ? kv_count_kernel<8, 1> : kv_count_kernel<32, 1>;
+    auto count2 = few ? kv_count_kernel<8, 2> : kv_count_kernel<32, 2>;
+    auto list = few ? kv_list_kernel<8> : kv_list_kernel<32>;
+    for (auto count : {count0, count1, count2}) {
+      count<<<grid, 1024, 0, stream>>>(t, w, keep, recent, c);
+      if (int rc = ditk_check_launch(what)) return rc;
+    }
+    list<<<grid, 1024, 0, stream>>>(t, w, keep, recent, c, slots, new_lengths);
+    if (int rc = ditk_check_launch(what)) return rc;
+  }
   if (m == 0) return 0;
   const int per = head_dim == 128 ? 16 : 32;
   auto kern = head_dim == 128 ? kv_move_kernel<4> : kv_move_kernel<3>;

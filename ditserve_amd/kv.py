@@ -314,8 +314,9 @@ def evict(cache, table, lengths, out_table, keep, recent=0, max_len=None):
     status = _status(device)
     status.poll()
     new = torch.empty(batch, dtype=torch.int32, device=device)
-    slots = torch.empty(batch * hk * keep, dtype=torch.int32, device=device)
+    size = _lib.load().ditk_kv_evict_workspace(batch, hk, most, keep)
+    space = torch.empty(size, dtype=torch.uint8, device=device)
     _call(device, "ditk_kv_evict", *cache._kv(), *cache._weights(), cache.pages, cache.page, tp, ldt, width,
-          _ptr(lengths), most, op, ldo, out_width, _ptr(new), keep, recent, _ptr(slots), batch, hk, d,
+          _ptr(lengths), most, op, ldo, out_width, _ptr(new), keep, recent, _ptr(space), size, batch, hk, d,
           _ptr(status.host))
     return new

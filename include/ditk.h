@@ -510,14 +510,15 @@ int ditk_kv_attn(const void* q, int64_t ldq, const void* k_cache, int64_t k_ps, 
  * Of each (sequence, key head) the last `recent` slots and those of the others with the largest
  * weights (ties: the lowest slot; NaN counts as -inf), min(length, keep) in all, copied in their
  * order, with their weights, into the first slots of out_table's pages (other pages than
- * table's; out_width * page >= min(keep, width * page, max_len)).  slots: workspace of
- * batch * kv_heads * keep ints.
+ * table's; out_width * page >= min(keep, width * page, max_len)).  workspace: 16-byte aligned, this
+ * call's alone, of ditk_kv_evict_workspace bytes (most: the smaller of width * page and max_len).
  */
+int64_t ditk_kv_evict_workspace(int batch, int kv_heads, int most, int keep);
 int ditk_kv_evict(void* k_cache, int64_t k_ps, int64_t k_hs, void* v_cache, int64_t v_ps, int64_t v_hs,
                   float* weights, int64_t w_ps, int64_t w_hs, int pages, int page, const int32_t* table, int64_t ldt,
                   int width, const int32_t* lengths, int max_len, const int32_t* out_table, int64_t ldo, int out_width,
-                  int32_t* new_lengths, int keep, int recent, int32_t* slots, int batch, int kv_heads, int head_dim,
-                  int32_t* status, ditk_stream_t stream);
+                  int32_t* new_lengths, int keep, int recent, void* workspace, int64_t workspace_bytes, int batch,
+                  int kv_heads, int head_dim, int32_t* status, ditk_stream_t stream);
 
 #ifdef __cplusplus
 }

@@ -201,7 +201,9 @@ def kept_slots(w, n, keep, recent):
 @pytest.mark.parametrize("lens,keep,recent,hk,d,page", [
     ([1], 1, 0, 1, 64, 16), ([1, 2, 3], 2, 1, 2, 128, 16), ([100, 7, 0, 64], 20, 5, 3, 64, 16),
     ([5000, 300], 1000, 100, 2, 128, 64), ([2000], 1999, 0, 1, 64, 32), ([700, 650], 64, 64, 2, 128, 256),
-    ([33, 65, 129], 33, 32, 1, 128, 32), ([70000], 600, 17, 1, 64, 128)])
+    ([33, 65, 129], 33, 32, 1, 128, 32), ([70000], 600, 17, 1, 64, 128),
+    ([1024], 511, 1, 2, 64, 64), ([1025, 4096], 1024, 0, 1, 64, 16), ([4097, 8192], 3, 1, 1, 64, 32), ([8193], 8192, 100, 1, 64, 64),
+    ([32768], 16000, 0, 1, 64, 128), ([32769, 20, 9000], 8193, 8192, 1, 64, 128), ([131073, 50], 40000, 33, 1, 64, 256)])
 @pytest.mark.parametrize("kind", ["random", "ties", "odd"])
 def test_evict(lens, keep, recent, hk, d, page, kind):
     stay = [min(n, keep) for n in lens]

@@ -22,8 +22,8 @@ APPEND = dict(new_k=E, ldk=128, new_v=F, ldv=128, **CACHE, **PAGES, new=G, cu=No
               stream=None)
 ATTN = dict(q=E, ldq=256, **CACHE, add=0, **PAGES, max_len=64, o=F, ldo=256, lse=None, space=None, size=0, batch=2, heads=4,
             hk=2, d=64, scale=0.1, status=H, stream=None)
-EVICT = dict(**{**CACHE, "w": E}, **PAGES, max_len=64, out_table=F, ldo=2, out_width=2, new=G, keep=32, recent=4, slots=A,
-             batch=2, hk=2, d=64, status=H, stream=None)
+EVICT = dict(**{**CACHE, "w": E}, **PAGES, max_len=64, out_table=F, ldo=2, out_width=2, new=G, keep=32, recent=4, space=A,
+             size=1 << 20, batch=2, hk=2, d=64, status=H, stream=None)
 
 COMMON = [
     (dict(batch=-1), "sequences"), (dict(batch=65536), "sequences"), (dict(hk=0), "key head"), (dict(d=96), "head_dim"),
@@ -53,7 +53,8 @@ def test_attn_refuses(change, word):
 @pytest.mark.parametrize("change,word", COMMON + [
     (dict(w=None), "no weights"), (dict(keep=0), "keep"), (dict(recent=-1), "recent"), (dict(recent=33), "recent"),
     (dict(max_len=-1), "max_len"), (dict(out_table=None), "null table"), (dict(out_width=1), "32 stay"),
-    (dict(new=None), "null output"), (dict(slots=None), "null output")])
+    (dict(new=None), "null output"), (dict(space=None), "null output"), (dict(space=A + 8), "null output"),
+    (dict(size=4 * 2 * 2 * 32 - 4), "workspace"), (dict(width=4096, ldt=4096, max_len=65536, size=1 << 19), "workspace")])
 def test_evict_refuses(change, word):
     refused("ditk_kv_evict", tuple({**EVICT, **change}.values()), word)
 
