@@ -238,6 +238,28 @@ struct Counts {
   int parts;
 };
 
+// counts of bins tid and 1024 + tid of a digit: in all parts, and in those before `part`.  Eight parts' loads at a time
+// (8 rows of 131072 slots, 16 parts: launches of 11 to 13 us take 7 to 9).
+__device__ __forceinline__ void sum_parts(const Counts& c, int64_t row, int digit, int parts, int part, int (&all)[2],
+                                          int (&before)[2]) {
+  all[0] = all[1] = before[0] = before[1] = 0;
+  const int* from = c.digits + (row * c.parts * 3 + digit) * kBins + threadIdx.x;
+  for (int p = 0; p < parts; p += 8) {
+    int v[8][2];
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) v[k][i] = from[(int64_t)min(p + k, parts - 1) * 3 * kBins + i * 1024];
+#pragma unroll
+    for (int k = 0; k < 8; ++k)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        all[i] += p + k < parts ? v[k][i] : 0;
+        before[i] += p + k < part ? v[k][i] : 0;
+      }
+  }
+}
+
 // counts of digit PASS of a part; PASS > 0: finds the digit before it first
 template <int KPT, int PASS>
 __global__ __launch_bounds__(1024) void kv_count_kernel(KvPages t, KvWeights w, int keep, int recent, Counts c) {
@@ -252,10 +274,8 @@ __global__ __launch_bounds__(1024) void kv_count_kernel(KvPages t, KvWeights w, 
   uint32_t key[KPT], top = 0, mask = 0;
   load_keys<KPT>(t, w, b, h, first, x.old, key);
   if (PASS > 0) {
-    int v[2] = {0, 0};
-    for (int p = 0; p < parts; ++p)
-#pragma unroll
-      for (int i = 0; i < 2; ++i) v[i] += c.digits[((row * c.parts + p) * 3 + PASS - 1) * kBins + i * 1024 + tid];
+    int v[2], mine[2];
+    sum_parts(c, row, PASS - 1, parts, part, v, mine);
     counts[tid] = v[0];
     counts[1024 + tid] = v[1];
     __syncthreads();
@@ -313,12 +333,8 @@ __global__ __launch_bounds__(1024) void kv_list_kernel(KvPages t, KvWeights w, i
   if (x.sort) {
     const int parts = (x.old - 1) / (KPT * 1024) + 1;
     load_keys<KPT>(t, w, b, h, first, x.old, key);
-    int v[2] = {0, 0}, mine[2] = {0, 0};  // all parts' counts of the last digit, and those of the parts before
-    for (int p = 0; p < parts; ++p) {
-      if (p == part) mine[0] = v[0], mine[1] = v[1];
-#pragma unroll
-      for (int i = 0; i < 2; ++i) v[i] += c.digits[((row * c.parts + p) * 3 + 2) * kBins + i * 1024 + tid];
-    }
+    int v[2], mine[2];  // counts of the last digit
+    sum_parts(c, row, 2, parts, part, v, mine);
     counts[tid] = v[0];
     counts[1024 + tid] = v[1];
     if (tid < 2) before[tid] = 0;
