@@ -42,6 +42,7 @@
 // projections feed joint attention, and take its output, without a gather or
 // scatter copy.  Results are bitwise those of the gathered layout.
 #include <algorithm>
+#include <cmath>
 #include <mutex>
 
 #include "ditk_common.h"
@@ -181,21 +182,35 @@ __global__ __launch_bounds__(256, 1) void flash_fwd_asm(
   const int b = blockIdx.x;
   const int j = b >> 3;
   int t = CAUSAL ? b : ((j / chunk) * 8 + (b & 7)) * chunk + j % chunk;
-  int seg = -1, head = 0, npass = 0;
+  int seg = -1, head = 0, npass = 0, pk = 0;
   if constexpr (CAUSAL) {
-    for (int m = 0, prev = cu_q[0]; m < nseg; ++m) {
-      const int next = cu_q[m + 1];
-      const int ntile = (next - prev + BM - 1) / BM;
-      if (t < ntile * heads) {
-        seg = m;
+    // 64 segments at a time, one a lane: their items and padded keys, summed up over the lanes
+    const int lane = threadIdx.x & 63;
+    for (int m = 0; m < nseg; m += 64) {
+      const int i = min(m + lane, nseg - 1);
+      const int ntile = m + lane < nseg ? (cu_q[i + 1] - cu_q[i] + BM - 1) / BM : 0;
+      const int pad = m + lane < nseg ? (cu_k[i + 1] - cu_k[i] + BN - 1) / BN : 0;
+      int items = ntile * heads, pads = pad;
+      for (int off = 1; off < 64; off <<= 1) {
+        const int x = __shfl_up(items, off, 64), y = __shfl_up(pads, off, 64);
+        items += lane >= off ? x : 0;
+        pads += lane >= off ? y : 0;
+      }
+      const uint64_t past = __ballot(items > t);
+      if (past != 0) {
+        const int at = __builtin_ctzll(past);
+        const int nt = __builtin_amdgcn_readlane(ntile, at);
+        seg = m + at;
         npass = 1;
+        t -= __builtin_amdgcn_readlane(items, at) - nt * heads;
+        pk += (__builtin_amdgcn_readlane(pads, at) - __builtin_amdgcn_readlane(pad, at)) * BN;
         head = t % heads;
-        t = ntile - 1 - t / heads;
+        t = nt - 1 - t / heads;
         if ((heads & 7) == 0) head = (head & 7) * (heads >> 3) + (head >> 3);
         break;
       }
-      t -= ntile * heads;
-      prev = next;
+      t -= __builtin_amdgcn_readlane(items, 63);
+      pk += __builtin_amdgcn_readlane(pads, 63) * BN;
     }
   } else
   for (int m = 0, prev = cu_q[0]; m < nseg; ++m) {
@@ -236,7 +251,7 @@ __global__ __launch_bounds__(256, 1) void flash_fwd_asm(
     vlim[0] = min(qrow0 + ahead, k_len) - 8 * hh;
     vlim[1] = min(qrow1 + ahead, k_len) - 8 * hh;
   }
-  const int pk = padded_key_start(cu_k, seg);
+  if constexpr (!CAUSAL) pk = padded_key_start(cu_k, seg);
   // Q rows past the segment end read its last row (their outputs are not stored);
   // the body forms each lane's 64-bit row address from qbase, its row and ldq
   const uint64_t qbase = (uint64_t)(uintptr_t)(Q + head * ql.hs + seg * ql.sa);
@@ -514,9 +529,25 @@ int item_queries(int Tq, int nseg, int heads, int np, bool equal) {
   return most * heads <= ncu ? 128 : 256;
 }
 
-// Queries per work item of a causal launch: 128 when 256-query items would not fill the CUs
-int causal_item_queries(int Tq, int Tk, int nseg, int heads) {
-  return (int64_t)((Tq + 255) / 256) * heads < 2 * ditk_cu_count() ? 128 : 256;
+// Queries per work item of a causal launch, 128 or 256, whichever a time model says is done first (the choice changes no
+// result).  An item of one block a wave takes about 9 us and 0.85 a key tile (head_dim 64: 0.6), one of two 10 and 1.5
+// (0.95) or, while the CUs are not all busy, 1.18 (0.75): its start, Q's load and O's store are not hidden, and with all
+// CUs busy the matrix clock falls.  The longest run first, so a launch ends after its work divided by the CUs, plus what
+// the last round lacks of a whole one, or with its longest item.  Only totals are known here: segments count as equal.
+// 32 heads over 8: 1024 queries 24.9 us by 128 and 32.6 by 256, 2048 51.6 and 55.7, 4096 155 and 130; 8 of 2841 in all
+// 49.4 and 45.2; 512 after 8000 keys 120 and 157; head_dim 64, 8 heads, 16000 queries 337 and 262.
+int causal_item_queries(int Tq, int Tk, int nseg, int heads, int head_dim) {
+  const double ncu = ditk_cu_count(), n = (double)Tq / nseg, ahead = Tk > Tq ? (double)(Tk - Tq) / nseg : 0.0;
+  auto time = [&](double bm, double start, double busy, double light) {
+    const double tiles = std::ceil(n / bm), items = tiles * heads * nseg;
+    const double tile = items > ncu ? busy : light;
+    const double least = start + tile * std::ceil((ahead + std::min(bm, n)) / BN);
+    const double most = std::ceil((ahead + n) / BN), longest = start + tile * most;
+    const double rounds = items / ncu;
+    return std::max(start + light * most, rounds * (least + longest) / 2 + (std::ceil(rounds) - rounds) * least);
+  };
+  const bool wide = head_dim == 128;
+  return time(128, 9, wide ? 0.85 : 0.6, wide ? 0.85 : 0.6) <= time(256, 10, wide ? 1.5 : 0.95, wide ? 1.18 : 0.75) ? 128 : 256;
 }
 
 // shared checks and launch of both attention entry points; sl2 = the factor that
@@ -603,28 +634,30 @@ DITK_EXPORT int ditk_joint_attn_q_prescaled(const void* q_a, const void* q_b, in
                       cu_a, cu_b);
 }
 
-DITK_EXPORT int ditk_flash_attn_causal(const void* q, int64_t ldq, const void* k, int64_t ldk, const void* vt,
-                                       int64_t vt_ld, void* o, int64_t ldo, float* lse, int64_t lse_ld,
+DITK_EXPORT int ditk_flash_attn_causal(const void* q, int64_t ldq, const void* k, int64_t ldk, const void* v, int64_t ldv,
+                                       void* vt, int64_t vt_ld, void* o, int64_t ldo, float* lse, int64_t lse_ld,
                                        const int32_t* cu_q, const int32_t* cu_k, int nseg, int Tq, int Tk, int heads,
                                        int kv_heads, int head_dim, float softmax_scale, hipStream_t stream) {
   const char* what = "ditk_flash_attn_causal";
   DITK_REQUIRE(softmax_scale >= 1e-30f && softmax_scale <= 1e30f, "%s: softmax_scale must be in 1e-30..1e30", what);
-  DITK_REQUIRE(cu_q && cu_k && (Tq == 0 || (q && o)) && (Tk == 0 || (k && vt)), "%s: null tensor", what);
+  DITK_REQUIRE(cu_q && cu_k && (Tq == 0 || (q && o)) && (Tk == 0 || (k && v && vt)), "%s: null tensor", what);
   DITK_REQUIRE(head_dim == 64 || head_dim == 128, "%s: head_dim must be 64 or 128, got %d", what, head_dim);
   DITK_REQUIRE(nseg > 0 && Tq >= 0 && Tk >= 0 && Tq < (1 << 30) && Tk < (1 << 30), "%s: bad sizes", what);
   DITK_REQUIRE(heads > 0 && kv_heads > 0 && heads % kv_heads == 0, "%s: %d query heads for %d key heads", what, heads,
                kv_heads);
-  DITK_REQUIRE(ldq % 8 == 0 && ldk % 8 == 0 && ldo % 8 == 0 && vt_ld % 8 == 0 && vt_ld >= ditk_vt_columns(Tk, nseg),
+  DITK_REQUIRE(ldq % 8 == 0 && ldk % 8 == 0 && ldv % 8 == 0 && ldv >= 0 && ldo % 8 == 0 && vt_ld % 8 == 0 &&
+                   vt_ld >= ditk_vt_columns(Tk, nseg),
                "%s: leading dims must be multiples of 8, vt_ld at least ditk_vt_columns", what);
-  DITK_REQUIRE(((uintptr_t)q % 16) == 0 && ((uintptr_t)k % 16) == 0 && ((uintptr_t)vt % 16) == 0 &&
-                   ((uintptr_t)o % 16) == 0, "%s: misaligned tensor", what);
+  DITK_REQUIRE(((uintptr_t)q % 16) == 0 && ((uintptr_t)k % 16) == 0 && ((uintptr_t)v % 16) == 0 &&
+                   ((uintptr_t)vt % 16) == 0 && ((uintptr_t)o % 16) == 0, "%s: misaligned tensor", what);
   // the kernel addresses a 64-row K tile, HD Vt rows, and a row's bytes, with 32 bits
   DITK_REQUIRE(ldq >= 0 && ldk >= 0 && ldo >= 0 && ldq < (1ll << 30) && ldo < (1ll << 30) && ldk < (1ll << 23) &&
                    vt_ld < (1ll << 23), "%s: rows too long for 32-bit lane offsets", what);
   if (Tq == 0) return 0;
-  const int qb = causal_item_queries(Tq, Tk, nseg, heads) / 128;
+  const int qb = causal_item_queries(Tq, Tk, nseg, heads, head_dim) / 128;
   const int64_t nblocks = ((int64_t)(Tq + 128 * qb - 1) / (128 * qb) + nseg) * heads;
-  DITK_REQUIRE(nblocks < (1ll << 24), "%s: grid too large", what);
+  DITK_REQUIRE(nblocks < (1ll << 24) && kv_heads <= 65535, "%s: grid too large", what);
+  if (int rc = ditk_transpose_v(v, ldv, vt, vt_ld, Tk, kv_heads, head_dim, cu_k, nseg, stream)) return rc;
   const bool stream_out = (int64_t)Tq * heads * head_dim * 2 >= (64ll << 20);
   auto kern = head_dim == 128 ? (qb == 2 ? flash_fwd_asm<128, false, false, 2, true> : flash_fwd_asm<128, false, false, 1, true>)
                               : (qb == 2 ? flash_fwd_asm<64, false, false, 2, true> : flash_fwd_asm<64, false, false, 1, true>);

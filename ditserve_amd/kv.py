@@ -20,13 +20,14 @@ invalid cu_seqlens table is.  The pages a call writes must belong to one sequenc
 that are only read may be shared.  The reference has no counterpart: its models attend over
 whole videos.
 """
+import ctypes
 import math
 
 import torch
 
 from . import _lib, ops
 from .mx import _apart
-from .ops import _call, _check, _one_device, _ptr, _rows
+from .ops import _call, _check, _extent, _one_device, _ptr, _row_view
 
 PAGES = (16, 32, 64, 128, 256)
 HEAD_DIMS = (64, 128)
@@ -36,8 +37,13 @@ _BF16 = torch.bfloat16
 class PageStatus(ops.TableStatus):
     """TableStatus of the page tables and lengths that kv's calls were given."""
 
+    def __init__(self, device):
+        super().__init__(device)
+        self.address = self.host.data_ptr()
+        self._word = ctypes.c_int32.from_address(self.address)
+
     def poll(self):
-        if self.host.item() != 0:
+        if self._word.value:
             self.host.zero_()
             raise _lib.DitkError("an invalid page table reached the cache kernels (a length outside the table or "
                                  "max_len, or a page that the cache lacks); it was clamped into bounds, so those "
@@ -72,32 +78,36 @@ class PagedCache:
     weights  [pages, kv_heads, page] fp32, the attention weight each slot has gathered
              (optional; decode_attn writes it, evict reads it)"""
 
-    __slots__ = ("k", "v", "weights")
+    __slots__ = ("_k", "_v", "_w", "_dims", "_strides")
 
     def __init__(self, k, v, weights=None):
+        strides = []
         for t, name in ((k, "k"), (v, "v")):
             _check(t, name, _BF16, 4)
-            pages, heads, page, d = t.shape
+            pages, heads, page, d = dims = tuple(t.shape)
             ps, hs, ss, unit = t.stride()
             if page not in PAGES or d not in HEAD_DIMS:
-                raise ValueError(f"{name} must be [pages, kv_heads, {PAGES}, {HEAD_DIMS}], got {tuple(t.shape)}")
+                raise ValueError(f"{name} must be [pages, kv_heads, {PAGES}, {HEAD_DIMS}], got {dims}")
             if pages == 0 or heads == 0:
-                raise ValueError(f"{name} has no pages or no heads: {tuple(t.shape)}")
+                raise ValueError(f"{name} has no pages or no heads: {dims}")
             if unit != 1 or ss != d or ps % 8 or hs % 8 or t.data_ptr() % 16 or \
                     (pages > 1 and ps < page * d) or (heads > 1 and hs < page * d):
                 raise ValueError(f"{name}'s slots must be contiguous within a (page, head) and 16-byte aligned, got "
                                  f"strides {t.stride()}")
+            strides += [ps, hs]
         if v.shape != k.shape:
             raise ValueError(f"v must be {tuple(k.shape)}, got {tuple(v.shape)}")
         _one_device(k.device, ("v", v), ("weights", weights))
         if weights is not None:
             _check(weights, "weights", torch.float32, 3)
             ps, hs, unit = weights.stride()
-            if weights.shape != k.shape[:3] or unit != 1 or (k.shape[0] > 1 and ps < k.shape[2]) or \
-                    (k.shape[1] > 1 and hs < k.shape[2]):
-                raise ValueError(f"weights must be {tuple(k.shape[:3])} with unit slot stride, got "
-                                 f"{tuple(weights.shape)}, strides {weights.stride()}")
-        self.k, self.v, self.weights = k, v, weights
+            if tuple(weights.shape) != dims[:3] or unit != 1 or (pages > 1 and ps < page) or (heads > 1 and hs < page):
+                raise ValueError(f"weights must be {dims[:3]} with unit slot stride, got {tuple(weights.shape)}, strides "
+                                 f"{weights.stride()}")
+            strides += [ps, hs]
+        else:
+            strides += [0, 0]
+        self._k, self._v, self._w, self._dims, self._strides = k, v, weights, dims, strides
         _status(k.device)
 
     @classmethod
@@ -107,41 +117,35 @@ class PagedCache:
         w = torch.empty((pages, kv_heads, page), dtype=torch.float32, device=device) if weights else None
         return cls(k, v, w)
 
-    @property
-    def pages(self):
-        return self.k.shape[0]
-
-    @property
-    def kv_heads(self):
-        return self.k.shape[1]
-
-    @property
-    def page(self):
-        return self.k.shape[2]
-
-    @property
-    def head_dim(self):
-        return self.k.shape[3]
-
-    @property
-    def device(self):
-        return self.k.device
+    k = property(lambda self: self._k)
+    v = property(lambda self: self._v)
+    weights = property(lambda self: self._w)
+    pages = property(lambda self: self._dims[0])
+    kv_heads = property(lambda self: self._dims[1])
+    page = property(lambda self: self._dims[2])
+    head_dim = property(lambda self: self._dims[3])
+    device = property(lambda self: self._k.device)
 
     def record_stream(self, stream):
         """Mark the cache as in use by `stream` (for steps on a side stream)."""
-        for t in (self.k, self.v, self.weights):
+        for t in (self._k, self._v, self._w):
             if t is not None:
                 t.record_stream(stream)
 
-    def _kv(self):
-        (kp, kh, _, _), (vp, vh, _, _) = self.k.stride(), self.v.stride()
-        return self.k.data_ptr(), kp, kh, self.v.data_ptr(), vp, vh
+    def _args(self, weights=True):
+        """Addresses and strides of keys, values and (unless not wanted) weights."""
+        s = self._strides
+        w = (self._w.data_ptr(), s[4], s[5]) if weights and self._w is not None else (None, 0, 0)
+        return (self._k.data_ptr(), s[0], s[1], self._v.data_ptr(), s[2], s[3], *w)
 
-    def _weights(self, used=True):
-        if self.weights is None or not used:
-            return None, 0, 0
-        ps, hs, _ = self.weights.stride()
-        return self.weights.data_ptr(), ps, hs
+    def _spans(self):
+        """First and last byte of keys, values and weights."""
+        pages, heads, page, d = self._dims
+        for t, (ps, hs), size in ((self._k, self._strides[:2], 2 * d), (self._v, self._strides[2:4], 2 * d),
+                                  (self._w, self._strides[4:], 4)):
+            if t is not None:
+                first = t.data_ptr()
+                yield first, first + ((pages - 1) * ps + (heads - 1) * hs) * t.element_size() + page * size
 
 
 def _cache_check(cache):
@@ -171,35 +175,12 @@ def _lengths(t, device):
     return t.shape[0]
 
 
-def _outside(fn, cache, *tensors):
-    """Refuse rows and tables that lie between a cache's first and last byte."""
-    spans = []
-    for c in (cache.k, cache.v, cache.weights):
-        if c is not None:
-            (pages, heads, page), (ps, hs) = c.shape[:3], c.stride()[:2]
-            first, size = c.data_ptr(), c.element_size()
-            spans.append((first, first + ((pages - 1) * ps + (heads - 1) * hs + page * (c.shape[3] if size == 2 else 1)) * size))
-    for t in tensors:
-        if t is not None:
-            first = t.data_ptr()
-            rows = t.shape[0]
-            last = first + ((rows - 1) * t.stride(0) + (t.shape[1] if t.dim() == 2 else 1)) * t.element_size() if rows else first
-            for a, b in spans:
-                if first < b and a < last:
-                    raise ValueError(f"{fn}: an operand lies in the cache")
-
-
-def _rows_of(t, name, rows, cols, device):
-    if t.__class__ is not torch.Tensor or t.dtype is not _BF16 or t.dim() != 2 or t.device != device:
-        _check(t, name, _BF16, 2)
-        _one_device(device, (name, t))
-    n, wide = t.shape
-    if wide != cols or (rows is not None and n != rows):
-        raise ValueError(f"{name} must be [{'rows' if rows is None else rows}, {cols}], got {tuple(t.shape)}")
-    ld = _rows(t, name)
-    if n > 1 and ld < cols:
-        raise ValueError(f"{name}'s rows overlap: strides {t.stride()}")
-    return ld
+def _outside(fn, cache, *spans):
+    """Refuse operands (first and last byte) that lie between a cache's first and last byte."""
+    for a, b in cache._spans():
+        for first, last in spans:
+            if first < b and a < last:
+                raise ValueError(f"{fn}: an operand lies in the cache")
 
 
 def append(cache, k, v, table, lengths, segments=None):
@@ -210,26 +191,32 @@ def append(cache, k, v, table, lengths, segments=None):
     whose pages must be in the table already.  Returns the new lengths, a new int32 tensor;
     `lengths` itself stays.  The slots' weights, if the cache has any, become 0."""
     _cache_check(cache)
-    device, hk, d = cache.k.device, cache.kv_heads, cache.head_dim
+    device, (pages, hk, page, d) = cache._k.device, cache._dims
+    wide = hk * d
     batch = _lengths(lengths, device)
-    ldk = _rows_of(k, "k", None, hk * d, device)
-    T = k.shape[0]
-    ldv = _rows_of(v, "v", T, hk * d, device)
+    T, ldk = _row_view(k, "k", wide, device)
+    rows, ldv = _row_view(v, "v", wide, device)
+    if rows != T:
+        raise ValueError(f"k and v must have the same rows, got {T} and {rows}")
     tp, ldt, width = _table(table, "table", batch, device)
-    cu = None
+    kp, vp, lp, cu = k.data_ptr(), v.data_ptr(), lengths.data_ptr(), None
+    spans = [(kp, kp + 2 * ((T - 1) * ldk + wide) * (T > 0)), (vp, vp + 2 * ((T - 1) * ldv + wide) * (T > 0)),
+             (tp, tp + 4 * batch * ldt), (lp, lp + 4 * batch)]
     if segments is not None:
         if segments.nseg != batch or segments.total != T:
             raise ValueError(f"segments are {segments.nseg} of {segments.total} rows, lengths {batch} and k {T}")
-        cu = segments.dev
-        _one_device(device, ("segments", cu))
+        if segments.dev.device != device:
+            _one_device(device, ("segments", segments.dev))
+        cu = segments.dev.data_ptr()
+        spans.append((cu, cu + 4 * batch + 4))
     elif T != batch:
         raise ValueError(f"k must have one row for each of the {batch} sequences, got {T} (or pass segments)")
     status = _status(device)
     status.poll()
     new = torch.empty(batch, dtype=torch.int32, device=device)
-    _outside("append", cache, k, v, table, lengths, cu)
-    _call(device, "ditk_kv_append", _ptr(k), ldk, _ptr(v), ldv, *cache._kv(), *cache._weights(), cache.pages, cache.page,
-          tp, ldt, width, _ptr(lengths), _ptr(new), _ptr(cu), batch, T, hk, d, _ptr(status.host))
+    _outside("append", cache, *spans)
+    _call(device, "ditk_kv_append", kp, ldk, vp, ldv, *cache._args(), pages, page, tp, ldt, width, lp, new.data_ptr(), cu,
+          batch, T, hk, d, status.address)
     return new
 
 
@@ -245,18 +232,20 @@ def decode_attn(q, cache, table, lengths, heads, softmax_scale=None, max_len=Non
     bf16, and with return_lse lse [batch, heads] fp32 (natural log).  A sequence without
     slots gives zeros and -inf.  A sequence's result does not depend on the others."""
     _cache_check(cache)
-    device, hk, d = cache.k.device, cache.kv_heads, cache.head_dim
+    device, (pages, hk, page, d) = cache._k.device, cache._dims
     batch = _lengths(lengths, device)
     heads = int(heads)
     if heads <= 0 or heads % hk:
         raise ValueError(f"heads must be a multiple of the cache's {hk}, got {heads}")
-    ldq = _rows_of(q, "q", batch, heads * d, device)
+    rows, ldq = _row_view(q, "q", heads * d, device)
+    if rows != batch:
+        raise ValueError(f"q must have one row for each of the {batch} sequences, got {rows}")
     tp, ldt, width = _table(table, "table", batch, device)
     if weights not in (None, "set", "add"):
         raise ValueError(f"weights must be None, 'set' or 'add', got {weights!r}")
-    if weights is not None and cache.weights is None:
+    if weights is not None and cache._w is None:
         raise ValueError("the cache has no weights")
-    most = width * cache.page
+    most = width * page
     if max_len is not None:
         if max_len < 0:
             raise ValueError(f"max_len must not be negative, got {max_len}")
@@ -267,17 +256,20 @@ def decode_attn(q, cache, table, lengths, heads, softmax_scale=None, max_len=Non
     if out is None:
         out, ldo = torch.empty((batch, heads * d), dtype=_BF16, device=device), heads * d
     else:
-        ldo = _rows_of(out, "out", batch, heads * d, device)
-        _outside("decode_attn", cache, out)
+        rows, ldo = _row_view(out, "out", heads * d, device)
+        if rows != batch:
+            raise ValueError(f"out must have one row for each of the {batch} sequences, got {rows}")
+        _outside("decode_attn", cache, _extent(out))
         _apart("decode_attn", (out,), (q, table, lengths))
     status = _status(device)
     status.poll()
     lse = torch.empty((batch, heads), dtype=torch.float32, device=device) if return_lse else None
-    size = _lib.load().ditk_kv_attn_workspace(batch, heads, d, most, weights is not None)
+    # (up to 512 slots without weights take one launch and no workspace)
+    size = _lib.load().ditk_kv_attn_workspace(batch, heads, d, most, weights is not None) if weights or most > 512 else 0
     space = torch.empty(size, dtype=torch.uint8, device=device) if size else None
-    _call(device, "ditk_kv_attn", _ptr(q), ldq, *cache._kv(), *cache._weights(weights is not None), int(weights == "add"),
-          cache.pages, cache.page, tp, ldt, width, _ptr(lengths), most, _ptr(out), ldo, _ptr(lse), _ptr(space), size,
-          batch, heads, hk, d, scale, _ptr(status.host))
+    _call(device, "ditk_kv_attn", q.data_ptr(), ldq, *cache._args(weights is not None), int(weights == "add"), pages, page,
+          tp, ldt, width, lengths.data_ptr(), most, out.data_ptr(), ldo, _ptr(lse), _ptr(space), size, batch, heads, hk, d,
+          scale, status.address)
     return (out, lse) if return_lse else out
 
 
@@ -292,8 +284,8 @@ def evict(cache, table, lengths, out_table, keep, recent=0, max_len=None):
     max_len: the longest length there can be (default: what the table holds).  Returns the new
     lengths, a new int32 tensor."""
     _cache_check(cache)
-    device, hk, d = cache.k.device, cache.kv_heads, cache.head_dim
-    if cache.weights is None:
+    device, (pages, hk, page, d) = cache._k.device, cache._dims
+    if cache._w is None:
         raise ValueError("the cache has no weights")
     batch = _lengths(lengths, device)
     keep, recent = int(keep), int(recent)
@@ -302,13 +294,13 @@ def evict(cache, table, lengths, out_table, keep, recent=0, max_len=None):
     tp, ldt, width = _table(table, "table", batch, device)
     op, ldo, out_width = _table(out_table, "out_table", batch, device)
     _apart("evict", (out_table,), (table,))
-    most = width * cache.page
+    most = width * page
     if max_len is not None:
         if max_len < 0:
             raise ValueError(f"max_len must not be negative, got {max_len}")
         most = min(most, int(max_len))
-    if out_width * cache.page < min(keep, most):
-        raise ValueError(f"out_table holds {out_width * cache.page} slots, {min(keep, most)} stay")
+    if out_width * page < min(keep, most):
+        raise ValueError(f"out_table holds {out_width * page} slots, {min(keep, most)} stay")
     keep = max(min(keep, most), 1)
     recent = min(recent, keep)
     status = _status(device)
@@ -316,7 +308,6 @@ def evict(cache, table, lengths, out_table, keep, recent=0, max_len=None):
     new = torch.empty(batch, dtype=torch.int32, device=device)
     size = _lib.load().ditk_kv_evict_workspace(batch, hk, most, keep)
     space = torch.empty(size, dtype=torch.uint8, device=device)
-    _call(device, "ditk_kv_evict", *cache._kv(), *cache._weights(), cache.pages, cache.page, tp, ldt, width,
-          _ptr(lengths), most, op, ldo, out_width, _ptr(new), keep, recent, _ptr(space), size, batch, hk, d,
-          _ptr(status.host))
+    _call(device, "ditk_kv_evict", *cache._args(), pages, page, tp, ldt, width, _ptr(lengths), most, op, ldo, out_width,
+          _ptr(new), keep, recent, _ptr(space), size, batch, hk, d, status.address)
     return new

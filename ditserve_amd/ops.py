@@ -98,6 +98,22 @@ def _rows(t, name):
     return st[0]
 
 
+def _row_view(t, name, cols, device):
+    """(rows, row stride) of a bf16 row view of `cols` columns on `device` whose rows lie apart, or the refusal."""
+    if t.__class__ is not torch.Tensor or t.dtype is not _BF16 or t.dim() != 2 or t.device != device:
+        _check(t, name, _BF16, 2)
+        _one_device(device, (name, t))
+    n, wide = t.shape
+    if wide != cols:
+        raise ValueError(f"{name} must have {cols} columns, got {tuple(t.shape)}")
+    ld, unit = t.stride()
+    if unit != 1 or ld & 7 or t.data_ptr() & 15:
+        _rows(t, name)
+    if ld < cols and n > 1:
+        raise ValueError(f"{name}'s rows overlap: strides {t.stride()}")
+    return n, ld
+
+
 class Segments:
     """Packed-batch segment table: host list of offsets + device int32 copy.
 
@@ -686,38 +702,37 @@ def flash_attn_causal(q, k, v, seg_q, seg_k, heads, kv_heads, head_dim, softmax_
         raise ValueError(f"heads must be a multiple of kv_heads, got {heads} and {kv_heads}")
     if head_dim not in (64, 128):
         raise ValueError(f"head_dim must be 64 or 128, got {head_dim}")
-    for t, n, h in ((q, "q", heads), (k, "k", kv_heads), (v, "v", kv_heads)):
-        _check(t, n, _BF16, 2)
-        if t.shape[1] != h * head_dim:
-            raise ValueError(f"{n} must have {h * head_dim} columns, got {t.shape[1]}")
-    Tq, Tk, device = q.shape[0], k.shape[0], q.device
-    if v.shape[0] != Tk:
-        raise ValueError(f"k and v must have the same rows, got {Tk} and {v.shape[0]}")
-    if seg_q.nseg != seg_k.nseg:
+    _check(q, "q", _BF16, 2)
+    device = q.device
+    Tq, ldq = _row_view(q, "q", heads * head_dim, device)
+    Tk, ldk = _row_view(k, "k", kv_heads * head_dim, device)
+    rows, ldv = _row_view(v, "v", kv_heads * head_dim, device)
+    if rows != Tk:
+        raise ValueError(f"k and v must have the same rows, got {Tk} and {rows}")
+    nseg, cu_q, cu_k = seg_q.nseg, seg_q.dev, seg_k.dev
+    if nseg != seg_k.nseg:
         raise ValueError("cu_seqlens_q and cu_seqlens_k must describe the same number of segments")
     if seg_q.total != Tq or seg_k.total != Tk:
         raise ValueError("cu_seqlens totals must match the packed token counts")
-    _one_device(device, ("k", k), ("v", v), ("seg_q", seg_q.dev), ("seg_k", seg_k.dev))
-    ldq, ldk, ldv = _rows(q, "q"), _rows(k, "k"), _rows(v, "v")
+    if cu_q.device != device or cu_k.device != device:
+        _one_device(device, ("seg_q", cu_q), ("seg_k", cu_k))
     if out is None:
         out, ldo = torch.empty((Tq, heads * head_dim), dtype=_BF16, device=device), heads * head_dim
     else:
-        _check(out, "out", _BF16, 2)
-        _one_device(device, ("out", out))
-        if out.shape != q.shape:
+        rows, ldo = _row_view(out, "out", heads * head_dim, device)
+        if rows != Tq:
             raise ValueError(f"out must be {tuple(q.shape)}, got {tuple(out.shape)}")
-        ldo = _rows(out, "out")
         for t, n in ((q, "q"), (k, "k"), (v, "v")):
             if _overlap(out, t) and not _beside(out, t):
                 raise ValueError(f"out overlaps {n}")
     scale = 1.0 / math.sqrt(head_dim) if softmax_scale is None else float(softmax_scale)
     lse = torch.empty((heads, Tq), dtype=torch.float32, device=device) if return_lse else None
     if Tq:
-        cols = vt_columns(Tk, seg_k.nseg)
-        vt = torch.empty((kv_heads, head_dim, cols), dtype=_BF16, device=device)
-        _call(device, "ditk_transpose_v", _ptr(v), ldv, _ptr(vt), cols, Tk, kv_heads, head_dim, _ptr(seg_k.dev), seg_k.nseg)
-        _call(device, "ditk_flash_attn_causal", _ptr(q), ldq, _ptr(k), ldk, _ptr(vt), cols, _ptr(out), ldo, _ptr(lse), Tq,
-              _ptr(seg_q.dev), _ptr(seg_k.dev), seg_q.nseg, Tq, Tk, heads, kv_heads, head_dim, scale)
+        cols = ((Tk + 63) // 64 + nseg) * 64  # vt_columns
+        vt = torch.empty(kv_heads * head_dim * cols, dtype=_BF16, device=device)
+        _call(device, "ditk_flash_attn_causal", q.data_ptr(), ldq, k.data_ptr(), ldk, v.data_ptr(), ldv, vt.data_ptr(), cols,
+              out.data_ptr(), ldo, _ptr(lse), Tq, cu_q.data_ptr(), cu_k.data_ptr(), nseg, Tq, Tk, heads, kv_heads, head_dim,
+              scale)
     return (out, lse) if return_lse else out
 
 
