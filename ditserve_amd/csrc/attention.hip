@@ -6,7 +6,7 @@
 // (cu_k = 512-row text blocks) and SD3.5 joint attention (image+text joint
 // segments) are all this one kernel.
 //
-// V is consumed transposed: Vt [heads][HD][Tpad], where segment m's keys start
+// V is consumed transposed (by causal attention as it is): Vt [heads][HD][Tpad], where segment m's keys start
 // at the 64-aligned column pk[m] = 64 * sum_{m'<m} ceil(len_k[m'] / 64) and the
 // padding columns are zero.  ditk_transpose_v produces it.
 //
@@ -51,6 +51,8 @@
 #include "attn_d64_clobbers.h"
 #include "attn_d64p_clobbers.h"
 #include "attn_d64j_clobbers.h"
+#include "attn_d128c_clobbers.h"
+#include "attn_d64c_clobbers.h"
 
 namespace {
 
@@ -139,9 +141,24 @@ __device__ __forceinline__ int padded_key_start(const int32_t* __restrict__ cu, 
       [qa1lo] "a"((uint32_t)qa[1]), [qa1hi] "a"((uint32_t)(qa[1] >> 32)), [krow0] "a"(krow_of[0]),                  \
       [krow1] "a"(krow_of[1]), [krow2] "a"(krow_of[2]), [krow3] "a"(krow_of[3])
 // Causal (plain q): how many keys each lane's queries see, less 8 (lane / 32), and the
-// first key tile that is not whole to every query of the wave
+// first key tile that is not whole to every query of the wave; V's rows, a tile of them
+// and their DMA offsets (in AGPRs: the body copies them)
 #define DITK_ATTN_ASM_OPERANDS_CAUSAL                                                                               \
-  DITK_ATTN_ASM_OPERANDS, [vlim0] "v"(vlim[0]), [vlim1] "v"(vlim[1]), [kdiag] "s"(su(kdiag))
+  [qbase_lo] "s"(su((uint32_t)qbase)), [qbase_hi] "s"(su((uint32_t)(qbase >> 32))), [kdma_lo] "s"(su((uint32_t)kdma)), \
+      [kdma_hi] "s"(su((uint32_t)(kdma >> 32))), [vdma_lo] "s"(su((uint32_t)vdma)),                               \
+      [vdma_hi] "s"(su((uint32_t)(vdma >> 32))), [lds_k] "s"(su(lds_k)), [lds_v] "s"(su(lds_v)),                   \
+      [nkt] "s"(su(nkt)), [valid_last] "s"(su(valid_last)), [ktile] "s"(su(ktile)), [wave1k] "s"(su(wave1k)),      \
+      [lds_o] "s"(su(lds_o)), [npass] "s"(su(npass)), [ldqb] "s"(su(ldqb)), [sc] "s"(sc), [qend] "s"(su(q_end)),     \
+      [ldob] "s"(su(ldob)), [obase_lo] "s"(su((uint32_t)obase)), [obase_hi] "s"(su((uint32_t)(obase >> 32))),       \
+      [has_lse] "s"(su(has_lse)), [ont] "s"(su(stream_out)), [lsebase] "s"(su64(lsebase)),                          \
+      [kaddr0] "v"(kaddr[0]), [kaddr1] "v"(kaddr[1]), [kaddr2] "v"(kaddr[2]), [kaddr3] "v"(kaddr[3]),             \
+      [vaddr0] "v"(vaddr[0]), [vaddr1] "v"(vaddr[1]), [vaddr2] "v"(vaddr[2]), [vaddr3] "v"(vaddr[3]),             \
+      [koff0] "v"(koff[0]), [koff1] "v"(koff[1]), [koff2] "v"(koff[2]), [koff3] "v"(koff[3]),                     \
+      [koffl0] "v"(koffl[0]), [koffl1] "v"(koffl[1]), [koffl2] "v"(koffl[2]), [koffl3] "v"(koffl[3]),             \
+      [voff0] "a"(voff[0]), [voff1] "a"(voff[1]), [voff2] "a"(voff[2]), [voff3] "a"(voff[3]),                     \
+      [voffl0] "a"(voffl[0]), [voffl1] "a"(voffl[1]), [voffl2] "a"(voffl[2]), [voffl3] "a"(voffl[3]),             \
+      [flag] "s"(su(lds_f)), [lane] "v"(lanev), [qrow0] "v"(qrow0), [qrow1] "v"(qrow1), [vlim0] "v"(vlim[0]),       \
+      [vlim1] "v"(vlim[1]), [kdiag] "s"(su(kdiag)), [vtile] "s"(su(vtile))
 // Row r, head h of segment m of an operand lies at base + h * hs + m * sa + r * ld
 // (elements).  Packed rows: hs = head_dim, sa = 0.  A [batch, heads, rows, head_dim]
 // tensor read in place: hs and ld its head and row strides, sa = batch stride -
@@ -182,19 +199,17 @@ __global__ __launch_bounds__(256, 1) void flash_fwd_asm(
   const int b = blockIdx.x;
   const int j = b >> 3;
   int t = CAUSAL ? b : ((j / chunk) * 8 + (b & 7)) * chunk + j % chunk;
-  int seg = -1, head = 0, npass = 0, pk = 0;
+  int seg = -1, head = 0, npass = 0;
   if constexpr (CAUSAL) {
-    // 64 segments at a time, one a lane: their items and padded keys, summed up over the lanes
+    // 64 segments at a time, one a lane: their items, summed up over the lanes
     const int lane = threadIdx.x & 63;
     for (int m = 0; m < nseg; m += 64) {
       const int i = min(m + lane, nseg - 1);
       const int ntile = m + lane < nseg ? (cu_q[i + 1] - cu_q[i] + BM - 1) / BM : 0;
-      const int pad = m + lane < nseg ? (cu_k[i + 1] - cu_k[i] + BN - 1) / BN : 0;
-      int items = ntile * heads, pads = pad;
+      int items = ntile * heads;
       for (int off = 1; off < 64; off <<= 1) {
-        const int x = __shfl_up(items, off, 64), y = __shfl_up(pads, off, 64);
+        const int x = __shfl_up(items, off, 64);
         items += lane >= off ? x : 0;
-        pads += lane >= off ? y : 0;
       }
       const uint64_t past = __ballot(items > t);
       if (past != 0) {
@@ -203,14 +218,12 @@ __global__ __launch_bounds__(256, 1) void flash_fwd_asm(
         seg = m + at;
         npass = 1;
         t -= __builtin_amdgcn_readlane(items, at) - nt * heads;
-        pk += (__builtin_amdgcn_readlane(pads, at) - __builtin_amdgcn_readlane(pad, at)) * BN;
         head = t % heads;
         t = nt - 1 - t / heads;
         if ((heads & 7) == 0) head = (head & 7) * (heads >> 3) + (head >> 3);
         break;
       }
       t -= __builtin_amdgcn_readlane(items, 63);
-      pk += __builtin_amdgcn_readlane(pads, 63) * BN;
     }
   } else
   for (int m = 0, prev = cu_q[0]; m < nseg; ++m) {
@@ -251,7 +264,7 @@ __global__ __launch_bounds__(256, 1) void flash_fwd_asm(
     vlim[0] = min(qrow0 + ahead, k_len) - 8 * hh;
     vlim[1] = min(qrow1 + ahead, k_len) - 8 * hh;
   }
-  if constexpr (!CAUSAL) pk = padded_key_start(cu_k, seg);
+  const int pk = CAUSAL ? 0 : padded_key_start(cu_k, seg);
   // Q rows past the segment end read its last row (their outputs are not stored);
   // the body forms each lane's 64-bit row address from qbase, its row and ldq
   const uint64_t qbase = (uint64_t)(uintptr_t)(Q + head * ql.hs + seg * ql.sa);
@@ -275,7 +288,10 @@ __global__ __launch_bounds__(256, 1) void flash_fwd_asm(
       qa[qb] = (uint64_t)(uintptr_t)(src + (int64_t)head * HD + hh * 8);
     }
   }
-  const uint64_t vdma = (uint64_t)(uintptr_t)(Vt + (int64_t)kv_head * vt_hs + pk);
+  // (causal: Vt is V, its rows vt_ld apart and its heads vt_hs)
+  const uint64_t vdma = (uint64_t)(uintptr_t)(Vt + (int64_t)kv_head * vt_hs + (CAUSAL ? (int64_t)k_beg * vt_ld : pk));
+  const uint32_t vtile = (uint32_t)(BN * vt_ld * 2);
+  (void)vtile;
   const uint32_t ktile = (uint32_t)(BN * ldk * 2);
   const uint32_t ldkb = (uint32_t)(ldk * 2);
   // LDS read bases (bytes within a stage): K rows permuted by kperm, 16-byte
@@ -289,7 +305,8 @@ __global__ __launch_bounds__(256, 1) void flash_fwd_asm(
   const uint32_t lds_o = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) u32x4_t*)&Os[0] +
                          (uint32_t)wave_u * (32 * OPITCH);
   const uint32_t lds_f = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint32_t*)&Fs[wave_u];
-  uint32_t kaddr[4], vaddr[4], koff[4] = {}, koffl[4] = {}, voff[4] = {};
+  uint32_t kaddr[4], vaddr[4], koff[4] = {}, koffl[4] = {}, voff[4] = {}, voffl[4] = {};
+  (void)voffl;
   const int lrow = lane >> 3;
   const int lsw0 = ((lane & 7) ^ ((lane >> 4) & 7)) * 8;
   const int lsw1 = ((lane & 7) ^ (((lane >> 4) + 4) & 7)) * 8;
@@ -297,6 +314,12 @@ __global__ __launch_bounds__(256, 1) void flash_fwd_asm(
   for (int i = 0; i < 4; ++i) {
     kaddr[i] = lds_k + (uint32_t)(kr * 8 + ((i * 2 + hh) ^ kg)) * 16;
     vaddr[i] = lds_v + (uint32_t)(l32 * 8 + ((i * 2 + hh) ^ vg)) * 16;
+    if constexpr (CAUSAL) {
+      // V stage: rows of HD dims, the 64-byte pieces of a row swizzled by it so that 4 rows of one piece lie in
+      // different banks.  Transposing reads of d tile i: lane 16 g + 4 r + c reads 4 dims of row 8 (g / 2) + r.
+      const int r = (lane >> 2) & 3, row = 8 * hh + r, piece = HD == 128 ? i ^ r : (i & 1) ^ (r >> 1);
+      vaddr[i] = lds_v + (uint32_t)(row * HD * 2 + piece * 64 + ((lane >> 4) & 1) * 32 + (lane & 3) * 8);
+    }
   }
 #pragma unroll
   for (int i = 0; i < ND; ++i) {
@@ -308,6 +331,13 @@ __global__ __launch_bounds__(256, 1) void flash_fwd_asm(
     koffl[i] = min(krow, (uint32_t)(valid_rows - 1)) * ldkb + kcolb;
     if constexpr (JOINT) krow_of[i] = krow;
     voff[i] = (uint32_t)((int64_t)(g * 8 + lrow) * vt_ld + ((g & 1) ? lsw1 : lsw0)) * 2;
+    if constexpr (CAUSAL) {  // 64 slots of 16 bytes: 4 (head_dim 64: 8) rows
+      constexpr int CH = HD / 8;
+      const int row = g * (64 / CH) + lane / CH, piece = (lane % CH) >> 2;
+      const int from = (HD == 128 ? piece ^ (row & 3) : piece ^ ((row >> 1) & 1)) * 4 + (lane & 3);
+      voff[i] = (uint32_t)(row * vt_ld * 2) + (uint32_t)from * 16;
+      voffl[i] = (uint32_t)(min(row, valid_rows - 1) * vt_ld * 2) + (uint32_t)from * 16;
+    }
   }
   const uint32_t wave1k = (uint32_t)wave_u * 1024u;
   const uint32_t lanev = (uint32_t)lane;
@@ -324,19 +354,19 @@ __global__ __launch_bounds__(256, 1) void flash_fwd_asm(
   if constexpr (CAUSAL && HD == 128 && QB == 2) {
     asm volatile(
 #include "attn_d128c_body.inc"
-        : : DITK_ATTN_ASM_OPERANDS_CAUSAL : DITK_D128_CLOBBERS "vcc", "scc", "memory");
+        : : DITK_ATTN_ASM_OPERANDS_CAUSAL : DITK_D128C_CLOBBERS "vcc", "scc", "memory");
   } else if constexpr (CAUSAL && HD == 128 && QB == 1) {
     asm volatile(
 #include "attn_d128cq1_body.inc"
-        : : DITK_ATTN_ASM_OPERANDS_CAUSAL : DITK_D128_CLOBBERS "vcc", "scc", "memory");
+        : : DITK_ATTN_ASM_OPERANDS_CAUSAL : DITK_D128C_CLOBBERS "vcc", "scc", "memory");
   } else if constexpr (CAUSAL && HD == 64 && QB == 2) {
     asm volatile(
 #include "attn_d64c_body.inc"
-        : : DITK_ATTN_ASM_OPERANDS_CAUSAL : DITK_D64_CLOBBERS "vcc", "scc", "memory");
+        : : DITK_ATTN_ASM_OPERANDS_CAUSAL : DITK_D64C_CLOBBERS "vcc", "scc", "memory");
   } else if constexpr (CAUSAL && HD == 64 && QB == 1) {
     asm volatile(
 #include "attn_d64cq1_body.inc"
-        : : DITK_ATTN_ASM_OPERANDS_CAUSAL : DITK_D64_CLOBBERS "vcc", "scc", "memory");
+        : : DITK_ATTN_ASM_OPERANDS_CAUSAL : DITK_D64C_CLOBBERS "vcc", "scc", "memory");
   } else if constexpr (HD == 128 && !PRE && QB == 2) {
     asm volatile(
 #include "attn_d128_body.inc"
@@ -635,35 +665,32 @@ DITK_EXPORT int ditk_joint_attn_q_prescaled(const void* q_a, const void* q_b, in
 }
 
 DITK_EXPORT int ditk_flash_attn_causal(const void* q, int64_t ldq, const void* k, int64_t ldk, const void* v, int64_t ldv,
-                                       void* vt, int64_t vt_ld, void* o, int64_t ldo, float* lse, int64_t lse_ld,
+                                       void* o, int64_t ldo, float* lse, int64_t lse_ld,
                                        const int32_t* cu_q, const int32_t* cu_k, int nseg, int Tq, int Tk, int heads,
                                        int kv_heads, int head_dim, float softmax_scale, hipStream_t stream) {
   const char* what = "ditk_flash_attn_causal";
   DITK_REQUIRE(softmax_scale >= 1e-30f && softmax_scale <= 1e30f, "%s: softmax_scale must be in 1e-30..1e30", what);
-  DITK_REQUIRE(cu_q && cu_k && (Tq == 0 || (q && o)) && (Tk == 0 || (k && v && vt)), "%s: null tensor", what);
+  DITK_REQUIRE(cu_q && cu_k && (Tq == 0 || (q && o)) && (Tk == 0 || (k && v)), "%s: null tensor", what);
   DITK_REQUIRE(head_dim == 64 || head_dim == 128, "%s: head_dim must be 64 or 128, got %d", what, head_dim);
   DITK_REQUIRE(nseg > 0 && Tq >= 0 && Tk >= 0 && Tq < (1 << 30) && Tk < (1 << 30), "%s: bad sizes", what);
   DITK_REQUIRE(heads > 0 && kv_heads > 0 && heads % kv_heads == 0, "%s: %d query heads for %d key heads", what, heads,
                kv_heads);
-  DITK_REQUIRE(ldq % 8 == 0 && ldk % 8 == 0 && ldv % 8 == 0 && ldv >= 0 && ldo % 8 == 0 && vt_ld % 8 == 0 &&
-                   vt_ld >= ditk_vt_columns(Tk, nseg),
-               "%s: leading dims must be multiples of 8, vt_ld at least ditk_vt_columns", what);
+  DITK_REQUIRE(ldq % 8 == 0 && ldk % 8 == 0 && ldv % 8 == 0 && ldo % 8 == 0,
+               "%s: leading dims must be multiples of 8", what);
   DITK_REQUIRE(((uintptr_t)q % 16) == 0 && ((uintptr_t)k % 16) == 0 && ((uintptr_t)v % 16) == 0 &&
-                   ((uintptr_t)vt % 16) == 0 && ((uintptr_t)o % 16) == 0, "%s: misaligned tensor", what);
-  // the kernel addresses a 64-row K tile, HD Vt rows, and a row's bytes, with 32 bits
-  DITK_REQUIRE(ldq >= 0 && ldk >= 0 && ldo >= 0 && ldq < (1ll << 30) && ldo < (1ll << 30) && ldk < (1ll << 23) &&
-                   vt_ld < (1ll << 23), "%s: rows too long for 32-bit lane offsets", what);
+                   ((uintptr_t)o % 16) == 0, "%s: misaligned tensor", what);
+  // the kernel addresses a tile of 64 K or V rows, and a row's bytes, with 32 bits
+  DITK_REQUIRE(ldq >= 0 && ldk >= 0 && ldv >= 0 && ldo >= 0 && ldq < (1ll << 30) && ldo < (1ll << 30) &&
+                   ldk < (1ll << 23) && ldv < (1ll << 23), "%s: rows too long for 32-bit lane offsets", what);
   if (Tq == 0) return 0;
   const int qb = causal_item_queries(Tq, Tk, nseg, heads, head_dim) / 128;
   const int64_t nblocks = ((int64_t)(Tq + 128 * qb - 1) / (128 * qb) + nseg) * heads;
-  DITK_REQUIRE(nblocks < (1ll << 24) && kv_heads <= 65535, "%s: grid too large", what);
-  if (int rc = ditk_transpose_v(v, ldv, vt, vt_ld, Tk, kv_heads, head_dim, cu_k, nseg, stream)) return rc;
+  DITK_REQUIRE(nblocks < (1ll << 24), "%s: grid too large", what);
   const bool stream_out = (int64_t)Tq * heads * head_dim * 2 >= (64ll << 20);
   auto kern = head_dim == 128 ? (qb == 2 ? flash_fwd_asm<128, false, false, 2, true> : flash_fwd_asm<128, false, false, 1, true>)
                               : (qb == 2 ? flash_fwd_asm<64, false, false, 2, true> : flash_fwd_asm<64, false, false, 1, true>);
   kern<<<(unsigned)nblocks, 256, 0, stream>>>(
-      (const bf16_t*)q, ldq, (const bf16_t*)k, ldk, (const bf16_t*)vt, vt_ld, (int64_t)head_dim * vt_ld, (bf16_t*)o, ldo,
-      lse, lse_ld, cu_q, cu_k, nseg, heads, 1, 1, stream_out, softmax_scale * 1.4426950408889634f, RowLayout{head_dim, 0},
+      (const bf16_t*)q, ldq, (const bf16_t*)k, ldk, (const bf16_t*)v, ldv, head_dim, (bf16_t*)o, ldo, lse, lse_ld, cu_q, cu_k, nseg, heads, 1, 1, stream_out, softmax_scale * 1.4426950408889634f, RowLayout{head_dim, 0},
       RowLayout{head_dim, 0}, nullptr, nullptr, nullptr, nullptr, nullptr, heads / kv_heads);
   return ditk_check_launch(what);
 }

@@ -45,8 +45,8 @@ v_accvgpr_write, an s_nop between an M0 write and the DMA that reads it.
 
 Usage: python gen_attn.py [dir/any]  (writes attn_d128_body.inc, attn_d128p_body.inc,
 attn_d64_body.inc, attn_d64p_body.inc, attn_d64j_body.inc and their
-*_clobbers.h, and attn_d128c_body.inc and attn_d64c_body.inc, into that directory,
-default beside this file)
+*_clobbers.h, and the causal attn_d128c and attn_d64c ones, into that directory, default
+beside this file)
 """
 import os
 import sys
@@ -93,12 +93,14 @@ def configure(hd, pre=False, joint=False, qb=2, causal=False):
     last key that a query of the workgroup sees, and from tile %[kdiag] on, the first that
     is not seen whole by every query of the wave, a tile's scores are set to -inf where they
     are not seen, out of line, once they are complete (mask_scores).  The tile that holds a
-    segment's last key is such a tile for every wave, so no row sums are masked."""
+    segment's last key is such a tile for every wave, so no row sums are masked.  V comes as
+    rows, like K (no transposed copy): its stage holds 64 rows of HD dims, and a Vt fragment
+    is two transposing reads, each of 4 keys x 16 dims a group of 16 lanes."""
     global QB, BM, KRING, KA, VRING, VA
     QB, BM = qb, 128 * qb
     KRING, KA, VRING, VA = (3, 2, 6, 4) if qb == 2 else (6, 4, 10, 8)
     global HD, NC, DT, NF, ND, KSTAGE_BYTES, VSTAGE_BYTES, O_A, Q_A, KF_A, VF_A, LAST_AGPR
-    global PRE, TMP, RING, DTMP, RS0, RS1, NEGM, NEGB, LRUN, KOFF, LAST_VGPR, EPI_T, EPI_L, JOINT, CAUSAL
+    global PRE, TMP, RING, DTMP, RS0, RS1, NEGM, NEGB, LRUN, KOFF, LAST_VGPR, EPI_T, EPI_L, JOINT, CAUSAL, VOFF
     assert pre or not joint
     assert not (causal and pre)
     HD, PRE, JOINT, CAUSAL = hd, pre, joint, causal
@@ -111,7 +113,8 @@ def configure(hd, pre=False, joint=False, qb=2, causal=False):
     else:
         RING = 4                       # exp temporaries: a ring of four score pairs
         RS0, RS1, NEGM, LRUN, KOFF, DTMP, NEGB = 200, 202, 204, 206, 208, 212, None
-        LAST_VGPR = 215
+        VOFF = 216                     # causal: V DMA source offsets (switched as K's)
+        LAST_VGPR = 219 if causal else 215
         EPI_T, EPI_L = TMP, DTMP
     NC, DT = hd // 16, hd // 32
     NF = 4 * DT
@@ -376,7 +379,29 @@ def vdma_m0(g, i, stage):
 
 
 def vdma_go(g, i):
-    g(f"global_load_lds_dwordx4 %[voff{i}], {sp(S_VDMA)}")
+    g(f"global_load_lds_dwordx4 {vr(VOFF + i) if CAUSAL else f'%[voff{i}]'}, {sp(S_VDMA)}")
+
+
+def vdma_next(g):
+    """V DMA base: the next tile's columns of Vt, or (causal) rows of V."""
+    g(f"s_add_u32 {s_(S_VDMA)}, {s_(S_VDMA)}, {'%[vtile]' if CAUSAL else BN * 2}")
+    g(f"s_addc_u32 {s_(S_VDMA + 1)}, {s_(S_VDMA + 1)}, 0")
+
+
+def voff_set(g, name):
+    """Causal: V DMA offsets from the AGPR operands `name` (voff, or voffl: rows past the end
+    read the last row)."""
+    for i in range(ND):
+        g(f"v_accvgpr_read_b32 {vr(VOFF + i)}, %[{name}{i}]")
+
+
+def clamp_voff(g, cmp):
+    """The last tile's V DMA offsets when the scalar compare `cmp` holds."""
+    skip = g.new_label("noclampv")
+    g(cmp)
+    g(f"s_cbranch_scc0 {skip}")
+    voff_set(g, "voffl")
+    g.label(skip)
 
 
 def kdma_block(g, stage):
@@ -416,6 +441,12 @@ def k_read(g, chunk, kk, stage):
 
 def v_read(g, f, stage):
     grp, d = f // DT, f % DT
+    if CAUSAL:  # keys 16 grp + 8 (lane / 32) + 0..3, then + 4..7
+        for half in range(2):
+            off = stage * VSTAGE_BYTES + (16 * grp + 4 * half) * HD * 2
+            g(f"ds_read_b64_tr_b16 {ar(vf_reg(f % VRING) + 2 * half, 2)}, %[vaddr{d}] offset:{off}")
+            g.lds_issue(("v", f) if half else ("v", f, "first half"))
+        return
     g(f"ds_read_b128 {ar(vf_reg(f % VRING), 4)}, %[vaddr{grp}] offset:{stage * VSTAGE_BYTES + d * 4096}")
     g.lds_issue(("v", f))
 
@@ -700,6 +731,9 @@ def tile(g, a):
         g(f"s_add_u32 {s_(S_KDMA)}, {s_(S_KDMA)}, %[kdma_lo]")
         g(f"s_addc_u32 {s_(S_KDMA + 1)}, {s_(S_KDMA + 1)}, %[kdma_hi]")
         clamp_koff(g, f"s_cmp_eq_u32 {s_(S_T0)}, {s_(S_NKT1)}")
+        if CAUSAL:
+            g(f"s_add_u32 {s_(S_T0)}, {s_(S_KT)}, 1")
+            clamp_voff(g, f"s_cmp_eq_u32 {s_(S_T0)}, {s_(S_NKT1)}")
     dmas = ([(lambda i=i: kdma_m0(g, i, a), lambda i=i: kdma_go(g, i)) for i in range(ND)] +
             [(lambda i=i: vdma_m0(g, i, b), lambda i=i: vdma_go(g, i)) for i in range(ND)])
     # phase 1: S(kt+1) into set b || P(kt) keys 32..63 from set a
@@ -741,8 +775,7 @@ def tile(g, a):
     # publish this tile's DMA: own loads landed, then the workgroup barrier
     g("s_waitcnt vmcnt(0)")
     g("s_barrier")
-    g(f"s_add_u32 {s_(S_VDMA)}, {s_(S_VDMA)}, {BN * 2}")
-    g(f"s_addc_u32 {s_(S_VDMA + 1)}, {s_(S_VDMA + 1)}, 0")
+    vdma_next(g)
     g(f"s_add_u32 {s_(S_KT)}, {s_(S_KT)}, 1")
     # the next tile's first K reads: K(kt+2), in stage a
     for c in range(KA):
@@ -908,9 +941,11 @@ def first_vt_dma(g):
     """DMA Vt(0) into Vt stage 0; the Vt DMA base then points at tile 1."""
     g(f"s_mov_b32 {s_(S_VDMA)}, %[vdma_lo]")
     g(f"s_mov_b32 {s_(S_VDMA + 1)}, %[vdma_hi]")
+    if CAUSAL:
+        voff_set(g, "voff")
+        clamp_voff(g, f"s_cmp_eq_u32 {s_(S_NKT1)}, 0")
     vdma_block(g, 0)
-    g(f"s_add_u32 {s_(S_VDMA)}, {s_(S_VDMA)}, {BN * 2}")
-    g(f"s_addc_u32 {s_(S_VDMA + 1)}, {s_(S_VDMA + 1)}, 0")
+    vdma_next(g)
 
 
 def prologue(g, empty):
@@ -929,7 +964,7 @@ def prologue(g, empty):
     # Q fragments straight into AGPRs, then the DMAs of K(0) (K stage 0), K(1)
     # (K stage 1; K(0) again when there is one tile) and Vt(0) (Vt stage 0), all
     # before the first wait so that their latencies overlap
-    if PRE:
+    if PRE or CAUSAL:
         g("s_nop 4")  # the AGPR operands were written just before the body
     for qb in range(QB):
         if JOINT:  # per-lane 64-bit row address in its source
@@ -1225,14 +1260,14 @@ def generate():
     return g.lines
 
 
-def clobbers(hd, pre=False, joint=False):
+def clobbers(hd, pre=False, joint=False, causal=False):
     """One header for both block counts: the two-block body owns more registers."""
-    configure(hd, pre, joint)
+    configure(hd, pre, joint, causal=causal)
     regs = ([f"v{i}" for i in range(LAST_VGPR + 1)] + [f"a{i}" for i in range(LAST_AGPR + 1)] +
             [f"s{i}" for i in (SGPRS_JOINT if joint else SGPRS)])
     rows = [", ".join(f'"{r}"' for r in regs[i:i + 16]) for i in range(0, len(regs), 16)]
-    name = f"{hd}{'j' if joint else 'p' if pre else ''}"
-    return (f"// Registers the generated flash_fwd_asm<{hd}, {str(pre).lower()}, {str(joint).lower()}> body owns (gen_attn.py register map).\n"
+    name = f"{hd}{'c' if causal else 'j' if joint else 'p' if pre else ''}"
+    return (f"// Registers the generated {'causal ' if causal else ''}flash_fwd_asm<{hd}, {str(pre).lower()}, {str(joint).lower()}> body owns (gen_attn.py register map).\n"
             f"#define DITK_D{name.upper()}_CLOBBERS \\\n" + "".join(f"  {r}, \\\n" for r in rows) + "\n")
 
 
@@ -1257,7 +1292,9 @@ def main(argv):
             write_body(os.path.join(out, f"attn_{name}{'' if qb == 2 else 'q1'}_body.inc"), hd, pre, joint, qb)
         with open(os.path.join(out, f"attn_{name}_clobbers.h"), "w") as f:
             f.write(clobbers(hd, pre, joint))
-    for hd in (128, 64):  # causal: the registers of the plain body
+    for hd in (128, 64):
+        with open(os.path.join(out, f"attn_d{hd}c_clobbers.h"), "w") as f:
+            f.write(clobbers(hd, causal=True))
         for qb in (2, 1):
             write_body(os.path.join(out, f"attn_d{hd}c{'' if qb == 2 else 'q1'}_body.inc"), hd, qb=qb, causal=True)
     return 0

@@ -728,9 +728,7 @@ def flash_attn_causal(q, k, v, seg_q, seg_k, heads, kv_heads, head_dim, softmax_
     scale = 1.0 / math.sqrt(head_dim) if softmax_scale is None else float(softmax_scale)
     lse = torch.empty((heads, Tq), dtype=torch.float32, device=device) if return_lse else None
     if Tq:
-        cols = ((Tk + 63) // 64 + nseg) * 64  # vt_columns
-        vt = torch.empty(kv_heads * head_dim * cols, dtype=_BF16, device=device)
-        _call(device, "ditk_flash_attn_causal", q.data_ptr(), ldq, k.data_ptr(), ldk, v.data_ptr(), ldv, vt.data_ptr(), cols,
+        _call(device, "ditk_flash_attn_causal", q.data_ptr(), ldq, k.data_ptr(), ldk, v.data_ptr(), ldv,
               out.data_ptr(), ldo, _ptr(lse), Tq, cu_q.data_ptr(), cu_k.data_ptr(), nseg, Tq, Tk, heads, kv_heads, head_dim,
               scale)
     return (out, lse) if return_lse else out

@@ -463,13 +463,12 @@ int ditk_mx_matvec_plan(int M, int N, int K, int* plan);
 /*
  * Causal attention of packed prompts with grouped heads (heads a multiple of kv_heads: query head h
  * reads key head h / (heads / kv_heads)).  A segment's queries are the last of its keys: query i of
- * nq sees the keys j <= i + nk - nq; one that sees none gives zeros and lse -inf.  vt: workspace of
- * kv_heads * head_dim rows of vt_ld >= ditk_vt_columns(Tk, nseg) for the transposed v, this call's
- * alone; the rest as ditk_flash_attn_varlen.
+ * nq sees the keys j <= i + nk - nq; one that sees none gives zeros and lse -inf.  v as k; the rest as
+ * ditk_flash_attn_varlen.
  * No reference counterpart: the reference's attention is non-causal with one key head a query head.
  */
-int ditk_flash_attn_causal(const void* q, int64_t ldq, const void* k, int64_t ldk, const void* v, int64_t ldv, void* vt,
-                           int64_t vt_ld, void* o, int64_t ldo, float* lse, int64_t lse_ld, const int32_t* cu_q,
+int ditk_flash_attn_causal(const void* q, int64_t ldq, const void* k, int64_t ldk, const void* v, int64_t ldv,
+                           void* o, int64_t ldo, float* lse, int64_t lse_ld, const int32_t* cu_q,
                            const int32_t* cu_k, int nseg, int Tq, int Tk, int heads, int kv_heads, int head_dim,
                            float softmax_scale, ditk_stream_t stream);
 

@@ -88,15 +88,15 @@ def test_cpu_tensors_are_refused():
         kv.evict(k, k, k, k, 2)
 
 
-CAUSAL = dict(q=A, ldq=256, k=B, ldk=128, v=G, ldv=128, vt=C, vt_ld=128, o=D, ldo=256, lse=None, lse_ld=0, cu_q=E, cu_k=F, nseg=1, Tq=64,
+CAUSAL = dict(q=A, ldq=256, k=B, ldk=128, v=G, ldv=128, o=D, ldo=256, lse=None, lse_ld=0, cu_q=E, cu_k=F, nseg=1, Tq=64,
               Tk=64, heads=4, hk=2, d=64, scale=0.1, stream=None)
 
 
 @pytest.mark.parametrize("change,word", [
     (dict(scale=0.0), "softmax_scale"), (dict(scale=float("inf")), "softmax_scale"), (dict(cu_q=None), "null"),
-    (dict(q=None), "null"), (dict(vt=None), "null"), (dict(d=96), "head_dim"), (dict(nseg=0), "sizes"), (dict(Tk=-1), "sizes"),
+    (dict(q=None), "null"), (dict(d=96), "head_dim"), (dict(nseg=0), "sizes"), (dict(Tk=-1), "sizes"),
     (dict(Tq=1 << 30), "sizes"), (dict(heads=3), "query heads"), (dict(hk=0), "query heads"), (dict(ldq=252), "leading"),
-    (dict(vt_ld=64), "leading"), (dict(ldv=124), "leading"), (dict(v=None), "null"), (dict(v=G + 2), "misaligned"), (dict(q=A + 8), "misaligned"), (dict(o=D + 8), "misaligned"),
-    (dict(ldk=1 << 23), "32-bit"), (dict(ldo=1 << 30), "32-bit"), (dict(Tq=(1 << 30) - 1), "grid")])
+    (dict(ldv=124), "leading"), (dict(v=None), "null"), (dict(v=G + 2), "misaligned"), (dict(q=A + 8), "misaligned"), (dict(o=D + 8), "misaligned"),
+    (dict(ldk=1 << 23), "32-bit"), (dict(ldv=1 << 23), "32-bit"), (dict(ldo=1 << 30), "32-bit"), (dict(Tq=(1 << 30) - 1), "grid")])
 def test_causal_refuses(change, word):
     refused("ditk_flash_attn_causal", tuple({**CAUSAL, **change}.values()), word)
