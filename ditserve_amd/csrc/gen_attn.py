@@ -439,13 +439,19 @@ def k_read(g, chunk, kk, stage):
     g.lds_issue(("k", chunk, kk))
 
 
+def v_read_half(g, f, stage, half):
+    """Causal: keys 16 grp + 8 (lane / 32) + 0..3, or + 4..7, of fragment f."""
+    grp, d = f // DT, f % DT
+    off = stage * VSTAGE_BYTES + (16 * grp + 4 * half) * HD * 2
+    g(f"ds_read_b64_tr_b16 {ar(vf_reg(f % VRING) + 2 * half, 2)}, %[vaddr{d}] offset:{off}")
+    g.lds_issue(("v", f) if half else ("v", f, "first half"))
+
+
 def v_read(g, f, stage):
     grp, d = f // DT, f % DT
-    if CAUSAL:  # keys 16 grp + 8 (lane / 32) + 0..3, then + 4..7
-        for half in range(2):
-            off = stage * VSTAGE_BYTES + (16 * grp + 4 * half) * HD * 2
-            g(f"ds_read_b64_tr_b16 {ar(vf_reg(f % VRING) + 2 * half, 2)}, %[vaddr{d}] offset:{off}")
-            g.lds_issue(("v", f) if half else ("v", f, "first half"))
+    if CAUSAL:
+        v_read_half(g, f, stage, 0)
+        v_read_half(g, f, stage, 1)
         return
     g(f"ds_read_b128 {ar(vf_reg(f % VRING), 4)}, %[vaddr{grp}] offset:{stage * VSTAGE_BYTES + d * 4096}")
     g.lds_issue(("v", f))
@@ -484,9 +490,15 @@ def s_phase(g, s_set, kstage, vstage=None, items=None, dma=None, first=False):
                 if kk == 0 and qb == 0 and c + KA < NC:
                     k_read(g, c + KA, 0, kstage)
                     k_read(g, c + KA, 1, kstage)
-                if kk == 0 and qb == 0 and c == NC - 1 and vstage is not None:
+                if kk == 0 and qb == 0 and c == NC - 1 and vstage is not None and not CAUSAL:
                     for f in range(VA):
                         v_read(g, f, vstage)
+                if CAUSAL and vstage is not None:  # spread over the slots that read no K any more
+                    free = 2 * QB * min(KA, NC)
+                    first = slot - (2 * QB * NC - free)
+                    if first >= 0:
+                        for i in range(2 * VA * first // free, 2 * VA * (first + 1) // free):
+                            v_read_half(g, i // 2, vstage, i % 2)
                 if d:
                     d[1]()
                 if items is not None:
@@ -504,7 +516,9 @@ def o_phase(g, p_set, vstage, items=None):
             if qb == 0 and f % 2 == 0:
                 g.lds_wait(("v", f + 1))
             mfma_o(g, p_set, qb, d, grp, f % VRING)
-            if qb == 0 and f + VA < NF:
+            if CAUSAL and QB == 2 and f + VA < NF:  # a half after each block's MFMA
+                v_read_half(g, f + VA, vstage, qb)
+            elif qb == 0 and f + VA < NF:
                 v_read(g, f + VA, vstage)
             if items is not None:
                 items[slot]()
