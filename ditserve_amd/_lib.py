@@ -86,7 +86,9 @@ SIGNATURES = {
                                c_int64, _P]),
     "ditk_mx_matvec_plan": (c_int, [c_int, c_int, c_int, ctypes.POINTER(c_int)]),
     "ditk_flash_attn_causal": (c_int, [_P, c_int64, _P, c_int64, _P, c_int64, _P, c_int64, _P, c_int64, _P, _P,
-                                       c_int, c_int, c_int, c_int, c_int, c_int, c_float, _P]),
+                                       c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_int, _P, c_int64,
+                                       c_int64, _P]),
+    "ditk_causal_few_parts": (c_int, [c_int, c_int, c_int]),
     "ditk_kv_append": (c_int, [_P, c_int64, _P, c_int64, _P, c_int64, c_int64, _P, c_int64, c_int64, _P, c_int64, c_int64,
                                c_int, c_int, _P, c_int64, c_int, _P, _P, _P, c_int, c_int, c_int, c_int, _P, _P]),
     "ditk_kv_attn_workspace": (c_int64, [c_int, c_int, c_int, c_int, c_int]),

@@ -45,6 +45,7 @@
 #include <cmath>
 #include <mutex>
 
+#include "causal_few.h"
 #include "ditk_common.h"
 #include "attn_d128_clobbers.h"
 #include "attn_d128p_clobbers.h"
@@ -205,7 +206,9 @@ __global__ __launch_bounds__(256, 1) void flash_fwd_asm(
     const int lane = threadIdx.x & 63;
     for (int m = 0; m < nseg; m += 64) {
       const int i = min(m + lane, nseg - 1);
-      const int ntile = m + lane < nseg ? (cu_q[i + 1] - cu_q[i] + BM - 1) / BM : 0;
+      const int nq = cu_q[i + 1] - cu_q[i];
+      const bool mine = m + lane < nseg && !few_queries(nq, cu_k[i + 1] - cu_k[i], group);
+      const int ntile = mine ? (nq + BM - 1) / BM : 0;
       int items = ntile * heads;
       for (int off = 1; off < 64; off <<= 1) {
         const int x = __shfl_up(items, off, 64);
@@ -664,11 +667,17 @@ DITK_EXPORT int ditk_joint_attn_q_prescaled(const void* q_a, const void* q_b, in
                       cu_a, cu_b);
 }
 
+DITK_EXPORT int ditk_causal_few_parts(int nq, int nk, int group) {
+  return group > 0 && nq < (1 << 30) ? few_parts(nq, nk, group) : 0;
+}
+
 DITK_EXPORT int ditk_flash_attn_causal(const void* q, int64_t ldq, const void* k, int64_t ldk, const void* v, int64_t ldv,
                                        void* o, int64_t ldo, float* lse, int64_t lse_ld,
                                        const int32_t* cu_q, const int32_t* cu_k, int nseg, int Tq, int Tk, int heads,
-                                       int kv_heads, int head_dim, float softmax_scale, hipStream_t stream) {
+                                       int kv_heads, int head_dim, float softmax_scale, int kinds, void* workspace,
+                                       int64_t workspace_bytes, int64_t few_parts, hipStream_t stream) {
   const char* what = "ditk_flash_attn_causal";
+  DITK_REQUIRE(kinds >= 1 && kinds <= 3, "%s: bad kinds %d", what, kinds);
   DITK_REQUIRE(softmax_scale >= 1e-30f && softmax_scale <= 1e30f, "%s: softmax_scale must be in 1e-30..1e30", what);
   DITK_REQUIRE(cu_q && cu_k && (Tq == 0 || (q && o)) && (Tk == 0 || (k && v)), "%s: null tensor", what);
   DITK_REQUIRE(head_dim == 64 || head_dim == 128, "%s: head_dim must be 64 or 128, got %d", what, head_dim);
@@ -683,6 +692,15 @@ DITK_EXPORT int ditk_flash_attn_causal(const void* q, int64_t ldq, const void* k
   DITK_REQUIRE(ldq >= 0 && ldk >= 0 && ldv >= 0 && ldo >= 0 && ldq < (1ll << 30) && ldo < (1ll << 30) &&
                    ldk < (1ll << 23) && ldv < (1ll << 23), "%s: rows too long for 32-bit lane offsets", what);
   if (Tq == 0) return 0;
+  const float sl2 = softmax_scale * 1.4426950408889634f;
+  if ((kinds & 2) && Tk >= kFewKeys) {
+    DITK_REQUIRE(few_parts > 0 && few_parts < (1ll << 31) && workspace && ((uintptr_t)workspace % 16) == 0 &&
+                     workspace_bytes >= causal_few_workspace(few_parts, kv_heads, head_dim),
+                 "%s: the workspace does not hold %lld parts", what, (long long)few_parts);
+    if (int rc = causal_few_launch(q, ldq, k, ldk, v, ldv, o, ldo, lse, lse_ld, cu_q, cu_k, nseg, heads, kv_heads, head_dim,
+                                   sl2, workspace, few_parts, stream)) return rc;
+  }
+  if (!(kinds & 1)) return 0;
   const int qb = causal_item_queries(Tq, Tk, nseg, heads, head_dim) / 128;
   const int64_t nblocks = ((int64_t)(Tq + 128 * qb - 1) / (128 * qb) + nseg) * heads;
   DITK_REQUIRE(nblocks < (1ll << 24), "%s: grid too large", what);
@@ -690,7 +708,7 @@ DITK_EXPORT int ditk_flash_attn_causal(const void* q, int64_t ldq, const void* k
   auto kern = head_dim == 128 ? (qb == 2 ? flash_fwd_asm<128, false, false, 2, true> : flash_fwd_asm<128, false, false, 1, true>)
                               : (qb == 2 ? flash_fwd_asm<64, false, false, 2, true> : flash_fwd_asm<64, false, false, 1, true>);
   kern<<<(unsigned)nblocks, 256, 0, stream>>>(
-      (const bf16_t*)q, ldq, (const bf16_t*)k, ldk, (const bf16_t*)v, ldv, head_dim, (bf16_t*)o, ldo, lse, lse_ld, cu_q, cu_k, nseg, heads, 1, 1, stream_out, softmax_scale * 1.4426950408889634f, RowLayout{head_dim, 0},
+      (const bf16_t*)q, ldq, (const bf16_t*)k, ldk, (const bf16_t*)v, ldv, head_dim, (bf16_t*)o, ldo, lse, lse_ld, cu_q, cu_k, nseg, heads, 1, 1, stream_out, sl2, RowLayout{head_dim, 0},
       RowLayout{head_dim, 0}, nullptr, nullptr, nullptr, nullptr, nullptr, heads / kv_heads);
   return ditk_check_launch(what);
 }

@@ -1,16 +1,9 @@
 // Attention of one new token of each sequence over its paged keys and values (kv_common.h), split over the
 // sequence's slots and joined.
 //
-// The G query heads of a key head make the columns of one matrix product: a wave takes 32 slots at a time,
-//   S^T = K Q^T         (A = 16 slots x 32 dims straight from the pages, B = Q)
-//   O^T += V^T P^T      (A = V^T by transposing LDS reads, B = P^T)
-// with v_mfma_f32_16x16x32_bf16.  Row m of score tile t is slot 8 (m / 4) + 4 t + m % 4, so that the accumulators of both
-// tiles are the 8 consecutive slots a lane of the second product's B operand holds: no shuffles between the two.
-// P is taken as the sum of two bf16 numbers (16 bits of it at least), so that only the output is rounded to 8 bits: the
-// matrix pipe is idle most of the time anyway.
-//
-// Scores are in log2 units; m, l and O stay fp32.  A chunk's length goes by the sequence's own length alone, so a
-// sequence's result does not depend on what it is batched with.
+// The query heads of a key head, 16 at a time, are the columns of a wave's products (attn_chunk.h).  A chunk's length
+// goes by the sequence's own length alone, so a sequence's result does not depend on what it is batched with.
+#include "attn_chunk.h"
 #include "kv_common.h"
 
 namespace {
@@ -53,157 +46,40 @@ struct Args {
   float scale2;   // softmax scale times log2 e
 };
 
+// Pages of a sequence, 64 of them (1024 slots at least) in a wave's lanes
 template <int HD>
-__device__ __forceinline__ int v_swizzle(int row) {
-  return HD == 128 ? (row & 3) | ((row >> 3) & 1) << 2 : ((row >> 1) & 1) | ((row >> 3) & 1) << 1;
-}
-
-__device__ __forceinline__ float group_maxf(float v) {
-  v = fmaxf(v, __shfl_xor(v, 16, 64));
-  return fmaxf(v, __shfl_xor(v, 32, 64));
-}
-__device__ __forceinline__ float group_sumf(float v) {
-  v += __shfl_xor(v, 16, 64);
-  return v + __shfl_xor(v, 32, 64);
-}
-
-typedef short s16x4 __attribute__((ext_vector_type(4)));
-
-// What a wave gathers of one chunk: lane (quad, col) holds dims 16 j + 4 quad .. + 3 of query head `col`'s sums of
-// p v, its m and its l.
-template <int HD, bool SCORES>
-struct Chunk {
-  static constexpr int NC = HD / 32, ND = HD / 16, CH = HD / 8, RPL = 64 / CH;  // RPL: rows of V a load of the wave covers
-  f32x4_t o[ND];
-  float m, l;
-
-  // slots [s0, s1) of sequence b (n slots) and key head kvh, for nq query heads from head0 on; vt: 32 HD bf16 of LDS
-  __device__ __forceinline__ void run(const Args& a, int b, int n, int s0, int s1, int kvh, int head0, int nq, char* vt) {
-    const int lane = threadIdx.x & 63, col = lane & 15, quad = lane >> 4;
-    const int pl = a.t.page_log2, low = (1 << pl) - 1, last = max(n - 1, 0);
-    bf16x8_t q[NC];
-    const bf16_t* qr = a.q + b * a.ldq + (int64_t)(head0 + min(col, nq - 1)) * HD + quad * 8;
-#pragma unroll
-    for (int i = 0; i < NC; ++i) q[i] = *reinterpret_cast<const bf16x8_t*>(qr + i * 32);
-#pragma unroll
-    for (int j = 0; j < ND; ++j) o[j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-    m = -INFINITY;
-    l = 0.f;
-    int page = 0, first = 0;
-    for (int t0 = s0; t0 < s1; t0 += 32) {
-      // pages of the next 1024 slots, one a lane
-      if (((t0 - s0) & 1023) == 0) {
-        first = t0 >> pl;
-        const int i = min(first + lane, last >> pl), p = a.t.table[b * a.t.ldt + i];
-        page = (unsigned)p < (unsigned)a.t.pages ? p : -1;
-        if (page < 0 && (first + lane) << pl < s1) *a.t.status = 1;
-      }
-      // the tile's two halves of 16 slots lie in one page each; slots past the last read it
-      const int g0 = __builtin_amdgcn_readlane(page, (min(t0, last) >> pl) - first);
-      const int g1 = __builtin_amdgcn_readlane(page, (min(t0 + 16, last) >> pl) - first);
-      const bool ok0 = g0 >= 0, ok1 = g1 >= 0;
-      const int p0 = max(g0, 0), p1 = max(g1, 0);
-      const bf16_t* kb0 = a.k.p + p0 * a.k.ps + kvh * a.k.hs;
-      const bf16_t* kb1 = a.k.p + p1 * a.k.ps + kvh * a.k.hs;
-      const bf16_t* vb0 = a.v.p + p0 * a.v.ps + kvh * a.v.hs;
-      const bf16_t* vb1 = a.v.p + p1 * a.v.ps + kvh * a.v.hs;
-      bf16x8_t k[2][NC];
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int slot = min(t0 + 8 * (col >> 2) + 4 * i + (col & 3), last);
-        const bf16_t* kr = (col < 8 ? kb0 : kb1) + (int64_t)(slot & low) * HD + quad * 8;
-#pragma unroll
-        for (int c = 0; c < NC; ++c) k[i][c] = *reinterpret_cast<const bf16x8_t*>(kr + c * 32);
-      }
-      u32x4_t v[32 / RPL];
-#pragma unroll
-      for (int i = 0; i < 32 / RPL; ++i) {
-        const int row = i * RPL + lane / CH, slot = min(t0 + row, last);
-        v[i] = *reinterpret_cast<const u32x4_t*>((i * RPL < 16 ? vb0 : vb1) + (int64_t)(slot & low) * HD + (lane % CH) * 8);
-      }
-      // values of absent slots may be anything: they count as 0
-      const int n0 = ok0 ? min(s1 - t0, 16) : 0, n1 = ok1 ? s1 - t0 - 16 : 0;
-      const bool whole = n0 == 16 && n1 >= 16;
-      if (!whole) {
-#pragma unroll
-        for (int i = 0; i < 32 / RPL; ++i) {
-          const int row = i * RPL + lane / CH;
-          if (i * RPL < 16 ? row >= n0 : row - 16 >= n1) v[i] = u32x4_t{0, 0, 0, 0};
-        }
-      }
-      f32x4_t s[2];
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        s[i] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int c = 0; c < NC; ++c) s[i] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(k[i][c], q[c], s[i], 0, 0, 0);
-      }
-      float x[8], top = -INFINITY;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        x[e] = s[e >> 2][e & 3] * a.scale2;
-        const int row = quad * 8 + e;
-        if (!whole && (row < 16 ? row >= n0 : row - 16 >= n1)) x[e] = -INFINITY;
-        top = fmaxf(top, x[e]);
-      }
-      if (SCORES) {
-        if (col < nq) {
-          float* sr = a.score + ((int64_t)b * a.heads + head0 + col) * a.ld_score + t0 + quad * 8;
-          *reinterpret_cast<f32x4_t*>(sr) = f32x4_t{x[0], x[1], x[2], x[3]};
-          *reinterpret_cast<f32x4_t*>(sr + 4) = f32x4_t{x[4], x[5], x[6], x[7]};
-        }
-      }
-      const float mn = fmaxf(m, group_maxf(top));
-      if (__any(mn > m)) {
-        const float al = mn == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m - mn);
-        l *= al;
-#pragma unroll
-        for (int j = 0; j < ND; ++j)
-#pragma unroll
-          for (int r = 0; r < 4; ++r) o[j][r] *= al;
-        m = mn;
-      }
-      const float base = m == -INFINITY ? 0.f : m;
-      bf16x8_t hi, lo;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float p = __builtin_amdgcn_exp2f(x[e] - base);
-        l += p;
-        // hi cut off, so that lo is not negative, and lo not 0 unless p is: an infinite value stays one
-        const float cut = __uint_as_float(__float_as_uint(p) & 0xffff0000u);
-        hi[e] = __builtin_bit_cast(__bf16, (uint16_t)(__float_as_uint(p) >> 16));
-        lo[e] = (__bf16)fmaxf(p - cut, fminf(p, 1.17549435e-38f));
-      }
-#pragma unroll
-      for (int i = 0; i < 32 / RPL; ++i) {
-        const int row = i * RPL + lane / CH, ch = lane % CH;
-        *reinterpret_cast<u32x4_t*>(vt + row * (HD * 2) + (((ch >> 1) ^ v_swizzle<HD>(row)) * 32) + (ch & 1) * 16) = v[i];
-      }
-      // lane i of a quad reads 8 bytes of row i / 4 and gets 4 rows of column i
-#pragma unroll
-      for (int j = 0; j < ND; ++j) {
-        s16x4 w[2];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const int row = quad * 8 + 4 * i + (col >> 2);
-          const char* p = vt + row * (HD * 2) + ((j ^ v_swizzle<HD>(row)) * 32) + (col & 3) * 8;
-          w[i] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)p);
-        }
-        union { s16x4 h[2]; bf16x8_t f; } f;
-        f.h[0] = w[0];
-        f.h[1] = w[1];
-        o[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f.f, hi, o[j], 0, 0, 0);
-        o[j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(f.f, lo, o[j], 0, 0, 0);
-      }
+struct PagedSrc {
+  const Args& a;
+  int b, kvh, last;
+  int page = 0, first = 0;
+  int64_t k0, k1, v0, v1;  // offsets of the halves' first slots
+  bool ok0, ok1;
+  __device__ __forceinline__ void tile(int t0, int s0, int s1) {
+    const int pl = a.t.page_log2, low = (1 << pl) - 1;
+    if (((t0 - s0) & 1023) == 0) {
+      first = t0 >> pl;
+      const int lane = threadIdx.x & 63, i = min(first + lane, last >> pl), p = a.t.table[b * a.t.ldt + i];
+      page = (unsigned)p < (unsigned)a.t.pages ? p : -1;
+      if (page < 0 && (first + lane) << pl < s1) *a.t.status = 1;
     }
-    l = group_sumf(l);
+    // a half of 16 slots lies in one page; one behind the last slot stands where the first half does
+    const int t1 = t0 + 16 <= last ? t0 + 16 : t0;
+    const int g0 = __builtin_amdgcn_readlane(page, (t0 >> pl) - first), g1 = __builtin_amdgcn_readlane(page, (t1 >> pl) - first);
+    ok0 = g0 >= 0;
+    ok1 = g1 >= 0;
+    k0 = max(g0, 0) * a.k.ps + (t0 & low) * HD;
+    k1 = max(g1, 0) * a.k.ps + (t1 & low) * HD;
+    v0 = max(g0, 0) * a.v.ps + (t0 & low) * HD;
+    v1 = max(g1, 0) * a.v.ps + (t1 & low) * HD;
   }
+  __device__ __forceinline__ bool ok(int half) const { return half ? ok1 : ok0; }
+  __device__ __forceinline__ const bf16_t* k(int half) const { return a.k.p + kvh * a.k.hs + (half ? k1 : k0); }
+  __device__ __forceinline__ const bf16_t* v(int half) const { return a.v.p + kvh * a.v.hs + (half ? v1 : v0); }
+  __device__ __forceinline__ int k_stride() const { return HD; }
+  __device__ __forceinline__ int v_stride() const { return HD; }
 };
 
-// 1 / l, 0 for a row without slots
-__device__ __forceinline__ float inverse(float l) { return l > 0.f || l != l ? 1.f / l : 0.f; }
-__device__ __forceinline__ void store_lse(const Args& a, int64_t row, float m, float l, bool scores) {
-  const float e = l > 0.f || l != l ? m + __builtin_amdgcn_logf(l) : -INFINITY;
+__device__ __forceinline__ void store_lse(const Args& a, int64_t row, float e, bool scores) {
   if (a.lse != nullptr) a.lse[row] = e * 0.6931471805599453f;
   if (scores) a.lse2[row] = e;
 }
@@ -211,9 +87,9 @@ __device__ __forceinline__ void store_lse(const Args& a, int64_t row, float m, f
 // A wave takes one chunk of one (sequence, key head, 16 query heads) after another; units go round the waves in
 // order: a sequence's chunks, and for each its heads, which lie side by side in a page.
 template <int HD, bool SCORES>
-__global__ __launch_bounds__(256, 3) void kv_attn_kernel(Args a) {
-  using C = Chunk<HD, SCORES>;
-  __shared__ __align__(16) char lds[4 * 32 * HD * 2];
+__global__ __launch_bounds__(256, 2) void kv_attn_kernel(Args a) {
+  using C = Chunk<HD>;
+  __shared__ __align__(256) char lds[4 * 32 * HD * 2];
   __shared__ int sums[4], ends[256], lens[256];
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
   const int col = lane & 15, quad = lane >> 4;
@@ -260,10 +136,13 @@ __global__ __launch_bounds__(256, 3) void kv_attn_kernel(Args a) {
     const int kvh = hg / groups, g0 = (hg - kvh * groups) * 16;
     const int csl = chunk_slots(n), s0 = chunk * csl, s1 = min(n, s0 + csl);
     const int nq = min(a.group - g0, 16), head0 = kvh * a.group + g0;  // query heads of this unit
+    const int64_t row = (int64_t)b * a.heads + head0 + min(col, nq - 1);
     C x;
-    x.run(a, b, n, s0, s1, kvh, head0, nq, lds + wave * (32 * HD * 2));
+    PagedSrc<HD> src{a, b, kvh, max(n - 1, 0)};
+    x.run(src, a.q + b * a.ldq + (int64_t)(head0 + min(col, nq - 1)) * HD + quad * 8, a.scale2, s0, s1,
+                          n, n, SCORES && col < nq ? a.score + row * a.ld_score : nullptr,
+                          lds + wave * (32 * HD * 2));
     if (col < nq) {
-      const int64_t row = (int64_t)b * a.heads + head0 + col;
       if (nch == 1) {
         const float inv = inverse(x.l);
         bf16_t* ob = a.o + b * a.ldo + (int64_t)(head0 + col) * HD + quad * 4;
@@ -271,7 +150,7 @@ __global__ __launch_bounds__(256, 3) void kv_attn_kernel(Args a) {
         for (int j = 0; j < C::ND; ++j)
           *reinterpret_cast<u32x2_t*>(ob + j * 16) = u32x2_t{pack_bf2(x.o[j][0] * inv, x.o[j][1] * inv),
                                                             pack_bf2(x.o[j][2] * inv, x.o[j][3] * inv)};
-        if (quad == 0) store_lse(a, row, x.m, x.l, SCORES);
+        if (quad == 0) store_lse(a, row, row_lse2(x.m, x.l), SCORES);
       } else {
         float* pb = a.part + (row * a.nchunk + chunk) * HD + quad * 4;
 #pragma unroll
@@ -287,9 +166,9 @@ __global__ __launch_bounds__(256, 3) void kv_attn_kernel(Args a) {
 // join them through LDS, by the join kernel's operations in its order.
 template <int HD, bool SCORES>
 __global__ __launch_bounds__(512) void kv_attn_short_kernel(Args a) {
-  using C = Chunk<HD, SCORES>;
+  using C = Chunk<HD>;
   constexpr int OP = HD + 4;  // floats of a row of LDS
-  __shared__ __align__(16) char lds[8 * 16 * OP * 4];
+  __shared__ __align__(256) char lds[8 * 16 * OP * 4];
   __shared__ float stat[2][16][8];
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
   const int col = lane & 15, quad = lane >> 4, groups = (a.group + 15) / 16;
@@ -298,8 +177,12 @@ __global__ __launch_bounds__(512) void kv_attn_short_kernel(Args a) {
   const int n = kv_length(a.t, b, hg == 0 && tid == 0), csl = chunk_slots(n), nch = chunks_of(n);
   const int s0 = min(wave * csl, n), s1 = min(n, s0 + csl);
   const int nq = min(a.group - g0, 16), head0 = kvh * a.group + g0;
+  const int64_t row = (int64_t)b * a.heads + head0 + min(col, nq - 1);
   C x;
-  x.run(a, b, n, s0, s1, kvh, head0, nq, lds + wave * (16 * OP * 4));
+  PagedSrc<HD> src{a, b, kvh, max(n - 1, 0)};
+  x.run(src, a.q + b * a.ldq + (int64_t)(head0 + min(col, nq - 1)) * HD + quad * 8, a.scale2, s0, s1,
+                       n, n, SCORES && col < nq ? a.score + row * a.ld_score : nullptr,
+                       lds + wave * (16 * OP * 4));
   if (quad == 0) {
     stat[0][col][wave] = x.m;
     stat[1][col][wave] = x.l;
@@ -310,31 +193,13 @@ __global__ __launch_bounds__(512) void kv_attn_short_kernel(Args a) {
   for (int j = 0; j < C::ND; ++j) *reinterpret_cast<f32x4_t*>(ob + j * 16) = x.o[j];
   __syncthreads();
   for (int i = tid; i < nq * (HD / 4); i += 512) {
-#pragma clang fp contract(off)  // products rounded, then added, as where the join reads them
     const int r = i / (HD / 4), d = (i % (HD / 4)) * 4;
-    float m[8], f[8], top = -INFINITY;
-#pragma unroll
-    for (int c = 0; c < 8; ++c) {
-      m[c] = stat[0][r][c];
-      top = fmaxf(top, m[c]);
-    }
-    float l[8];
-    f32x4_t y = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int c = 0; c < 8; ++c) {
-      f[c] = m[c] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[c] - top);
-      if (nch == 1) f[c] = 1.f;
-      l[c] = stat[1][r][c] * f[c];
-      const f32x4_t z = *reinterpret_cast<const f32x4_t*>(reinterpret_cast<const float*>(lds) + (c * 16 + r) * OP + d);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) y[e] += z[e] * f[c];
-    }
-    // wave_sum's order of eight lanes
-    const float lt = ((l[0] + l[4]) + (l[2] + l[6])) + ((l[1] + l[5]) + (l[3] + l[7]));
+    float top, lt;
+    const f32x4_t y = join8<HD>(reinterpret_cast<const float*>(lds), stat, r, d, top, lt);
     const float inv = inverse(lt);
     *reinterpret_cast<u32x2_t*>(a.o + b * a.ldo + (int64_t)(head0 + r) * HD + d) =
         u32x2_t{pack_bf2(y[0] * inv, y[1] * inv), pack_bf2(y[2] * inv, y[3] * inv)};
-    if (d == 0) store_lse(a, (int64_t)b * a.heads + head0 + r, top, lt, SCORES);
+    if (d == 0) store_lse(a, (int64_t)b * a.heads + head0 + r, row_lse2(top, lt), SCORES);
   }
 }
 
@@ -392,7 +257,7 @@ __global__ __launch_bounds__(256) void kv_join_kernel(Args a) {
     const float inv = inverse(lt);
     *reinterpret_cast<u32x2_t*>(a.o + b * a.ldo + (int64_t)head * HD + d) =
         u32x2_t{pack_bf2(y[0] * inv, y[1] * inv), pack_bf2(y[2] * inv, y[3] * inv)};
-    if (tid == 0) store_lse(a, row, top, lt, SCORES);
+    if (tid == 0) store_lse(a, row, row_lse2(top, lt), SCORES);
   }
 }
 
@@ -497,7 +362,7 @@ DITK_EXPORT int ditk_kv_attn(const void* q, int64_t ldq, const void* k_cache, in
     kern<<<(unsigned)(batch * a.hgroups), 512, 0, stream>>>(a);
     if (int rc = ditk_check_launch(what)) return rc;
   } else {
-    const int most_wgs = 3 * ditk_cu_count();
+    const int most_wgs = 2 * ditk_cu_count();  // (3 a CU, with fewer registers, spill: 1 x 8192 slots 20 us for 18)
     auto kern = head_dim == 128 ? (s ? kv_attn_kernel<128, true> : kv_attn_kernel<128, false>)
                                 : (s ? kv_attn_kernel<64, true> : kv_attn_kernel<64, false>);
     kern<<<(unsigned)(wgs < most_wgs ? wgs : most_wgs), 256, 0, stream>>>(a);

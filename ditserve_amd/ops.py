@@ -728,10 +728,33 @@ def flash_attn_causal(q, k, v, seg_q, seg_k, heads, kv_heads, head_dim, softmax_
     scale = 1.0 / math.sqrt(head_dim) if softmax_scale is None else float(softmax_scale)
     lse = torch.empty((heads, Tq), dtype=torch.float32, device=device) if return_lse else None
     if Tq:
+        kinds, parts = _causal_kinds(seg_q, seg_k, heads // kv_heads)
+        size = parts * kv_heads * (head_dim + 2) * 4
+        space = torch.empty(size, dtype=torch.uint8, device=device) if size else None
         _call(device, "ditk_flash_attn_causal", q.data_ptr(), ldq, k.data_ptr(), ldk, v.data_ptr(), ldv,
               out.data_ptr(), ldo, _ptr(lse), Tq, cu_q.data_ptr(), cu_k.data_ptr(), nseg, Tq, Tk, heads, kv_heads, head_dim,
-              scale)
+              scale, kinds, _ptr(space), size, parts)
     return (out, lse) if return_lse else out
+
+
+def _causal_kinds(seg_q, seg_k, group):
+    """(the kernels of ditk_flash_attn_causal that the segments need: 1, 2 (few queries over many keys) or 3 for both;
+    the parts that the second leaves for each key head, or a bound where only the device knows the segments)."""
+    Tk = seg_k.total
+    if Tk < 1024:
+        return 1, 0
+    q, k = seg_q.cu, seg_k.cu
+    if q is None or k is None:
+        # of each segment 128 rows at most, and rows times chunks at most 2048, or rows times (keys / 128 + 1)
+        n = min(seg_q.nseg, Tk // 1024)
+        return 3, min(2048 * n, Tk + 128 * n, 128 * group * seg_q.total)
+    few, kinds, parts = _lib.load().ditk_causal_few_parts, 0, 0
+    for a, b, c, d in zip(q, q[1:], k, k[1:]):
+        if a < b:
+            p = few(b - a, d - c, group)
+            kinds |= 2 if p else 1
+            parts += p
+    return kinds or 1, parts
 
 
 def flash_attn_bhsd(q, k, v, softmax_scale=None):

@@ -464,13 +464,21 @@ int ditk_mx_matvec_plan(int M, int N, int K, int* plan);
  * Causal attention of packed prompts with grouped heads (heads a multiple of kv_heads: query head h
  * reads key head h / (heads / kv_heads)).  A segment's queries are the last of its keys: query i of
  * nq sees the keys j <= i + nk - nq; one that sees none gives zeros and lse -inf.  v as k; the rest as
- * ditk_flash_attn_varlen.
+ * ditk_flash_attn_varlen.  kinds: the kernels that the segments need, 1 or (ditk_causal_few_parts > 0)
+ * 2, or 3 for both (a caller that does not know the lengths); segments of a kernel not named stay as
+ * they are.  Kernel 2 takes a workspace (this call's alone) of few_parts * kv_heads * (head_dim + 2)
+ * floats, few_parts at least the segments' sum (2048 a segment of 1024 keys or more is always enough).
  * No reference counterpart: the reference's attention is non-causal with one key head a query head.
  */
 int ditk_flash_attn_causal(const void* q, int64_t ldq, const void* k, int64_t ldk, const void* v, int64_t ldv,
                            void* o, int64_t ldo, float* lse, int64_t lse_ld, const int32_t* cu_q,
                            const int32_t* cu_k, int nseg, int Tq, int Tk, int heads, int kv_heads, int head_dim,
-                           float softmax_scale, ditk_stream_t stream);
+                           float softmax_scale, int kinds, void* workspace, int64_t workspace_bytes,
+                           int64_t few_parts, ditk_stream_t stream);
+
+/* The parts for each key head that a segment of nq queries and nk keys with `group` query heads a key head needs of
+ * ditk_flash_attn_causal's workspace: 0 unless it has few queries over many keys. */
+int ditk_causal_few_parts(int nq, int nk, int group);
 
 /*
  * Paged key-value caches.  A cache of `pages` pages of `page` slots (16, 32, 64, 128 or 256) holds

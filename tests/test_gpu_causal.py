@@ -58,6 +58,9 @@ CASES = [
     # queries that see no key: more queries than keys, and no keys
     ([100, 300], [30, 77], 4, 2, 128), ([5, 300, 7], [0, 1, 0], 8, 8, 64), ([0, 0], [0, 9], 2, 1, 128),
     ([513], [256], 3, 3, 64), ([9000], None, 2, 1, 128), ([3000, 2500], None, 24, 8, 64),
+    # few queries over many keys, among others
+    ([1], [1024], 1, 1, 64), ([1, 16, 3, 32, 33], [5000, 1024, 1023, 4097, 4097], 8, 2, 128), ([128, 0, 7], [1100, 3000, 1600], 5, 5, 64),
+    ([10, 300, 2], [9000, 1300, 1025], 12, 1, 128), ([100], [2000], 6, 6, 128), ([18, 1], [1030, 70000], 7, 1, 64),
 ]
 
 
@@ -76,8 +79,8 @@ def test_causal(lens_q, lens_k, heads, hk, d, fused):
 @pytest.mark.parametrize("d", [64, 128])
 def test_packed_is_alone(d):
     """Each segment bitwise what it is alone, whatever work items the launches take; with device tables too."""
-    lens_q, heads, hk = [1500, 3, 700, 4100, 64], 16, 4
-    lens_k = [1500, 40, 700, 4100, 2064]
+    lens_q, heads, hk = [1500, 3, 700, 4100, 64, 20, 1], 16, 4
+    lens_k = [1500, 40, 700, 4100, 2064, 3020, 1024]
     q, k, v = prompt(lens_q, lens_k, heads, hk, d, 3)
     q[::37] *= 5.0  # maxima that rise late
     k[::53] *= 4.0

@@ -89,10 +89,14 @@ def test_cpu_tensors_are_refused():
 
 
 CAUSAL = dict(q=A, ldq=256, k=B, ldk=128, v=G, ldv=128, o=D, ldo=256, lse=None, lse_ld=0, cu_q=E, cu_k=F, nseg=1, Tq=64,
-              Tk=64, heads=4, hk=2, d=64, scale=0.1, stream=None)
+              Tk=64, heads=4, hk=2, d=64, scale=0.1, kinds=3, space=H,
+              size=1 << 20, parts=8, stream=None)
 
 
 @pytest.mark.parametrize("change,word", [
+    (dict(kinds=0), "kinds"), (dict(kinds=4), "kinds"), (dict(nseg=1 << 22, Tk=2000), "too many"),
+    (dict(Tk=2000, space=None), "workspace"), (dict(Tk=2000, space=H + 8), "workspace"), (dict(Tk=2000, parts=0), "workspace"),
+    (dict(Tk=2000, size=8 * 2 * 66 * 4 - 1), "workspace"),
     (dict(scale=0.0), "softmax_scale"), (dict(scale=float("inf")), "softmax_scale"), (dict(cu_q=None), "null"),
     (dict(q=None), "null"), (dict(d=96), "head_dim"), (dict(nseg=0), "sizes"), (dict(Tk=-1), "sizes"),
     (dict(Tq=1 << 30), "sizes"), (dict(heads=3), "query heads"), (dict(hk=0), "query heads"), (dict(ldq=252), "leading"),
