@@ -45,6 +45,7 @@
 #include <cmath>
 #include <mutex>
 
+#include "attn_chunk.h"
 #include "causal_few.h"
 #include "ditk_common.h"
 #include "attn_d128_clobbers.h"
@@ -159,7 +160,7 @@ __device__ __forceinline__ int padded_key_start(const int32_t* __restrict__ cu, 
       [voff0] "a"(voff[0]), [voff1] "a"(voff[1]), [voff2] "a"(voff[2]), [voff3] "a"(voff[3]),                     \
       [voffl0] "a"(voffl[0]), [voffl1] "a"(voffl[1]), [voffl2] "a"(voffl[2]), [voffl3] "a"(voffl[3]),             \
       [flag] "s"(su(lds_f)), [lane] "v"(lanev), [qrow0] "v"(qrow0), [qrow1] "v"(qrow1), [vlim0] "v"(vlim[0]),       \
-      [vlim1] "v"(vlim[1]), [kdiag] "s"(su(kdiag)), [vtile] "s"(su(vtile))
+      [vlim1] "v"(vlim[1]), [kdiag] "s"(su(kdiag)), [vtile] "s"(su(vtile)), [odd] "s"(su(lds_odd))
 // Row r, head h of segment m of an operand lies at base + h * hs + m * sa + r * ld
 // (elements).  Packed rows: hs = head_dim, sa = 0.  A [batch, heads, rows, head_dim]
 // tensor read in place: hs and ld its head and row strides, sa = batch stride -
@@ -180,11 +181,11 @@ __global__ __launch_bounds__(256, 1) void flash_fwd_asm(
   static_assert(!CAUSAL || !PRE, "causal: plain q");
   constexpr int NW = 4, BM = 128 * QB;  // QB 32-query blocks per wave
   constexpr int ND = HD / 32;  // DMA instructions per wave and operand per tile
-  __shared__ u32x4_t Ks[2][BN * HD / 8];
+  __shared__ __align__(CAUSAL ? 256 : 16) u32x4_t Ks[2][BN * HD / 8];
   __shared__ u32x4_t Vs[2][HD * 8];
   constexpr int OPITCH = HD * 2 + 8;  // output staging row pitch (bytes), 32 rows per wave
   __shared__ u32x4_t Os[4 * 32 * OPITCH / 16];
-  __shared__ __align__(16) uint32_t Fs[NW];  // rescale flags of one-block waves
+  __shared__ __align__(16) uint32_t Fs[CAUSAL ? 2 * NW : NW];  // rescale flags of one-block waves; causal: odd outputs
   // A work item is np consecutive BM-query tiles of one (segment, head), run as
   // passes of the body (the next pass's loads issued under the current pass's
   // last key tile).  Items in segment-major order (segment, then head, then
@@ -308,6 +309,8 @@ __global__ __launch_bounds__(256, 1) void flash_fwd_asm(
   const uint32_t lds_o = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) u32x4_t*)&Os[0] +
                          (uint32_t)wave_u * (32 * OPITCH);
   const uint32_t lds_f = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) uint32_t*)&Fs[wave_u];
+  const uint32_t lds_odd = lds_f + 4 * NW;
+  (void)lds_odd;
   uint32_t kaddr[4], vaddr[4], koff[4] = {}, koffl[4] = {}, voff[4] = {}, voffl[4] = {};
   (void)voffl;
   const int lrow = lane >> 3;
@@ -410,6 +413,33 @@ __global__ __launch_bounds__(256, 1) void flash_fwd_asm(
     asm volatile(
 #include "attn_d64pq1_body.inc"
         : : DITK_ATTN_ASM_OPERANDS_PRE : DITK_D64P_CLOBBERS "vcc", "scc", "memory");
+  }
+  if constexpr (CAUSAL) {
+    // A wave with an output that is not finite does its rows again, 16 at a time, by the products that take each value
+    // only where it is seen (attn_chunk.h); K's stage is free once all waves are here, the first stores done by then.
+    // 0.1 us of an item without one.
+    __syncthreads();
+    if (Fs[NW + wave_u] != 0) {
+      asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+      const int col = lane & 15, quad = lane >> 4;
+      const bf16_t *kb = Kp + (int64_t)kv_head * HD + (int64_t)k_beg * ldk, *vb = Vt + (int64_t)kv_head * vt_hs + (int64_t)k_beg * vt_ld;
+      for (int r0 = __builtin_amdgcn_readfirstlane(qrow0 - l32); r0 < min(qrow0 - l32 + 32 * QB, q_end); r0 += 16) {
+        const int rows = min(16, q_end - r0), row = r0 + min(col, rows - 1), ahead = k_len - q_end + 1;
+        Chunk<HD, true> x;
+        RowsSrc src{kb, vb, (int)ldk, (int)vt_ld, k_len - 1};
+        x.run(src, Q + (int64_t)row * ldq + (int64_t)head * HD + quad * 8, sc, 0, max(r0 + rows - 1 + ahead, 0),
+              row + ahead, r0 + ahead, nullptr, reinterpret_cast<char*>(&Ks[0][0]) + wave_u * (32 * HD * 2));
+        if (col < rows) {
+          const float inv = inverse(x.l);
+          bf16_t* ob = O + (int64_t)row * ldo + (int64_t)head * HD + quad * 4;
+#pragma unroll
+          for (int j = 0; j < HD / 16; ++j)
+            *reinterpret_cast<u32x2_t*>(ob + j * 16) = u32x2_t{pack_bf2(x.o[j][0] * inv, x.o[j][1] * inv),
+                                                              pack_bf2(x.o[j][2] * inv, x.o[j][3] * inv)};
+          if (quad == 0 && lse != nullptr) lse[(int64_t)head * lse_ld + row] = row_lse2(x.m, x.l) * 0.6931471805599453f;
+        }
+      }
+    }
   }
 }
 

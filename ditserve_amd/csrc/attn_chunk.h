@@ -38,7 +38,8 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 // the half's first row (for a half behind the last key or that is absent: at some row), k_stride() and v_stride() are the
 // rows' distances, and ok(half) says whether the half is there.  All of it is uniform.
 // The next tile's loads are issued as soon as this one's registers are free: the scores are made and the values in LDS.
-template <int HD>
+// EACH: the queries may see different numbers of keys.
+template <int HD, bool EACH>
 struct Chunk {
   static constexpr int NC = HD / 32, ND = HD / 16, CH = HD / 8, RPL = 64 / CH;  // RPL: rows of V a load of the wave covers
   f32x4_t o[ND];
@@ -113,7 +114,9 @@ struct Chunk {
 #pragma unroll
       for (int i = 0; i < 32 / RPL; ++i) *reinterpret_cast<u32x4_t*>((i & 1 ? w4 : w) + i * RPL * (HD * 2)) = x.v[i];
     }
-    if (t0 + 32 < s1) load(src, t0 + 32, s0, s1, x);
+    // a value that some queries do not see and that is not finite would reach them (0 times it is NaN) through the product
+    const bool odd = EACH && !whole && !all_finite(x.v);
+    if (!odd && t0 + 32 < s1) load(src, t0 + 32, s0, s1, x);
     float y[8], top = -INFINITY;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
@@ -137,6 +140,11 @@ struct Chunk {
       m = mn;
     }
     const float base = m == -INFINITY ? 0.f : m;
+    if (odd) {
+      step_odd(y, base, t0, n0, n1, lim, vt);
+      if (t0 + 32 < s1) load(src, t0 + 32, s0, s1, x);
+      return;
+    }
     bf16x8_t hi, lo;
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
@@ -170,6 +178,40 @@ struct Chunk {
     }
   }
 
+  static __device__ __forceinline__ bool all_finite(const u32x4_t (&v)[32 / RPL]) {
+    uint32_t bad = 0;
+#pragma unroll
+    for (int i = 0; i < 32 / RPL; ++i)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) bad |= ((v[i][e] & 0x7f80u) == 0x7f80u) | ((v[i][e] & 0x7f800000u) == 0x7f800000u);
+    return !__any(bad != 0);
+  }
+
+  // P and O of a tile with values that are not finite, each of them only where it is seen: products one by one
+  __device__ __forceinline__ void step_odd(const float (&y)[8], float base, int t0, int n0, int n1, int lim, const char* vt) {
+    const int lane = threadIdx.x & 63, col = lane & 15, quad = lane >> 4;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float mine = __builtin_amdgcn_exp2f(y[e] - base);
+      l += mine;
+#pragma unroll 1
+      for (int g = 0; g < 4; ++g) {
+        const int in = 4 * g + (e & 3), row = (e & 4) * 4 + in;
+        const float p = __shfl(mine, g * 16 + col, 64);
+        if (in >= (e < 4 ? n0 : n1) || t0 + row >= lim) continue;
+#pragma unroll
+        for (int j = 0; j < ND; ++j) {
+          const u32x2_t w = *reinterpret_cast<const u32x2_t*>(vt + row * (HD * 2) + (j ^ v_swizzle<HD>(row)) * 32 + quad * 8);
+#pragma unroll
+          for (int r = 0; r < 2; ++r) {
+            o[j][2 * r] = fmaf(p, __uint_as_float(w[r] << 16), o[j][2 * r]);
+            o[j][2 * r + 1] = fmaf(p, __uint_as_float(w[r] & 0xffff0000u), o[j][2 * r + 1]);
+          }
+        }
+      }
+    }
+  }
+
   // keys [s0, s1); qr: this lane's query row, + 8 quad; vt: 32 HD bf16 of LDS, aligned to 256 bytes
   template <class Src>
   __device__ __forceinline__ void run(Src& src, const bf16_t* qr, float scale2, int s0, int s1, int lim, int all_see,
@@ -186,6 +228,22 @@ struct Chunk {
     for (int t0 = s0; t0 < s1; t0 += 32) step(src, x, q, scale2, t0, s0, s1, lim, all_see, score, vt);
     l = group_sumf(l);
   }
+};
+
+// Packed rows
+struct RowsSrc {
+  const bf16_t *kb, *vb;  // first key's row of the head
+  int ldk, ldv, last;
+  int t0 = 0, t1 = 0;
+  __device__ __forceinline__ void tile(int t, int, int) {
+    t0 = t;
+    t1 = t + 16 <= last ? t + 16 : t;
+  }
+  __device__ __forceinline__ bool ok(int) const { return true; }
+  __device__ __forceinline__ const bf16_t* k(int half) const { return kb + (int64_t)(half ? t1 : t0) * ldk; }
+  __device__ __forceinline__ const bf16_t* v(int half) const { return vb + (int64_t)(half ? t1 : t0) * ldv; }
+  __device__ __forceinline__ int k_stride() const { return ldk; }
+  __device__ __forceinline__ int v_stride() const { return ldv; }
 };
 
 // 1 / l, 0 for a row without keys

@@ -22,21 +22,6 @@ struct Args {
   int64_t parts;
 };
 
-struct RowsSrc {
-  const bf16_t *kb, *vb;  // first key's row of the head
-  int ldk, ldv, last;
-  int t0 = 0, t1 = 0;
-  __device__ __forceinline__ void tile(int t, int, int) {
-    t0 = t;
-    t1 = t + 16 <= last ? t + 16 : t;
-  }
-  __device__ __forceinline__ bool ok(int) const { return true; }
-  __device__ __forceinline__ const bf16_t* k(int half) const { return kb + (int64_t)(half ? t1 : t0) * ldk; }
-  __device__ __forceinline__ const bf16_t* v(int half) const { return vb + (int64_t)(half ? t1 : t0) * ldv; }
-  __device__ __forceinline__ int k_stride() const { return ldk; }
-  __device__ __forceinline__ int v_stride() const { return ldv; }
-};
-
 struct Seg {
   int q0, nq, k0, nk, parts, units;
 };
@@ -55,7 +40,7 @@ __device__ __forceinline__ Seg seg_of(const Args& a, int m) {
 // side by side.
 template <int HD>
 __global__ __launch_bounds__(256, 2) void causal_few_kernel(Args a) {
-  using C = Chunk<HD>;
+  using C = Chunk<HD, true>;
   __shared__ __align__(256) char lds[4 * 32 * HD * 2];
   __shared__ int ends[256], froms[256], sums[2][4];
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;

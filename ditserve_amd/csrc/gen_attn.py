@@ -95,7 +95,10 @@ def configure(hd, pre=False, joint=False, qb=2, causal=False):
     are not seen, out of line, once they are complete (mask_scores).  The tile that holds a
     segment's last key is such a tile for every wave, so no row sums are masked.  V comes as
     rows, like K (no transposed copy): its stage holds 64 rows of HD dims, and a Vt fragment
-    is two transposing reads, each of 4 keys x 16 dims a group of 16 lanes."""
+    is two transposing reads, each of 4 keys x 16 dims a group of 16 lanes.  A value that is
+    not finite makes NaN (times 0) of queries that do not see it too: the epilogue says by a
+    word of LDS (%[odd]) whether any output is not finite, and the wrapper then does the
+    wave's rows again, each value only where it is seen."""
     global QB, BM, KRING, KA, VRING, VA
     QB, BM = qb, 128 * qb
     KRING, KA, VRING, VA = (3, 2, 6, 4) if qb == 2 else (6, 4, 10, 8)
@@ -1091,6 +1094,9 @@ def epilogue(g, negm_of=None):
     g(f"v_lshl_add_u32 {vr(ra)}, {vr(t0)}, 4, {vr(ra)}")
     g(f"v_add_u32 {vr(ra)}, %[lds_o], {vr(ra)}")
     g(f"s_lshl_b32 {s_(S_T1)}, %[ldob], {rpr.bit_length() - 1}")   # rpr rows of output
+    odd = EB + 60  # causal: 0, or NaN once an output is not finite
+    if CAUSAL:
+        g(f"v_mov_b32 {vr(odd)}, 0")
     for qb in range(QB):
         lt, inv, t = EPI_L + 0, EPI_L + 1, EPI_L + 2
         xa = xaddr_to(g, EPI_L + 3, lane)
@@ -1124,6 +1130,8 @@ def epilogue(g, negm_of=None):
                     g(f"v_accvgpr_read_b32 {vr(EB + 8 + k)}, {ar(base + k)}")
                 for k in range(4):
                     g(f"v_mul_f32 {vr(EB + 8 + k)}, {vr(EB + 8 + k)}, {vr(inv)}")
+                for k in range(4 if CAUSAL else 0):
+                    g(f"v_fma_f32 {vr(odd)}, 0, {vr(EB + 8 + k)}, {vr(odd)}")
                 g(f"v_cvt_pk_bf16_f32 {vr(w0)}, {vr(EB + 8)}, {vr(EB + 9)}")
                 g(f"v_cvt_pk_bf16_f32 {vr(w1)}, {vr(EB + 10)}, {vr(EB + 11)}")
                 g(f"ds_write_b64 {vr(wa)}, {vr(w0, 2)} offset:{(d * 32 + gg * 8) * 2}")
@@ -1209,6 +1217,14 @@ def epilogue(g, negm_of=None):
         g(f"global_store_dword {vr(EB + 13)}, {vr(EB + 12)}, %[lsebase]")
         g.label(skip)
         g(f"s_mov_b64 exec, {sp(S_EXEC)}")
+    if CAUSAL:
+        g(f"v_cmp_u_f32 vcc, {vr(odd)}, {vr(odd)}")
+        g("s_cmp_lg_u64 vcc, 0")
+        g(f"s_cselect_b32 {s_(S_T0)}, 1, 0")
+        g(f"v_mov_b32 {vr(odd)}, {s_(S_T0)}")
+        g(f"v_mov_b32 {vr(odd + 1)}, %[odd]")
+        g(f"ds_write_b32 {vr(odd + 1)}, {vr(odd)}")
+        g("s_waitcnt lgkmcnt(0)")
 
 
 def generate():

@@ -88,7 +88,7 @@ __device__ __forceinline__ void store_lse(const Args& a, int64_t row, float e, b
 // order: a sequence's chunks, and for each its heads, which lie side by side in a page.
 template <int HD, bool SCORES>
 __global__ __launch_bounds__(256, 2) void kv_attn_kernel(Args a) {
-  using C = Chunk<HD>;
+  using C = Chunk<HD, false>;
   __shared__ __align__(256) char lds[4 * 32 * HD * 2];
   __shared__ int sums[4], ends[256], lens[256];
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
@@ -166,7 +166,7 @@ __global__ __launch_bounds__(256, 2) void kv_attn_kernel(Args a) {
 // join them through LDS, by the join kernel's operations in its order.
 template <int HD, bool SCORES>
 __global__ __launch_bounds__(512) void kv_attn_short_kernel(Args a) {
-  using C = Chunk<HD>;
+  using C = Chunk<HD, false>;
   constexpr int OP = HD + 4;  // floats of a row of LDS
   __shared__ __align__(256) char lds[8 * 16 * OP * 4];
   __shared__ float stat[2][16][8];

@@ -696,8 +696,8 @@ def flash_attn_causal(q, k, v, seg_q, seg_k, heads, kv_heads, head_dim, softmax_
     them: query i of nq sees the keys j <= i + nk - nq (with earlier keys in front, the next part of
     a prompt; a query that sees none gives zeros and an lse of -inf).  Returns out
     [Tq, heads * head_dim] (and lse [heads, Tq] fp32, natural log, when return_lse).  A segment's
-    result does not depend on what it is packed with.  Values must be finite: an infinity or NaN
-    may also reach queries of the same 256 that do not see it."""
+    result does not depend on what it is packed with, nor a query's on keys and values that it
+    does not see, whatever they hold."""
     if heads <= 0 or kv_heads <= 0 or heads % kv_heads:
         raise ValueError(f"heads must be a multiple of kv_heads, got {heads} and {kv_heads}")
     if head_dim not in (64, 128):

@@ -118,6 +118,38 @@ def test_masked_keys_may_be_anything():
     assert torch.isnan(out[190].float()).all() and torch.isnan(out[500].float()).all()
 
 
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("heads,hk", [(4, 2), (40, 8)])
+def test_values_that_are_not_seen(d, heads, hk):
+    """Values that are not finite reach the queries that see them and no others, in items of 128 and 256 queries and in
+    segments of few queries over many keys."""
+    lens_q, lens_k = [700, 1900, 5, 30], [700, 1900, 2005, 1100]
+    q, k, v = prompt(lens_q, lens_k, heads, hk, d, 21)
+    cq, ck = cu_of(lens_q), cu_of(lens_k)
+    bad = [(0, 300, 1, math.nan), (0, 301, 2, math.inf), (0, 690, 3, -math.inf), (1, 1000, 0, math.inf), (1, 1001, 0, -math.inf),
+           (2, 2002, 5, math.nan), (3, 1080, 7, math.inf), (3, 1099, 8, math.nan)]  # (segment, key, dim of the last head, value)
+    clean = v.clone()
+    for m, key, dim, x in bad:
+        v[ck[m] + key, (hk - 1) * d + dim] = x
+        clean[ck[m] + key, (hk - 1) * d + dim] = 0.25
+    seg_q, seg_k = ops.Segments(cq, DEV), ops.Segments(ck, DEV)
+    out, lse = ops.flash_attn_causal(q, k, v, seg_q, seg_k, heads, hk, d, return_lse=True)
+    want = torch.zeros(out.shape, device=DEV)
+    hit = torch.zeros(out.shape, dtype=torch.bool, device=DEV)
+    for m, key, dim, x in bad:
+        first = cq[m] + key - (lens_k[m] - lens_q[m])  # the first query that sees the key
+        for h in range(heads - heads // hk, heads):
+            want[first:cq[m + 1], h * d + dim] += x
+            hit[first:cq[m + 1], h * d + dim] = True
+    assert torch.equal(torch.isnan(out.float())[hit], torch.isnan(want)[hit])
+    assert torch.equal(torch.nan_to_num(out.float())[hit] > 0, torch.nan_to_num(want)[hit] > 0)
+    assert bool((out.float().abs()[hit & ~torch.isnan(want)] == math.inf).all())
+    # the rest as without them
+    ref = ops.flash_attn_causal(q, k, clean, seg_q, seg_k, heads, hk, d)
+    good = torch.where(hit, ref, out)
+    check(q, k, clean, lens_q, lens_k, heads, hk, d, good, lse)
+
+
 def test_offsets_past_32_bits():
     """Rows of a buffer past 4 GiB, on both sides."""
     n, heads, hk, d = 700, 2, 1, 128
