@@ -60,7 +60,7 @@ CASES = [
     ([513], [256], 3, 3, 64), ([9000], None, 2, 1, 128), ([3000, 2500], None, 24, 8, 64),
     # few queries over many keys, among others
     ([1], [1024], 1, 1, 64), ([1, 16, 3, 32, 33], [5000, 1024, 1023, 4097, 4097], 8, 2, 128), ([128, 0, 7], [1100, 3000, 1600], 5, 5, 64),
-    ([10, 300, 2], [9000, 1300, 1025], 12, 1, 128), ([100], [2000], 6, 6, 128), ([18, 1], [1030, 70000], 7, 1, 64),
+    ([10, 300, 2], [9000, 1300, 1025], 12, 1, 128), ([1, 2, 1] * 100, [1024, 3, 1030] * 100, 2, 1, 64), ([3, 70, 0] * 45, None, 4, 2, 64), ([100], [2000], 6, 6, 128), ([18, 1], [1030, 70000], 7, 1, 64),
 ]
 
 

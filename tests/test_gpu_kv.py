@@ -43,7 +43,7 @@ DECODE = [
     ([1], 1, 1, 128, 16), ([500], 12, 2, 128, 16), ([0, 5, 33, 0], 8, 8, 64, 32), ([31, 32, 33, 64, 65], 32, 8, 128, 64),
     ([255, 256, 257, 1000], 40, 8, 128, 128), ([700, 3], 16, 1, 64, 256), ([511, 513, 129, 127], 9, 3, 128, 16),
     ([4097, 1, 300], 7, 1, 128, 64), ([33000, 12000], 4, 2, 128, 32), ([40001], 34, 2, 64, 16), ([300], 17, 1, 128, 32),
-    ([0], 4, 4, 128, 16), ([2, 1, 2, 1] * 30, 2, 1, 64, 16),
+    ([0], 4, 4, 128, 16), ([2, 1, 2, 1] * 30, 2, 1, 64, 16), ([3, 0, 600, 1] * 75, 2, 1, 64, 16), ([1] * 599 + [1100], 1, 1, 64, 32),
 ]
 
 
