@@ -138,8 +138,9 @@ __device__ __forceinline__ void count_digits(const uint32_t (&key)[KPT], int fir
   }
 }
 
-// the digit of the want-th largest, and how many of its keys are wanted: counts in LDS, two a thread
-__device__ __forceinline__ void find_digit(const int* counts, int& want, int& digit, int (*sums)[16], int* pick) {
+// the digit of the want-th largest, how many of its keys are wanted, and whether that is all of them (then the digits
+// below do not matter: with them 0, the threshold is at or below each of these keys): counts in LDS, two a thread
+__device__ __forceinline__ bool find_digit(const int* counts, int& want, int& digit, int (*sums)[16], int* pick) {
   const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
   const int hi = kBins - 1 - 2 * tid, v0 = counts[hi], v1 = counts[hi - 1];
   int incl = v0 + v1;
@@ -153,13 +154,17 @@ __device__ __forceinline__ void find_digit(const int* counts, int& want, int& di
   for (int i = 0; i < wave; ++i) incl += sums[0][i];
   const int before = incl - v0 - v1;
   if (before < want && want <= incl) {
-    pick[0] = before + v0 >= want ? hi : hi - 1;
-    pick[1] = before + v0 >= want ? want - before : want - before - v0;
+    const bool in0 = before + v0 >= want;
+    pick[0] = in0 ? hi : hi - 1;
+    pick[1] = in0 ? want - before : want - before - v0;
+    pick[2] = pick[1] == (in0 ? v0 : v1);
   }
   __syncthreads();
   digit = pick[0];
   want = pick[1];
+  const bool all = pick[2] != 0;
   __syncthreads();
+  return all;
 }
 
 // Writes this workgroup's slots that stay: those above `top`, and those equal to it while fewer than `want` of them came
@@ -202,7 +207,7 @@ template <int KPT>
 __global__ __launch_bounds__(1024) void kv_select_kernel(KvPages t, KvWeights w, int keep, int recent,
                                                          int32_t* __restrict__ slots, int32_t* __restrict__ new_lengths) {
   __shared__ int counts[3][kBins];
-  __shared__ int sums[2][16], pick[2];
+  __shared__ int sums[2][16], pick[3];
   const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x;
   const Row x = row_of(t, b, keep, recent, tid == 0);
   int32_t* out = slots + ((int64_t)b * gridDim.x + h) * keep;
@@ -214,14 +219,20 @@ __global__ __launch_bounds__(1024) void kv_select_kernel(KvPages t, KvWeights w,
     for (int i = tid; i < 3 * kBins; i += 1024) counts[0][i] = 0;
     load_keys<KPT>(t, w, b, h, 0, x.old, key);
     __syncthreads();
+    bool all = false;
 #pragma unroll
     for (int k = 0; k < 3; ++k) {
+      if (all) break;
       count_digits<KPT>(key, 0, x.old, top, mask, kShift[k], counts[k]);
       __syncthreads();
       int d;
-      find_digit(counts[k], want, d, sums, pick);
+      all = find_digit(counts[k], want, d, sums, pick);
       top |= (uint32_t)d << kShift[k];
       mask = ~0u << kShift[k];
+    }
+    if (all) {  // every key that agrees with `top` stays, as one above it (no key is below 2^21, -inf's first digit)
+      top -= 1;
+      want = 0;
     }
   } else {
 #pragma unroll
@@ -234,7 +245,7 @@ __global__ __launch_bounds__(1024) void kv_select_kernel(KvPages t, KvWeights w,
 struct Counts {
   int* digits;  // [rows][parts][3][kBins]
   int* above;   // [rows][parts][2]: keys above the first digit, and at it but above the second
-  int* pick;    // [rows][2][2]: digits found, and how many are wanted of what agrees with them
+  int* pick;    // [rows][2][2]: digits found, and how many are wanted of what agrees with them (0: all of it)
   int parts;
 };
 
@@ -264,13 +275,20 @@ __device__ __forceinline__ void sum_parts(const Counts& c, int64_t row, int digi
 template <int KPT, int PASS>
 __global__ __launch_bounds__(1024) void kv_count_kernel(KvPages t, KvWeights w, int keep, int recent, Counts c) {
   __shared__ int counts[kBins];
-  __shared__ int sums[2][16], pick[2];
+  __shared__ int sums[2][16], pick[3];
   const int part = blockIdx.x, h = blockIdx.y, b = blockIdx.z, tid = threadIdx.x;
   const Row x = row_of(t, b, keep, recent, false);
   const int first = part * (KPT * 1024);
   if (!x.sort || first >= x.old) return;
   const int64_t row = (int64_t)b * gridDim.y + h;
   const int parts = (x.old - 1) / (KPT * 1024) + 1;
+  if (PASS == 2 && c.pick[row * 4 + 1] == 0) {  // the first digit was enough
+    if (tid == 0) {
+      c.above[(row * c.parts + part) * 2 + 1] = 0;
+      if (part == 0) c.pick[row * 4 + 2] = c.pick[row * 4 + 3] = 0;
+    }
+    return;
+  }
   uint32_t key[KPT], top = 0, mask = 0;
   load_keys<KPT>(t, w, b, h, first, x.old, key);
   if (PASS > 0) {
@@ -284,28 +302,29 @@ __global__ __launch_bounds__(1024) void kv_count_kernel(KvPages t, KvWeights w, 
       top = (uint32_t)c.pick[row * 4] << kShift[0];
       want = c.pick[row * 4 + 1];
     }
-    find_digit(counts, want, d, sums, pick);
+    const bool all = find_digit(counts, want, d, sums, pick);
     top |= (uint32_t)d << kShift[PASS - 1];
     if (part == 0 && tid == 0) {
       c.pick[row * 4 + 2 * (PASS - 1)] = d;
-      c.pick[row * 4 + 2 * (PASS - 1) + 1] = want;
+      c.pick[row * 4 + 2 * (PASS - 1) + 1] = all ? 0 : want;
     }
-    // this part's keys above, among those that agree with the digits before
+    // this part's keys above (all: and at it), among those that agree with the digits before
     const uint32_t agree = PASS == 1 ? 0u : ~0u << kShift[0];
     mask = ~0u << kShift[PASS - 1];
     int na = 0;
 #pragma unroll
     for (int i = 0; i < KPT; ++i) {
       const bool in = first + (tid >> 6) * (KPT * 64) + i * 64 + (tid & 63) < x.old && (key[i] & agree) == (top & agree);
-      na += __popcll(__ballot(in && (key[i] & mask) > top));
+      na += __popcll(__ballot(in && (key[i] & mask) > top - all));
     }
     if ((tid & 63) == 0) sums[1][tid >> 6] = na;
     __syncthreads();
     if (tid == 0) {
-      int all = 0;
-      for (int i = 0; i < 16; ++i) all += sums[1][i];
-      c.above[(row * c.parts + part) * 2 + PASS - 1] = all;
+      int n = 0;
+      for (int i = 0; i < 16; ++i) n += sums[1][i];
+      c.above[(row * c.parts + part) * 2 + PASS - 1] = n;
     }
+    if (all) return;
   }
   counts[tid] = counts[1024 + tid] = 0;
   __syncthreads();
@@ -319,7 +338,7 @@ template <int KPT>
 __global__ __launch_bounds__(1024) void kv_list_kernel(KvPages t, KvWeights w, int keep, int recent, Counts c,
                                                        int32_t* __restrict__ slots, int32_t* __restrict__ new_lengths) {
   __shared__ int counts[kBins];
-  __shared__ int sums[2][16], pick[2], before[2];
+  __shared__ int sums[2][16], pick[3], before[2];
   const int part = blockIdx.x, h = blockIdx.y, b = blockIdx.z, tid = threadIdx.x;
   const Row x = row_of(t, b, keep, recent, part == 0 && tid == 0);
   const int64_t row = (int64_t)b * gridDim.y + h;
@@ -333,22 +352,27 @@ __global__ __launch_bounds__(1024) void kv_list_kernel(KvPages t, KvWeights w, i
   if (x.sort) {
     const int parts = (x.old - 1) / (KPT * 1024) + 1;
     load_keys<KPT>(t, w, b, h, first, x.old, key);
-    int v[2], mine[2];  // counts of the last digit
-    sum_parts(c, row, 2, parts, part, v, mine);
-    counts[tid] = v[0];
-    counts[1024 + tid] = v[1];
     if (tid < 2) before[tid] = 0;
-    __syncthreads();
+    top = (uint32_t)c.pick[row * 4] << kShift[0] | (uint32_t)c.pick[row * 4 + 2] << kShift[1];
     want = c.pick[row * 4 + 3];
-    int d;
-    find_digit(counts, want, d, sums, pick);
-    top = (uint32_t)c.pick[row * 4] << kShift[0] | (uint32_t)c.pick[row * 4 + 2] << kShift[1] | (uint32_t)d;
     int na = 0;
+    if (want == 0) {  // all that agrees with the digits found stays
+      top -= 1;
+      __syncthreads();
+    } else {
+      int v[2], mine[2], d;  // counts of the last digit
+      sum_parts(c, row, 2, parts, part, v, mine);
+      counts[tid] = v[0];
+      counts[1024 + tid] = v[1];
+      __syncthreads();
+      find_digit(counts, want, d, sums, pick);
+      top |= (uint32_t)d;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int bin = i * 1024 + tid;
-      if (bin > d) na += mine[i];
-      if (bin == d) before[1] = mine[i];
+      for (int i = 0; i < 2; ++i) {
+        const int bin = i * 1024 + tid;
+        if (bin > d) na += mine[i];
+        if (bin == d) before[1] = mine[i];
+      }
     }
     for (int p = tid; p < part; p += 1024) na += c.above[(row * c.parts + p) * 2] + c.above[(row * c.parts + p) * 2 + 1];
     if (na) atomicAdd(&before[0], na);  // (whole numbers: no order matters)

@@ -204,7 +204,7 @@ def kept_slots(w, n, keep, recent):
     ([33, 65, 129], 33, 32, 1, 128, 32), ([70000], 600, 17, 1, 64, 128),
     ([1024], 511, 1, 2, 64, 64), ([1025, 4096], 1024, 0, 1, 64, 16), ([4097, 8192], 3, 1, 1, 64, 32), ([8193], 8192, 100, 1, 64, 64),
     ([32768], 16000, 0, 1, 64, 128), ([32769, 20, 9000], 8193, 8192, 1, 64, 128), ([131073, 50], 40000, 33, 1, 64, 256)])
-@pytest.mark.parametrize("kind", ["random", "ties", "odd"])
+@pytest.mark.parametrize("kind", ["random", "ties", "steps", "odd"])
 def test_evict(lens, keep, recent, hk, d, page, kind):
     stay = [min(n, keep) for n in lens]
     cache, table, lengths, out_table, keys, values = paged(lens, hk, d, page, sum(lens), weights=True, more=stay)
@@ -212,6 +212,8 @@ def test_evict(lens, keep, recent, hk, d, page, kind):
     w = torch.randn(cache.weights.shape, generator=g, device=DEV)
     if kind == "ties":
         w = torch.round(w * 2) / 2  # zeros of both signs among them
+    elif kind == "steps":  # few values far apart: digits that leave nothing to decide, and ones that do
+        w = torch.exp2(torch.randint(-3, 3, w.shape, generator=g, device=DEV).float()) + (torch.rand(w.shape, generator=g, device=DEV) < 0.3) * w.abs()
     elif kind == "odd":
         pick = torch.randint(0, 6, w.shape, generator=g, device=DEV)
         for i, x in enumerate((NAN, math.inf, -math.inf, 1e-42, -0.0)):
