@@ -36,7 +36,8 @@ typedef short s16x4 __attribute__((ext_vector_type(4)));
 //
 // Src says where keys are: tile(t0, s0, s1) looks up the tile's two halves of 16 keys; then k(half) and v(half) point at
 // the half's first row (for a half behind the last key or that is absent: at some row), k_stride() and v_stride() are the
-// rows' distances, and ok(half) says whether the half is there.  All of it is uniform.
+// rows' distances, and ok(half) says whether the half is there.  All of it is uniform.  Src::once: whether the rows are
+// read past the caches.
 // The next tile's loads are issued as soon as this one's registers are free: the scores are made and the values in LDS.
 // EACH: the queries may see different numbers of keys.
 template <int HD, bool EACH>
@@ -51,6 +52,12 @@ struct Chunk {
     int n0, n1;  // keys that are there of its halves
   };
 
+  template <bool ONCE, class T>
+  static __device__ __forceinline__ T fetch(const T* p) {
+    if constexpr (ONCE) return __builtin_nontemporal_load(p);
+    return *p;
+  }
+
   template <class Src>
   __device__ __forceinline__ void load(Src& src, int t0, int s0, int s1, Tile& x) const {
     const int lane = threadIdx.x & 63, col = lane & 15, quad = lane >> 4;
@@ -61,10 +68,10 @@ struct Chunk {
         const bf16_t *kr = src.k(h), *vr = src.v(h);
         const uint32_t ko = (uint32_t)col * src.k_stride() + quad * 8, vo = (uint32_t)(lane / CH) * src.v_stride() + (lane % CH) * 8;
 #pragma unroll
-        for (int c = 0; c < NC; ++c) x.k[h][c] = *reinterpret_cast<const bf16x8_t*>(kr + ko + c * 32);
+        for (int c = 0; c < NC; ++c) x.k[h][c] = fetch<Src::once>(reinterpret_cast<const bf16x8_t*>(kr + ko + c * 32));
 #pragma unroll
         for (int i = 0; i < 16 / RPL; ++i)
-          x.v[h * (16 / RPL) + i] = *reinterpret_cast<const u32x4_t*>(vr + (int64_t)i * RPL * src.v_stride() + vo);
+          x.v[h * (16 / RPL) + i] = fetch<Src::once>(reinterpret_cast<const u32x4_t*>(vr + (int64_t)i * RPL * src.v_stride() + vo));
       }
     } else {
 #pragma unroll
@@ -73,11 +80,11 @@ struct Chunk {
         const bf16_t *kr = src.k(h), *vr = src.v(h);
         const uint32_t ko = (uint32_t)min(col, most) * src.k_stride() + quad * 8;
 #pragma unroll
-        for (int c = 0; c < NC; ++c) x.k[h][c] = *reinterpret_cast<const bf16x8_t*>(kr + ko + c * 32);
+        for (int c = 0; c < NC; ++c) x.k[h][c] = fetch<Src::once>(reinterpret_cast<const bf16x8_t*>(kr + ko + c * 32));
 #pragma unroll
         for (int i = 0; i < 16 / RPL; ++i)
-          x.v[h * (16 / RPL) + i] = *reinterpret_cast<const u32x4_t*>(
-              vr + (uint32_t)min(i * RPL + lane / CH, most) * src.v_stride() + (lane % CH) * 8);
+          x.v[h * (16 / RPL) + i] = fetch<Src::once>(reinterpret_cast<const u32x4_t*>(
+              vr + (uint32_t)min(i * RPL + lane / CH, most) * src.v_stride() + (lane % CH) * 8));
       }
     }
     x.n0 = src.ok(0) ? min(s1 - t0, 16) : 0;
@@ -232,6 +239,7 @@ struct Chunk {
 
 // Packed rows
 struct RowsSrc {
+  static constexpr bool once = false;
   const bf16_t *kb, *vb;  // first key's row of the head
   int ldk, ldv, last;
   int t0 = 0, t1 = 0;

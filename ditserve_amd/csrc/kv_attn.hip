@@ -46,9 +46,12 @@ struct Args {
   float scale2;   // softmax scale times log2 e
 };
 
-// Pages of a sequence, 64 of them (1024 slots at least) in a wave's lanes
-template <int HD>
+// Pages of a sequence, 64 of them (1024 slots at least) in a wave's lanes.  ONCE: a long cache's rows go past the caches
+// (16 x 32768 slots 410 -> 397 us, 1 x 131072 105 -> 94, 64 x 2000 112 -> 108; not where scores are written
+// beside: 469 -> 475).
+template <int HD, bool ONCE>
 struct PagedSrc {
+  static constexpr bool once = ONCE;
   const Args& a;
   int b, kvh, last;
   int page = 0, first = 0;
@@ -138,7 +141,7 @@ __global__ __launch_bounds__(256, 2) void kv_attn_kernel(Args a) {
     const int nq = min(a.group - g0, 16), head0 = kvh * a.group + g0;  // query heads of this unit
     const int64_t row = (int64_t)b * a.heads + head0 + min(col, nq - 1);
     C x;
-    PagedSrc<HD> src{a, b, kvh, max(n - 1, 0)};
+    PagedSrc<HD, !SCORES> src{a, b, kvh, max(n - 1, 0)};
     x.run(src, a.q + b * a.ldq + (int64_t)(head0 + min(col, nq - 1)) * HD + quad * 8, a.scale2, s0, s1,
                           n, n, SCORES && col < nq ? a.score + row * a.ld_score : nullptr,
                           lds + wave * (32 * HD * 2));
@@ -179,7 +182,7 @@ __global__ __launch_bounds__(512) void kv_attn_short_kernel(Args a) {
   const int nq = min(a.group - g0, 16), head0 = kvh * a.group + g0;
   const int64_t row = (int64_t)b * a.heads + head0 + min(col, nq - 1);
   C x;
-  PagedSrc<HD> src{a, b, kvh, max(n - 1, 0)};
+  PagedSrc<HD, false> src{a, b, kvh, max(n - 1, 0)};
   x.run(src, a.q + b * a.ldq + (int64_t)(head0 + min(col, nq - 1)) * HD + quad * 8, a.scale2, s0, s1,
                        n, n, SCORES && col < nq ? a.score + row * a.ld_score : nullptr,
                        lds + wave * (16 * OP * 4));
