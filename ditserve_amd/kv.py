@@ -27,7 +27,7 @@ import torch
 
 from . import _lib, ops
 from .mx import _apart
-from .ops import _call, _check, _extent, _one_device, _ptr, _row_view
+from .ops import _call, _check, _extent, _meet, _one_device, _ptr, _row_view
 
 PAGES = (16, 32, 64, 128, 256)
 HEAD_DIMS = (64, 128)
@@ -55,8 +55,8 @@ _STATUS = {}
 
 def _status(device):
     st = _STATUS.get(device)
-    if st is None:
-        st = _STATUS[device] = PageStatus(device)
+    if st is None:  # (one word for good, also if two threads come here at once)
+        st = _STATUS.setdefault(device, PageStatus(device))
     return st
 
 
@@ -67,6 +67,27 @@ def check_tables(device=None):
     if device.index is None:
         device = torch.device(device.type, torch.cuda.current_device())
     _status(device).check()
+
+
+def _levels(pages, heads, ps, hs, size):
+    """[(stride, count, what lies below)] of a tensor's (page, head) blocks, the smallest stride first; None if they overlap."""
+    levels = []
+    for stride, count in sorted((x for x in ((ps, pages), (hs, heads)) if x[1] > 1)):
+        if stride < size:
+            return None
+        levels.append((stride, count, size))
+        size += (count - 1) * stride
+    return levels
+
+
+def _meet_blocks(delta, levels, size):
+    """Whether a block of two tensors of the same strides, the second `delta` behind the first, is in both."""
+    if not levels:
+        return abs(delta) < size
+    stride, count, below = levels[-1]
+    near = -delta // stride
+    return any(abs(delta + i * stride) < below and _meet_blocks(delta + i * stride, levels[:-1], size)
+               for i in (near, near + 1) if abs(i) < count)
 
 
 class PagedCache:
@@ -90,18 +111,21 @@ class PagedCache:
                 raise ValueError(f"{name} must be [pages, kv_heads, {PAGES}, {HEAD_DIMS}], got {dims}")
             if pages == 0 or heads == 0:
                 raise ValueError(f"{name} has no pages or no heads: {dims}")
-            if unit != 1 or ss != d or ps % 8 or hs % 8 or t.data_ptr() % 16 or \
-                    (pages > 1 and ps < page * d) or (heads > 1 and hs < page * d):
-                raise ValueError(f"{name}'s slots must be contiguous within a (page, head) and 16-byte aligned, got "
-                                 f"strides {t.stride()}")
+            levels = _levels(pages, heads, ps, hs, page * d)
+            if unit != 1 or ss != d or ps % 8 or hs % 8 or t.data_ptr() % 16 or levels is None:
+                raise ValueError(f"{name}'s slots must be contiguous within a (page, head), which must not overlap, and "
+                                 f"16-byte aligned, got strides {t.stride()}")
             strides += [ps, hs]
         if v.shape != k.shape:
             raise ValueError(f"v must be {tuple(k.shape)}, got {tuple(v.shape)}")
         _one_device(k.device, ("v", v), ("weights", weights))
+        if _meet(_extent(k), _extent(v)) and (strides[:2] != strides[2:] or
+                                              _meet_blocks((v.data_ptr() - k.data_ptr()) // 2, levels, page * d)):
+            raise ValueError("k and v overlap")
         if weights is not None:
             _check(weights, "weights", torch.float32, 3)
             ps, hs, unit = weights.stride()
-            if tuple(weights.shape) != dims[:3] or unit != 1 or (pages > 1 and ps < page) or (heads > 1 and hs < page):
+            if tuple(weights.shape) != dims[:3] or unit != 1 or _levels(pages, heads, ps, hs, page) is None:
                 raise ValueError(f"weights must be {dims[:3]} with unit slot stride, got {tuple(weights.shape)}, strides "
                                  f"{weights.stride()}")
             strides += [ps, hs]
@@ -201,7 +225,7 @@ def append(cache, k, v, table, lengths, segments=None):
     tp, ldt, width = _table(table, "table", batch, device)
     kp, vp, lp, cu = k.data_ptr(), v.data_ptr(), lengths.data_ptr(), None
     spans = [(kp, kp + 2 * ((T - 1) * ldk + wide) * (T > 0)), (vp, vp + 2 * ((T - 1) * ldv + wide) * (T > 0)),
-             (tp, tp + 4 * batch * ldt), (lp, lp + 4 * batch)]
+             (tp, tp + 4 * (batch * ldt - ldt + width)), (lp, lp + 4 * batch)]
     if segments is not None:
         if segments.nseg != batch or segments.total != T:
             raise ValueError(f"segments are {segments.nseg} of {segments.total} rows, lengths {batch} and k {T}")
@@ -261,6 +285,8 @@ def decode_attn(q, cache, table, lengths, heads, softmax_scale=None, max_len=Non
             raise ValueError(f"out must have one row for each of the {batch} sequences, got {rows}")
         _outside("decode_attn", cache, _extent(out))
         _apart("decode_attn", (out,), (q, table, lengths))
+    if weights is not None:
+        _outside("decode_attn", cache, _extent(q), _extent(table), _extent(lengths))
     status = _status(device)
     status.poll()
     lse = torch.empty((batch, heads), dtype=torch.float32, device=device) if return_lse else None
@@ -301,6 +327,7 @@ def evict(cache, table, lengths, out_table, keep, recent=0, max_len=None):
         most = min(most, int(max_len))
     if out_width * page < min(keep, most):
         raise ValueError(f"out_table holds {out_width * page} slots, {min(keep, most)} stay")
+    _outside("evict", cache, _extent(table), _extent(out_table), _extent(lengths))
     keep = max(min(keep, most), 1)
     recent = min(recent, keep)
     status = _status(device)

@@ -168,6 +168,40 @@ def test_append(before, counts, hk, d, page, layout):
         assert torch.equal(get(cache.k, table[0], after[0])[-1], k.reshape(T, hk, d)[0])
 
 
+def test_overlapping_operands_are_refused():
+    pages, hk, page, d = 6, 2, 16, 64
+    x = torch.zeros((pages, 2 * hk, page, d), dtype=torch.bfloat16, device=DEV)
+    w = torch.zeros((pages, hk, page), device=DEV)
+    cache = kv.PagedCache(x[:, ::2], x[:, 1::2], w)  # heads of keys and of values in turn
+    kv.PagedCache(x[:3, :hk], x[3:, :hk])
+    one, block = x[:, :hk], page * d
+    for k, v in ((one, one), (one, x[:, 1:1 + hk]), (one[1:], one[:-1]), (x[:, ::2], x[:, :hk]),
+                 (one, x.view(-1)[block // 2:].as_strided(one.shape, one.stride()))):
+        with pytest.raises(ValueError, match="overlap"):
+            kv.PagedCache(k, v)
+    for strides in ((block, block), (block, 2 * block), (0, block), (block // 2, 6 * block)):  # pages that overlap heads
+        with pytest.raises(ValueError, match="overlap"):
+            kv.PagedCache(x.as_strided(one.shape, (*strides, d, 1)), torch.zeros_like(one))
+    with pytest.raises(ValueError, match="weights"):
+        kv.PagedCache(x[:, ::2], x[:, 1::2], w.as_strided(w.shape, (page, page, 1)))
+    # operands that lie in the cache
+    inside = x.view(-1).view(torch.int32)
+    table, lengths, fine = inside[:8].view(2, 4), inside[:2], torch.zeros((2, 4), dtype=torch.int32, device=DEV)
+    n, q = torch.zeros(2, dtype=torch.int32, device=DEV), torch.zeros((2, hk * d), dtype=torch.bfloat16, device=DEV)
+    for bad in ((table, n, fine), (fine, lengths, fine.clone()), (fine, n, table)):
+        with pytest.raises(ValueError, match="lies in the cache"):
+            kv.evict(cache, *bad, 4)
+    for bad in ((x.view(-1)[:2 * hk * d].view(2, hk * d), fine, n), (q, table, n), (q, fine, lengths)):
+        with pytest.raises(ValueError, match="lies in the cache"):
+            kv.decode_attn(bad[0], cache, *bad[1:], hk, weights="set")
+    # a table that is a few columns of one that the cache follows is none
+    flat = torch.zeros(4096 + pages * 2 * hk * block, dtype=torch.bfloat16, device=DEV)
+    rows, rest = flat[:4096].view(torch.int32).view(2, 1024), flat[4096:].view(x.shape)
+    rows[1] = 1
+    beside = kv.PagedCache(rest[:, :hk], rest[:, hk:])
+    assert kv.append(beside, q, q, rows[:, 1020:], n).tolist() == [1, 1]
+
+
 def test_append_past_the_table():
     """Rows that no page is there for are not written; the length stops where the table does."""
     cache, table, _, _, _ = paged([40, 30], 2, 64, 16, 12)

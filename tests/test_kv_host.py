@@ -88,6 +88,22 @@ def test_cpu_tensors_are_refused():
         kv.evict(k, k, k, k, 2)
 
 
+@pytest.mark.parametrize("pages,heads,ps,hs,size", [
+    (1, 1, 0, 0, 8), (4, 1, 8, 3, 8), (4, 1, 7, 0, 8), (1, 3, 0, 16, 8), (3, 2, 16, 8, 8), (3, 2, 8, 24, 8), (3, 2, 8, 16, 8),
+    (3, 4, 40, 8, 8), (3, 4, 24, 8, 8), (2, 3, 100, 16, 8), (5, 2, 8, 8, 8), (2, 2, 64, 32, 8)])
+def test_overlapping_blocks(pages, heads, ps, hs, size):
+    """What is said of the blocks of one cache, and of two, is what counting their elements says."""
+    starts = [i * ps + j * hs for i in range(pages) for j in range(heads)]
+    cells = [x + i for x in starts for i in range(size)]
+    levels = kv._levels(pages, heads, ps, hs, size)
+    if levels is None:  # (levels of a stride below what they hold are not taken, though some of them interleave)
+        assert len(set(cells)) < len(cells)
+        return
+    assert len(set(cells)) == len(cells)
+    for delta in range(-max(cells) - 2, max(cells) + 3):
+        assert kv._meet_blocks(delta, levels, size) == any(x + delta in set(cells) for x in cells), delta
+
+
 CAUSAL = dict(q=A, ldq=256, k=B, ldk=128, v=G, ldv=128, o=D, ldo=256, lse=None, lse_ld=0, cu_q=E, cu_k=F, nseg=1, Tq=64,
               Tk=64, heads=4, hk=2, d=64, scale=0.1, kinds=3, space=H,
               size=1 << 20, parts=8, stream=None)
