@@ -69,25 +69,35 @@ def check_tables(device=None):
     _status(device).check()
 
 
-def _levels(pages, heads, ps, hs, size):
-    """[(stride, count, what lies below)] of a tensor's (page, head) blocks, the smallest stride first; None if they overlap."""
-    levels = []
-    for stride, count in sorted((x for x in ((ps, pages), (hs, heads)) if x[1] > 1)):
-        if stride < size:
-            return None
-        levels.append((stride, count, size))
-        size += (count - 1) * stride
-    return levels
+def _span(pages, heads, ps, hs, size):
+    """From the first to the last element of a tensor's (page, head) blocks of `size`; 0 if blocks overlap."""
+    if pages > 1 and heads > 1 and ps < hs:
+        pages, heads, ps, hs = heads, pages, hs, ps
+    if heads > 1:
+        if hs < size:
+            return 0
+        size += (heads - 1) * hs
+    if pages > 1:
+        if ps < size:
+            return 0
+        size += (pages - 1) * ps
+    return size
 
 
-def _meet_blocks(delta, levels, size):
-    """Whether a block of two tensors of the same strides, the second `delta` behind the first, is in both."""
-    if not levels:
-        return abs(delta) < size
-    stride, count, below = levels[-1]
-    near = -delta // stride
-    return any(abs(delta + i * stride) < below and _meet_blocks(delta + i * stride, levels[:-1], size)
-               for i in (near, near + 1) if abs(i) < count)
+def _nearest(delta, stride, count):
+    """delta and a multiple of stride, less than `count` of them either way, where that is nearest to 0 on both sides."""
+    if count == 1:
+        return (delta,)
+    i = -delta // stride
+    return [delta + j * stride for j in (i, i + 1) if abs(j) < count]
+
+
+def _meet_blocks(delta, pages, heads, ps, hs, size):
+    """Whether two tensors of the same strides, of which _span is not 0, the second `delta` elements behind the first,
+    share an element."""
+    if pages > 1 and heads > 1 and ps < hs:
+        pages, heads, ps, hs = heads, pages, hs, ps
+    return any(abs(y) < size for x in _nearest(delta, ps, pages) for y in _nearest(x, hs, heads))
 
 
 class PagedCache:
@@ -99,40 +109,46 @@ class PagedCache:
     weights  [pages, kv_heads, page] fp32, the attention weight each slot has gathered
              (optional; decode_attn writes it, evict reads it)"""
 
-    __slots__ = ("_k", "_v", "_w", "_dims", "_strides")
+    __slots__ = ("_k", "_v", "_w", "_dims", "_strides", "_bytes")
 
     def __init__(self, k, v, weights=None):
-        strides = []
+        strides, ends = [], []
         for t, name in ((k, "k"), (v, "v")):
-            _check(t, name, _BF16, 4)
+            if t.__class__ is not torch.Tensor or t.dtype is not _BF16 or not t.is_cuda or t.dim() != 4:
+                _check(t, name, _BF16, 4)
             pages, heads, page, d = dims = tuple(t.shape)
             ps, hs, ss, unit = t.stride()
             if page not in PAGES or d not in HEAD_DIMS:
                 raise ValueError(f"{name} must be [pages, kv_heads, {PAGES}, {HEAD_DIMS}], got {dims}")
             if pages == 0 or heads == 0:
                 raise ValueError(f"{name} has no pages or no heads: {dims}")
-            levels = _levels(pages, heads, ps, hs, page * d)
-            if unit != 1 or ss != d or ps % 8 or hs % 8 or t.data_ptr() % 16 or levels is None:
+            first, span = t.data_ptr(), _span(pages, heads, ps, hs, page * d)
+            if unit != 1 or ss != d or (ps | hs) & 7 or first & 15 or not span:
                 raise ValueError(f"{name}'s slots must be contiguous within a (page, head), which must not overlap, and "
                                  f"16-byte aligned, got strides {t.stride()}")
-            strides += [ps, hs]
+            strides += (ps, hs)
+            ends.append((first, first + 2 * span))
         if v.shape != k.shape:
             raise ValueError(f"v must be {tuple(k.shape)}, got {tuple(v.shape)}")
-        _one_device(k.device, ("v", v), ("weights", weights))
-        if _meet(_extent(k), _extent(v)) and (strides[:2] != strides[2:] or
-                                              _meet_blocks((v.data_ptr() - k.data_ptr()) // 2, levels, page * d)):
+        device = k.device
+        if v.device != device or (weights is not None and weights.device != device):
+            _one_device(device, ("v", v), ("weights", weights))
+        if _meet(*ends) and (strides[:2] != strides[2:] or _meet_blocks((ends[1][0] - ends[0][0]) // 2, *dims[:2], ps, hs,
+                                                                        page * d)):
             raise ValueError("k and v overlap")
         if weights is not None:
             _check(weights, "weights", torch.float32, 3)
             ps, hs, unit = weights.stride()
-            if tuple(weights.shape) != dims[:3] or unit != 1 or _levels(pages, heads, ps, hs, page) is None:
+            span = _span(pages, heads, ps, hs, page)
+            if tuple(weights.shape) != dims[:3] or unit != 1 or not span:
                 raise ValueError(f"weights must be {dims[:3]} with unit slot stride, got {tuple(weights.shape)}, strides "
                                  f"{weights.stride()}")
-            strides += [ps, hs]
+            strides += (ps, hs)
         else:
-            strides += [0, 0]
+            span, strides = 0, strides + [0, 0]
+        self._bytes = ends[0][1] - ends[0][0], ends[1][1] - ends[1][0], 4 * span
         self._k, self._v, self._w, self._dims, self._strides = k, v, weights, dims, strides
-        _status(k.device)
+        _status(device)
 
     @classmethod
     def empty(cls, pages, kv_heads, head_dim, page=64, device="cuda", weights=True):
@@ -164,12 +180,9 @@ class PagedCache:
 
     def _spans(self):
         """First and last byte of keys, values and weights."""
-        pages, heads, page, d = self._dims
-        for t, (ps, hs), size in ((self._k, self._strides[:2], 2 * d), (self._v, self._strides[2:4], 2 * d),
-                                  (self._w, self._strides[4:], 4)):
-            if t is not None:
-                first = t.data_ptr()
-                yield first, first + ((pages - 1) * ps + (heads - 1) * hs) * t.element_size() + page * size
+        k, v, w = self._k.data_ptr(), self._v.data_ptr(), self._w.data_ptr() if self._w is not None else 0
+        a, b, c = self._bytes
+        return (k, k + a), (v, v + b), (w or k, (w or k) + c)
 
 
 def _cache_check(cache):
@@ -201,10 +214,12 @@ def _lengths(t, device):
 
 def _outside(fn, cache, *spans):
     """Refuse operands (first and last byte) that lie between a cache's first and last byte."""
-    for a, b in cache._spans():
-        for first, last in spans:
-            if first < b and a < last:
-                raise ValueError(f"{fn}: an operand lies in the cache")
+    own = cache._spans()
+    (a, b), (c, d), (e, f) = own
+    low, high = min(a, c, e), max(b, d, f)
+    for span in spans:
+        if span[0] < high and low < span[1] and any(_meet(span, x) for x in own):
+            raise ValueError(f"{fn}: an operand lies in the cache")
 
 
 def append(cache, k, v, table, lengths, segments=None):

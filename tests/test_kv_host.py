@@ -95,13 +95,13 @@ def test_overlapping_blocks(pages, heads, ps, hs, size):
     """What is said of the blocks of one cache, and of two, is what counting their elements says."""
     starts = [i * ps + j * hs for i in range(pages) for j in range(heads)]
     cells = [x + i for x in starts for i in range(size)]
-    levels = kv._levels(pages, heads, ps, hs, size)
-    if levels is None:  # (levels of a stride below what they hold are not taken, though some of them interleave)
+    span = kv._span(pages, heads, ps, hs, size)
+    if span == 0:
         assert len(set(cells)) < len(cells)
         return
-    assert len(set(cells)) == len(cells)
+    assert len(set(cells)) == len(cells) and span == max(cells) + 1
     for delta in range(-max(cells) - 2, max(cells) + 3):
-        assert kv._meet_blocks(delta, levels, size) == any(x + delta in set(cells) for x in cells), delta
+        assert kv._meet_blocks(delta, pages, heads, ps, hs, size) == any(x + delta in set(cells) for x in cells), delta
 
 
 CAUSAL = dict(q=A, ldq=256, k=B, ldk=128, v=G, ldv=128, o=D, ldo=256, lse=None, lse_ld=0, cu_q=E, cu_k=F, nseg=1, Tq=64,
