@@ -210,11 +210,7 @@ __global__ __launch_bounds__(256, 1) void flash_fwd_asm(
       const int nq = cu_q[i + 1] - cu_q[i];
       const bool mine = m + lane < nseg && !few_queries(nq, cu_k[i + 1] - cu_k[i], group);
       const int ntile = mine ? (nq + BM - 1) / BM : 0;
-      int items = ntile * heads;
-      for (int off = 1; off < 64; off <<= 1) {
-        const int x = __shfl_up(items, off, 64);
-        items += lane >= off ? x : 0;
-      }
+      const int items = wave_scan(ntile * heads);
       const uint64_t past = __ballot(items > t);
       if (past != 0) {
         const int at = __builtin_ctzll(past);

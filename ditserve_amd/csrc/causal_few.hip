@@ -54,12 +54,8 @@ __global__ __launch_bounds__(256, 2) void causal_few_kernel(Args a) {
       units += s.units;
       parts += s.parts;
     }
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) {
-    const int x = __shfl_up(units, off, 64), y = __shfl_up(parts, off, 64);
-    units += lane >= off ? x : 0;
-    parts += lane >= off ? y : 0;
-  }
+  units = wave_scan(units);
+  parts = wave_scan(parts);
   if (lane == 63) sums[0][wave] = units, sums[1][wave] = parts;
   __syncthreads();
   for (int w = 0; w < wave; ++w) {

@@ -124,6 +124,17 @@ __device__ __forceinline__ float wave_max(float v) {
   return v;
 }
 
+// sums over the lanes up to and with each: within rows of 16 lanes, then of the rows before
+__device__ __forceinline__ int wave_scan(int x) {
+  x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xF, 0xF, true);   // row_shr:1
+  x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xF, 0xF, true);   // row_shr:2
+  x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xF, 0xF, true);   // row_shr:4
+  x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xF, 0xF, true);   // row_shr:8
+  x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xA, 0xF, false);  // row 0's last lane to row 1, row 2's to row 3
+  x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xC, 0xF, false);  // lane 31 to rows 2 and 3
+  return x;
+}
+
 // segment of token t in cu[0..nseg] (cu[0] = 0, nondecreasing); tokens at or
 // beyond cu[nseg] map to nseg - 1.
 __device__ __forceinline__ int find_segment(const int32_t* __restrict__ cu, int nseg, int t) {

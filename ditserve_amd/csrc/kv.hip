@@ -69,12 +69,10 @@ __global__ __launch_bounds__(256) void kv_append_kernel(KvPages t, KvTensor kc, 
   }
 }
 
-// fp32 -> uint32 whose order is the floats': -0 is 0, and a NaN is -inf
+// fp32 -> uint32 whose order is the floats', from -inf's 0x7fffff to +inf's 0xff800000: -0 is 0, and a NaN is -inf
 __device__ __forceinline__ uint32_t order_of(float f) {
-  uint32_t u = __float_as_uint(f);
-  if (f != f) u = 0xff800000u;
-  if (u == 0x80000000u) u = 0;
-  return u & 0x80000000u ? ~u : u | 0x80000000u;
+  const uint32_t u = __float_as_uint(fmaxf(f + 0.f, -INFINITY));
+  return u ^ ((uint32_t)((int)u >> 31) | 0x80000000u);
 }
 
 // The slots that stay, ascending, of a (sequence, key head): of its `old` slots before the recent ones those above a
@@ -87,7 +85,10 @@ __device__ __forceinline__ uint32_t order_of(float f) {
 // each of every part: counts of the first digit; that digit from all parts' counts, and counts of the second; the same
 // for the third; the threshold and the list (kv_count_kernel, kv_list_kernel).  Counts have a place for each part, so
 // that nothing has to be cleared and no order matters.
-constexpr int kBins = 2048;
+//
+// Latency bounds it: reads that wait for each other, and some 300 vector operations a wave on the few CUs that have one
+// of the workgroups.  64 rows of 8192 slots 10 us; 8 of 131072 in 16 parts 4.5, 6, 6 and 8 us for the four launches.
+constexpr int kBins = 2048, kCopies = 4;
 constexpr int kShift[3] = {21, 10, 0};
 
 struct Row {
@@ -105,61 +106,99 @@ __device__ __forceinline__ Row row_of(const KvPages& t, int b, int keep, int rec
   return x;
 }
 
+// A thread's keys, 0 behind the last slot.  Its table entries (of slots that the call's lengths may have) are asked for before the sequence's
+// length is there, and its weights become keys after whatever else a launch reads is asked for: 64 rows of 8192 slots
+// 12.2 -> 10.6 us.
 template <int KPT>
-__device__ __forceinline__ void load_keys(const KvPages& t, const KvWeights& w, int b, int h, int first, int old,
-                                          uint32_t (&key)[KPT]) {
-  const int base = first + (threadIdx.x >> 6) * (KPT * 64) + (threadIdx.x & 63);
+struct Keys {
   int page[KPT];
+  float raw[KPT];
+  uint32_t key[KPT];
+
+  __device__ __forceinline__ int slot(int first, int i) const {
+    return first + (int)(threadIdx.x >> 6) * (KPT * 64) + (int)(threadIdx.x & 63) + i * 64;
+  }
+  __device__ __forceinline__ void load_pages(const KvPages& t, int b, int first) {
+    if (t.most == 0) return;  // (no table: no keys either)
+    const int32_t* row = t.table + b * t.ldt;
 #pragma unroll
-  for (int i = 0; i < KPT; ++i) page[i] = base + i * 64 < old ? t.table[b * t.ldt + ((base + i * 64) >> t.page_log2)] : 0;
+    for (int i = 0; i < KPT; ++i) page[i] = row[(uint32_t)min(slot(first, i), t.most - 1) >> t.page_log2];
+  }
+  // (of a page that the cache lacks, and behind the last slot, some other weight: without branches all loads go out at once)
+  __device__ __forceinline__ void load_weights(const KvPages& t, const KvWeights& w, int h, int first, int old) {
+    const float* row = w.p + h * w.hs;
+    bool bad = false;
+#pragma unroll
+    for (int i = 0; i < KPT; ++i) {
+      const int at = slot(first, i);
+      const bool ok = (unsigned)page[i] < (unsigned)t.pages;
+      bad |= !ok && at < old;
+      raw[i] = row[(uint64_t)(ok ? (uint32_t)page[i] : 0u) * (uint32_t)w.ps + (at & ((1 << t.page_log2) - 1))];
+    }
+    if (bad) *t.status = 1;
+  }
+  __device__ __forceinline__ void make(const KvPages& t, int first, int old) {
+#pragma unroll
+    for (int i = 0; i < KPT; ++i)
+      key[i] = slot(first, i) < old ? order_of((unsigned)page[i] < (unsigned)t.pages ? raw[i] : -INFINITY) : 0u;
+  }
+  // every slot stays, or none: keys above a threshold of 0, or not
+  __device__ __forceinline__ void make_all(int first, int old, bool stay) {
+#pragma unroll
+    for (int i = 0; i < KPT; ++i) key[i] = stay && slot(first, i) < old ? 1u : 0u;
+  }
+};
+
+// counts[d] += keys of this workgroup whose k-th digit is d and that agree with `top` above it.  Neighbouring lanes count in
+// kCopies places, so that keys of few digits (a first digit is a sign, an exponent and two bits) meet less.
+template <int KPT>
+__device__ __forceinline__ void count_digits(const uint32_t (&key)[KPT], int k, uint32_t top, int (*counts)[kCopies]) {
+  int* mine = counts[0] + (threadIdx.x % kCopies);
 #pragma unroll
   for (int i = 0; i < KPT; ++i) {
-    const int at = base + i * 64;
-    const bool ok = (unsigned)page[i] < (unsigned)t.pages;
-    if (!ok) *t.status = 1;
-    key[i] = order_of(at < old && ok ? w.p[page[i] * w.ps + h * w.hs + (at & ((1 << t.page_log2) - 1))] : -INFINITY);
+    const uint32_t d = k == 0 ? key[i] >> kShift[0] : k == 1 ? (key[i] >> kShift[1]) % kBins : key[i] % (1u << kShift[1]);
+    if (k == 0 ? key[i] != 0 : (key[i] ^ top) < 1u << kShift[k - 1]) atomicAdd(&mine[d * kCopies], 1);
   }
 }
 
-// counts[d] += keys of this workgroup that have digit d and agree with `top` where `mask` says
-template <int KPT>
-__device__ __forceinline__ void count_digits(const uint32_t (&key)[KPT], int first, int old, uint32_t top, uint32_t mask,
-                                             int shift, int* counts) {
-  const int lane = threadIdx.x & 63, base = first + (threadIdx.x >> 6) * (KPT * 64) + lane;
+__device__ __forceinline__ void clear_counts(int (*counts)[kCopies]) {
 #pragma unroll
-  for (int i = 0; i < KPT; ++i) {
-    const bool in = base + i * 64 < old && (key[i] & mask) == top;
-    const int d = (int)(key[i] >> shift) & (kBins - 1) & (int)(~mask >> shift);
-    // lanes that share the first one's digit count as one
-    const uint64_t any = __ballot(in);
-    if (any == 0) continue;
-    const int lead = __builtin_ctzll(any), d0 = __builtin_amdgcn_readlane(d, lead);
-    const uint64_t same = __ballot(in && d == d0);
-    if (lane == lead) atomicAdd(&counts[d0], __popcll(same));
-    else if (in && d != d0) atomicAdd(&counts[d], 1);
+  for (int i = 0; i < 2; ++i) *reinterpret_cast<u32x4_t*>(counts[i * 1024 + threadIdx.x]) = u32x4_t{0, 0, 0, 0};
+}
+
+// counts of a thread's two digits, 2047 - 2 tid and the one below: the larger first
+__device__ __forceinline__ void my_digits(const int (*counts)[kCopies], int (&v)[2]) {
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const u32x4_t x = *reinterpret_cast<const u32x4_t*>(counts[kBins - 1 - 2 * threadIdx.x - i]);
+    v[i] = (int)((x[0] + x[1]) + (x[2] + x[3]));
   }
+}
+
+// sum of the first `wave` of 16 numbers in LDS (read side by side: one after another they cost a latency each)
+__device__ __forceinline__ int sum_before(const int (&sums)[16], int wave) {
+  int x[16], n = 0;
+#pragma unroll
+  for (int i = 0; i < 16; ++i) x[i] = sums[i];
+#pragma unroll
+  for (int i = 0; i < 16; ++i) n += i < wave ? x[i] : 0;
+  return n;
 }
 
 // the digit of the want-th largest, how many of its keys are wanted, and whether that is all of them (then the digits
-// below do not matter: with them 0, the threshold is at or below each of these keys): counts in LDS, two a thread
-__device__ __forceinline__ bool find_digit(const int* counts, int& want, int& digit, int (*sums)[16], int* pick) {
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-  const int hi = kBins - 1 - 2 * tid, v0 = counts[hi], v1 = counts[hi - 1];
-  int incl = v0 + v1;
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) {
-    const int o = __shfl_up(incl, off, 64);
-    if (lane >= off) incl += o;
-  }
+// below do not matter: with them 0, the threshold is at or below each of these keys): v as my_digits gives it
+__device__ __forceinline__ bool find_digit(const int (&v)[2], int& want, int& digit, int (*sums)[16], int* pick) {
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, hi = kBins - 1 - 2 * tid;
+  int incl = wave_scan(v[0] + v[1]);
   if (lane == 63) sums[0][wave] = incl;
   __syncthreads();
-  for (int i = 0; i < wave; ++i) incl += sums[0][i];
-  const int before = incl - v0 - v1;
+  incl += sum_before(sums[0], wave);
+  const int before = incl - v[0] - v[1];
   if (before < want && want <= incl) {
-    const bool in0 = before + v0 >= want;
+    const bool in0 = before + v[0] >= want;
     pick[0] = in0 ? hi : hi - 1;
-    pick[1] = in0 ? want - before : want - before - v0;
-    pick[2] = pick[1] == (in0 ? v0 : v1);
+    pick[1] = in0 ? want - before : want - before - v[0];
+    pick[2] = pick[1] == (in0 ? v[0] : v[1]);
   }
   __syncthreads();
   digit = pick[0];
@@ -172,115 +211,116 @@ __device__ __forceinline__ bool find_digit(const int* counts, int& want, int& di
 // Writes this workgroup's slots that stay: those above `top`, and those equal to it while fewer than `want` of them came
 // before.  at, tie: slots that stay, and equal ones, in the parts before.
 template <int KPT>
-__device__ __forceinline__ void write_list(const uint32_t (&key)[KPT], const Row& x, int first, uint32_t top, int want, int at,
-                                           int tie, int (*sums)[16], int32_t* out) {
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, base = first + wave * (KPT * 64);
-  const bool all = x.n <= x.m;
-  if (!all && !x.sort) return;
+__device__ __forceinline__ void write_list(const uint32_t (&key)[KPT], int first, uint32_t top, int want, int at, int tie,
+                                           int (*sums)[16], int32_t* out) {
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   int na = 0, nt = 0;
 #pragma unroll
   for (int i = 0; i < KPT; ++i) {
-    const bool in = base + i * 64 + lane < x.old;
-    na += __popcll(__ballot(in && (all || key[i] > top)));
-    nt += __popcll(__ballot(in && !all && key[i] == top));
+    na += __popcll(__ballot(key[i] > top));
+    nt += __popcll(__ballot(key[i] == top));
   }
   if (lane == 0) sums[0][wave] = na, sums[1][wave] = nt;
   __syncthreads();
-  for (int i = 0; i < wave; ++i) {
-    at += sums[0][i];
-    tie += sums[1][i];
-  }
-  at += min(tie, want);
-  const uint64_t before = (1ull << lane) - 1;
+  tie = __builtin_amdgcn_readfirstlane(tie + sum_before(sums[1], wave));
+  at = __builtin_amdgcn_readfirstlane(at + sum_before(sums[0], wave) + min(tie, want));
 #pragma unroll
   for (int i = 0; i < KPT; ++i) {
-    const int slot = base + i * 64 + lane;
-    const bool in = slot < x.old, eq = in && !all && key[i] == top;
-    const uint64_t eqs = __ballot(eq);
-    const bool stay = in && (all || key[i] > top || (eq && tie + __popcll(eqs & before) < want));
-    const uint64_t stays = __ballot(stay);
-    if (stay) out[at + __popcll(stays & before)] = slot;
+    const uint64_t eqs = __ballot(key[i] == top);
+    uint64_t stays = __ballot(key[i] > top);
+    if (tie < want) {
+      const bool low = tie + (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(eqs >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)eqs, 0)) < want;
+      stays |= eqs & __ballot(low);
+      tie += __popcll(eqs);
+    }
+    if (stays >> lane & 1)
+      out[at + (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(stays >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)stays, 0))] =
+          first + wave * (KPT * 64) + i * 64 + lane;
     at += __popcll(stays);
-    tie += __popcll(eqs);
   }
 }
 
 template <int KPT>
 __global__ __launch_bounds__(1024) void kv_select_kernel(KvPages t, KvWeights w, int keep, int recent,
                                                          int32_t* __restrict__ slots, int32_t* __restrict__ new_lengths) {
-  __shared__ int counts[3][kBins];
+  __shared__ __align__(16) int counts[2][kBins][kCopies];
   __shared__ int sums[2][16], pick[3];
   const int h = blockIdx.x, b = blockIdx.y, tid = threadIdx.x;
+  Keys<KPT> keys;
+  keys.load_pages(t, b, 0);
   const Row x = row_of(t, b, keep, recent, tid == 0);
   int32_t* out = slots + ((int64_t)b * gridDim.x + h) * keep;
   if (h == 0 && tid == 0) new_lengths[b] = x.m;
   for (int i = tid; i < x.r; i += 1024) out[x.m - x.r + i] = x.old + i;
-  uint32_t key[KPT], top = 0, mask = 0;
+  uint32_t top = 0;
   int want = x.want;
   if (x.sort) {
-    for (int i = tid; i < 3 * kBins; i += 1024) counts[0][i] = 0;
-    load_keys<KPT>(t, w, b, h, 0, x.old, key);
+    keys.load_weights(t, w, h, 0, x.old);
+    clear_counts(counts[0]);
     __syncthreads();
+    keys.make(t, 0, x.old);
     bool all = false;
 #pragma unroll
     for (int k = 0; k < 3; ++k) {
       if (all) break;
-      count_digits<KPT>(key, 0, x.old, top, mask, kShift[k], counts[k]);
+      if (k < 2) clear_counts(counts[(k + 1) & 1]);  // (read two digits ago)
+      count_digits<KPT>(keys.key, k, top, counts[k & 1]);
       __syncthreads();
-      int d;
-      all = find_digit(counts[k], want, d, sums, pick);
+      int d, v[2];
+      my_digits(counts[k & 1], v);
+      all = find_digit(v, want, d, sums, pick);
       top |= (uint32_t)d << kShift[k];
-      mask = ~0u << kShift[k];
     }
     if (all) {  // every key that agrees with `top` stays, as one above it (no key is below 2^21, -inf's first digit)
       top -= 1;
       want = 0;
     }
   } else {
-#pragma unroll
-    for (int i = 0; i < KPT; ++i) key[i] = 0;
+    keys.make_all(0, x.old, x.n <= x.m);
+    want = 0;
   }
-  write_list<KPT>(key, x, 0, top, want, 0, 0, sums, out);
+  write_list<KPT>(keys.key, 0, top, want, 0, 0, sums, out);
 }
 
 // what the launches for long rows keep of a row
 struct Counts {
-  int* digits;  // [rows][parts][3][kBins]
+  uint32_t* digits;  // [rows][parts][3][kBins / 2]: counts of 16 bits (a part holds 32768 keys at most), the lower digit's first
   int* above;   // [rows][parts][2]: keys above the first digit, and at it but above the second
   int* pick;    // [rows][2][2]: digits found, and how many are wanted of what agrees with them (0: all of it)
   int parts;
 };
 
-// counts of bins tid and 1024 + tid of a digit: in all parts, and in those before `part`.  Eight parts' loads at a time
-// (8 rows of 131072 slots, 16 parts: launches of 11 to 13 us take 7 to 9).
+// counts of this thread's two digits (as my_digits): in all parts, and in those before `part`.  Sixteen parts' loads at a
+// time.
 __device__ __forceinline__ void sum_parts(const Counts& c, int64_t row, int digit, int parts, int part, int (&all)[2],
                                           int (&before)[2]) {
   all[0] = all[1] = before[0] = before[1] = 0;
-  const int* from = c.digits + (row * c.parts * 3 + digit) * kBins + threadIdx.x;
-  for (int p = 0; p < parts; p += 8) {
-    int v[8][2];
+  const uint32_t* from = c.digits + (row * c.parts * 3 + digit) * (kBins / 2) + kBins / 2 - 1 - threadIdx.x;
+  for (int p = 0; p < parts; p += 16) {
+    uint32_t v[16];
 #pragma unroll
-    for (int k = 0; k < 8; ++k)
+    for (int k = 0; k < 16; ++k) v[k] = from[(int64_t)min(p + k, parts - 1) * 3 * (kBins / 2)];
 #pragma unroll
-      for (int i = 0; i < 2; ++i) v[k][i] = from[(int64_t)min(p + k, parts - 1) * 3 * kBins + i * 1024];
-#pragma unroll
-    for (int k = 0; k < 8; ++k)
+    for (int k = 0; k < 16; ++k) {
+      const int n[2] = {(int)(v[k] >> 16), (int)(v[k] & 0xffffu)};
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        all[i] += p + k < parts ? v[k][i] : 0;
-        before[i] += p + k < part ? v[k][i] : 0;
+        all[i] += p + k < parts ? n[i] : 0;
+        before[i] += p + k < part ? n[i] : 0;
       }
+    }
   }
 }
 
 // counts of digit PASS of a part; PASS > 0: finds the digit before it first
 template <int KPT, int PASS>
 __global__ __launch_bounds__(1024) void kv_count_kernel(KvPages t, KvWeights w, int keep, int recent, Counts c) {
-  __shared__ int counts[kBins];
+  __shared__ __align__(16) int counts[kBins][kCopies];
   __shared__ int sums[2][16], pick[3];
-  const int part = blockIdx.x, h = blockIdx.y, b = blockIdx.z, tid = threadIdx.x;
+  const int part = blockIdx.x, h = blockIdx.y, b = blockIdx.z, tid = threadIdx.x, first = part * (KPT * 1024);
+  Keys<KPT> keys;
+  keys.load_pages(t, b, first);
   const Row x = row_of(t, b, keep, recent, false);
-  const int first = part * (KPT * 1024);
   if (!x.sort || first >= x.old) return;
   const int64_t row = (int64_t)b * gridDim.y + h;
   const int parts = (x.old - 1) / (KPT * 1024) + 1;
@@ -291,101 +331,94 @@ __global__ __launch_bounds__(1024) void kv_count_kernel(KvPages t, KvWeights w, 
     }
     return;
   }
-  uint32_t key[KPT], top = 0, mask = 0;
-  load_keys<KPT>(t, w, b, h, first, x.old, key);
+  uint32_t top = 0;
+  keys.load_weights(t, w, h, first, x.old);
+  clear_counts(counts);
   if constexpr (PASS > 0) {
     int v[2], mine[2];
     sum_parts(c, row, PASS - 1, parts, part, v, mine);
-    counts[tid] = v[0];
-    counts[1024 + tid] = v[1];
-    __syncthreads();
     int want = x.want, d;
     if (PASS == 2) {
       top = (uint32_t)c.pick[row * 4] << kShift[0];
       want = c.pick[row * 4 + 1];
     }
-    const bool all = find_digit(counts, want, d, sums, pick);
+    // this part's keys above the digit (all: and at it), among those that agree with the digits before
+    const uint32_t past = PASS == 2 ? top + (1u << kShift[0]) : 0u;
+    const bool all = find_digit(v, want, d, sums, pick);
+    keys.make(t, first, x.old);
     top |= (uint32_t)d << kShift[PASS - 1];
     if (part == 0 && tid == 0) {
       c.pick[row * 4 + 2 * (PASS - 1)] = d;
       c.pick[row * 4 + 2 * (PASS - 1) + 1] = all ? 0 : want;
     }
-    // this part's keys above (all: and at it), among those that agree with the digits before
-    const uint32_t agree = PASS == 1 ? 0u : ~0u << kShift[0];
-    mask = ~0u << kShift[PASS - 1];
+    const uint32_t least = all ? top : top + (1u << kShift[PASS - 1]);
     int na = 0;
 #pragma unroll
-    for (int i = 0; i < KPT; ++i) {
-      const bool in = first + (tid >> 6) * (KPT * 64) + i * 64 + (tid & 63) < x.old && (key[i] & agree) == (top & agree);
-      na += __popcll(__ballot(in && (key[i] & mask) > top - all));
-    }
+    for (int i = 0; i < KPT; ++i) na += __popcll(__ballot(keys.key[i] - least < past - least));
     if ((tid & 63) == 0) sums[1][tid >> 6] = na;
     __syncthreads();
-    if (tid == 0) {
-      int n = 0;
-      for (int i = 0; i < 16; ++i) n += sums[1][i];
-      c.above[(row * c.parts + part) * 2 + PASS - 1] = n;
-    }
+    if (tid == 0) c.above[(row * c.parts + part) * 2 + PASS - 1] = sum_before(sums[1], 16);
     if (all) return;
+  } else {
+    __syncthreads();
+    keys.make(t, first, x.old);
   }
-  counts[tid] = counts[1024 + tid] = 0;
+  count_digits<KPT>(keys.key, PASS, top, counts);
   __syncthreads();
-  count_digits<KPT>(key, first, x.old, top, mask, kShift[PASS], counts);
-  __syncthreads();
-#pragma unroll
-  for (int i = 0; i < 2; ++i) c.digits[((row * c.parts + part) * 3 + PASS) * kBins + i * 1024 + tid] = counts[i * 1024 + tid];
+  int n[2];
+  my_digits(counts, n);
+  c.digits[((row * c.parts + part) * 3 + PASS) * (kBins / 2) + kBins / 2 - 1 - tid] = (uint32_t)n[0] << 16 | (uint32_t)n[1];
 }
 
 template <int KPT>
 __global__ __launch_bounds__(1024) void kv_list_kernel(KvPages t, KvWeights w, int keep, int recent, Counts c,
                                                        int32_t* __restrict__ slots, int32_t* __restrict__ new_lengths) {
-  __shared__ int counts[kBins];
   __shared__ int sums[2][16], pick[3], before[2];
   const int part = blockIdx.x, h = blockIdx.y, b = blockIdx.z, tid = threadIdx.x;
+  const int first = part * (KPT * 1024);
+  Keys<KPT> keys;
+  keys.load_pages(t, b, first);
   const Row x = row_of(t, b, keep, recent, part == 0 && tid == 0);
   const int64_t row = (int64_t)b * gridDim.y + h;
   int32_t* out = slots + row * keep;
   if (part == 0 && h == 0 && tid == 0) new_lengths[b] = x.m;
   for (int i = part * 1024 + tid; i < x.r; i += gridDim.x * 1024) out[x.m - x.r + i] = x.old + i;
-  const int first = part * (KPT * 1024);
   if (first >= x.old) return;
-  uint32_t key[KPT], top = 0;
+  uint32_t top = 0;
   int want = x.want, at = first, tie = 0;  // (all stay: every slot before)
   if (x.sort) {
     const int parts = (x.old - 1) / (KPT * 1024) + 1;
-    load_keys<KPT>(t, w, b, h, first, x.old, key);
+    keys.load_weights(t, w, h, first, x.old);
     if (tid < 2) before[tid] = 0;
+    int na = 0;
+    for (int p = tid; p < part; p += 1024) na += c.above[(row * c.parts + p) * 2] + c.above[(row * c.parts + p) * 2 + 1];
     top = (uint32_t)c.pick[row * 4] << kShift[0] | (uint32_t)c.pick[row * 4 + 2] << kShift[1];
     want = c.pick[row * 4 + 3];
-    int na = 0;
     if (want == 0) {  // all that agrees with the digits found stays
       top -= 1;
       __syncthreads();
     } else {
       int v[2], mine[2], d;  // counts of the last digit
       sum_parts(c, row, 2, parts, part, v, mine);
-      counts[tid] = v[0];
-      counts[1024 + tid] = v[1];
-      __syncthreads();
-      find_digit(counts, want, d, sums, pick);
+      find_digit(v, want, d, sums, pick);
       top |= (uint32_t)d;
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        const int bin = i * 1024 + tid;
+        const int bin = kBins - 1 - 2 * tid - i;
         if (bin > d) na += mine[i];
         if (bin == d) before[1] = mine[i];
       }
     }
-    for (int p = tid; p < part; p += 1024) na += c.above[(row * c.parts + p) * 2] + c.above[(row * c.parts + p) * 2 + 1];
+    keys.make(t, first, x.old);
     if (na) atomicAdd(&before[0], na);  // (whole numbers: no order matters)
     __syncthreads();
     at = before[0];
     tie = before[1];
   } else {
-#pragma unroll
-    for (int i = 0; i < KPT; ++i) key[i] = 0;
+    keys.make_all(first, x.old, x.n <= x.m);
+    want = 0;
   }
-  write_list<KPT>(key, x, first, top, want, at, tie, sums, out);
+  write_list<KPT>(keys.key, first, top, want, at, tie, sums, out);
 }
 
 // Copies the slots that stay into the pages of `to`: 16 slots of a (key head, sequence) a workgroup, 16 bytes a thread.
@@ -464,7 +497,7 @@ DITK_EXPORT int64_t ditk_kv_evict_workspace(int batch, int kv_heads, int most, i
   if (batch <= 0 || kv_heads <= 0 || most < 0 || most >= (1 << 30) || keep <= 0) return 0;
   const int64_t rows = (int64_t)batch * kv_heads;
   const SelectPlan pl = select_plan(most);
-  return 4 * (rows * keep + (pl.parts > 1 ? rows * ((int64_t)pl.parts * (3 * kBins + 2) + 4) : 0));
+  return 4 * (rows * keep + (pl.parts > 1 ? rows * ((int64_t)pl.parts * (3 * kBins / 2 + 2) + 4) : 0));
 }
 
 DITK_EXPORT int ditk_kv_evict(void* k_cache, int64_t k_ps, int64_t k_hs, void* v_cache, int64_t v_ps, int64_t v_hs,
@@ -479,6 +512,7 @@ DITK_EXPORT int ditk_kv_evict(void* k_cache, int64_t k_ps, int64_t k_hs, void* v
   if (int rc = kv_check_tensor(what, k_cache, k_ps, k_hs, page, head_dim)) return rc;
   if (int rc = kv_check_tensor(what, v_cache, v_ps, v_hs, page, head_dim)) return rc;
   DITK_REQUIRE(weights != nullptr, "%s: the cache has no weights", what);
+  DITK_REQUIRE(w_ps >= 0 && w_ps < (1ll << 32), "%s: the weights' pages are too far apart", what);
   DITK_REQUIRE(keep > 0 && recent >= 0 && recent <= keep && max_len >= 0, "%s: bad keep %d, recent %d or max_len %d",
                what, keep, recent, max_len);
   if (batch == 0) return 0;
@@ -503,9 +537,9 @@ DITK_EXPORT int ditk_kv_evict(void* k_cache, int64_t k_ps, int64_t k_hs, void* v
     if (int rc = ditk_check_launch(what)) return rc;
   } else {
     Counts c;
-    c.digits = slots + rows * keep;
-    c.above = c.digits + rows * pl.parts * 3 * kBins;
+    c.above = slots + rows * keep;
     c.pick = c.above + rows * pl.parts * 2;
+    c.digits = (uint32_t*)(c.pick + rows * 4);
     c.parts = pl.parts;
     const dim3 grid(pl.parts, kv_heads, batch);
     const bool few = pl.kpt == 8;

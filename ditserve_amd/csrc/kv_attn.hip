@@ -106,11 +106,7 @@ __global__ __launch_bounds__(256, 2) void kv_attn_kernel(Args a) {
       if (i == 0) lens[tid] = n;
       incl += chunks_of(n);
     }
-#pragma unroll
-  for (int off = 1; off < 64; off <<= 1) {
-    const int o = __shfl_up(incl, off, 64);
-    if (lane >= off) incl += o;
-  }
+  incl = wave_scan(incl);
   if (lane == 63) sums[wave] = incl;
   __syncthreads();
   for (int w = 0; w < wave; ++w) incl += sums[w];

@@ -51,10 +51,10 @@ def test_attn_refuses(change, word):
 
 
 @pytest.mark.parametrize("change,word", COMMON + [
-    (dict(w=None), "no weights"), (dict(keep=0), "keep"), (dict(recent=-1), "recent"), (dict(recent=33), "recent"),
+    (dict(w=None), "no weights"), (dict(w_ps=1 << 32), "too far"), (dict(keep=0), "keep"), (dict(recent=-1), "recent"), (dict(recent=33), "recent"),
     (dict(max_len=-1), "max_len"), (dict(out_table=None), "null table"), (dict(out_width=1), "32 stay"),
     (dict(new=None), "null output"), (dict(space=None), "null output"), (dict(space=A + 8), "null output"),
-    (dict(size=4 * 2 * 2 * 32 - 4), "workspace"), (dict(width=4096, ldt=4096, max_len=65536, size=1 << 19), "workspace")])
+    (dict(size=4 * 2 * 2 * 32 - 4), "workspace"), (dict(width=4096, ldt=4096, max_len=65536, size=1 << 18), "workspace")])
 def test_evict_refuses(change, word):
     refused("ditk_kv_evict", tuple({**EVICT, **change}.values()), word)
 
