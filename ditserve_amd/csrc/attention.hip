@@ -589,24 +589,24 @@ int item_queries(int Tq, int nseg, int heads, int np, bool equal) {
 }
 
 // Queries per work item of a causal launch, 128 or 256, whichever a time model says is done first (the choice changes no
-// result).  An item of one block a wave takes about 9 us and 0.85 a key tile (head_dim 64: 0.6), one of two 10 and 1.5
-// (0.95) or, while the CUs are not all busy, 1.18 (0.75): its start, Q's load and O's store are not hidden, and with all
-// CUs busy the matrix clock falls.  The longest run first, so a launch ends after its work divided by the CUs, plus what
-// the last round lacks of a whole one, or with its longest item.  Only totals are known here: segments count as equal.
-// 32 heads over 8: 1024 queries 24.9 us by 128 and 32.6 by 256, 2048 51.6 and 55.7, 4096 155 and 130; 8 of 2841 in all
-// 49.4 and 45.2; 512 after 8000 keys 120 and 157; head_dim 64, 8 heads, 16000 queries 337 and 262.
+// result).  An item of one block a wave takes 6 us (its launch, the first loads, the epilogue) and 0.93 a key tile while
+// all CUs are busy, 0.78 with few of them; one of two blocks 7.5 and 1.55 or 1.0 (head_dim 64: 4.5, 0.65 and 0.6; 5.3,
+// 0.95 and 0.7).  The longest run first: whole rounds of the CUs at the mean, then what is left of a round at the shortest
+// items' length, but no less than the longest item.  Only totals are known here: segments count as equal.
+// Measured, 128 and 256: 32 heads over 8, 1024 queries 22.4 us and 30.8, 2048 48.0 and 51.5, 4096 152 and 123; 8 of 355
+// 34.5 and 35.1; 512 after 7488 keys 107 and 147; two of 1024 after 6001 with 40 heads 297 and 283; 40 of 300 with 12
+// heads 58.7 and 66.0; head_dim 64, 32 heads: 2048 36.2 and 37.8, 4096 112 and 79.
 int causal_item_queries(int Tq, int Tk, int nseg, int heads, int head_dim) {
   const double ncu = ditk_cu_count(), n = (double)Tq / nseg, ahead = Tk > Tq ? (double)(Tk - Tq) / nseg : 0.0;
   auto time = [&](double bm, double start, double busy, double light) {
-    const double tiles = std::ceil(n / bm), items = tiles * heads * nseg;
-    const double tile = items > ncu ? busy : light;
-    const double least = start + tile * std::ceil((ahead + std::min(bm, n)) / BN);
-    const double most = std::ceil((ahead + n) / BN), longest = start + tile * most;
-    const double rounds = items / ncu;
-    return std::max(start + light * most, rounds * (least + longest) / 2 + (std::ceil(rounds) - rounds) * least);
+    const double rounds = std::ceil(n / bm) * heads * nseg / ncu, whole = std::floor(rounds), rest = rounds - whole;
+    const double least = std::ceil((ahead + std::min(bm, n)) / BN), most = std::ceil((ahead + n) / BN);
+    const double tail = rest > 0 ? start + (light + (busy - light) * rest) * least : 0.0;
+    const double longest = start + (light + (busy - light) * (whole > 0 ? 0.5 : rest)) * most;
+    return std::max(longest, whole * (start + busy * (least + most) / 2) + tail);
   };
-  const bool wide = head_dim == 128;
-  return time(128, 9, wide ? 0.85 : 0.6, wide ? 0.85 : 0.6) <= time(256, 10, wide ? 1.5 : 0.95, wide ? 1.18 : 0.75) ? 128 : 256;
+  return head_dim == 128 ? (time(128, 6, 0.93, 0.78) <= time(256, 7.5, 1.55, 1.0) ? 128 : 256)
+                         : (time(128, 4.5, 0.65, 0.6) <= time(256, 5.3, 0.95, 0.7) ? 128 : 256);
 }
 
 // shared checks and launch of both attention entry points; sl2 = the factor that
