@@ -261,28 +261,49 @@ __device__ __forceinline__ float row_lse2(float m, float l) {
   return l > 0.f || l != l ? m + __builtin_amdgcn_logf(l) : -INFINITY;
 }
 
+// Factors of two neighbouring parts, and the top and l of their sum.  (A part without a finite score is 0, or NaN and stays
+// it.)  Parts are joined in such pairs first, wherever that is done, by these operations.
+struct Pair {
+  float m, l, fa, fb;
+};
+__device__ __forceinline__ Pair join_pair(float ma, float la, float mb, float lb) {
+  Pair p;
+  p.m = fmaxf(ma, mb);
+  p.fa = ma == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(ma - p.m);
+  p.fb = mb == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(mb - p.m);
+  p.l = fmaf(lb, p.fb, la * p.fa);
+  return p;
+}
+__device__ __forceinline__ f32x4_t join_pair(const Pair& p, f32x4_t a, f32x4_t b) {
+  f32x4_t y;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) y[e] = fmaf(b[e], p.fb, a[e] * p.fa);
+  return y;
+}
+
 // Joins the parts of eight waves, a wave's 16 rows of HD + 4 floats in `lds` and its m and l in stat[0..1][row][wave]:
-// the sum of four dims from d on of row r, its top and its l.  Products are rounded, then added in order.  (A part
-// without a finite score is 0, or NaN and stays it.)
+// the sum of four dims from d on of row r, its top and its l.  Products are rounded, then added in order.
 template <int HD>
 __device__ __forceinline__ f32x4_t join8(const float* lds, const float (*stat)[16][8], int r, int d, float& top, float& lt) {
 #pragma clang fp contract(off)
-  float m[8], l[8];
+  Pair p[4];
   top = -INFINITY;
 #pragma unroll
-  for (int c = 0; c < 8; ++c) {
-    m[c] = stat[0][r][c];
-    top = fmaxf(top, m[c]);
+  for (int c = 0; c < 4; ++c) {
+    p[c] = join_pair(stat[0][r][2 * c], stat[1][r][2 * c], stat[0][r][2 * c + 1], stat[1][r][2 * c + 1]);
+    top = fmaxf(top, p[c].m);
   }
   f32x4_t y = {0.f, 0.f, 0.f, 0.f};
+  float l[4];
 #pragma unroll
-  for (int c = 0; c < 8; ++c) {
-    const float f = m[c] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(m[c] - top);
-    l[c] = stat[1][r][c] * f;
-    const f32x4_t z = *reinterpret_cast<const f32x4_t*>(lds + (c * 16 + r) * (HD + 4) + d);
+  for (int c = 0; c < 4; ++c) {
+    const float f = p[c].m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(p[c].m - top);
+    l[c] = p[c].l * f;
+    const float* at = lds + (c * 2 * 16 + r) * (HD + 4) + d;
+    const f32x4_t z = join_pair(p[c], *reinterpret_cast<const f32x4_t*>(at), *reinterpret_cast<const f32x4_t*>(at + 16 * (HD + 4)));
 #pragma unroll
     for (int e = 0; e < 4; ++e) y[e] += z[e] * f;
   }
-  lt = ((l[0] + l[4]) + (l[2] + l[6])) + ((l[1] + l[5]) + (l[3] + l[7]));  // wave_sum's order of eight lanes
+  lt = (l[0] + l[2]) + (l[1] + l[3]);  // wave_sum's order of four lanes
   return y;
 }

@@ -40,6 +40,7 @@ struct Args {
   float* lse2;    // [batch * heads] log2 units, for the weights
   float* part;    // [batch * heads][nchunk][HD]
   float* ml;      // [batch * heads][nchunk][2]
+  int* twos;      // whether parts are of two chunks each
   float* score;   // [batch * heads][ld_score], or null
   int64_t ld_score;
   int heads, group, nchunk, batch, hgroups;  // hgroups: (key head, 16 of its query heads) pairs
@@ -89,28 +90,40 @@ __device__ __forceinline__ void store_lse(const Args& a, int64_t row, float e, b
 
 // A wave takes one chunk of one (sequence, key head, 16 query heads) after another; units go round the waves in
 // order: a sequence's chunks, and for each its heads, which lie side by side in a page.
+//
+// With two chunks or more a wave, units are two neighbouring chunks and leave one part, joined as the join kernel joins
+// the parts of two (the bits are the same): half as much is written and read again (4 KB for 128 slots of 8 query heads,
+// 64 KB of keys and values).  32 heads over 8: 64 sequences of 2000 slots 107 -> 96 us, 256 437 -> 402, 16 of 32768 398
+// -> 363; with fewer units waves would stand idle (64 ragged ones 51 and 58), and where scores are written nothing is won
+// (16 of 32768 470 and 475).
 template <int HD, bool SCORES>
 __global__ __launch_bounds__(256, 2) void kv_attn_kernel(Args a) {
   using C = Chunk<HD, false>;
   __shared__ __align__(256) char lds[4 * 32 * HD * 2];
-  __shared__ int sums[4], ends[256], lens[256];
+  __shared__ int sums[2][4], ends[256], lens[256];
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6), lane = tid & 63;
   const int col = lane & 15, quad = lane >> 4;
 
   // chunks up to and with thread t's sequences, [t per, t per + per)
   const int per = (a.batch + 255) / 256;
-  int incl = 0;
+  int incl = 0, pairs = 0;
   for (int i = 0; i < per; ++i)
     if (tid * per + i < a.batch) {
-      const int n = kv_length(a.t, tid * per + i, blockIdx.x == 0);
+      const int n = kv_length(a.t, tid * per + i, blockIdx.x == 0), nch = chunks_of(n);
       if (i == 0) lens[tid] = n;
-      incl += chunks_of(n);
+      incl += nch;
+      pairs += (nch + 1) >> 1;
     }
   incl = wave_scan(incl);
-  if (lane == 63) sums[wave] = incl;
+  pairs = wave_scan(pairs);
+  if (lane == 63) sums[0][wave] = incl, sums[1][wave] = pairs;
   __syncthreads();
-  for (int w = 0; w < wave; ++w) incl += sums[w];
+  const int chunks = (sums[0][0] + sums[0][1]) + (sums[0][2] + sums[0][3]);
+  const int two = !SCORES && (int64_t)chunks * a.hgroups >= (int64_t)gridDim.x * 4 * 2;  // 1: units of two chunks
+  if (two) incl = pairs;
+  for (int w = 0; w < wave; ++w) incl += sums[two][w];
   ends[tid] = incl;
+  if (blockIdx.x == 0 && tid == 0) *a.twos = two;
   __syncthreads();
   int end[4];  // (every wave keeps all of them)
 #pragma unroll
@@ -119,28 +132,37 @@ __global__ __launch_bounds__(256, 2) void kv_attn_kernel(Args a) {
 
   for (int u = blockIdx.x * 4 + wave; u < units; u += gridDim.x * 4) {
     const int c = u / a.hgroups, hg = u - c * a.hgroups;
-    // the thread whose sequences hold chunk c, then the sequence
+    // the thread whose sequences hold unit c, then the sequence
     int th = 0;
 #pragma unroll
     for (int i = 0; i < 4; ++i) th += __popcll(__ballot(end[i] <= c));
-    int b = th * per, chunk = c - (th ? ends[th - 1] : 0), n = lens[th], nch = chunks_of(n);
-    while (chunk >= nch && b + 1 < a.batch) {
-      chunk -= nch;
+    int b = th * per, part = c - (th ? ends[th - 1] : 0), n = lens[th], nch = chunks_of(n);
+    while (part >= (nch + two) >> two && b + 1 < a.batch) {
+      part -= (nch + two) >> two;
       n = kv_length(a.t, ++b, false);
       nch = chunks_of(n);
     }
     b = __builtin_amdgcn_readfirstlane(b);
     n = __builtin_amdgcn_readfirstlane(n);
-    chunk = __builtin_amdgcn_readfirstlane(min(chunk, a.nchunk - 1));
+    part = __builtin_amdgcn_readfirstlane(min(part, (a.nchunk - 1) >> two));
     const int kvh = hg / groups, g0 = (hg - kvh * groups) * 16;
-    const int csl = chunk_slots(n), s0 = chunk * csl, s1 = min(n, s0 + csl);
+    const int csl = chunk_slots(n), s0 = (part << two) * csl, s1 = min(n, s0 + csl), s2 = two ? min(n, s1 + csl) : s1;
     const int nq = min(a.group - g0, 16), head0 = kvh * a.group + g0;  // query heads of this unit
     const int64_t row = (int64_t)b * a.heads + head0 + min(col, nq - 1);
     C x;
     PagedSrc<HD, !SCORES> src{a, b, kvh, max(n - 1, 0)};
-    x.run(src, a.q + b * a.ldq + (int64_t)(head0 + min(col, nq - 1)) * HD + quad * 8, a.scale2, s0, s1,
-                          n, n, SCORES && col < nq ? a.score + row * a.ld_score : nullptr,
-                          lds + wave * (32 * HD * 2));
+    x.run(src, a.q + b * a.ldq + (int64_t)(head0 + min(col, nq - 1)) * HD + quad * 8, a.scale2, s0, s1, n, n,
+          SCORES && col < nq ? a.score + row * a.ld_score : nullptr, lds + wave * (32 * HD * 2));
+    if (!SCORES && s1 < s2) {
+      const C y = x;
+      x.run(src, a.q + b * a.ldq + (int64_t)(head0 + min(col, nq - 1)) * HD + quad * 8, a.scale2, s1, s2, n, n, nullptr,
+            lds + wave * (32 * HD * 2));
+      const Pair p = join_pair(y.m, y.l, x.m, x.l);
+      x.m = p.m;
+      x.l = p.l;
+#pragma unroll
+      for (int j = 0; j < C::ND; ++j) x.o[j] = join_pair(p, y.o[j], x.o[j]);
+    }
     if (col < nq) {
       if (nch == 1) {
         const float inv = inverse(x.l);
@@ -151,10 +173,10 @@ __global__ __launch_bounds__(256, 2) void kv_attn_kernel(Args a) {
                                                             pack_bf2(x.o[j][2] * inv, x.o[j][3] * inv)};
         if (quad == 0) store_lse(a, row, row_lse2(x.m, x.l), SCORES);
       } else {
-        float* pb = a.part + (row * a.nchunk + chunk) * HD + quad * 4;
+        float* pb = a.part + (row * a.nchunk + part) * HD + quad * 4;
 #pragma unroll
         for (int j = 0; j < C::ND; ++j) *reinterpret_cast<f32x4_t*>(pb + j * 16) = x.o[j];
-        if (quad == 0) *reinterpret_cast<u32x2_t*>(a.ml + (row * a.nchunk + chunk) * 2) =
+        if (quad == 0) *reinterpret_cast<u32x2_t*>(a.ml + (row * a.nchunk + part) * 2) =
             u32x2_t{__float_as_uint(x.m), __float_as_uint(x.l)};
       }
     }
@@ -202,12 +224,13 @@ __global__ __launch_bounds__(512) void kv_attn_short_kernel(Args a) {
   }
 }
 
-// Joins the chunks of one query head.  HD / 4 threads add up every SUB-th chunk, 16 bytes each, and the SUB sums are
-// added in order: the order goes by the row's own chunks alone.  (A part without a finite score is 0, or NaN and stays it.)
+// Joins the parts of one query head: those of two chunks as units of two leave them, or two at a time.  HD / 4 threads add
+// up every SUB-th, 16 bytes each, and the SUB sums are added in order: the order goes by the row's own chunks alone.
 template <int HD, bool SCORES>
 __global__ __launch_bounds__(256) void kv_join_kernel(Args a) {
   constexpr int TPR = HD / 4, SUB = 256 / TPR;
-  __shared__ float f[kMaxChunks];
+  static_assert(kMaxChunks == 2 * 256, "a pair of chunks a thread");
+  __shared__ float f[256], fa[256], fb[256];
   __shared__ float red[2][4];
   __shared__ __align__(16) float acc[SUB][HD];
   const int head = blockIdx.x, b = blockIdx.y, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -215,37 +238,54 @@ __global__ __launch_bounds__(256) void kv_join_kernel(Args a) {
   if (nch == 1) return;
   const int64_t row = (int64_t)b * a.heads + head;
   const float* ml = a.ml + row * a.nchunk * 2;
-  float mc[kMaxChunks / 256], lc[kMaxChunks / 256], top = -INFINITY;
-#pragma unroll
-  for (int i = 0; i < kMaxChunks / 256; ++i) {
-    const int c = i * 256 + tid;
-    mc[i] = c < nch ? ml[2 * c] : -INFINITY;
-    lc[i] = c < nch ? ml[2 * c + 1] : 0.f;
-    top = fmaxf(top, mc[i]);
+  const int np = (nch + 1) >> 1, odd = nch & 1;  // pairs; whether the last is one chunk
+  // (both places are read before the word that says which counts is there)
+  const int last = nch - 1, at0 = min(tid, last), at1 = min(2 * tid, last), at2 = min(2 * tid + 1, last);
+  const u32x2_t e0 = *reinterpret_cast<const u32x2_t*>(ml + 2 * at0), e1 = *reinterpret_cast<const u32x2_t*>(ml + 2 * at1),
+                e2 = *reinterpret_cast<const u32x2_t*>(ml + 2 * at2);
+  const bool two = *a.twos != 0;
+  Pair p{-INFINITY, 0.f, 1.f, 0.f};
+  if (tid < np) {
+    p.m = __uint_as_float(two ? e0[0] : e1[0]);
+    p.l = __uint_as_float(two ? e0[1] : e1[1]);
+    if (!two && !(odd && tid == np - 1)) p = join_pair(p.m, p.l, __uint_as_float(e2[0]), __uint_as_float(e2[1]));
   }
-  top = wave_max<64>(top);
+  fa[tid] = p.fa;
+  fb[tid] = p.fb;
+  float top = wave_max<64>(p.m);
   if (lane == 0) red[0][wave] = top;
   __syncthreads();
   top = fmaxf(fmaxf(red[0][0], red[0][1]), fmaxf(red[0][2], red[0][3]));
-  float lt = 0.f;
-#pragma unroll
-  for (int i = 0; i < kMaxChunks / 256; ++i) {
-    const float fc = mc[i] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(mc[i] - top);
-    f[i * 256 + tid] = fc;
-    lt += lc[i] * fc;
-  }
-  lt = wave_sum<64>(lt);
+  const float fc = p.m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(p.m - top);
+  f[tid] = fc;
+  float lt = wave_sum<64>(fmaf(p.l, fc, 0.f));  // (a rounded product)
   if (lane == 0) red[1][wave] = lt;
   __syncthreads();
   lt = red[1][0] + red[1][1] + red[1][2] + red[1][3];
   const int sub = tid / TPR, d = (tid % TPR) * 4;
   const float* part = a.part + row * a.nchunk * HD + d;
   f32x4_t x = {0.f, 0.f, 0.f, 0.f};
+  if (two) {
 #pragma unroll 8
-  for (int c = sub; c < nch; c += SUB) {
-    const f32x4_t y = *reinterpret_cast<const f32x4_t*>(part + (int64_t)c * HD);
+    for (int c = sub; c < np; c += SUB) {
+      const f32x4_t y = *reinterpret_cast<const f32x4_t*>(part + (int64_t)c * HD);
 #pragma unroll
-    for (int r = 0; r < 4; ++r) x[r] += y[r] * f[c];
+      for (int r = 0; r < 4; ++r) x[r] = fmaf(y[r], f[c], x[r]);
+    }
+  } else {
+#pragma unroll 4
+    for (int c = sub; c < nch >> 1; c += SUB) {
+      const f32x4_t ya = *reinterpret_cast<const f32x4_t*>(part + (int64_t)(2 * c) * HD);
+      const f32x4_t yb = *reinterpret_cast<const f32x4_t*>(part + (int64_t)(2 * c + 1) * HD);
+      const f32x4_t y = join_pair(Pair{0.f, 0.f, fa[c], fb[c]}, ya, yb);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) x[r] = fmaf(y[r], f[c], x[r]);
+    }
+    if (odd && (np - 1) % SUB == sub) {
+      const f32x4_t y = *reinterpret_cast<const f32x4_t*>(part + (int64_t)last * HD);
+#pragma unroll
+      for (int r = 0; r < 4; ++r) x[r] = fmaf(y[r], f[np - 1], x[r]);
+    }
   }
   *reinterpret_cast<f32x4_t*>(&acc[sub][d]) = x;
   __syncthreads();
@@ -283,20 +323,22 @@ __global__ __launch_bounds__(256) void kv_weights_kernel(Args a, int add) {
     if (i + r < n) w[r] = add ? w[r] + sum[r] : sum[r];
 }
 
-// floats of the workspace's parts, each a multiple of 4
+// floats of the workspace's parts, each a multiple of 64 (scores are written in whole lines: 16 bytes off one, 16 x 32768
+// slots took 457 us for 443)
 struct Space {
-  int64_t part, ml, lse2, score, ld_score;
-  int64_t floats() const { return part + ml + lse2 + score; }
+  int64_t part, ml, twos, lse2, score, ld_score;
+  int64_t floats() const { return part + ml + twos + lse2 + score; }
 };
 Space space_of(int batch, int heads, int head_dim, int most, bool weights) {
   const int64_t rows = (int64_t)batch * heads, nc = chunks_bound(most);
   Space s{};
   if (nc > kShortChunks) {
     s.part = rows * nc * head_dim;
-    s.ml = (rows * nc * 2 + 3) & ~(int64_t)3;
+    s.ml = (rows * nc * 2 + 63) & ~(int64_t)63;
+    s.twos = 64;
   }
   if (weights) {
-    s.lse2 = (rows + 3) & ~(int64_t)3;
+    s.lse2 = (rows + 63) & ~(int64_t)63;
     s.ld_score = (most + 31) & ~31;
     s.score = rows * s.ld_score;
   }
@@ -343,7 +385,8 @@ DITK_EXPORT int ditk_kv_attn(const void* q, int64_t ldq, const void* k_cache, in
   a.lse = lse;
   a.part = (float*)workspace;
   a.ml = a.part + sp.part;
-  a.lse2 = a.ml + sp.ml;
+  a.twos = (int*)(a.ml + sp.ml);
+  a.lse2 = a.ml + sp.ml + sp.twos;
   a.score = a.lse2 + sp.lse2;
   a.ld_score = sp.ld_score;
   a.heads = heads;

@@ -86,6 +86,26 @@ def test_decode_layouts_and_batches(layout, d, page):
         assert torch.equal(alone[0], out[b])
 
 
+@pytest.mark.parametrize("batch,heads,hk,d,page", [(72, 16, 8, 64, 16), (100, 40, 2, 128, 64), (300, 8, 8, 64, 32)])
+def test_decode_of_many(batch, heads, hk, d, page):
+    """More chunks than waves: each sequence bitwise what it is alone; lengths around those of a chunk, of two and of none."""
+    some = [1100, 128 * 9, 128 * 9 + 1, 1025, 1024, 64 * 3, 65, 64, 1, 0, 2000, 128 * 14, 128 * 14 + 31, 8192, 8193]
+    lens = [some[i % len(some)] if i % 3 == 0 else 1300 + 7 * i % 640 for i in range(batch)]
+    cache, table, lengths, keys, values = paged(lens, hk, d, page, batch)
+    cache.v[table[3, 0].long(), 0, 5, 7] = math.inf
+    q = queries(batch, heads, d, 8)
+    out, lse = kv.decode_attn(q, cache, table, lengths, heads, return_lse=True)
+    kv.check_tables()
+    picked = [i for i in range(batch) if i != 3 and i % 3 == 0][:24] + [1, batch - 2]
+    pick = torch.tensor(picked, device=DEV)
+    check_decode(q[pick], cache, [lens[i] for i in picked], [keys[i] for i in picked], [values[i] for i in picked], heads,
+                 out[pick], lse[pick])
+    assert bool((out[3].view(hk, heads // hk, d)[0, :, 7] == math.inf).all()) and int(torch.isfinite(out[3]).sum()) == heads * d - heads // hk
+    for b in {3, *picked}:
+        alone, e = kv.decode_attn(q[b:b + 1], cache, table[b:b + 1], lengths[b:b + 1], heads, return_lse=True)
+        assert torch.equal(alone[0], out[b]) and torch.equal(e[0], lse[b])
+
+
 def test_decode_infinite_values():
     """An infinite value of a slot that is held is infinite in the output, one of a slot that is not stays out."""
     cache, table, lengths, _, _ = paged([40, 300], 1, 128, 16, 3)
