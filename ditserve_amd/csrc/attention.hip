@@ -41,6 +41,16 @@
 // operand (text tokens) — for Q, K and O alike, so SD3.5's image and text
 // projections feed joint attention, and take its output, without a gather or
 // scatter copy.  Results are bitwise those of the gathered layout.
+//
+// CAUSAL (plain q): a segment's queries are the last of its keys, query i of nq sees the keys
+// j <= i + nk - nq, and `group` query heads read one key head.  Work is cut as above; a work item's
+// key loop ends behind the last key that one of its queries sees, and only the tiles that some
+// query of a wave does not see whole take a mask, out of line: 2 vector operations a score, 2 or 3
+// tiles an item.  V is staged as rows, like K, and read by transposing LDS reads: a transposed copy was a
+// launch of its own (77 keys 5 of 12 us).  The matrix pipe bounds long prompts (16384 queries,
+// 32 heads of 128 over 8: 1.76 ms, 1.25 PFLOP/s of what is seen, at the clock that the power leaves), a
+// work item's start and end short ones (6 us of 10 for 128 queries).  Segments of few queries
+// over many keys go to causal_few.hip.
 #include <algorithm>
 #include <cmath>
 #include <mutex>

@@ -2,6 +2,9 @@
 //
 // The rows of a key head are its (query, query head) pairs.  A wave takes a chunk of a segment's keys for 16 rows of a key
 // head (attn_chunk.h) and leaves its part in a workspace; a second kernel joins them in the chunks' order.
+//
+// 32 heads over 8 of 128: 16 queries after 8192 keys 25 + 10 us, the latency of a chunk's tiles and of the join's parts;
+// 32 segments of 4 after 4000 106 + 10 (4.9 TB/s), memory.
 #include "attn_chunk.h"
 #include "causal_few.h"
 

@@ -26,7 +26,8 @@ namespace {
 constexpr int kCuLds = 1024;
 
 // Rows of new keys and values into the slots behind each sequence's last: row i of segment b goes to slot lengths[b] + i.
-// A thread moves 16 bytes of K and of V; `per` of them make a row.
+// A thread moves 16 bytes of K and of V; `per` of them make a row.  Memory bounds it: 16384 rows of 8 heads of 128, 134 MB
+// read and written, 28 us (4.8 TB/s); one row each of 64 sequences 3.5 us, a launch and three reads after one another.
 template <int LOG_CH>
 __global__ __launch_bounds__(256) void kv_append_kernel(KvPages t, KvTensor kc, KvTensor vc, KvWeights w,
                                                         const bf16_t* __restrict__ k, int64_t ldk,

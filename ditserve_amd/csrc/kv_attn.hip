@@ -3,6 +3,10 @@
 //
 // The query heads of a key head, 16 at a time, are the columns of a wave's products (attn_chunk.h).  A chunk's length
 // goes by the sequence's own length alone, so a sequence's result does not depend on what it is batched with.
+//
+// Each slot is read once and gives 2 operations a byte and query head: memory bounds it.  32 heads over 8 of 128: 16
+// sequences of 32768 slots 360 us (5.9 TB/s), 64 of 2000 90 (5.8), one of 131072 (40 heads) 89 (6.0); where few waves
+// have a unit each, the latency of a chunk's tiles: one of 8192 14 us.
 #include "attn_chunk.h"
 #include "kv_common.h"
 
@@ -184,7 +188,8 @@ __global__ __launch_bounds__(256, 2) void kv_attn_kernel(Args a) {
 }
 
 // Sequences of up to 8 chunks in one launch: eight waves take a chunk each of a (sequence, key head, 16 query heads) and
-// join them through LDS, by the join kernel's operations in its order.
+// join them through LDS, by the join kernel's operations in its order.  One sequence of 500 slots, 12 heads over 2: 9 us,
+// the latency of lengths, pages, two tiles and the join.
 template <int HD, bool SCORES>
 __global__ __launch_bounds__(512) void kv_attn_short_kernel(Args a) {
   using C = Chunk<HD, false>;
@@ -301,6 +306,7 @@ __global__ __launch_bounds__(256) void kv_join_kernel(Args a) {
 }
 
 // Weights of a key head's slots: the probabilities summed over its query heads, in their order.  Four slots a thread.
+// Memory: 80 MB of scores and weights of 16 x 32768 slots 17 us (4.7 TB/s).
 __global__ __launch_bounds__(256) void kv_weights_kernel(Args a, int add) {
   const int b = blockIdx.z, kvh = blockIdx.y, i = (blockIdx.x * 256 + threadIdx.x) * 4;
   const int n = kv_length(a.t, b, false);
