@@ -507,6 +507,7 @@ int64_t ditk_kv_attn_workspace(int batch, int heads, int head_dim, int most, int
  * kv_heads) over its slots: o [batch, heads * head_dim] bf16, lse [batch][heads] fp32 natural log
  * (may be NULL).  weights not NULL: the probabilities of each slot, summed over the query heads of
  * its key head, are written there (add != 0: added).  workspace: 16-byte aligned, this call's alone.
+ * batch * heads is less than 2^22.
  */
 int ditk_kv_attn(const void* q, int64_t ldq, const void* k_cache, int64_t k_ps, int64_t k_hs, const void* v_cache,
                  int64_t v_ps, int64_t v_hs, float* weights, int64_t w_ps, int64_t w_hs, int add, int pages, int page,
@@ -520,6 +521,7 @@ int ditk_kv_attn(const void* q, int64_t ldq, const void* k_cache, int64_t k_ps, 
  * order, with their weights, into the first slots of out_table's pages (other pages than
  * table's; out_width * page >= min(keep, width * page, max_len)).  workspace: 16-byte aligned, this
  * call's alone, of ditk_kv_evict_workspace bytes (most: the smaller of width * page and max_len).
+ * w_ps is less than 2^32.
  */
 int64_t ditk_kv_evict_workspace(int batch, int kv_heads, int most, int keep);
 int ditk_kv_evict(void* k_cache, int64_t k_ps, int64_t k_hs, void* v_cache, int64_t v_ps, int64_t v_hs,
