@@ -9,7 +9,7 @@ int kv_check_pages(const char* what, const void* table, const void* lengths, con
   DITK_REQUIRE(page == 16 || page == 32 || page == 64 || page == 128 || page == 256,
                "%s: a page holds 16, 32, 64, 128 or 256 slots, got %d", what, page);
   DITK_REQUIRE(pages > 0, "%s: the cache has no pages", what);
-  DITK_REQUIRE(status != nullptr && (batch == 0 || (table && lengths)), "%s: null table", what);
+  DITK_REQUIRE(status != nullptr && (batch == 0 || ((table || width == 0) && lengths)), "%s: null table", what);
   DITK_REQUIRE(width >= 0 && ldt >= width && (int64_t)width * page < (1ll << 30), "%s: bad page table", what);
   return 0;
 }

@@ -188,6 +188,23 @@ def test_append(before, counts, hk, d, page, layout):
         assert torch.equal(get(cache.k, table[0], after[0])[-1], k.reshape(T, hk, d)[0])
 
 
+def test_tables_without_pages():
+    """No columns: nothing is held, written or moved."""
+    cache = kv.PagedCache.empty(2, 2, 64, 16, DEV)
+    before = cache.k.clone()
+    none, zero = torch.empty((3, 0), dtype=torch.int32, device=DEV), torch.zeros(3, dtype=torch.int32, device=DEV)
+    q = queries(3, 4, 64, 1)
+    for weights in (None, "set", "add"):
+        out, lse = kv.decode_attn(q, cache, none, zero, 4, weights=weights, return_lse=True)
+        assert not out.any() and bool((lse == -math.inf).all())
+    assert kv.evict(cache, none, zero, none.clone(), 4).tolist() == [0, 0, 0]
+    kv.check_tables()
+    assert kv.append(cache, q[:, :128], q[:, 128:], none, zero).tolist() == [0, 0, 0]
+    with pytest.raises(_lib.DitkError):
+        kv.check_tables()
+    assert torch.equal(cache.k.view(torch.int16), before.view(torch.int16))
+
+
 def test_overlapping_operands_are_refused():
     pages, hk, page, d = 6, 2, 16, 64
     x = torch.zeros((pages, 2 * hk, page, d), dtype=torch.bfloat16, device=DEV)
