@@ -31,6 +31,26 @@ __device__ __forceinline__ float group_sumf(float v) {
 
 typedef short s16x4 __attribute__((ext_vector_type(4)));
 
+// Factors of two neighbouring parts, and the top and l of their sum.  (A part without a finite score is 0, or NaN and stays
+// it.)  Parts are joined in such pairs first, wherever that is done, by these operations.
+struct Pair {
+  float m, l, fa, fb;
+};
+__device__ __forceinline__ Pair join_pair(float ma, float la, float mb, float lb) {
+  Pair p;
+  p.m = fmaxf(ma, mb);
+  p.fa = ma == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(ma - p.m);
+  p.fb = mb == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(mb - p.m);
+  p.l = fmaf(lb, p.fb, la * p.fa);
+  return p;
+}
+__device__ __forceinline__ f32x4_t join_pair(const Pair& p, f32x4_t a, f32x4_t b) {
+  f32x4_t y;
+#pragma unroll
+  for (int e = 0; e < 4; ++e) y[e] = fmaf(b[e], p.fb, a[e] * p.fa);
+  return y;
+}
+
 // What a wave gathers of one range: lane (quad, col) holds dims 16 j + 4 quad .. + 3 of query row `col`'s sums of
 // p v, and its m and its l.
 //
@@ -223,17 +243,39 @@ struct Chunk {
   template <class Src>
   __device__ __forceinline__ void run(Src& src, const bf16_t* qr, float scale2, int s0, int s1, int lim, int all_see,
                                       float* score, char* vt) {
+    run_two(src, qr, scale2, s0, s1, s1, lim, all_see, score, vt);
+  }
+
+  // keys [s0, s1) and [s1, s2) (whole tiles up to s1), each by itself, then joined; the second's first tile is asked for
+  // with the first's last
+  template <class Src>
+  __device__ __forceinline__ void run_two(Src& src, const bf16_t* qr, float scale2, int s0, int s1, int s2, int lim,
+                                          int all_see, float* score, char* vt) {
     Tile x;
-    if (s0 < s1) load(src, s0, s0, s1, x);
+    if (s0 < s2) load(src, s0, s0, s2, x);
     bf16x8_t q[NC];
 #pragma unroll
     for (int i = 0; i < NC; ++i) q[i] = *reinterpret_cast<const bf16x8_t*>(qr + i * 32);
+    clear();
+    for (int t0 = s0; t0 < s1; t0 += 32) step(src, x, q, scale2, t0, s0, s2, lim, all_see, score, vt);
+    l = group_sumf(l);
+    if (s1 >= s2) return;
+    const Chunk y = *this;
+    clear();
+    for (int t0 = s1; t0 < s2; t0 += 32) step(src, x, q, scale2, t0, s0, s2, lim, all_see, score, vt);
+    l = group_sumf(l);
+    const Pair p = join_pair(y.m, y.l, m, l);
+    m = p.m;
+    l = p.l;
+#pragma unroll
+    for (int j = 0; j < ND; ++j) o[j] = join_pair(p, y.o[j], o[j]);
+  }
+
+  __device__ __forceinline__ void clear() {
 #pragma unroll
     for (int j = 0; j < ND; ++j) o[j] = f32x4_t{0.f, 0.f, 0.f, 0.f};
     m = -INFINITY;
     l = 0.f;
-    for (int t0 = s0; t0 < s1; t0 += 32) step(src, x, q, scale2, t0, s0, s1, lim, all_see, score, vt);
-    l = group_sumf(l);
   }
 };
 
@@ -259,26 +301,6 @@ __device__ __forceinline__ float inverse(float l) { return l > 0.f || l != l ? 1
 // log2 of a row's sum, -inf without keys
 __device__ __forceinline__ float row_lse2(float m, float l) {
   return l > 0.f || l != l ? m + __builtin_amdgcn_logf(l) : -INFINITY;
-}
-
-// Factors of two neighbouring parts, and the top and l of their sum.  (A part without a finite score is 0, or NaN and stays
-// it.)  Parts are joined in such pairs first, wherever that is done, by these operations.
-struct Pair {
-  float m, l, fa, fb;
-};
-__device__ __forceinline__ Pair join_pair(float ma, float la, float mb, float lb) {
-  Pair p;
-  p.m = fmaxf(ma, mb);
-  p.fa = ma == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(ma - p.m);
-  p.fb = mb == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(mb - p.m);
-  p.l = fmaf(lb, p.fb, la * p.fa);
-  return p;
-}
-__device__ __forceinline__ f32x4_t join_pair(const Pair& p, f32x4_t a, f32x4_t b) {
-  f32x4_t y;
-#pragma unroll
-  for (int e = 0; e < 4; ++e) y[e] = fmaf(b[e], p.fb, a[e] * p.fa);
-  return y;
 }
 
 // Joins the parts of eight waves, a wave's 16 rows of HD + 4 floats in `lds` and its m and l in stat[0..1][row][wave]:

@@ -155,18 +155,9 @@ __global__ __launch_bounds__(256, 2) void kv_attn_kernel(Args a) {
     const int64_t row = (int64_t)b * a.heads + head0 + min(col, nq - 1);
     C x;
     PagedSrc<HD, !SCORES> src{a, b, kvh, max(n - 1, 0)};
-    x.run(src, a.q + b * a.ldq + (int64_t)(head0 + min(col, nq - 1)) * HD + quad * 8, a.scale2, s0, s1, n, n,
-          SCORES && col < nq ? a.score + row * a.ld_score : nullptr, lds + wave * (32 * HD * 2));
-    if (!SCORES && s1 < s2) {
-      const C y = x;
-      x.run(src, a.q + b * a.ldq + (int64_t)(head0 + min(col, nq - 1)) * HD + quad * 8, a.scale2, s1, s2, n, n, nullptr,
-            lds + wave * (32 * HD * 2));
-      const Pair p = join_pair(y.m, y.l, x.m, x.l);
-      x.m = p.m;
-      x.l = p.l;
-#pragma unroll
-      for (int j = 0; j < C::ND; ++j) x.o[j] = join_pair(p, y.o[j], x.o[j]);
-    }
+    const bf16_t* qr = a.q + b * a.ldq + (int64_t)(head0 + min(col, nq - 1)) * HD + quad * 8;
+    if constexpr (SCORES) x.run(src, qr, a.scale2, s0, s1, n, n, col < nq ? a.score + row * a.ld_score : nullptr, lds + wave * (32 * HD * 2));
+    else x.run_two(src, qr, a.scale2, s0, s1, s2, n, n, nullptr, lds + wave * (32 * HD * 2));
     if (col < nq) {
       if (nch == 1) {
         const float inv = inverse(x.l);
