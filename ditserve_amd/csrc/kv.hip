@@ -143,10 +143,17 @@ struct Keys {
     for (int i = 0; i < KPT; ++i)
       key[i] = slot(first, i) < old ? order_of((unsigned)page[i] < (unsigned)t.pages ? raw[i] : -INFINITY) : 0u;
   }
-  // every slot stays, or none: keys above a threshold of 0, or not
-  __device__ __forceinline__ void make_all(int first, int old, bool stay) {
+  // every slot stays, or none: keys above a threshold of 0, or not.  (No weights are read: pages that the cache lacks are
+  // reported here.)
+  __device__ __forceinline__ void make_all(const KvPages& t, int first, int old, bool stay) {
+    bool bad = false;
 #pragma unroll
-    for (int i = 0; i < KPT; ++i) key[i] = stay && slot(first, i) < old ? 1u : 0u;
+    for (int i = 0; i < KPT; ++i) {
+      const bool mine = slot(first, i) < old;
+      bad |= mine && (unsigned)page[i] >= (unsigned)t.pages;
+      key[i] = stay && mine ? 1u : 0u;
+    }
+    if (bad) *t.status = 1;
   }
 };
 
@@ -277,7 +284,7 @@ __global__ __launch_bounds__(1024) void kv_select_kernel(KvPages t, KvWeights w,
       want = 0;
     }
   } else {
-    keys.make_all(0, x.old, x.n <= x.m);
+    keys.make_all(t, 0, x.old, x.n <= x.m);
     want = 0;
   }
   write_list<KPT>(keys.key, 0, top, want, 0, 0, sums, out);
@@ -416,13 +423,15 @@ __global__ __launch_bounds__(1024) void kv_list_kernel(KvPages t, KvWeights w, i
     at = before[0];
     tie = before[1];
   } else {
-    keys.make_all(first, x.old, x.n <= x.m);
+    keys.make_all(t, first, x.old, x.n <= x.m);
     want = 0;
   }
   write_list<KPT>(keys.key, first, top, want, at, tie, sums, out);
 }
 
 // Copies the slots that stay into the pages of `to`: 16 slots of a (key head, sequence) a workgroup, 16 bytes a thread.
+// One whose page the cache lacks becomes zeros, weight too, and is reported (of the recent ones no other kernel sees the
+// pages): the slots behind it keep their places, as in every key head.
 // The old slots are not read again and go past the caches (134 MB copied 30.4 -> 26.0 us: 5.2 TB/s, what a copy reaches);
 // the next step reads the new ones.
 template <int LOG_CH>
@@ -435,7 +444,7 @@ __global__ __launch_bounds__(256) void kv_move_kernel(KvPages t, KvPages to, KvT
   if (j >= m) return;
   const int i = slots[((int64_t)b * gridDim.y + h) * keep + j], low = (1 << t.page_log2) - 1;
   bool ok, ok_to;
-  const int p = kv_page(t, b, i, ok, false), q = kv_page(to, b, j, ok_to, true);
+  const int p = kv_page(t, b, i, ok, true), q = kv_page(to, b, j, ok_to, true);
   if (!ok_to) return;
   const int64_t src = (((int64_t)(i & low) << LOG_CH) + c) * 8, dst = (((int64_t)(j & low) << LOG_CH) + c) * 8;
   u32x4_t k = {0, 0, 0, 0}, v = {0, 0, 0, 0};

@@ -322,6 +322,8 @@ def evict(cache, table, lengths, out_table, keep, recent=0, max_len=None):
     lowest).  A sequence of at most `keep` slots keeps them all.  What stays is copied, with
     its weights, in its order into the first slots of the pages of `out_table`, which must be
     other pages than the table's; those may be freed, or go on being read by who shares them.
+    (Slots of a page that the cache lacks have the lowest weight; one that has to stay becomes
+    zeros, with weight 0, besides being reported.)
     max_len: the longest length there can be (default: what the table holds).  Returns the new
     lengths, a new int32 tensor."""
     _cache_check(cache)

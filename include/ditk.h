@@ -521,7 +521,7 @@ int ditk_kv_attn(const void* q, int64_t ldq, const void* k_cache, int64_t k_ps, 
  * order, with their weights, into the first slots of out_table's pages (other pages than
  * table's; out_width * page >= min(keep, width * page, max_len)).  workspace: 16-byte aligned, this
  * call's alone, of ditk_kv_evict_workspace bytes (most: the smaller of width * page and max_len).
- * w_ps is less than 2^32.
+ * w_ps is less than 2^32.  Slots of a page that the cache lacks count as -inf; those that stay become zeros.
  */
 int64_t ditk_kv_evict_workspace(int batch, int kv_heads, int most, int keep);
 int ditk_kv_evict(void* k_cache, int64_t k_ps, int64_t k_hs, void* v_cache, int64_t v_ps, int64_t v_hs,

@@ -1,0 +1,82 @@
+"""Paged caches where tables are wrong, and where pages, heads and weights have strides of their own."""
+import math
+
+import pytest
+import torch
+
+from tests.kv_reference import DEV, NAN, paged
+
+pytestmark = pytest.mark.gpu
+
+if torch.cuda.is_available():
+    from ditserve_amd import _lib, kv
+
+
+def cache_of(lens, hk, d, page, seed, layout="plain", more=()):
+    """(cache, table, lengths, table of `more` slots): paged() with weights in wider rows of their own, NaN around them."""
+    cache, table, lengths, out_table, _, _ = paged(lens, hk, d, page, seed, layout=layout, more=more)
+    wide = torch.full((cache.pages, hk + 1, page + 12), NAN, device=DEV)
+    w = wide[:, :hk, 4:4 + page]
+    w.copy_(torch.rand(w.shape, generator=torch.Generator().manual_seed(seed)).to(DEV))
+    return kv.PagedCache(cache.k, cache.v, w), table, lengths, out_table, wide
+
+
+def evicted(cache, table, lens, out_table, keep, recent):
+    """(keys, values, weights, new lengths) by definition: slots of pages that the cache lacks have the lowest weight and
+    are zeros where they stay; what would go to such a page goes nowhere."""
+    k, v, w = (t.clone() for t in (cache.k, cache.v, cache.weights))
+    table, out_table, page = table.cpu().long(), out_table.cpu().long(), cache.page
+    there = lambda p: (p >= 0) & (p < cache.pages)  # noqa: E731
+    new = []
+    for b, n in enumerate(lens):
+        n = min(max(n, 0), table.shape[1] * page)
+        m = min(n, keep)
+        r = min(recent, m)
+        new.append(m)
+        i, j = torch.arange(n), torch.arange(m)
+        src, dst = table[b, i // page], out_table[b, j // page]
+        for h in range(cache.kv_heads):
+            old = cache.weights[src.clamp(0, cache.pages - 1).to(DEV), h, (i % page).to(DEV)].cpu()
+            old = torch.where(there(src), old, torch.full_like(old, -math.inf))[:n - r]
+            stay = torch.cat([torch.sort(old, descending=True, stable=True).indices[:m - r].sort().values, i[n - r:]])
+            for to, of in ((k, cache.k), (v, cache.v), (w, cache.weights)):
+                x = of[src[stay].clamp(0, cache.pages - 1).to(DEV), h, (stay % page).to(DEV)]
+                x[~there(src[stay]).to(DEV)] = 0
+                ok = there(dst)
+                to[dst[ok].to(DEV), h, (j % page)[ok].to(DEV)] = x[ok.to(DEV)]
+    return k, v, w, new
+
+
+def same(got, want):
+    return torch.equal(torch.nan_to_num(got.float(), 77.0), torch.nan_to_num(want.float(), 77.0))
+
+
+def check_evict(cache, table, lengths, out_table, wide, keep, recent, lens, reported, max_len=None):
+    before = wide.clone()
+    k, v, w, new = evicted(cache, table, lens, out_table, keep, recent)
+    got = kv.evict(cache, table, lengths, out_table, keep, recent, max_len=max_len)
+    if reported:
+        with pytest.raises(_lib.DitkError):
+            kv.check_tables()
+    kv.check_tables()
+    assert got.tolist() == new
+    assert same(cache.k, k) and same(cache.v, v) and same(cache.weights, w)
+    hk, page = cache.kv_heads, cache.page
+    assert same(wide[:, hk:], before[:, hk:]) and same(wide[:, :, :4], before[:, :, :4])
+    assert same(wide[:, :, 4 + page:], before[:, :, 4 + page:])
+
+
+@pytest.mark.parametrize("n,page", [(200, 16), (40000, 128)])  # one workgroup, parts of a row
+@pytest.mark.parametrize("where,keep,recent", [
+    ("old", 0.5, 10), ("last", 0.5, 10), ("all", 1.0, 10), ("all", 2.0, 0), ("dropped", 0.25, None), ("last", 0.25, None)])
+@pytest.mark.parametrize("bad", [-1, None, 2**31 - 1, -2**31])
+def test_evict_reports_bad_pages(n, page, where, keep, recent, bad):
+    """A page that the cache lacks, among slots that weights decide on, among the recent ones, where every slot stays, and
+    where only recent ones do: reported, its slots zeros where they stay, the other sequence as ever."""
+    keep = int(n * keep)
+    recent = keep if recent is None else recent
+    stay = [min(n, keep), min(90, keep)]
+    cache, table, lengths, out_table, wide = cache_of([n, 90], 2, 64, page, 5, more=stay)
+    slot = {"old": n // 3, "last": n - 1, "all": n // 2, "dropped": 5}[where]
+    table[0, slot // page] = cache.pages if bad is None else bad
+    check_evict(cache, table, lengths, out_table, wide, keep, recent, [n, 90], True)
