@@ -100,6 +100,24 @@ def _meet_blocks(delta, pages, heads, ps, hs, size):
     return any(abs(y) < size for x in _nearest(delta, ps, pages) for y in _nearest(x, hs, heads))
 
 
+def _blocks_meet(delta, a, b):
+    """Whether two tensors' blocks (pages, heads, page stride, head stride, size), of which _span is not 0, the second's
+    `delta` behind the first's, share an element.  Exact where their strides are the same, or the larger ones are (what
+    lies in between counts as a tensor's own then); else whether their spans meet."""
+    levels, sizes = [], []
+    for pages, heads, ps, hs, size in (a, b):
+        levels.append(sorted(((st, n) for n, st in ((pages, ps), (heads, hs)) if n > 1), reverse=True))
+        sizes.append(size)
+    same = 0
+    while same < len(levels[0]) and levels[0][same] == levels[1][same]:
+        same += 1
+    sizes = [size + sum((n - 1) * st for st, n in own[same:]) for size, own in zip(sizes, levels)]
+    starts = [delta]
+    for st, n in levels[0][:same]:
+        starts = [y for x in starts for y in _nearest(x, st, n)]
+    return any(-sizes[1] < y < sizes[0] for y in starts)
+
+
 class PagedCache:
     """Keys and values in pages.
 
@@ -107,7 +125,7 @@ class PagedCache:
              head_dim 64 or 128.  A (page, head)'s slots are contiguous; the first two strides
              are free (k and v may be halves of one buffer)
     weights  [pages, kv_heads, page] fp32, the attention weight each slot has gathered
-             (optional; decode_attn writes it, evict reads it)"""
+             (optional; decode_attn writes it, evict reads it); none of them in a key or value"""
 
     __slots__ = ("_k", "_v", "_w", "_dims", "_strides", "_bytes")
 
@@ -143,6 +161,12 @@ class PagedCache:
             if tuple(weights.shape) != dims[:3] or unit != 1 or not span:
                 raise ValueError(f"weights must be {dims[:3]} with unit slot stride, got {tuple(weights.shape)}, strides "
                                  f"{weights.stride()}")
+            first = weights.data_ptr()
+            for end, st in zip(ends, (strides[:2], strides[2:])):
+                if _meet(end, (first, first + 4 * span)) and _blocks_meet(
+                        first - end[0], (*dims[:2], 2 * st[0], 2 * st[1], 2 * page * d),
+                        (*dims[:2], 4 * ps, 4 * hs, 4 * page)):
+                    raise ValueError("weights overlap k or v")
             strides += (ps, hs)
         else:
             span, strides = 0, strides + [0, 0]

@@ -80,3 +80,38 @@ def test_evict_reports_bad_pages(n, page, where, keep, recent, bad):
     slot = {"old": n // 3, "last": n - 1, "all": n // 2, "dropped": 5}[where]
     table[0, slot // page] = cache.pages if bad is None else bad
     check_evict(cache, table, lengths, out_table, wide, keep, recent, [n, 90], True)
+
+
+def test_weights_apart():
+    """Weights in the buffer of keys and values: refused where they share an element with them, taken where they lie between."""
+    pages, hk, page, d = 5, 2, 16, 64
+    block = page * d
+    for head_first in (False, True):
+        # a record of keys, values and weights for each page (or head), then heads (or pages) in it
+        n, m = (hk, pages) if head_first else (pages, hk)
+        line = 2 * m * block + 2 * m * page
+        x = torch.zeros(n * line, dtype=torch.bfloat16, device=DEV)
+        f = x.view(torch.float32)
+        ps, hs = (block, line) if head_first else (line, block)
+        wps, whs = (page, line // 2) if head_first else (line // 2, page)
+        k, v = (x.as_strided((pages, hk, page, d), (ps, hs, d, 1), i * m * block) for i in range(2))
+        w = lambda off: f.as_strided((pages, hk, page), (wps, whs, 1), off)  # noqa: E731
+        first = m * block  # floats up to a record's weights
+        assert kv.PagedCache(k, v, w(first)).weights is not None
+        for off in (0, 4, first - page, first - 4, first - 1, m * block // 2):
+            with pytest.raises(ValueError, match="overlap"):
+                kv.PagedCache(k, v, w(off))
+    # each head's weights behind its keys and values
+    line = 2 * block + 2 * page
+    x = torch.zeros(pages * hk * line, dtype=torch.bfloat16, device=DEV)
+    f = x.view(torch.float32)
+    k, v = (x.as_strided((pages, hk, page, d), (hk * line, line, d, 1), i * block) for i in range(2))
+    w = lambda off: f.as_strided((pages, hk, page), (hk * line // 2, line // 2, 1), off)  # noqa: E731
+    kv.PagedCache(k, v, w(block))
+    for off in (0, block - 1, block // 2):
+        with pytest.raises(ValueError, match="overlap"):
+            kv.PagedCache(k, v, w(off))
+    # another order than theirs
+    with pytest.raises(ValueError, match="overlap"):
+        kv.PagedCache(k, v, f.as_strided((pages, hk, page), (page, pages * page, 1), 0))
+    kv.PagedCache(k, v, torch.zeros((pages, hk, page), device=DEV))

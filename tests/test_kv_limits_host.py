@@ -1,0 +1,39 @@
+"""Further checks of the paged cache's entry points, before any launch (no GPU)."""
+import random
+
+from ditserve_amd import kv
+
+
+def test_blocks_of_two_tensors():
+    """Whether keys or values and weights share a byte: never missed, and exact where both have the same order and strides or
+    the same stride of pages with contiguous heads."""
+    r = random.Random(1)
+    seen = [0, 0]  # cases that do not meet, and that do
+    for _ in range(1200):
+        pages, heads = r.randint(1, 4), r.randint(1, 3)
+        sizes = [r.randint(1, 6), r.randint(1, 6)]
+        exact = True
+        kind = r.randrange(3)
+        if kind == 0:  # the same strides, pages or heads outside
+            inner, outside = max(sizes) + r.randint(0, 9), r.random() < 0.5
+            outer = inner * (heads if outside else pages) + r.randint(0, 20)
+            strides = [(outer, inner) if outside else (inner, outer)] * 2
+        elif kind == 1:  # the same outer stride, insides contiguous
+            outer = sum(sizes) * heads + r.randint(0, 20)
+            strides = [(outer, sizes[0]), (outer, sizes[1])]
+        else:
+            exact = False
+            strides = [(sizes[i] * heads + r.randint(0, 5), sizes[i]) for i in range(2)]
+        a, b = [(pages, heads, *st, size) for st, size in zip(strides, sizes)]
+        if not kv._span(*a) or not kv._span(*b):
+            continue
+        cells = [{i * ps + j * hs + e for i in range(p) for j in range(h) for e in range(n)} for p, h, ps, hs, n in (a, b)]
+        far = max(map(max, cells)) + 2
+        for delta in range(-far, far + 1, r.randint(1, 3)):
+            want = any(x + delta in cells[0] for x in cells[1])
+            got = kv._blocks_meet(delta, a, b)
+            assert got or not want, (delta, a, b)
+            if exact:
+                assert got == want, (delta, a, b)
+                seen[want] += 1
+    assert min(seen) > 1000
