@@ -364,7 +364,8 @@ DITK_EXPORT int ditk_kv_attn(const void* q, int64_t ldq, const void* k_cache, in
   DITK_REQUIRE(batch == 0 || (q && o), "%s: null tensor", what);
   DITK_REQUIRE(ldq % 8 == 0 && ldo % 8 == 0 && ((uintptr_t)q % 16) == 0 && ((uintptr_t)o % 16) == 0,
                "%s: rows must be 16-byte aligned", what);
-  DITK_REQUIRE(max_len >= 0 && softmax_scale > 0.f, "%s: bad max_len or softmax_scale", what);
+  DITK_REQUIRE(max_len >= 0, "%s: bad max_len %d", what, max_len);
+  DITK_REQUIRE(softmax_scale >= 1e-30f && softmax_scale <= 1e30f, "%s: softmax_scale must be in 1e-30..1e30", what);
   if (batch == 0) return 0;
   const int most = width * page < max_len ? width * page : max_len;
   const Space sp = space_of(batch, heads, head_dim, most, weights != nullptr);

@@ -314,8 +314,8 @@ def decode_attn(q, cache, table, lengths, heads, softmax_scale=None, max_len=Non
             raise ValueError(f"max_len must not be negative, got {max_len}")
         most = min(most, int(max_len))
     scale = 1.0 / math.sqrt(d) if softmax_scale is None else float(softmax_scale)
-    if not 0 < scale < math.inf:
-        raise ValueError(f"softmax_scale must be positive and finite, got {scale}")
+    if not 1e-30 <= scale <= 1e30:  # (scores are scaled in fp32)
+        raise ValueError(f"softmax_scale must be in 1e-30..1e30, got {scale}")
     if out is None:
         out, ldo = torch.empty((batch, heads * d), dtype=_BF16, device=device), heads * d
     else:

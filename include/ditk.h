@@ -507,7 +507,7 @@ int64_t ditk_kv_attn_workspace(int batch, int heads, int head_dim, int most, int
  * kv_heads) over its slots: o [batch, heads * head_dim] bf16, lse [batch][heads] fp32 natural log
  * (may be NULL).  weights not NULL: the probabilities of each slot, summed over the query heads of
  * its key head, are written there (add != 0: added).  workspace: 16-byte aligned, this call's alone.
- * batch * heads is less than 2^22.
+ * batch * heads is less than 2^22, softmax_scale in 1e-30..1e30 (ditk_flash_attn_causal too).
  */
 int ditk_kv_attn(const void* q, int64_t ldq, const void* k_cache, int64_t k_ps, int64_t k_hs, const void* v_cache,
                  int64_t v_ps, int64_t v_hs, float* weights, int64_t w_ps, int64_t w_hs, int add, int pages, int page,

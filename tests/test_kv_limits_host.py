@@ -1,7 +1,20 @@
 """Further checks of the paged cache's entry points, before any launch (no GPU)."""
 import random
 
-from ditserve_amd import kv
+import pytest
+
+from ditserve_amd import _lib, kv
+
+if not _lib.LIB_PATH.exists():
+    pytest.skip("libditk.so not built (run python -m ditserve_amd.build)", allow_module_level=True)
+
+from tests.test_kv_host import ATTN, refused  # noqa: E402
+
+
+@pytest.mark.parametrize("scale", [1e-31, 1e31, 1e39, float("inf"), -1.0])
+def test_attn_refuses_scales_beyond_fp32(scale):
+    """Scores are scaled in fp32: a scale that is no number there, or near its ends, is refused, as for prompts."""
+    refused("ditk_kv_attn", tuple({**ATTN, "scale": scale}.values()), "softmax_scale")
 
 
 def test_blocks_of_two_tensors():
