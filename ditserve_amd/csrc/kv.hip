@@ -14,10 +14,15 @@ int kv_check_pages(const char* what, const void* table, const void* lengths, con
   return 0;
 }
 
-int kv_check_tensor(const char* what, const void* p, int64_t ps, int64_t hs, int page, int head_dim) {
+int kv_check_tensor(const char* what, const void* p, int64_t ps, int64_t hs) {
   DITK_REQUIRE(p != nullptr, "%s: null cache", what);
   DITK_REQUIRE(((uintptr_t)p % 16) == 0 && ps % 8 == 0 && hs % 8 == 0 && ps >= 0 && hs >= 0,
                "%s: the cache's heads must be 16-byte aligned", what);
+  return 0;
+}
+
+int kv_check_weights(const char* what, const float* p, int64_t ps, int64_t hs) {
+  DITK_REQUIRE(p == nullptr || (((uintptr_t)p % 4) == 0 && ps >= 0 && hs >= 0), "%s: bad strides or address of the weights", what);
   return 0;
 }
 
@@ -468,8 +473,9 @@ DITK_EXPORT int ditk_kv_append(const void* k, int64_t ldk, const void* v, int64_
                                int T, int kv_heads, int head_dim, int32_t* status, hipStream_t stream) {
   const char* what = "ditk_kv_append";
   if (int rc = kv_check_pages(what, table, lengths, status, batch, width, ldt, pages, page, kv_heads, head_dim)) return rc;
-  if (int rc = kv_check_tensor(what, k_cache, k_ps, k_hs, page, head_dim)) return rc;
-  if (int rc = kv_check_tensor(what, v_cache, v_ps, v_hs, page, head_dim)) return rc;
+  if (int rc = kv_check_tensor(what, k_cache, k_ps, k_hs)) return rc;
+  if (int rc = kv_check_tensor(what, v_cache, v_ps, v_hs)) return rc;
+  if (int rc = kv_check_weights(what, weights, w_ps, w_hs)) return rc;
   const int64_t row = (int64_t)kv_heads * head_dim;
   DITK_REQUIRE(T >= 0 && T < (1 << 30) && row < (1 << 30) && (T == 0 || (k && v)), "%s: bad rows", what);
   DITK_REQUIRE(cu_seqlens != nullptr || T == batch, "%s: %d rows for %d sequences", what, T, batch);
@@ -519,10 +525,11 @@ DITK_EXPORT int ditk_kv_evict(void* k_cache, int64_t k_ps, int64_t k_hs, void* v
   const char* what = "ditk_kv_evict";
   if (int rc = kv_check_pages(what, table, lengths, status, batch, width, ldt, pages, page, kv_heads, head_dim)) return rc;
   if (int rc = kv_check_pages(what, out_table, lengths, status, batch, out_width, ldo, pages, page, kv_heads, head_dim)) return rc;
-  if (int rc = kv_check_tensor(what, k_cache, k_ps, k_hs, page, head_dim)) return rc;
-  if (int rc = kv_check_tensor(what, v_cache, v_ps, v_hs, page, head_dim)) return rc;
+  if (int rc = kv_check_tensor(what, k_cache, k_ps, k_hs)) return rc;
+  if (int rc = kv_check_tensor(what, v_cache, v_ps, v_hs)) return rc;
+  if (int rc = kv_check_weights(what, weights, w_ps, w_hs)) return rc;
   DITK_REQUIRE(weights != nullptr, "%s: the cache has no weights", what);
-  DITK_REQUIRE(w_ps >= 0 && w_ps < (1ll << 32), "%s: the weights' pages are too far apart", what);
+  DITK_REQUIRE(w_ps < (1ll << 32), "%s: the weights' pages are too far apart", what);
   DITK_REQUIRE(keep > 0 && recent >= 0 && recent <= keep && max_len >= 0, "%s: bad keep %d, recent %d or max_len %d",
                what, keep, recent, max_len);
   if (batch == 0) return 0;

@@ -357,8 +357,9 @@ DITK_EXPORT int ditk_kv_attn(const void* q, int64_t ldq, const void* k_cache, in
                              float softmax_scale, int32_t* status, hipStream_t stream) {
   const char* what = "ditk_kv_attn";
   if (int rc = kv_check_pages(what, table, lengths, status, batch, width, ldt, pages, page, kv_heads, head_dim)) return rc;
-  if (int rc = kv_check_tensor(what, k_cache, k_ps, k_hs, page, head_dim)) return rc;
-  if (int rc = kv_check_tensor(what, v_cache, v_ps, v_hs, page, head_dim)) return rc;
+  if (int rc = kv_check_tensor(what, k_cache, k_ps, k_hs)) return rc;
+  if (int rc = kv_check_tensor(what, v_cache, v_ps, v_hs)) return rc;
+  if (int rc = kv_check_weights(what, weights, w_ps, w_hs)) return rc;
   DITK_REQUIRE(heads > 0 && heads <= 65535 && heads % kv_heads == 0, "%s: %d query heads for %d key heads", what, heads,
                kv_heads);
   DITK_REQUIRE(batch == 0 || (q && o), "%s: null tensor", what);

@@ -48,4 +48,5 @@ __device__ __forceinline__ int kv_page(const KvPages& t, int b, int i, bool& ok,
 // host checks shared by the entry points
 int kv_check_pages(const char* what, const void* table, const void* lengths, const void* status, int batch, int width,
                    int64_t ldt, int pages, int page, int kv_heads, int head_dim);
-int kv_check_tensor(const char* what, const void* p, int64_t ps, int64_t hs, int page, int head_dim);
+int kv_check_tensor(const char* what, const void* p, int64_t ps, int64_t hs);
+int kv_check_weights(const char* what, const float* p, int64_t ps, int64_t hs);  // (none: fine)

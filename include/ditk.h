@@ -483,8 +483,8 @@ int ditk_causal_few_parts(int nq, int nk, int group);
 /*
  * Paged key-value caches.  A cache of `pages` pages of `page` slots (16, 32, 64, 128 or 256) holds
  * keys and values [page][head_dim] bf16 (head_dim 64 or 128), contiguous, for each (page, key head),
- * with a page stride *_ps and a head stride *_hs (elements, multiples of 8); weights (fp32, may be
- * NULL) one for each (page, key head, slot).  Slot i of sequence b is slot i % page of page
+ * with a page stride *_ps and a head stride *_hs (elements, multiples of 8, not negative); weights
+ * (fp32, may be NULL) one for each (page, key head, slot), in no key's or value's memory.  Slot i of sequence b is slot i % page of page
  * table[b * ldt + i / page]; the table's rows hold `width` pages and lengths[b] slots are filled.
  * A length outside [0, min(width * page, max_len)] is clamped; a page outside [0, pages) is neither
  * read nor written and its slots count as absent; either sets *status (pinned host memory) to 1.

@@ -8,13 +8,20 @@ from ditserve_amd import _lib, kv
 if not _lib.LIB_PATH.exists():
     pytest.skip("libditk.so not built (run python -m ditserve_amd.build)", allow_module_level=True)
 
-from tests.test_kv_host import ATTN, refused  # noqa: E402
+from tests.test_kv_host import APPEND, ATTN, EVICT, G, refused  # noqa: E402
 
 
 @pytest.mark.parametrize("scale", [1e-31, 1e31, 1e39, float("inf"), -1.0])
 def test_attn_refuses_scales_beyond_fp32(scale):
     """Scores are scaled in fp32: a scale that is no number there, or near its ends, is refused, as for prompts."""
     refused("ditk_kv_attn", tuple({**ATTN, "scale": scale}.values()), "softmax_scale")
+
+
+@pytest.mark.parametrize("change", [dict(w=G + 2), dict(w=G, w_hs=-16), dict(w=G, w_ps=-32)])
+@pytest.mark.parametrize("name,args", [
+    ("ditk_kv_append", APPEND), ("ditk_kv_attn", {**ATTN, "space": G, "size": 1 << 20}), ("ditk_kv_evict", EVICT)])
+def test_weights_are_checked(name, args, change):
+    refused(name, tuple({**args, **change}.values()), "weights")
 
 
 def test_blocks_of_two_tensors():
