@@ -727,6 +727,7 @@ DITK_EXPORT int ditk_flash_attn_causal(const void* q, int64_t ldq, const void* k
   // the kernel addresses a tile of 64 K or V rows, and a row's bytes, with 32 bits
   DITK_REQUIRE(ldq >= 0 && ldk >= 0 && ldv >= 0 && ldo >= 0 && ldq < (1ll << 30) && ldo < (1ll << 30) &&
                    ldk < (1ll << 23) && ldv < (1ll << 23), "%s: rows too long for 32-bit lane offsets", what);
+  DITK_REQUIRE(Tq <= 1 || ldo >= (int64_t)heads * head_dim, "%s: rows of o overlap", what);
   if (Tq == 0) return 0;
   const float sl2 = softmax_scale * 1.4426950408889634f;
   if ((kinds & 2) && Tk >= kFewKeys) {

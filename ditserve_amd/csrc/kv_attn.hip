@@ -365,6 +365,8 @@ DITK_EXPORT int ditk_kv_attn(const void* q, int64_t ldq, const void* k_cache, in
   DITK_REQUIRE(batch == 0 || (q && o), "%s: null tensor", what);
   DITK_REQUIRE(ldq % 8 == 0 && ldo % 8 == 0 && ((uintptr_t)q % 16) == 0 && ((uintptr_t)o % 16) == 0,
                "%s: rows must be 16-byte aligned", what);
+  const int64_t row = (int64_t)heads * head_dim;
+  DITK_REQUIRE(batch <= 1 || (ldq >= row && ldo >= row), "%s: rows of q or o overlap", what);
   DITK_REQUIRE(max_len >= 0, "%s: bad max_len %d", what, max_len);
   DITK_REQUIRE(softmax_scale >= 1e-30f && softmax_scale <= 1e30f, "%s: softmax_scale must be in 1e-30..1e30", what);
   if (batch == 0) return 0;

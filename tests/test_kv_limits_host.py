@@ -8,13 +8,23 @@ from ditserve_amd import _lib, kv
 if not _lib.LIB_PATH.exists():
     pytest.skip("libditk.so not built (run python -m ditserve_amd.build)", allow_module_level=True)
 
-from tests.test_kv_host import APPEND, ATTN, EVICT, G, refused  # noqa: E402
+from tests.test_kv_host import APPEND, ATTN, CAUSAL, EVICT, G, refused  # noqa: E402
 
 
 @pytest.mark.parametrize("scale", [1e-31, 1e31, 1e39, float("inf"), -1.0])
 def test_attn_refuses_scales_beyond_fp32(scale):
     """Scores are scaled in fp32: a scale that is no number there, or near its ends, is refused, as for prompts."""
     refused("ditk_kv_attn", tuple({**ATTN, "scale": scale}.values()), "softmax_scale")
+
+
+@pytest.mark.parametrize("change", [dict(ldq=128), dict(ldo=248), dict(ldq=-256), dict(ldo=-256), dict(ldo=0)])
+def test_attn_refuses_rows_that_overlap(change):
+    refused("ditk_kv_attn", tuple({**ATTN, **change}.values()), "rows")
+
+
+@pytest.mark.parametrize("ldo", [0, 128, 248])
+def test_causal_refuses_rows_that_overlap(ldo):
+    refused("ditk_flash_attn_causal", tuple({**CAUSAL, "ldo": ldo}.values()), "rows of o")
 
 
 @pytest.mark.parametrize("change", [dict(w=G + 2), dict(w=G, w_hs=-16), dict(w=G, w_ps=-32)])
