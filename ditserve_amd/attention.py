@@ -143,6 +143,7 @@ def causal_attn_varlen_func(q, k, v, cu_q, cu_k, max_q, max_k, softmax_scale=Non
     (tq, h, d), (tk, hk, _) = q.shape, k.shape
     if k.shape[2] != d or v.shape != k.shape:
         raise ValueError(f"k and v must be [Tk, Hk, {d}], got {tuple(k.shape)} and {tuple(v.shape)}")
+    ops._one_device(q.device, ("cu_seqlens_q", cu_q), ("cu_seqlens_k", cu_k))
     if cu_q.numel() != cu_k.numel():
         raise ValueError("cu_seqlens_q and cu_seqlens_k must have the same length")
     seg_q, seg_k = ops.Segments.pair_from_device(cu_q.to(torch.int32), tq, cu_k.to(torch.int32), tk)

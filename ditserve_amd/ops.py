@@ -140,8 +140,8 @@ class Segments:
         status = table_status(cu_dev.device)
         status.poll()
         obj = cls._clamped(torch.empty_like(cu_dev, memory_format=torch.contiguous_format), total)
-        _lib.call("ditk_check_cu_seqlens", _ptr(cu_dev.contiguous()), obj._nseg, obj._total, _ptr(obj.dev),
-                  _ptr(status.host), _stream())
+        _call(cu_dev.device, "ditk_check_cu_seqlens", _ptr(cu_dev.contiguous()), obj._nseg, obj._total, _ptr(obj.dev),
+              _ptr(status.host))
         return obj
 
     @classmethod
@@ -151,13 +151,14 @@ class Segments:
         cls._check_table(cu_k)
         if cu_q.numel() != cu_k.numel():
             raise ValueError("cu_seqlens_q and cu_seqlens_k must have the same length")
+        _one_device(cu_q.device, ("cu_seqlens_k", cu_k))
         status = table_status(cu_q.device)
         status.poll()
         own = torch.empty((2, cu_q.numel()), dtype=torch.int32, device=cu_q.device).unbind(0)
         q, k = cls._clamped(own[0], total_q), cls._clamped(own[1], total_k)
         cu_q, cu_k = cu_q.contiguous(), cu_k.contiguous()
-        _lib.call("ditk_check_cu_seqlens_pair", _ptr(cu_q), q._total, _ptr(q.dev), _ptr(cu_k), k._total, _ptr(k.dev),
-                  q._nseg, _ptr(status.host), _stream())
+        _call(cu_q.device, "ditk_check_cu_seqlens_pair", _ptr(cu_q), q._total, _ptr(q.dev), _ptr(cu_k), k._total,
+              _ptr(k.dev), q._nseg, _ptr(status.host))
         return q, k
 
     @staticmethod

@@ -1,9 +1,10 @@
-"""Further checks of the paged cache's entry points, before any launch (no GPU)."""
+"""Further checks of the paged cache's and the device tables' entry points, before any launch (no GPU)."""
 import random
 
 import pytest
+import torch
 
-from ditserve_amd import _lib, kv
+from ditserve_amd import _lib, attention, kv, ops
 
 if not _lib.LIB_PATH.exists():
     pytest.skip("libditk.so not built (run python -m ditserve_amd.build)", allow_module_level=True)
@@ -67,3 +68,60 @@ def test_blocks_of_two_tensors():
                 assert got == want, (delta, a, b)
                 seen[want] += 1
     assert min(seen) > 1000
+
+
+class Table:
+    """A device table, as far as the host looks at one."""
+
+    def __init__(self, device, n=3):
+        self.device, self.n, self.dtype = torch.device(device), n, torch.int32
+
+    def dim(self):
+        return 1
+
+    def numel(self):
+        return self.n
+
+    def to(self, dtype):
+        return self
+
+    def contiguous(self):
+        return self
+
+    def data_ptr(self):
+        return 0
+
+
+def test_tables_on_two_devices_are_refused(monkeypatch):
+    """The check of a pair of tables is one launch: both have to be on one device, the rows' own."""
+    def launched(*args):
+        raise AssertionError("launched")
+    for name in ("_call", "table_status"):
+        monkeypatch.setattr(ops, name, launched)
+    monkeypatch.setattr(ops._lib, "call", launched)
+    with pytest.raises(ValueError, match="cu_seqlens"):
+        ops.Segments.pair_from_device(Table("cuda:0"), 8, Table("cuda:1"), 8)
+    rows = torch.zeros((8, 2, 64), dtype=torch.bfloat16)  # (rows on the host)
+    for q, k in (("cuda:0", "cuda:1"), ("cuda:1", "cuda:0"), ("cuda:0", "cuda:0")):
+        with pytest.raises(ValueError):
+            attention.causal_attn_varlen_func(rows, rows, rows, Table(q), Table(k), 8, 8)
+
+
+def test_tables_are_checked_on_their_device(monkeypatch):
+    """The launch goes to the tables' device, which need not be the current one."""
+    seen = []
+
+    class Status:
+        host = torch.zeros(1, dtype=torch.int32)
+
+        def poll(self):
+            pass
+
+    empty = torch.empty
+    monkeypatch.setattr(ops, "table_status", lambda device: Status())
+    monkeypatch.setattr(ops, "_call", lambda device, name, *args: seen.append((str(device), name)))
+    monkeypatch.setattr(ops.torch, "empty", lambda *a, device=None, **kw: empty(*a, **kw))
+    monkeypatch.setattr(ops.torch, "empty_like", lambda t, **kw: empty(t.numel(), dtype=t.dtype))
+    ops.Segments.pair_from_device(Table("cuda:1"), 8, Table("cuda:1"), 8)
+    ops.Segments.from_device(Table("cuda:1"), 8)
+    assert seen == [("cuda:1", "ditk_check_cu_seqlens_pair"), ("cuda:1", "ditk_check_cu_seqlens")]
