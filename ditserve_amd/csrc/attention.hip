@@ -47,10 +47,12 @@
 // key loop ends behind the last key that one of its queries sees, and only the tiles that some
 // query of a wave does not see whole take a mask, out of line: 2 vector operations a score, 2 or 3
 // tiles an item.  V is staged as rows, like K, and read by transposing LDS reads: a transposed copy was a
-// launch of its own (77 keys 5 of 12 us).  The matrix pipe bounds long prompts (16384 queries,
-// 32 heads of 128 over 8: 1.76 ms, 1.25 PFLOP/s of what is seen, at the clock that the power leaves), a
-// work item's start and end short ones (6 us of 10 for 128 queries).  Segments of few queries
-// over many keys go to causal_few.hip.
+// launch of its own (77 keys 5 of 12 us).  Probabilities are rounded to bf16, 8 bits, as in all forms above: the second
+// product takes bf16, and a second operand for what that cuts off (attn_chunk.h) would make the matrix pipe's work 1.5 times
+// as much; outputs are 1.03-1.09 times as far from 64 bits as with probabilities in fp32.  The matrix pipe bounds long
+// prompts (16384 queries, 32 heads of 128 over 8: 1.76 ms, 1.25 PFLOP/s of what is seen, at the clock that the power
+// leaves), a work item's start and end short ones (6 us of 10 for 128 queries).  Segments of few queries over many keys go
+// to causal_few.hip.
 #include <algorithm>
 #include <cmath>
 #include <mutex>

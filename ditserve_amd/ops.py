@@ -696,9 +696,13 @@ def flash_attn_causal(q, k, v, seg_q, seg_k, heads, kv_heads, head_dim, softmax_
     h // (heads / kv_heads).  Segment m has as many keys as seg_k says; its queries are the last of
     them: query i of nq sees the keys j <= i + nk - nq (with earlier keys in front, the next part of
     a prompt; a query that sees none gives zeros and an lse of -inf).  Returns out
-    [Tq, heads * head_dim] (and lse [heads, Tq] fp32, natural log, when return_lse).  A segment's
-    result does not depend on what it is packed with, nor a query's on keys and values that it
-    does not see, whatever they hold."""
+    [Tq, heads * head_dim] (and lse [heads, Tq] fp32, natural log, when return_lse).
+
+    A segment's result is bitwise the same whatever it is packed with, as long as its values and the
+    sums of them (fp32, the weights up to 256) are finite.  What a query does not see, whatever it
+    holds, reaches its result as rounding only: the running maximum moves for 64 queries together,
+    and beside a value or an output that is not finite probabilities have 16 bits instead of
+    bf16's 8."""
     if heads <= 0 or kv_heads <= 0 or heads % kv_heads:
         raise ValueError(f"heads must be a multiple of kv_heads, got {heads} and {kv_heads}")
     if head_dim not in (64, 128):
