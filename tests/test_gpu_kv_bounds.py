@@ -1,10 +1,11 @@
-"""Paged caches where tables are wrong, and where pages, heads and weights have strides of their own."""
+"""Paged caches where tables and lengths are wrong, where pages, heads and weights have strides of their own, and where
+sequences are long enough for every size of chunk."""
 import math
 
 import pytest
 import torch
 
-from tests.kv_reference import DEV, NAN, paged
+from tests.kv_reference import DEV, NAN, attend64, check_out, errors32, get, paged
 
 pytestmark = pytest.mark.gpu
 
@@ -80,6 +81,83 @@ def test_evict_reports_bad_pages(n, page, where, keep, recent, bad):
     slot = {"old": n // 3, "last": n - 1, "all": n // 2, "dropped": 5}[where]
     table[0, slot // page] = cache.pages if bad is None else bad
     check_evict(cache, table, lengths, out_table, wide, keep, recent, [n, 90], True)
+
+
+@pytest.mark.parametrize("n,page", [(200, 16), (40000, 128)])
+def test_evict_into_bad_pages(n, page):
+    """What would go to a page that the cache lacks goes nowhere, and is reported."""
+    keep = n // 2
+    for bad in (-1, 2**31 - 1):
+        cache, table, lengths, out_table, wide = cache_of([n, 90], 2, 64, page, 6, more=[keep, 90])
+        out_table[0, 1] = bad
+        check_evict(cache, table, lengths, out_table, wide, keep, 16, [n, 90], True)
+        cache, table, lengths, out_table, wide = cache_of([n, 90], 2, 64, page, 6, more=[keep, 90])
+        out_table[0, 2] = cache.pages
+        check_evict(cache, table, lengths, out_table, wide, keep, 16, [n, 90], True)
+
+
+@pytest.mark.parametrize("n,page", [(190, 16), (40000, 128)])
+def test_evict_clamps_lengths(n, page):
+    """Lengths outside the table are clamped to it, and to max_len; both are reported."""
+    full = -(-n // page) * page
+    for given, holds in ((-5, 0), (-2**31, 0), (2**31 - 1, full), (full + 1, full)):
+        cache, table, lengths, out_table, wide = cache_of([full, 90], 1, 128, page, 7, more=[n // 2, 90])
+        lengths[0] = given
+        check_evict(cache, table, lengths, out_table, wide, n // 2, 9, [holds, 90], True)
+    cache, table, lengths, out_table, wide = cache_of([full, 90], 1, 128, page, 7, more=[100, 90])
+    check_evict(cache, table, lengths, out_table, wide, 100, 9, [150, 90], True, max_len=150)
+    cache, table, lengths, out_table, wide = cache_of([n, 90], 1, 128, page, 7, more=[100, 90])
+    check_evict(cache, table, lengths, out_table, wide, 100, 9, [n, 90], False, max_len=n)
+
+
+@pytest.mark.parametrize("layout", ["interleaved", "heads"])
+@pytest.mark.parametrize("lens,keep,recent,hk,d,page", [
+    ([300, 0, 41, 1], 40, 7, 3, 64, 16), ([5000, 900], 700, 64, 2, 128, 64), ([40000], 3000, 1, 2, 64, 256)])
+def test_evict_layouts(layout, lens, keep, recent, hk, d, page):
+    """Pages and heads in any order, weights in wider rows."""
+    cache, table, lengths, out_table, wide = cache_of(lens, hk, d, page, 8, layout, [min(n, keep) for n in lens])
+    check_evict(cache, table, lengths, out_table, wide, keep, recent, lens, False)
+
+
+def long_cache(lens, hk, d, page, seed):
+    """A cache made on the device, its pages in no order."""
+    g = torch.Generator(device=DEV).manual_seed(seed)
+    counts = [-(-n // page) for n in lens]
+    total = sum(counts) + 2
+    k = torch.randn((total, hk, page, d), generator=g, device=DEV).bfloat16()
+    v = (torch.randn((total, hk, page, d), generator=g, device=DEV) + 0.5).bfloat16()
+    order = torch.randperm(total, generator=g, device=DEV).int()
+    table = torch.full((len(lens), max(counts)), -1, dtype=torch.int32, device=DEV)
+    for b, c in enumerate(counts):
+        at = sum(counts[:b])
+        table[b, :c] = order[at:at + c]
+    return kv.PagedCache(k, v, torch.zeros((total, hk, page), device=DEV)), table, torch.tensor(lens, dtype=torch.int32, device=DEV)
+
+
+@pytest.mark.parametrize("lens,heads,hk,d,page", [
+    ([65536, 65537, 3], 2, 1, 64, 16), ([262144, 262145], 2, 1, 64, 256), ([262145, 1000], 20, 10, 64, 16),
+    ([300001], 3, 1, 128, 16), ([600000, 1024], 17, 1, 64, 16), ([540673], 1, 1, 64, 32)])
+def test_decode_long(lens, heads, hk, d, page):
+    """Around 65536 and 262144 slots, where chunks become longer, and beyond, where a unit's pages are read in several
+    parts, with one chunk a unit and with two: against 64 bits, and bitwise what each sequence is alone."""
+    cache, table, lengths = long_cache(lens, hk, d, page, sum(lens) + hk)
+    q = torch.randn((len(lens), heads * d), generator=torch.Generator().manual_seed(3)).bfloat16().to(DEV)
+    out, lse = kv.decode_attn(q, cache, table, lengths, heads, return_lse=True)
+    kv.check_tables()
+    weighed, e = kv.decode_attn(q, cache, table, lengths, heads, return_lse=True, weights="set")
+    assert torch.equal(weighed, out) and torch.equal(e, lse)
+    for b, n in enumerate(lens):
+        want, e, p, mass, size = attend64(q[b].view(heads, 1, d), get(cache.k, table[b], n).transpose(0, 1),
+                                          get(cache.v, table[b], n).transpose(0, 1))
+        score, rel = errors32(d, n, size)
+        check_out(out[b].view(heads, d), want[:, 0], mass[:, 0], rel)
+        # fp32: the score's loss, half a step an addition of the sum, the logarithm and its product
+        assert bool(((lse[b].double() - e[:, 0]).abs() <= score + (n + 4) * 2.0 ** -24 + 2.0 ** -22 * e[:, 0].abs()).all())
+        w = p[:, 0].view(hk, heads // hk, n).sum(1).t()
+        off = (get(cache.weights, table[b], n).double() - w).abs()
+        assert bool((off <= 2 * (2 * rel + 2.0 ** -19 + (heads // hk + 1) * 2.0 ** -24) * w + 2.0 ** -126).all())
+        alone, e = kv.decode_attn(q[b:b + 1], cache, table[b:b + 1], lengths[b:b + 1], heads, return_lse=True, max_len=n)
+        assert torch.equal(alone[0], out[b]) and torch.equal(e[0], lse[b])
 
 
 def test_weights_apart():
