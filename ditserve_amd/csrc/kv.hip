@@ -449,7 +449,8 @@ __global__ __launch_bounds__(256) void kv_move_kernel(KvPages t, KvPages to, KvT
   if (j >= m) return;
   const int i = slots[((int64_t)b * gridDim.y + h) * keep + j], low = (1 << t.page_log2) - 1;
   bool ok, ok_to;
-  const int p = kv_page(t, b, i, ok, true), q = kv_page(to, b, j, ok_to, true);
+  const int p = kv_page(t, b, i, ok, false), q = kv_page(to, b, j, ok_to, false);
+  if (!ok || !ok_to) *t.status = 1;  // (once both are there: a branch behind the first alone, 8 x 8192 slots 33 us for 32)
   if (!ok_to) return;
   const int64_t src = (((int64_t)(i & low) << LOG_CH) + c) * 8, dst = (((int64_t)(j & low) << LOG_CH) + c) * 8;
   u32x4_t k = {0, 0, 0, 0}, v = {0, 0, 0, 0};
@@ -497,7 +498,11 @@ DITK_EXPORT int ditk_kv_append(const void* k, int64_t ldk, const void* v, int64_
 }
 
 namespace {
-// launches of the selection: rows of up to 1024 * kpt slots by one workgroup each (parts 1), longer ones in parts
+// launches of the selection: rows of up to 1024 * kpt slots by one workgroup each (parts 1), longer ones in parts.  Parts of
+// 8192 slots put more CUs to a row, parts of 32768 leave fewer counts, which each workgroup of a row reads whole (sixteen
+// parts at a time: the border).  Eight key heads, the whole call, us with parts of 8192 and of 32768: 1 x 40000 slots 31 and 53,
+// 1 x 131072 49 and 71, 8 x 131072 289 and 278; beyond the border 1 x 262144 54 and 72, 1 x 524288 71 and 72, 8 x 262144
+// 350 and 334, 1 x 1000000 147 and 80, 4 x 1000000 500 and 301.
 struct SelectPlan {
   int kpt, parts;
 };
