@@ -50,9 +50,11 @@
 // launch of its own (77 keys 5 of 12 us).  Probabilities are rounded to bf16, 8 bits, as in all forms above: the second
 // product takes bf16, and a second operand for what that cuts off (attn_chunk.h) would make the matrix pipe's work 1.5 times
 // as much; outputs are 1.03-1.09 times as far from 64 bits as with probabilities in fp32.  The matrix pipe bounds long
-// prompts (16384 queries, 32 heads of 128 over 8: 1.76 ms, 1.25 PFLOP/s of what is seen, at the clock that the power
-// leaves), a work item's start and end short ones (6 us of 10 for 128 queries).  Segments of few queries over many keys go
-// to causal_few.hip.
+// prompts (16384 queries, 32 heads of 128 over 8: 1.69-1.76 ms, 1.25-1.30 PFLOP/s of what is seen, at the clock that the
+// power leaves), a work item's start and end short ones (6 us of 10 for 128 queries).  At head_dim 64 a score has half the
+// matrix work and the same 4.2 vector operations, an exp among them, and these bound it: 16384 queries 1.12 ms, the matrix
+// pipe busy 45% of the time (67% at 128), the vector pipe 47% at 4 cycles an operation and the exps' own cycles on top.
+// Segments of few queries over many keys go to causal_few.hip.
 #include <algorithm>
 #include <cmath>
 #include <mutex>
@@ -605,9 +607,9 @@ int item_queries(int Tq, int nseg, int heads, int np, bool equal) {
 // all CUs are busy, 0.78 with few of them; one of two blocks 7.5 and 1.55 or 1.0 (head_dim 64: 4.5, 0.65 and 0.6; 5.3,
 // 0.95 and 0.7).  The longest run first: whole rounds of the CUs at the mean, then what is left of a round at the shortest
 // items' length, but no less than the longest item.  Only totals are known here: segments count as equal.
-// Measured, 128 and 256: 32 heads over 8, 1024 queries 22.4 us and 30.8, 2048 48.0 and 51.5, 4096 152 and 123; 8 of 355
-// 34.5 and 35.1; 512 after 7488 keys 107 and 147; two of 1024 after 6001 with 40 heads 297 and 283; 40 of 300 with 12
-// heads 58.7 and 66.0; head_dim 64, 32 heads: 2048 36.2 and 37.8, 4096 112 and 79.
+// Measured, 128 and 256: 32 heads over 8, 1024 queries 21.5 us and 28.8, 2048 44.4 and 50.1, 4096 147 and 126; 8 of 355
+// 31.3 and 33.9; 512 after 7488 keys 105 and 147; two of 1024 after 6001 with 40 heads 298 and 288; 40 of 300 with 12
+// heads 56.3 and 63.6; head_dim 64, 32 heads: 2048 31.5 and 35.2, 4096 100 and 78.7.
 int causal_item_queries(int Tq, int Tk, int nseg, int heads, int head_dim) {
   const double ncu = ditk_cu_count(), n = (double)Tq / nseg, ahead = Tk > Tq ? (double)(Tk - Tq) / nseg : 0.0;
   auto time = [&](double bm, double start, double busy, double light) {

@@ -4,9 +4,11 @@
 // The query heads of a key head, 16 at a time, are the columns of a wave's products (attn_chunk.h).  A chunk's length
 // goes by the sequence's own length alone, so a sequence's result does not depend on what it is batched with.
 //
-// Each slot is read once and gives 2 operations a byte and query head: memory bounds it.  32 heads over 8 of 128: 16
-// sequences of 32768 slots 360 us (5.9 TB/s), 64 of 2000 90 (5.8), one of 131072 (40 heads) 89 (6.0); where few waves
-// have a unit each, the latency of a chunk's tiles: one of 8192 14 us.
+// Up to 16 query heads a key head, each slot is read once, and gives 2 operations a byte and query head: memory bounds it.
+// 32 heads over 8 of 128, this kernel: 16 sequences of 32768 slots 360 us (5.9 TB/s), 64 of 2000 90 (5.8), one of 131072 (40
+// heads) 89 (6.0); where few waves have a unit each, the latency of a chunk's tiles: one of 8192 14 us.  Of more than 16
+// heads, every 16 read the slots again, side by side in the list: 16 of 32768 with one key head 51 us for 16 query
+// heads (5.2 TB/s), 84 for 32 (3.2 of what there is).
 #include "attn_chunk.h"
 #include "kv_common.h"
 
@@ -51,8 +53,8 @@ struct Args {
   float scale2;   // softmax scale times log2 e
 };
 
-// Pages of a sequence, 64 of them (1024 slots at least) in a wave's lanes.  ONCE: a long cache's rows go past the caches
-// (16 x 32768 slots 410 -> 397 us, 1 x 131072 105 -> 94, 64 x 2000 112 -> 108; not where scores are written
+// Pages of a sequence, 64 of them (1024 slots at least) in a wave's lanes.  ONCE: a long cache's rows go past the caches,
+// also where more than 16 query heads read them more than once (16 x 32768 slots 410 -> 397 us, 1 x 131072 105 -> 94, 64 x 2000 112 -> 108; not where scores are written
 // beside: 469 -> 475).
 template <int HD, bool ONCE>
 struct PagedSrc {

@@ -17,7 +17,9 @@ Checks, streams and errors are those of ditserve_amd.ops.  A length outside what
 holds is clamped to it, and a page that the cache lacks is neither read nor written (its
 slots count as absent); both are reported by a later call or by check_tables(), as an
 invalid cu_seqlens table is.  The pages a call writes must belong to one sequence; pages
-that are only read may be shared.  The reference has no counterpart: its models attend over
+that are only read may be shared.  The cache serves single tokens: no call attends several
+new tokens over it, so the next part of a prompt (ops.flash_attn_causal) needs the keys and
+values of its earlier parts as packed rows as well.  The reference has no counterpart: its models attend over
 whole videos.
 """
 import ctypes
@@ -293,7 +295,12 @@ def decode_attn(q, cache, table, lengths, heads, softmax_scale=None, max_len=Non
     cache's weights what each slot gets from these queries (the probabilities, summed over
     the query heads of its key head), "add" adds it.  Returns out [batch, heads * head_dim]
     bf16, and with return_lse lse [batch, heads] fp32 (natural log).  A sequence without
-    slots gives zeros and -inf.  A sequence's result does not depend on the others."""
+    slots gives zeros and -inf.  A sequence's result does not depend on the others.
+
+    The workspace goes by max_len, not by the lengths: beyond 512 slots (head_dim + 2) * 4 bytes
+    for each query head and chunk (64 slots, 512 of long caches), and with weights 4 bytes for
+    each query head and slot: 64 sequences, 32 heads of 128, max_len 131072 take 0.27 GB, with
+    weights 1.35."""
     _cache_check(cache)
     device, (pages, hk, page, d) = cache._k.device, cache._dims
     batch = _lengths(lengths, device)
