@@ -52,7 +52,7 @@
 // as much; outputs are 1.03-1.09 times as far from 64 bits as with probabilities in fp32.  The matrix pipe bounds long
 // prompts (16384 queries, 32 heads of 128 over 8: 1.69-1.76 ms, 1.25-1.30 PFLOP/s of what is seen, at the clock that the
 // power leaves), a work item's start and end short ones (6 us of 10 for 128 queries).  At head_dim 64 a score has half the
-// matrix work and the same 4.2 vector operations, an exp among them, and these bound it: 16384 queries 1.12 ms, the matrix
+// matrix work and the same 4.2 vector operations, an exp among them, and these bound it: 16384 queries 1.1-1.2 ms, the matrix
 // pipe busy 45% of the time (67% at 128), the vector pipe 47% at 4 cycles an operation and the exps' own cycles on top.
 // Segments of few queries over many keys go to causal_few.hip.
 #include <algorithm>
